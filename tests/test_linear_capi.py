@@ -1,0 +1,168 @@
+"""Linear attention and the projection with an epilogue without a GPU: the header's entry points, what they refuse (before
+any launch), the host layer's refusals, the registered operators."""
+
+from __future__ import annotations
+
+import ctypes
+import importlib
+import re
+from pathlib import Path
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+ROOT = Path(__file__).resolve().parents[1]
+P = ctypes.c_void_p(1 << 20)  # never read: every call below is refused
+ODD = ctypes.c_void_p((1 << 20) + 8)
+
+
+@pytest.fixture(scope="module")
+def native():
+    return importlib.import_module("zonos3-mini_amd._native")
+
+
+def test_header_and_library_agree(native):
+    text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "zonos3_linear.h").read_text(), flags=re.S)
+    names = set(re.findall(r"\b(zlin_\w+)\s*\(", text))
+    assert names == set(native.LINEAR)
+    for n in names:
+        assert hasattr(native.lib(), n)
+
+
+def _refused(native, name, args, cases):
+    for over, match in cases:
+        assert set(over) <= set(args)
+        with pytest.raises(RuntimeError, match=match):
+            native.call(name, *{**args, **over}.values())
+
+
+def test_attn_fwd_refuses(native):
+    size = native.lib().zlin_attn_workspace_bytes
+    for bad in ((0, 0, 64, 4, 128, 128, 1), (0, 1, -1, 4, 128, 128, 1), (0, 1, 64, 4, 96, 128, 1), (0, 1, 64, 4, 128, 256, 1),
+                (0, 1, 64, 4, 128, 128, 3), (0, 1, 64, 0, 128, 128, 1)):
+        assert size(*bad) == 0
+    need = size(0, 2, 300, 4, 128, 128, 1)
+    assert 0 < need < size(0, 2, 3000, 4, 128, 128, 1)
+    args = dict(q=P, q_ld=512, k=P, k_ld=512, v=P, v_ld=512, dtype=1, g=P, g_ld=4, g_dtype=0, s_in=None, s_out=None, o=P,
+                cu=None, n_seqs=0, B=2, T=300, Hk=4, Hv=4, K=128, V=128, scale=1.0, ws=P, ws_bytes=need, stream=None)
+    _refused(native, "zlin_attn_fwd", args, [
+        (dict(B=0), "bad sizes"), (dict(T=-1), "bad sizes"), (dict(Hk=3), "multiple"), (dict(K=96), "K=96"),
+        (dict(V=32), "V=32"), (dict(dtype=2), "dtype code 2"), (dict(g_dtype=5), "dtype code 5"), (dict(q=None), "null"),
+        (dict(o=None), "null"), (dict(g=None), "null"), (dict(cu=P, n_seqs=2), "B == 1"), (dict(cu=P, B=1), "n_seqs=0"),
+        (dict(g_ld=3), "g rows 3 apart"), (dict(g_ld=0, g_dtype=1), "a head"), (dict(q_ld=504), "row strides"),
+        (dict(k_ld=516), "row strides"), (dict(v_ld=1 << 23), "row strides"), (dict(q=ODD), "16-byte"),
+        (dict(s_in=P, s_out=ctypes.c_void_p((1 << 20) + 4096)), "overlap"), (dict(ws=None), "workspace"),
+        (dict(ws_bytes=need - 1), "workspace"), (dict(B=1 << 20, T=1 << 12), "rows")])
+
+
+def test_attn_step_refuses(native):
+    args = dict(q=P, q_ld=512, k=P, k_ld=512, v=P, v_ld=512, dtype=1, g=P, g_ld=0, g_dtype=0, state=P, slots=None, n_slots=3,
+                o=P, B=3, Hk=4, Hv=4, K=128, V=128, scale=1.0, stream=None)
+    _refused(native, "zlin_attn_step", args, [
+        (dict(B=-1), "bad sizes"), (dict(Hv=6), "multiple"), (dict(K=32), "K=32"), (dict(V=192), "V=192"),
+        (dict(dtype=7), "dtype code 7"), (dict(state=None), "null"), (dict(n_slots=4), "without slots"),
+        (dict(g_dtype=1), "a head"), (dict(g_ld=2), "g rows 2 apart"), (dict(v_ld=513), "row strides"),
+        (dict(state=ODD), "16-byte"), (dict(B=1 << 22, n_slots=1 << 22), "rows")])
+    assert native.lib().zlin_attn_step(*{**args, "B": 0, "n_slots": 0}.values()) == native.OK  # nothing to do
+
+
+def test_gemm_act_refuses(native):
+    args = dict(x=P, x_ld=256, w=P, w_ld=256, bias=P, bias_dtype=1, act=2, res=P, r_ld=64, y=P, y_ld=64, M=4, N=64, K=256,
+                dtype=1, stream=None)
+    _refused(native, "zlin_gemm_act", args, [
+        (dict(dtype=0), "bf16 only"), (dict(bias_dtype=3), "bias dtype"), (dict(act=5), "activation 5"), (dict(act=-1), "activation"),
+        (dict(M=-1), "bad sizes"), (dict(N=0), "bad sizes"), (dict(K=0), "bad sizes"), (dict(w=None), "null"),
+        (dict(x_ld=255), "row strides"), (dict(w_ld=128), "row strides"), (dict(y_ld=63), "row strides"),
+        (dict(r_ld=63), "row strides"), (dict(y=ctypes.c_void_p((1 << 20) + 1)), "boundary"),
+        (dict(bias=ctypes.c_void_p((1 << 20) + 2), bias_dtype=0), "boundary")])
+    assert native.lib().zlin_gemm_act(*{**args, "M": 0}.values()) == native.OK
+
+
+def test_host_layer_refuses_cpu_tensors(gdn):
+    q = torch.zeros(1, 2, 1, 128)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        gdn.linear_attn_fwd(q, q, q, torch.zeros(1))
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        gdn.linear_attn_step(q[0], q[0], q[0], torch.zeros(1), torch.zeros(2, 1, 128, 128))
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        gdn.gemm_act(torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(3, 8, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="expected a tensor"):
+        gdn.gemm_act(None, None)
+
+
+def test_registered_operators(gdn):
+    z = torch.ops.zgdn
+    ops = importlib.import_module("zonos3-mini_amd.torch_ops")
+    assert {"linear_attn_fwd", "linear_attn_step", "gemm_act"} <= set(ops.OPERATORS)
+    writes = lambda n: {a.name for a in getattr(z, n).default._schema.arguments  # noqa: E731
+                        if a.alias_info is not None and a.alias_info.is_write}
+    assert writes("linear_attn_step") == {"state"} and not writes("linear_attn_fwd") and not writes("gemm_act")
+    with FakeTensorMode():
+        q, v = torch.empty(1, 70, 2, 128, dtype=torch.bfloat16), torch.empty(1, 70, 4, 64, dtype=torch.bfloat16)
+        o, s = z.linear_attn_fwd(q, q, v, torch.empty(4), None, None, torch.empty(6, dtype=torch.int32))
+        assert o.shape == v.shape and o.dtype == v.dtype and s.shape == (5, 4, 64, 128) and s.dtype == torch.float32
+        assert z.linear_attn_step(q[0], q[0], v[0], torch.empty(4), torch.empty(70, 4, 64, 128)).shape == (70, 4, 64)
+        y = z.gemm_act(q[0, :, 0], torch.empty(24, 128, dtype=torch.bfloat16), None, "silu", None)
+        assert y.shape == (70, 24) and y.dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_operators_run_what_the_direct_calls_run(gdn, cuda):
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(cuda)  # noqa: E731
+    q, k, v, a = r(1, 90, 2, 64), r(1, 90, 2, 64), r(1, 90, 2, 64), -r(1, 90, 2).abs()
+    assert all(torch.equal(x, y) for x, y in zip(gdn.linear_attn_fwd(q, k, v, a), torch.ops.zgdn.linear_attn_fwd(q, k, v, a)))
+    s1 = torch.zeros(90, 2, 64, 64, device=cuda)
+    s2 = s1.clone()
+    assert torch.equal(gdn.linear_attn_step(q[0], k[0], v[0], a[0], s1), torch.ops.zgdn.linear_attn_step(q[0], k[0], v[0], a[0], s2))
+    assert torch.equal(s1, s2) and bool(s1.any())
+    x, w = r(50, 64), r(40, 64)
+    assert torch.equal(gdn.gemm_act(x, w, activation="relu"), torch.ops.zgdn.gemm_act(x, w, None, "relu"))
+    tests = ("test_schema", "test_faketensor")
+    torch.library.opcheck(torch.ops.zgdn.linear_attn_fwd.default, (q, k, v, a), test_utils=tests)
+    torch.library.opcheck(torch.ops.zgdn.linear_attn_step.default, (q[0], k[0], v[0], a[0], s1), test_utils=tests)
+    torch.library.opcheck(torch.ops.zgdn.gemm_act.default, (x, w), test_utils=tests)
+
+
+@pytest.mark.gpu
+def test_host_layer_refuses(gdn, cuda):
+    """What the Python layer refuses, with messages, before a launch."""
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=cuda)  # noqa: E731
+    f32 = torch.float32
+    q, v, g = z(1, 8, 2, 64), z(1, 8, 2, 64), z(2, dt=f32)
+
+    def refused(match, f, *a, **k):
+        with pytest.raises(RuntimeError, match=match):
+            f(*a, **k)
+
+    fwd, step, gemm = gdn.linear_attn_fwd, gdn.linear_attn_step, gdn.gemm_act
+    refused("equal", fwd, q, q[:, :7], v, g)
+    refused("share a dtype", fwd, q, q, v.float(), g)
+    refused("not supported", fwd, q.half(), q.half(), v.half(), g)
+    refused("multiple", fwd, q, q, z(1, 8, 3, 64), z(3, dt=f32))
+    refused("64 or 128", fwd, z(1, 8, 2, 96), z(1, 8, 2, 96), v, g)
+    refused("a decay a head", fwd, q, q, v, g.to(torch.bfloat16))
+    refused("a decay a head", fwd, q, q, v, z(1, 7, 2, dt=f32))
+    refused("B == 1", fwd, z(2, 4, 2, 64), z(2, 4, 2, 64), z(2, 4, 2, 64), g, cu_seqlens=[0, 8])
+    refused("decreases", fwd, q, q, v, g, cu_seqlens=[0, 5, 4, 8])
+    refused("ends at", fwd, q, q, v, g, cu_seqlens=[0, 5])
+    refused("int32", fwd, q, q, v, g, cu_seqlens=torch.tensor([0, 8], device=cuda))
+    refused("initial_state", fwd, q, q, v, g, initial_state=z(2, 2, 64, 64, dt=f32))
+    refused("final_state", fwd, q, q, v, g, final_state=z(1, 2, 64, 64))
+    wide = z(3, 2, 64, 64, dt=f32)
+    two = z(2, 8, 2, 64)
+    refused("overlap", fwd, two, two, two, g, initial_state=wide[:2], final_state=wide[1:])
+    st = z(8, 2, 64, 64, dt=f32)
+    refused("states for", step, q[0], q[0], v[0], g, st[:7])
+    refused("slots", step, q[0], q[0], v[0], g, st, slots=torch.zeros(8, dtype=torch.int32, device=cuda))
+    refused("contiguous", step, q[0], q[0], v[0], g, z(8, 2, 64, 128, dt=f32)[..., :64])
+    x, w = z(4, 16), z(8, 16)
+    refused("activation", gemm, x, w, activation="tanh")
+    refused("bias", gemm, x, w, bias=z(7))
+    refused("residual", gemm, x, w, residual=z(4, 9))
+    refused("residual", gemm, x, w, residual=z(3, 8))
+    refused("expected bfloat16", gemm, x.float(), w)
+    refused("out", gemm, x, w, out=z(4, 16)[:, ::2])
+    refused("out", gemm, x, w, out=z(4, 9))
+    refused("w: expected", gemm, x, z(8, 17))

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libzonos3_gdn.so`` (the C ABI declared in ``include/zonos3_gdn.h``).
+"""ctypes binding of ``libzonos3_gdn.so`` (the C ABI declared in ``include/zonos3_gdn.h`` and
+``include/zonos3_linear.h``).
 
 The library is loaded after ``torch`` so that it binds to the HIP runtime torch already loaded (both carry
 the soname ``libamdhip64.so.7``); device pointers and streams then come straight from torch tensors.
@@ -19,6 +20,8 @@ F32, BF16 = 0, 1
 OK, EINVAL, EHIP, EUNSUPPORTED = 0, 1, 2, 3
 # bits of the chunked path's device status word (zgdn_chunk_status)
 STATUS_WAIT_GAVE_UP = 1
+# activation codes (enum zlin_act)
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 ABI_VERSION = 2  # zgdn_abi_version() of the library these signatures describe
 
 _P = c_void_p
@@ -85,6 +88,25 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
+# Entry points of include/zonos3_linear.h (the same library): name -> (restype, argtypes).
+LINEAR: dict[str, tuple] = {
+    "zlin_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "zlin_attn_fwd": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_long, c_int, _P, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
+         c_int, c_int, c_float, _P, c_size_t, _P],
+    ),
+    "zlin_attn_step": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_long, c_int, _P, c_long, c_int, _P, _P, c_int, _P, c_int, c_int, c_int, c_int,
+         c_int, c_float, _P],
+    ),
+    "zlin_gemm_act": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_int, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P],
+    ),
+}
+
 # Entry points of this package's own host layer, outside the published header: name -> (restype, argtypes).
 INTERNAL: dict[str, tuple] = {
     "zgdn_chunk32_slices": (c_int, [c_int, c_int, c_int, c_int]),
@@ -116,7 +138,7 @@ def lib() -> ctypes.CDLL:
             handle = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
         except OSError as exc:
             raise RuntimeError(f"cannot load {LIB_PATH}: {exc}") from exc
-        for name, (res, args) in (SIGNATURES | INTERNAL).items():
+        for name, (res, args) in (SIGNATURES | LINEAR | INTERNAL).items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

@@ -913,3 +913,187 @@ def serving_extend(x, in_proj, conv_weight, A_log, dt_bias, norm_weight, conv_co
                  state_live.data_ptr(), window.data_ptr(), win_len.data_ptr(), gated.data_ptr(), float(eps), float(scale),
                  workspace.data_ptr(), ws_bytes, stream)
     return gated
+
+
+# ------------------------------------------------------------- linear attention and the projections around it
+
+
+def _call_on(dev, name: str, *args) -> None:
+    """``_native.call`` with ``dev`` the current device (the library asks the current device for its CUs and launches
+    there)."""
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():
+        _native.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            _native.call(name, *args)
+
+
+def _linear_decay(g, lead: tuple, Hv: int, dev):
+    """(g, row stride, dtype code) of the log decays: float32 [Hv] (stride 0), or [*lead, Hv] read in place."""
+    if not isinstance(g, torch.Tensor):
+        raise RuntimeError("g: expected a tensor")
+    if g.dim() == 1:
+        _on_gpu("g", g, dev)
+        if not (g.dtype == torch.float32 and g.shape == (Hv,)):
+            raise RuntimeError(f"g: expected float32 [{Hv}] (a decay a head) or [{', '.join(map(str, lead))}, {Hv}]")
+        return g, 0, F32
+    g, ld = _rows_in_place("g", g, 1, dev)
+    if tuple(g.shape) != (*lead, Hv):
+        raise RuntimeError(f"g: expected float32 [{Hv}] (a decay a head) or [{', '.join(map(str, lead))}, {Hv}], "
+                           f"got {tuple(g.shape)}")
+    return g, ld, _code(g, "g")
+
+
+def _linear_qkv(q, k, v, lead_dims: int):
+    """The rows of q, k [*lead, Hk, K] and v [*lead, Hv, V], read in place where the kernels can, with their strides."""
+    dev = q.device if isinstance(q, torch.Tensor) else None
+    ve = 4 if isinstance(q, torch.Tensor) and q.dtype == torch.float32 else 8  # elements in 16 bytes
+    q, q_ld = _rows_in_place("q", q, 2, dev, ve, 16)
+    k, k_ld = _rows_in_place("k", k, 2, dev, ve, 16)
+    v, v_ld = _rows_in_place("v", v, 2, dev, ve, 16)
+    n = lead_dims
+    if not (q.dim() == n + 2 and k.shape == q.shape):
+        raise RuntimeError(f"q, k: expected equal [{'B, T' if n == 2 else 'B'}, Hk, K], got {tuple(q.shape)}, {tuple(k.shape)}")
+    if not (v.dim() == n + 2 and v.shape[:n] == q.shape[:n]):
+        raise RuntimeError(f"v: expected [{', '.join(map(str, q.shape[:n]))}, Hv, V], got {tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise RuntimeError("q, k, v: must share a dtype")
+    _code(q, "q")
+    (Hk, K), (Hv, V) = q.shape[n:], v.shape[n:]
+    if Hk < 1 or Hv < 1 or Hv % Hk != 0:
+        raise RuntimeError(f"value heads ({Hv}) must be a multiple of key heads ({Hk})")
+    if K not in (64, 128) or V not in (64, 128):
+        raise RuntimeError(f"head dims K={K}, V={V}; linear attention takes 64 or 128 each")
+    out = []
+    for t, ld in ((q, q_ld), (k, k_ld), (v, v_ld)):  # rows further apart than the kernels' 32-bit offsets reach
+        out.append((t, ld) if ld <= 1 << 22 else (t.contiguous(), t.shape[-1] * t.shape[-2]))
+    return out
+
+
+def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_state=True, cu_seqlens=None,
+                    final_state=None):
+    """Linear attention with a decay per head over whole sequences, chunked (C ABI ``zlin_attn_fwd``):
+    ``S_t = exp(g_t) S_{t-1} + v_t k_t^T``, ``o_t = S_t (scale q_t)``.
+
+    q, k [B, T, Hk, K], v [B, T, Hv, V], all bfloat16 or all float32, K and V each 64 or 128; value head h reads key head
+    ``h // (Hv / Hk)``. g: log decays, float32 [Hv] (one a head) or float32 / bfloat16 [B, T, Hv] (-inf forgets all that
+    was before; values below -200 count as -200, whose exponential is zero in float32). Packed sequences: B == 1 and
+    ``cu_seqlens`` int32 [N + 1] (a device table is not read on the host; a list or CPU tensor is checked, then
+    copied). initial_state [N, Hv, V, K] float32 or None (zeros). ``final_state`` may name an existing float32 tensor to
+    write (it may be ``initial_state`` itself: in place). q, k, v, g may be column slices of wider rows. ``scale``
+    defaults to ``K ** -0.5``. Returns (o [B, T, Hv, V] in q's dtype, final state or None); rows that no sequence of a
+    device table holds are not written."""
+    (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 2)
+    dev = q.device
+    B, T, Hk, K = q.shape
+    Hv, V = v.shape[2], v.shape[3]
+    if B < 1:
+        raise RuntimeError("q: no batch (B == 0)")
+    g, g_ld, g_code = _linear_decay(g, (B, T), Hv, dev)
+    n_seqs = B
+    if cu_seqlens is not None:
+        if B != 1:
+            raise RuntimeError("cu_seqlens: packed sequences need B == 1")
+        if _on_host(cu_seqlens):
+            cu = cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else [int(x) for x in cu_seqlens]
+            check_cu_seqlens(cu, T)
+            cu_seqlens = torch.tensor(cu, dtype=torch.int32).to(dev)
+        n_seqs = _cu_check(cu_seqlens, T, dev)
+    for name, t in (("initial_state", initial_state), ("final_state", final_state)):
+        if t is not None:
+            _on_gpu(name, t, dev)
+            if not (t.dtype == torch.float32 and t.shape == (n_seqs, Hv, V, K)):
+                raise RuntimeError(f"{name}: expected float32 [{n_seqs}, {Hv}, {V}, {K}], got {t.dtype} {tuple(t.shape)}")
+    if final_state is None and output_final_state:
+        final_state = torch.empty(n_seqs, Hv, V, K, device=dev, dtype=torch.float32)
+    o = torch.empty(B, T, Hv, V, device=dev, dtype=q.dtype)
+    code = _CODES[q.dtype]
+    size = int(_native.lib().zlin_attn_workspace_bytes(int(cu_seqlens is not None), n_seqs, T, Hv, K, V, code))
+    workspace = torch.empty(max(size, 16), device=dev, dtype=torch.uint8)
+    _call_on(dev, "zlin_attn_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, g.data_ptr(), g_ld,
+             g_code, _ptr(initial_state), _ptr(final_state), o.data_ptr(), _ptr(cu_seqlens), n_seqs, B, T, Hk, Hv, K, V,
+             K**-0.5 if scale is None else float(scale), workspace.data_ptr(), workspace.numel(), _stream(dev))
+    return o, final_state
+
+
+def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
+    """One token of linear attention for each of B streams, updating ``state`` in place (C ABI ``zlin_attn_step``):
+    ``S = exp(g) S + v k^T``, ``o = S (scale q)``.
+
+    q, k [B, Hk, K], v [B, Hv, V] (rows may be slices of a projection's), g float32 [Hv] or float32 / bfloat16 [B, Hv].
+    state [B, Hv, V, K] float32; with ``slots`` (int64 [B]) a table [n_slots, Hv, V, K] of which stream b has row
+    ``slots[b]``: a stream whose slot lies outside the table, or that an earlier stream of the call names, gets zeros and
+    touches no state. Returns o [B, Hv, V] in v's dtype."""
+    (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 1)
+    dev = q.device
+    B, Hk, K = q.shape
+    Hv, V = v.shape[1], v.shape[2]
+    g, g_ld, g_code = _linear_decay(g, (B,), Hv, dev)
+    _on_gpu("state", state, dev)
+    n_slots = state.shape[0] if state.dim() else 0
+    if not (state.dtype == torch.float32 and state.dim() == 4 and state.shape[1:] == (Hv, V, K)):
+        raise RuntimeError(f"state: expected float32 [{'B' if slots is None else 'n_slots'}, {Hv}, {V}, {K}], "
+                           f"got {state.dtype} {tuple(state.shape)}")
+    if slots is None:
+        if n_slots != B:
+            raise RuntimeError(f"state: {n_slots} states for {B} streams (slots name rows of a table)")
+    else:
+        _on_gpu("slots", slots, dev)
+        if not (slots.dtype == torch.int64 and slots.shape == (B,)):
+            raise RuntimeError(f"slots: expected int64 [{B}], got {slots.dtype} {tuple(slots.shape)}")
+    o = torch.empty(B, Hv, V, device=dev, dtype=v.dtype)
+    _call_on(dev, "zlin_attn_step", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, _CODES[q.dtype],
+             g.data_ptr(), g_ld, g_code, state.data_ptr(), _ptr(slots), n_slots, o.data_ptr(), B, Hk, Hv, K, V,
+             K**-0.5 if scale is None else float(scale), _stream(dev))
+    return o
+
+
+def _matrix_rows(name: str, t, cols: int | None, dev):
+    """A bfloat16 matrix with unit column stride on ``dev``, copied where its columns are not beside one another."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: must be a GPU tensor (got device {t.device}); there is no CPU path")
+    if t.device != dev:
+        raise RuntimeError(f"{name}: on {t.device}, expected {dev}")
+    if not (t.dim() == 2 and t.dtype == torch.bfloat16 and (cols is None or t.shape[1] == cols)):
+        raise RuntimeError(f"{name}: expected bfloat16 [rows, {'K' if cols is None else cols}], got {t.dtype} {tuple(t.shape)}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, max(t.stride(0), t.shape[1])
+
+
+def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
+    """``y = act(x w^T + bias) + residual`` on bf16 MFMA, sums and epilogue in float32, rounded once (C ABI
+    ``zlin_gemm_act``): a projection with its bias, activation and residual stream.
+
+    x [M, K], w [N, K] bfloat16 (any sizes; rows may be strided), bias [N] bfloat16 or float32, ``activation`` None,
+    "relu", "silu", "gelu" (erf) or "gelu_tanh", residual [M, N] bfloat16. Returns y [M, N] bfloat16: ``out`` when given
+    (unit column stride; it may be ``residual`` itself, and may overlap no other operand)."""
+    dev = x.device if isinstance(x, torch.Tensor) else None
+    x, x_ld = _matrix_rows("x", x, None, dev)
+    M, K = x.shape
+    w, w_ld = _matrix_rows("w", w, K, dev)
+    N = w.shape[0]
+    if N < 1 or K < 1:
+        raise RuntimeError(f"w: expected [N, K] with N, K >= 1, got {tuple(w.shape)}")
+    if activation not in _native.ACTIVATIONS:
+        raise RuntimeError(f"activation {activation!r}: one of {list(_native.ACTIVATIONS)}")
+    if bias is not None:
+        _on_gpu("bias", bias, dev)
+        if bias.shape != (N,):
+            raise RuntimeError(f"bias: expected [{N}], got {tuple(bias.shape)}")
+    if out is None:
+        out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+    elif not (isinstance(out, torch.Tensor) and out.device == dev and out.shape == (M, N) and out.dtype == torch.bfloat16
+              and (N == 1 or out.stride(1) == 1) and (M <= 1 or out.stride(0) >= N)):
+        raise RuntimeError(f"out: expected bfloat16 [{M}, {N}] on {dev} with unit column stride and rows apart")
+    r_ld = 0
+    if residual is not None:
+        residual, r_ld = _matrix_rows("residual", residual, N, dev)
+        if residual.shape[0] != M:
+            raise RuntimeError(f"residual: expected [{M}, {N}], got {tuple(residual.shape)}")
+    _call_on(dev, "zlin_gemm_act", x.data_ptr(), x_ld, w.data_ptr(), w_ld, _ptr(bias),
+             F32 if bias is None else _code(bias, "bias"), _native.ACTIVATIONS[activation], _ptr(residual), r_ld,
+             out.data_ptr(), max(out.stride(0), N), M, N, K, BF16, _stream(dev))
+    return out

@@ -19,6 +19,10 @@ state in place declare it in ``mutates_args``.
 | ``zgdn::l2norm`` | FLA ``l2norm_fwd`` (gdn.py:416-417); lm.py:570-571 |
 | ``zgdn::sigmoid`` | FLA ``fused_beta_sigmoid_fwd`` (gdn.py:423); lm.py:573 |
 | ``zgdn::gated_rmsnorm`` | FLA ``layer_norm_gated_fwd`` (gdn.py:435-445); lm.py:584-587 |
+
+Beside them, with no counterpart in the reference: ``zgdn::linear_attn_fwd`` (linear attention with a decay per head
+over sequences), ``zgdn::linear_attn_step`` (one token of it, states in place) and ``zgdn::gemm_act`` (a projection with
+bias, activation and residual).
 """
 
 from __future__ import annotations
@@ -194,5 +198,44 @@ def _(x, g, weight, eps=1e-5):
     return x.new_empty(x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
+# ------------------------------------------------------------- linear attention and the projections around it
+
+
+@torch.library.custom_op(f"{NS}::linear_attn_fwd", mutates_args=())
+def linear_attn_fwd(q: Tensor, k: Tensor, v: Tensor, g: Tensor, scale: Optional[float] = None,
+                    initial_state: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    return ops.linear_attn_fwd(q, k, v, g, scale=scale, initial_state=initial_state, cu_seqlens=cu_seqlens)
+
+
+@linear_attn_fwd.register_fake
+def _(q, k, v, g, scale=None, initial_state=None, cu_seqlens=None):
+    B, T, Hk, K = q.shape
+    Hv, V = v.shape[2], v.shape[3]
+    return v.new_empty(B, T, Hv, V), q.new_empty(_n_states(B, cu_seqlens), Hv, V, K, dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::linear_attn_step", mutates_args=("state",))
+def linear_attn_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor, scale: Optional[float] = None,
+                     slots: Optional[Tensor] = None) -> Tensor:
+    return ops.linear_attn_step(q, k, v, g, state, scale=scale, slots=slots)
+
+
+@linear_attn_step.register_fake
+def _(q, k, v, g, state, scale=None, slots=None):
+    return v.new_empty(v.shape)
+
+
+@torch.library.custom_op(f"{NS}::gemm_act", mutates_args=())
+def gemm_act(x: Tensor, w: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
+             residual: Optional[Tensor] = None) -> Tensor:
+    return ops.gemm_act(x, w, bias=bias, activation=activation, residual=residual)
+
+
+@gemm_act.register_fake
+def _(x, w, bias=None, activation=None, residual=None):
+    return x.new_empty(x.shape[0], w.shape[0])
+
+
 OPERATORS = ("recurrent_fwd", "decode_step", "chunk_fwd", "fused_decode_step", "serving_decode_step",
-             "attnres_route", "accent_shift", "causal_conv1d", "l2norm", "sigmoid", "gated_rmsnorm")
+             "attnres_route", "accent_shift", "causal_conv1d", "l2norm", "sigmoid", "gated_rmsnorm", "linear_attn_fwd",
+             "linear_attn_step", "gemm_act")

@@ -26,7 +26,7 @@ enum zlin_act { ZLIN_NONE = 0, ZLIN_RELU = 1, ZLIN_SILU = 2, ZLIN_GELU = 3 /* er
  * Bytes of workspace that zlin_attn_fwd needs for the same sizes (0 for sizes that it refuses). packed: 1 where
  * cu_seqlens is given (n_seqs sequences in T rows), else 0 (n_seqs = B batches of T rows).
  */
-size_t zlin_attn_workspace_bytes(int packed, int n_seqs, int T, int Hv, int K, int V, int dtype);
+size_t zlin_attn_workspace_bytes(int packed, int n_seqs, int T, int Hk, int Hv, int K, int V, int dtype);
 
 /*
  * Linear attention over whole sequences (chunked).

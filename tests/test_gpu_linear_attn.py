@@ -257,7 +257,7 @@ def test_rows_behind_the_last_sequence_stay(gdn, cuda):
     q, k, v, g = (d[n].to(cuda) for n in ("q", "k", "v", "g"))
     s0 = d["s0"].to(cuda)
     nat = gdn._native
-    ws = torch.empty(nat.lib().zlin_attn_workspace_bytes(1, 3, 200, 2, 64, 64, 1), dtype=torch.uint8, device=cuda)
+    ws = torch.empty(nat.lib().zlin_attn_workspace_bytes(1, 3, 200, 1, 2, 64, 64, 1), dtype=torch.uint8, device=cuda)
 
     def run(table):
         o = torch.full((200, 2, 64), 7.0, dtype=BF, device=cuda)

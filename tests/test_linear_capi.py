@@ -39,11 +39,12 @@ def _refused(native, name, args, cases):
 
 def test_attn_fwd_refuses(native):
     size = native.lib().zlin_attn_workspace_bytes
-    for bad in ((0, 0, 64, 4, 128, 128, 1), (0, 1, -1, 4, 128, 128, 1), (0, 1, 64, 4, 96, 128, 1), (0, 1, 64, 4, 128, 256, 1),
-                (0, 1, 64, 4, 128, 128, 3), (0, 1, 64, 0, 128, 128, 1)):
+    for bad in ((0, 0, 64, 4, 4, 128, 128, 1), (0, 1, -1, 4, 4, 128, 128, 1), (0, 1, 64, 4, 4, 96, 128, 1),
+                (0, 1, 64, 4, 4, 128, 256, 1), (0, 1, 64, 4, 4, 128, 128, 3), (0, 1, 64, 4, 0, 128, 128, 1),
+                (0, 1, 64, 3, 4, 128, 128, 1)):
         assert size(*bad) == 0
-    need = size(0, 2, 300, 4, 128, 128, 1)
-    assert 0 < need < size(0, 2, 3000, 4, 128, 128, 1)
+    need = size(0, 2, 300, 4, 4, 128, 128, 1)
+    assert 0 < need < size(0, 2, 3000, 4, 4, 128, 128, 1)
     args = dict(q=P, q_ld=512, k=P, k_ld=512, v=P, v_ld=512, dtype=1, g=P, g_ld=4, g_dtype=0, s_in=None, s_out=None, o=P,
                 cu=None, n_seqs=0, B=2, T=300, Hk=4, Hv=4, K=128, V=128, scale=1.0, ws=P, ws_bytes=need, stream=None)
     _refused(native, "zlin_attn_fwd", args, [

@@ -90,7 +90,7 @@ SIGNATURES: dict[str, tuple] = {
 
 # Entry points of include/zonos3_linear.h (the same library): name -> (restype, argtypes).
 LINEAR: dict[str, tuple] = {
-    "zlin_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "zlin_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "zlin_attn_fwd": (
         c_int,
         [_P, c_long, _P, c_long, _P, c_long, c_int, _P, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,

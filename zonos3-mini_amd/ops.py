@@ -1008,7 +1008,7 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
         final_state = torch.empty(n_seqs, Hv, V, K, device=dev, dtype=torch.float32)
     o = torch.empty(B, T, Hv, V, device=dev, dtype=q.dtype)
     code = _CODES[q.dtype]
-    size = int(_native.lib().zlin_attn_workspace_bytes(int(cu_seqlens is not None), n_seqs, T, Hv, K, V, code))
+    size = int(_native.lib().zlin_attn_workspace_bytes(int(cu_seqlens is not None), n_seqs, T, Hk, Hv, K, V, code))
     workspace = torch.empty(max(size, 16), device=dev, dtype=torch.uint8)
     _call_on(dev, "zlin_attn_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, g.data_ptr(), g_ld,
              g_code, _ptr(initial_state), _ptr(final_state), o.data_ptr(), _ptr(cu_seqlens), n_seqs, B, T, Hk, Hv, K, V,

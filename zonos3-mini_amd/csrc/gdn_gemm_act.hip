@@ -4,8 +4,8 @@
 // two tiles of w rows interleaved, so that a lane ends with 8 neighbouring columns of one row of y: bias, residual and y
 // are 16-byte accesses. Three forms, chosen by launch (below):
 //   gemm_act_tile   BM x BN tiles, both operands by direct-to-LDS loads in blocks of 64 of K, several blocks ahead;
-//   gemm_act_rows   few rows (a decode step): 16 x 16 tiles, K split over the workgroup's waves;
-//   gemm_act_any    rows off 16-byte boundaries, K not a multiple of 8: guarded loads through registers.
+//   gemm_act_split  few rows (a decode step): small tiles, K split over the workgroup's waves;
+//   gemm_act_any    rows off 16-byte boundaries, K not a multiple of 8: loads through registers.
 #include <algorithm>
 #include <atomic>
 
@@ -36,10 +36,10 @@ struct ActArgs {
 template <int ACT>
 __device__ __forceinline__ float act_of(float x) {
   if constexpr (ACT == ZLIN_RELU) return x > 0.f || x != x ? x : 0.f;
-  if constexpr (ACT == ZLIN_SILU) return x / (1.f + __expf(-x));
+  if constexpr (ACT == ZLIN_SILU) return silu_fast(x);
   if constexpr (ACT == ZLIN_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
   if constexpr (ACT == ZLIN_GELU_TANH)  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
-    return x / (1.f + __expf(-2.f * 0.79788456080286536f * (x + 0.044715f * x * x * x)));
+    return x * __builtin_amdgcn_rcpf(1.f + __expf(-2.f * 0.79788456080286536f * (x + 0.044715f * x * x * x)));
   return x;
 }
 
@@ -129,29 +129,34 @@ __device__ __forceinline__ void wait_and_meet() {  // at most N of the wave's lo
 // ------------------------------------------------------------------------------------------------------- tiles
 //
 // 8 waves, WM of them along the rows of x: BM x BN tiles, a wave BM / WM x BN / WN of it. Blocks of BK = 64 of K in NS
-// stages of LDS (128-byte rows, 16-byte chunk c of row r at c ^ f(r)): block kb computes while the NS - 1 after it land.
+// stages of LDS (128-byte rows, 16-byte chunk c of row r at c ^ f(r)): block kb computes while the next ones land. The
+// fragments of a block's second half are read under the products of its first, those of the next block's first half under
+// the products of its second: read when needed, LDS and matrix unit wait for each other (8192 x 4096 x 4096: 213 us read when needed, 211 so; the matrix unit runs at 85 % of the rate of the library's product, 178).
 // Fragment reads touch 16 rows, one chunk each: f spreads rows 0 .. 15 (x) and rows 8 a + b, b < 4 (w, whose fragments
 // interleave) over all 16 places of 256 bytes.
+// FOLD: the at most 16 columns behind the last full tile are formed by the tiles (row block tm, column tile tn: rows
+// 16 tn .. of its block), not by a column of tiles of their own (4096 x 2056 x 1024: 30.4 us, 24.9 so).
 
 constexpr int BK = 64;
 
 __device__ __forceinline__ int fx(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int fw(int r) { return (r >> 1 & 1) | (r >> 3 & 3) << 1; }
 
-template <int BM, int BN, int WM, int NS_>
+template <int BM, int BN, int WM, int NS_, bool FOLD>
 struct TileCfg {
   static constexpr int WN = 8 / WM;
   static constexpr int TM = BM / WM / 16, TN = BN / WN / 32;  // 16-row tiles of x, 32-row pairs of w, a wave
-  static constexpr int STAGE = (BM + BN) * 128;
+  static constexpr int STAGE = (BM + BN + (FOLD ? 16 : 0)) * 128;
   static constexpr int NS = NS_;
   static constexpr int LDS = NS * STAGE;
   static constexpr int PX = BM / 8 / 8, PW = BN / 8 / 8;  // 1 KiB pieces (8 rows) of each operand a wave
   static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;
+  static_assert(!FOLD || NS == 2, "the folded rows' two pieces are not counted");
 };
 
-template <int BM, int BN, int WM, int NS>
-__global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS>::PER_CU)) void gemm_act_tile_kernel(ActArgs a) {
-  using C = TileCfg<BM, BN, WM, NS>;
+template <int BM, int BN, int WM, int NS, bool FOLD>
+__global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS, FOLD>::PER_CU)) void gemm_act_tile_kernel(ActArgs a) {
+  using C = TileCfg<BM, BN, WM, NS, FOLD>;
   constexpr int TM = C::TM, TN = C::TN;
   extern __shared__ uint4 act_lds[];
   uint8_t* lds = reinterpret_cast<uint8_t*>(act_lds);
@@ -181,6 +186,19 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS>::PER_CU)) void ge
     cw[i] = (l & 7) ^ fw(r);
     ow[i] = (uint32_t)r * (uint32_t)a.w_ld * 2u + 16u * cw[i];
   }
+  // the folded columns: 16 rows of w, two pieces, by waves 0 and 1; their products by the wave that holds rows 16 tn
+  const int nf0 = a.tiles_n * BN;
+  const bool fold = FOLD && 16 * tn < BM, fold_mine = fold && wave == (16 * tn) / (BM / WM) + WM * (tn % C::WN);
+  au32x4 rf = {0u, 0u, 0u, 0u};
+  uint32_t of = 0;
+  int cf = 0;
+  af32x4 facc = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (FOLD) {
+    rf = rows_rsrc(a.w + (size_t)nf0 * a.w_ld, a.w_ld, a.N - nf0, a.K);
+    const int r = 8 * (wave & 1) + (l >> 3);
+    cf = (l & 7) ^ fx(r);
+    of = (uint32_t)r * (uint32_t)a.w_ld * 2u + 16u * cf;
+  }
   const int nk = (a.K + BK - 1) / BK, tail = a.K - (nk - 1) * BK;  // elements of the last block
   const uint32_t base = lds_at(lds);
   auto issue = [&](int kb, int stage) {
@@ -190,6 +208,9 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS>::PER_CU)) void ge
     for (int i = 0; i < C::PX; ++i) load_lds(rx, cut && 8 * cx[i] >= tail ? NOWHERE : ox[i], k, at + 8192 * i);
 #pragma unroll
     for (int i = 0; i < C::PW; ++i) load_lds(rw, cut && 8 * cw[i] >= tail ? NOWHERE : ow[i], k, at + BM * 128 + 8192 * i);
+    if constexpr (FOLD) {
+      if (fold && wave < 2) load_lds(rf, cut && 8 * cf >= tail ? NOWHERE : of, k, at + (BM + BN) * 128);
+    }
   };
 
   af32x4 acc[TN][2][TM];
@@ -199,190 +220,316 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS>::PER_CU)) void ge
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < TM; ++j) acc[i][u][j] = af32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int s = 0; s < NS - 1; ++s) issue(s, s);
   // w rows of fragment u of a pair: 8 (m / 4) + 4 u + m % 4
   const int rwl = wn + 8 * (m >> 2) + (m & 3), rxl = wm + m;
-  int st = 0;
-  for (int kb = 0; kb < nk; ++kb) {
-    wait_and_meet<(NS - 2) * (C::PX + C::PW)>();
-    issue(kb + NS - 1, st == 0 ? NS - 1 : st - 1);
-    const uint8_t* xs = lds + st * C::STAGE;
+  struct Frags {
+    abf16x8 x[TM], w[TN][2], fx_, fw_;
+  };
+  auto read = [&](Frags& f, int stage, int s) {
+    const uint8_t* xs = lds + stage * C::STAGE;
     const uint8_t* ws = xs + BM * 128;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      abf16x8 fb[TM], fa[TN][2];
+    for (int j = 0; j < TM; ++j)
+      f.x[j] = *reinterpret_cast<const abf16x8*>(xs + (rxl + 16 * j) * 128 + (((4 * s + g) ^ fx(rxl)) << 4));
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
-        fb[j] = *reinterpret_cast<const abf16x8*>(xs + (rxl + 16 * j) * 128 + (((4 * s + g) ^ fx(rxl)) << 4));
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          fa[i][u] = *reinterpret_cast<const abf16x8*>(ws + (rwl + 32 * i + 4 * u) * 128 + (((4 * s + g) ^ fw(rwl)) << 4));
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < TM; ++j) acc[i][u][j] = amfma(fa[i][u], fb[j], acc[i][u][j]);
+      for (int u = 0; u < 2; ++u)
+        f.w[i][u] = *reinterpret_cast<const abf16x8*>(ws + (rwl + 32 * i + 4 * u) * 128 + (((4 * s + g) ^ fw(rwl)) << 4));
+    if constexpr (FOLD) {
+      if (fold_mine) {
+        f.fx_ = *reinterpret_cast<const abf16x8*>(xs + (16 * tn + m) * 128 + (((4 * s + g) ^ fx(m)) << 4));
+        f.fw_ = *reinterpret_cast<const abf16x8*>(ws + (BN + m) * 128 + (((4 * s + g) ^ fx(m)) << 4));
+      }
     }
+  };
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][u][j] = amfma(f.w[i][u], f.x[j], acc[i][u][j]);
+    if constexpr (FOLD) {
+      if (fold_mine) facc = amfma(f.fw_, f.fx_, facc);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s) issue(s, s);
+  wait_and_meet<(NS - 2) * (C::PX + C::PW)>();
+  issue(NS - 1, NS - 1);
+  Frags f0, f1;
+  read(f0, 0, 0);
+  int st = 0;
+  for (int kb = 0; kb < nk; ++kb) {
+    read(f1, st, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f0);
+    __builtin_amdgcn_sched_barrier(0);
+    // block kb + 1 is there, and everybody has read all of block kb: its stage takes block kb + NS
+    wait_and_meet<(NS - 2) * (C::PX + C::PW)>();
+    issue(kb + NS, st);
     st = st == NS - 1 ? 0 : st + 1;
+    read(f0, st, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f1);
+    __builtin_amdgcn_sched_barrier(0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   with_act(a.act, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
+    if (a.vec == 8 && n0 + BN <= a.N) {  // whole column tiles: rows behind M read zeros and are dropped by the buffers' bounds
+      const int rows = min(BM, a.M - m0);
+      const Rsrc ry = raw_rsrc(a.y + (size_t)m0 * a.y_ld,
+                               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows - 1) * (uint32_t)a.y_ld * 2u + (uint32_t)a.N * 2u)));
+      const Rsrc rr = raw_rsrc(a.res + (size_t)m0 * a.r_ld,
+                               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows - 1) * (uint32_t)a.r_ld * 2u + (uint32_t)a.N * 2u)));
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const int n = n0 + wn + 32 * i + 8 * g;
-      float b[8];
+      for (int i = 0; i < TN; ++i) {
+        const int n = n0 + wn + 32 * i + 8 * g;
+        float b[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = a.bias != nullptr ? bias_at(a, min(n + e, a.N - 1)) : 0.f;
+        for (int e = 0; e < 8; ++e) b[e] = a.bias != nullptr ? bias_at(a, n + e) : 0.f;
+        au32x4 r[TM];
+        if (a.res != nullptr) {
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        float c[8];
+          for (int j = 0; j < TM; ++j)
+            r[j] = __builtin_amdgcn_raw_buffer_load_b128(rr, (uint32_t)(wm + 16 * j + m) * (uint32_t)a.r_ld * 2u + 2u * n, 0, 0);
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = acc[i][e >> 2][j][e & 3] + b[e];
-        finish<ACT>(a, m0 + wm + 16 * j + m, n, c);
+        for (int j = 0; j < TM; ++j) {
+          float c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[e] = act_of<ACT>(acc[i][e >> 2][j][e & 3] + b[e]);
+          if (a.res != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              c[e] += __uint_as_float(r[j][e / 2] << 16);
+              c[e + 1] += __uint_as_float(r[j][e / 2] & 0xffff0000u);
+            }
+          }
+          const au32x4 y = {pack_bf16x2(c[0], c[1]), pack_bf16x2(c[2], c[3]), pack_bf16x2(c[4], c[5]), pack_bf16x2(c[6], c[7])};
+          __builtin_amdgcn_raw_buffer_store_b128(y, ry, (uint32_t)(wm + 16 * j + m) * (uint32_t)a.y_ld * 2u + 2u * n, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < TN; ++i) {
+        const int n = n0 + wn + 32 * i + 8 * g;
+        float b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = a.bias != nullptr ? bias_at(a, min(n + e, a.N - 1)) : 0.f;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          float c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[e] = acc[i][e >> 2][j][e & 3] + b[e];
+          finish<ACT>(a, m0 + wm + 16 * j + m, n, c);
+        }
+      }
+    }
+    if constexpr (FOLD) {
+      if (fold_mine) {
+        const int n = nf0 + 4 * g;
+        float c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = facc[e] + (a.bias != nullptr ? bias_at(a, min(n + e, a.N - 1)) : 0.f);
+        finish<ACT>(a, m0 + 16 * tn + m, n, c);
       }
     }
   });
 }
 
-// ----------------------------------------------------------------------------------------------------- few rows
+// ---------------------------------------------------------------------------------------------- K split over waves
 //
-// 16 rows x 16 columns a workgroup, K in slices of 128 (256 bytes of a row), slice q to wave q % 8: such a call is the
-// weights' way from memory, so each wave keeps two slices of both operands on their way (direct-to-LDS, 4 rows x 256
-// contiguous bytes a load; chunk c of row r at c ^ r) and waits for nobody before its products. The 8 partial tiles are
-// added in LDS in wave order. The row tiles of one column tile run on one XCD and share its copy of the weights.
+// 16 R x 16 R tiles (R 1: a decode step's rows; R 2: more rows, still too few tiles of 64 x 128 for the CUs), K in slices of
+// SL = 128 / R elements, slice q to wave q % 8: such a call is the weights' way from memory and a few round trips, so each
+// wave keeps two slices of both operands on their way (direct-to-LDS, whole runs of 256 / R bytes of a row; chunk c of a
+// row at c ^ f(row)) and waits for nobody before its products. The 8 partial tiles are added in LDS in wave order. The row
+// tiles of one column tile run on one XCD and share its copy of the weights.
 
-constexpr int RW = 8, RSL = 128;                // waves, elements of a slice
-constexpr int RTILE = 16 * RSL * 2;             // bytes of one operand's slice: 4 KiB
-constexpr int ROWS_LDS = RW * 2 * 2 * RTILE;    // two slices of both, a wave: 128 KiB
+constexpr int RW = 8;  // waves
+template <int R>
+struct SplitCfg {
+  static constexpr int SL = 128 / R, RB = 2 * SL, CH = RB / 16;  // elements, bytes, chunks of a row's slice
+  static constexpr int OP = 16 * R * RB;                         // bytes of one operand's slice: 4 KiB
+  static constexpr int LDS = RW * 2 * 2 * OP;                    // two slices of both, a wave: 128 KiB
+  __device__ static __forceinline__ int f(int r) { return R == 1 ? r & 15 : (r >> 1) & 7; }
+};
 
-__global__ __launch_bounds__(64 * RW) void gemm_act_rows_kernel(ActArgs a) {
+struct __attribute__((packed, aligned(2))) Packed8 {
+  uint32_t w[4];
+};
+// 8 elements of a row from k on, wherever the row starts: zeros behind the rows and behind K.
+__device__ __forceinline__ uint4 fetch8(const uint16_t* base, long ld, int row, int rows, int k, int K) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (row >= rows || k >= K) return v;
+  const uint16_t* p = base + (size_t)row * ld + k;
+  if (k + 8 <= K) {
+    const Packed8 x = *reinterpret_cast<const Packed8*>(p);
+    return make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+  }
+  uint32_t u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = k + i < K ? p[i] : 0u;
+  return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+}
+
+// WIDE false: rows off 16-byte boundaries or K not a multiple of 8, the slices through registers.
+template <int R, bool WIDE>
+__global__ __launch_bounds__(64 * RW) void gemm_act_split_kernel(ActArgs a) {
+  using C = SplitCfg<R>;
   extern __shared__ uint4 act_lds[];
   uint8_t* lds = reinterpret_cast<uint8_t*>(act_lds);
   const int grp = blockIdx.x / (8 * a.tiles_m), in = blockIdx.x - grp * 8 * a.tiles_m;
   const int tn = grp * 8 + (in & 7), tm = in >> 3;
   if (tn >= a.tiles_n) return;
   const int wave = wave_id(), l = threadIdx.x & 63, m = l & 15, g = l >> 4;
-  const int m0 = __builtin_amdgcn_readfirstlane(16 * tm), n0 = __builtin_amdgcn_readfirstlane(16 * tn);
-  const au32x4 rx = rows_rsrc(a.x + (size_t)m0 * a.x_ld, a.x_ld, min(16, a.M - m0), a.K);
-  const au32x4 rw = rows_rsrc(a.w + (size_t)n0 * a.w_ld, a.w_ld, min(16, a.N - n0), a.K);
-  uint8_t* mine = lds + wave * 4 * RTILE;
+  const int m0 = __builtin_amdgcn_readfirstlane(16 * R * tm), n0 = __builtin_amdgcn_readfirstlane(16 * R * tn);
+  const au32x4 rx = rows_rsrc(a.x + (size_t)m0 * a.x_ld, a.x_ld, min(16 * R, a.M - m0), a.K);
+  const au32x4 rw = rows_rsrc(a.w + (size_t)n0 * a.w_ld, a.w_ld, min(16 * R, a.N - n0), a.K);
+  uint8_t* mine = lds + wave * 4 * C::OP;
   const uint32_t base = lds_at(mine);
+  uint4 vw[4], vx[4];
   auto issue = [&](int q, int half) {  // slice q of the wave's
-    const int k0 = (q * RW + wave) * RSL;
+    const int k0 = (q * RW + wave) * C::SL;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int r = 4 * p + g, c = m ^ r;  // the lane's row of the piece and the chunk its place holds
+    for (int p = 0; p < 4; ++p) {  // 1 KiB: 64 / CH rows
+      const int r = p * (64 / C::CH) + l / C::CH, c = (l % C::CH) ^ C::f(r);
+      if constexpr (!WIDE) {
+        vw[p] = fetch8(a.w, a.w_ld, n0 + r, a.N, k0 + 8 * c, a.K);
+        vx[p] = fetch8(a.x, a.x_ld, m0 + r, a.M, k0 + 8 * c, a.K);
+        continue;
+      }
       const bool there = k0 + 8 * c < a.K;
-      load_lds(rw, there ? (uint32_t)r * (uint32_t)a.w_ld * 2u + 16u * c : NOWHERE, (uint32_t)k0 * 2u, base + half * 2 * RTILE + 1024 * p);
-      load_lds(rx, there ? (uint32_t)r * (uint32_t)a.x_ld * 2u + 16u * c : NOWHERE, (uint32_t)k0 * 2u, base + half * 2 * RTILE + RTILE + 1024 * p);
+      load_lds(rw, there ? (uint32_t)r * (uint32_t)a.w_ld * 2u + 16u * c : NOWHERE, (uint32_t)k0 * 2u, base + half * 2 * C::OP + 1024 * p);
+      load_lds(rx, there ? (uint32_t)r * (uint32_t)a.x_ld * 2u + 16u * c : NOWHERE, (uint32_t)k0 * 2u, base + half * 2 * C::OP + C::OP + 1024 * p);
     }
   };
-  const int slices = (a.K + RSL * RW - 1) / (RSL * RW);  // (a wave's last may lie behind K: zeros)
-  af32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int slices = (a.K + C::SL * RW - 1) / (C::SL * RW);  // (a wave's last may lie behind K: zeros)
+  af32x4 acc[R][R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = af32x4{0.f, 0.f, 0.f, 0.f};
   issue(0, 0);
   for (int q = 0; q < slices; ++q) {
-    if (q + 1 < slices) {
+    if constexpr (!WIDE) {
+      uint8_t* at = mine + (q & 1) * 2 * C::OP + 16 * l;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        *reinterpret_cast<uint4*>(at + 1024 * p) = vw[p];
+        *reinterpret_cast<uint4*>(at + C::OP + 1024 * p) = vx[p];
+      }
+      if (q + 1 < slices) issue(q + 1, 0);
+    } else if (q + 1 < slices) {
       issue(q + 1, (q + 1) & 1);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const uint8_t* ws = mine + (q & 1) * 2 * RTILE;
+    const uint8_t* ws = mine + (q & 1) * 2 * C::OP;
 #pragma unroll
-    for (int s = 0; s < RSL / 32; ++s) {
-      const int at = m * 256 + (((4 * s + g) ^ m) << 4);
-      acc = amfma(*reinterpret_cast<const abf16x8*>(ws + at), *reinterpret_cast<const abf16x8*>(ws + RTILE + at), acc);
+    for (int s = 0; s < C::SL / 32; ++s) {
+      abf16x8 fa[R], fb[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int at = (16 * i + m) * C::RB + (((4 * s + g) ^ C::f(m)) << 4);
+        fa[i] = *reinterpret_cast<const abf16x8*>(ws + at);
+        fb[i] = *reinterpret_cast<const abf16x8*>(ws + C::OP + at);
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) acc[i][j] = amfma(fa[i], fb[j], acc[i][j]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the load after the next overwrites the slice)
   }
   __syncthreads();
-  float* part = reinterpret_cast<float*>(lds);  // [wave][lane][4]
-  *reinterpret_cast<af32x4*>(part + wave * 256 + 4 * l) = acc;
+  float* part = reinterpret_cast<float*>(lds);  // [tile][wave][lane][4]
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) *reinterpret_cast<af32x4*>(part + ((i * R + j) * RW + wave) * 256 + 4 * l) = acc[i][j];
   __syncthreads();
-  if (wave == 0) {
+  if (wave < R * R) {
     float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
-      const af32x4 p = *reinterpret_cast<const af32x4*>(part + w * 256 + 4 * l);
+      const af32x4 p = *reinterpret_cast<const af32x4*>(part + (wave * RW + w) * 256 + 4 * l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[e] += p[e];
     }
-    const int n = n0 + 4 * g;
+    const int n = n0 + 16 * (wave / R) + 4 * g;
     if (a.bias != nullptr) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[e] += bias_at(a, min(n + e, a.N - 1));
     }
-    with_act(a.act, [&](auto act) { finish<decltype(act)::value>(a, m0 + m, n, c); });
+    with_act(a.act, [&](auto act) { finish<decltype(act)::value>(a, m0 + 16 * (wave % R) + m, n, c); });
   }
 }
 
-// Any sizes and alignments: 64 x 64 tiles, 4 waves of 32 x 32, blocks of 64 of K through LDS (128-byte rows, 16-byte
-// chunks swizzled by row), each thread fetching 8 elements of a row at a time, one by one.
+// Any sizes and alignments: T x T tiles, 4 waves of T / 2 x T / 2, blocks of 64 of K through registers (loaded under the
+// products of the block before: 8 elements of a row at a time from wherever it starts, one by one at the end of K) into
+// LDS (128-byte rows, 16-byte chunks swizzled by row).
+template <int T>
 __global__ __launch_bounds__(256) void gemm_act_any_kernel(ActArgs a) {
-  __shared__ uint4 sx[64 * 8], sw[64 * 8];
-  const int n0 = (blockIdx.x % a.tiles_n) * 64, m0 = (blockIdx.x / a.tiles_n) * 64;
+  constexpr int W = T / 32, L = T / 32;  // 16-row tiles a wave and side; 8-element pieces a thread and operand
+  __shared__ uint4 sx[T * 8], sw[T * 8];
+  const int n0 = (blockIdx.x % a.tiles_n) * T, m0 = (blockIdx.x / a.tiles_n) * T;
   const int wave = wave_id(), l = threadIdx.x & 63, m = l & 15, g = l >> 4;
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  af32x4 acc[2][2];
+  const int wm = (wave & 1) * (T / 2), wn = (wave >> 1) * (T / 2);
+  af32x4 acc[W][W];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = af32x4{0.f, 0.f, 0.f, 0.f};
-  auto fetch = [&](const uint16_t* base, long ld, int row, int rows, int k) {
-    uint32_t u[8];
-    const uint16_t* p = base + (size_t)min(row, rows - 1) * ld;
+    for (int j = 0; j < W; ++j) acc[i][j] = af32x4{0.f, 0.f, 0.f, 0.f};
+  uint4 px[L], pw[L];
+  auto load = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t v = p[min(k + i, a.K - 1)];
-      u[i] = row < rows && k + i < a.K ? v : 0u;
+    for (int i = 0; i < L; ++i) {
+      const int e = threadIdx.x + 256 * i, r = e >> 3, c = e & 7;
+      px[i] = fetch8(a.x, a.x_ld, m0 + r, a.M, k0 + 8 * c, a.K);
+      pw[i] = fetch8(a.w, a.w_ld, n0 + r, a.N, k0 + 8 * c, a.K);
     }
-    return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
   };
+  load(0);
   for (int k0 = 0; k0 < a.K; k0 += 64) {
-    uint4 fx_[2], fw_[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = threadIdx.x + 256 * i, r = e >> 3, c = e & 7;
-      fx_[i] = fetch(a.x, a.x_ld, m0 + r, a.M, k0 + 8 * c);
-      fw_[i] = fetch(a.w, a.w_ld, n0 + r, a.N, k0 + 8 * c);
-    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L; ++i) {
       const int e = threadIdx.x + 256 * i, r = e >> 3, c = e & 7;
-      sx[r * 8 + (c ^ (r >> 1 & 7))] = fx_[i];
-      sw[r * 8 + (c ^ (r >> 1 & 7))] = fw_[i];
+      sx[r * 8 + (c ^ fx(r))] = px[i];
+      sw[r * 8 + (c ^ fx(r))] = pw[i];
     }
     __syncthreads();
+    if (k0 + 64 < a.K) load(k0 + 64);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      abf16x8 fa[2], fb[2];
+      abf16x8 fa[W], fb[W];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ra = wn + 16 * i + m, rb = wm + 16 * i + m;
-        fa[i] = __builtin_bit_cast(abf16x8, sw[ra * 8 + ((4 * s + g) ^ (ra >> 1 & 7))]);
-        fb[i] = __builtin_bit_cast(abf16x8, sx[rb * 8 + ((4 * s + g) ^ (rb >> 1 & 7))]);
+      for (int i = 0; i < W; ++i) {
+        fa[i] = __builtin_bit_cast(abf16x8, sw[(wn + 16 * i + m) * 8 + ((4 * s + g) ^ fx(m))]);
+        fb[i] = __builtin_bit_cast(abf16x8, sx[(wm + 16 * i + m) * 8 + ((4 * s + g) ^ fx(m))]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = amfma(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < W; ++j) acc[i][j] = amfma(fa[i], fb[j], acc[i][j]);
     }
   }
   with_act(a.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < W; ++i) {
       const int n = n0 + wn + 16 * i + 4 * g;
+      float b[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int e = 0; e < 4; ++e) b[e] = a.bias != nullptr ? bias_at(a, min(n + e, a.N - 1)) : 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
         float c[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = acc[i][j][e] + (a.bias != nullptr ? bias_at(a, min(n + e, a.N - 1)) : 0.f);
+        for (int e = 0; e < 4; ++e) c[e] = acc[i][j][e] + b[e];
         finish<decltype(act)::value>(a, m0 + wm + 16 * j + m, n, c);
       }
     }
@@ -403,14 +550,44 @@ bool lds_ready(F kernel, int bytes, std::atomic<signed char>* state) {
   return ok;
 }
 
-template <int BM, int BN, int WM, int NS>
-int launch_tiles(const char* fn, ActArgs a, hipStream_t s) {
-  using C = TileCfg<BM, BN, WM, NS>;
+template <int R, bool WIDE>
+int launch_split(const char* fn, ActArgs a, hipStream_t s) {
+  using C = SplitCfg<R>;
   static std::atomic<signed char> state[64];
-  if (!lds_ready(gemm_act_tile_kernel<BM, BN, WM, NS>, C::LDS, state)) return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
-  a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN;
+  if (!lds_ready(gemm_act_split_kernel<R, WIDE>, C::LDS, state)) return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
+  a.tiles_m = (a.M + 16 * R - 1) / (16 * R), a.tiles_n = (a.N + 16 * R - 1) / (16 * R);
+  hipLaunchKernelGGL((gemm_act_split_kernel<R, WIDE>), dim3((unsigned)((a.tiles_n + 7) / 8 * 8) * a.tiles_m), dim3(64 * RW), C::LDS, s, a);
+  return ZGDN_OK;
+}
+
+template <int T>
+int launch_any(ActArgs a, hipStream_t s) {
+  a.tiles_m = (a.M + T - 1) / T, a.tiles_n = (a.N + T - 1) / T;
+  hipLaunchKernelGGL(gemm_act_any_kernel<T>, dim3((unsigned)a.tiles_m * a.tiles_n), dim3(256), 0, s, a);
+  return ZGDN_OK;
+}
+
+// Which form takes the least time, by what each was measured to take (us, MI355X, graph replays): a fixed part and, a round
+// of workgroups over the CUs, a part for each block of K. `one`, `all`: with one workgroup a CU, with all that fit.
+struct Form {
+  int bm, bn, bk, per_cu;
+  double fixed, round, one, all;
+};
+double form_us(const Form& f, long M, long N, long K, long n_cu) {
+  const long tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn), blocks = (K + f.bk - 1) / f.bk;
+  const long rounds = (tiles + n_cu * f.per_cu - 1) / (n_cu * f.per_cu);
+  return f.fixed + rounds * f.round + blocks * (tiles <= n_cu ? f.one : rounds * f.all);
+}
+
+template <int BM, int BN, int WM, int NS, bool FOLD = false>
+int launch_tiles(const char* fn, ActArgs a, hipStream_t s) {
+  using C = TileCfg<BM, BN, WM, NS, FOLD>;
+  static std::atomic<signed char> state[64];
+  if (!lds_ready(gemm_act_tile_kernel<BM, BN, WM, NS, FOLD>, C::LDS, state))
+    return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
+  a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = FOLD ? a.N / BN : (a.N + BN - 1) / BN;
   const long per = ((long)a.tiles_m * a.tiles_n + 7) / 8;
-  hipLaunchKernelGGL((gemm_act_tile_kernel<BM, BN, WM, NS>), dim3((unsigned)(8 * per)), dim3(512), C::LDS, s, a);
+  hipLaunchKernelGGL((gemm_act_tile_kernel<BM, BN, WM, NS, FOLD>), dim3((unsigned)(8 * per)), dim3(512), C::LDS, s, a);
   return ZGDN_OK;
 }
 
@@ -447,29 +624,38 @@ extern "C" int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld,
   // wide loads: rows on 16-byte boundaries, and a tile's rows within 32-bit byte offsets of one another
   const bool wide = x_ld % 8 == 0 && w_ld % 8 == 0 && K % 8 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0 &&
                     x_ld < (1 << 21) && w_ld < (1 << 21) && K < (1 << 21);
+  if (y_ld >= (1 << 21) || r_ld >= (1 << 21)) a.vec = std::min(a.vec, 4);  // (likewise for the whole tiles' stores)
   hipStream_t s = (hipStream_t)stream;
   int st = ZGDN_OK;
+  // The fit's points (M x N x K, us), the form taken and the next best: 4 x 2056 x 1024 3.4 split 1, 4.0 split 2;
+  // 64 x 1024 x 2048 4.4 split 1, 4.9 split 2; 64 x 2056 x 1024 4.1 split 2, 6.1 split 1; 200 x 1024 x 2048 5.5 split 2,
+  // 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 2; 1000 x 2056 x 1024 12.4 tile 64 x 128, 13.9 128 x
+  // 128; 4096 x 2056 x 1024 23.8 tile 128 x 128 (its last 8 columns folded), 29.6 256 x 256; 30526 x 1024 x 2048 113
+  // tile 256 x 256, 134 128 x 128 and 128 x 256.
+  static const Form split1 = {16, 16, 1024, 1, 1.5, 1.0, 0.6, 0.6}, split2 = {32, 32, 512, 1, 1.5, 1.0, 0.7, 0.7};
+  static const Form t64 = {64, 128, 64, 2, 3.0, 0.0, 0.275, 0.52}, t128 = {128, 128, 64, 2, 3.0, 0.0, 0.66, 1.15};
+  static const Form t128w = {128, 256, 64, 1, 3.0, 0.0, 0.96, 0.98}, t256 = {256, 256, 64, 1, 3.0, 0.0, 1.62, 1.65};
+  static const Form any64 = {64, 64, 64, 2, 3.0, 0.0, 0.75, 1.0}, any128 = {128, 128, 64, 1, 3.0, 0.0, 1.2, 1.2};
+  const long n_cu = device_cus();
+  auto us = [&](const Form& f, long cols) { return form_us(f, M, cols, K, n_cu); };
+  const double s1 = us(split1, N), s2 = us(split2, N);
   if (!wide) {
-    a.tiles_m = (M + 63) / 64, a.tiles_n = (N + 63) / 64;
-    hipLaunchKernelGGL(gemm_act_any_kernel, dim3((unsigned)a.tiles_m * a.tiles_n), dim3(256), 0, s, a);
-  } else if (M <= 64) {
-    static std::atomic<signed char> state[64];
-    if (!lds_ready(gemm_act_rows_kernel, ROWS_LDS, state)) return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
-    a.tiles_m = (M + 15) / 16, a.tiles_n = (N + 15) / 16;
-    hipLaunchKernelGGL(gemm_act_rows_kernel, dim3((unsigned)((a.tiles_n + 7) / 8 * 8) * a.tiles_m), dim3(64 * RW), ROWS_LDS, s, a);
+    const double u1 = 2.1 * s1, u2 = 2.1 * s2, u3 = us(any64, N), u4 = us(any128, N), best = std::min(std::min(u1, u2), std::min(u3, u4));
+    st = best == u1   ? launch_split<1, false>(fn, a, s)
+         : best == u2 ? launch_split<2, false>(fn, a, s)
+         : best == u3 ? launch_any<64>(a, s)
+                      : launch_any<128>(a, s);
   } else {
-    // the tile whose rounds over the CUs take the least work, larger tiles doing more of it a time
-    const long n_cu = device_cus();
-    auto cost = [&](long bm, long bn, int per_cu, double eff) {
-      const long tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn), slots = n_cu * per_cu;
-      return (double)((tiles + slots - 1) / slots) * per_cu * bm * bn / eff;
-    };
-    const double c0 = cost(256, 256, 1, 1.0), c1 = cost(128, 256, 1, 0.8), c2 = cost(128, 128, 2, 0.65), c3 = cost(64, 128, 2, 0.5);
-    const double best = std::min(std::min(c0, c1), std::min(c2, c3));
-    st = best == c0 ? launch_tiles<256, 256, 2, 2>(fn, a, s)
-         : best == c1 ? launch_tiles<128, 256, 2, 3>(fn, a, s)
-         : best == c2 ? launch_tiles<128, 128, 2, 2>(fn, a, s)
-                      : launch_tiles<64, 128, 2, 3>(fn, a, s);
+    const int over = N % 128;  // columns behind the last whole tile of 128
+    const bool fold = over > 0 && over <= 16 && N / 128 >= 8;
+    const double u3 = us(t64, N), u4 = us(t128, fold ? N - over : N), u5 = us(t128w, N), u6 = us(t256, N);
+    const double best = std::min(std::min(std::min(s1, s2), std::min(u3, u4)), std::min(u5, u6));
+    st = best == s1   ? launch_split<1, true>(fn, a, s)
+         : best == s2 ? launch_split<2, true>(fn, a, s)
+         : best == u3 ? launch_tiles<64, 128, 2, 3>(fn, a, s)
+         : best == u4 ? (fold ? launch_tiles<128, 128, 2, 2, true>(fn, a, s) : launch_tiles<128, 128, 2, 2>(fn, a, s))
+         : best == u5 ? launch_tiles<128, 256, 2, 3>(fn, a, s)
+                      : launch_tiles<256, 256, 2, 2>(fn, a, s);
   }
   return st != ZGDN_OK ? st : check_launch(fn);
 }

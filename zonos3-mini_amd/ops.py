@@ -12,6 +12,7 @@ and 66).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -932,6 +933,8 @@ def _linear_decay(g, lead: tuple, Hv: int, dev):
     """(g, row stride, dtype code) of the log decays: float32 [Hv] (stride 0), or [*lead, Hv] read in place."""
     if not isinstance(g, torch.Tensor):
         raise RuntimeError("g: expected a tensor")
+    if g.dtype is torch.float32 and g.device == dev and g.shape == (*lead, Hv) and g.is_contiguous():
+        return g, Hv, F32
     if g.dim() == 1:
         _on_gpu("g", g, dev)
         if not (g.dtype == torch.float32 and g.shape == (Hv,)):
@@ -944,8 +947,30 @@ def _linear_decay(g, lead: tuple, Hv: int, dev):
     return g, ld, _code(g, "g")
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(packed: int, n_seqs: int, T: int, Hk: int, Hv: int, K: int, V: int, code: int) -> int:
+    return int(_native.lib().zlin_attn_workspace_bytes(packed, n_seqs, T, Hk, Hv, K, V, code))
+
+
+def _dense_qkv(q, k, v, lead_dims: int) -> bool:
+    """Whether q, k, v are what most calls hand over: dense tensors on one GPU, on 16-byte boundaries, of sizes that the
+    kernels take (checked in one expression: a small call's host time is near the kernel's own)."""
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        return False
+    qs, vs, n, dt, idx = q.shape, v.shape, lead_dims, q.dtype, q.get_device()
+    return (len(qs) == len(vs) == n + 2 and k.shape == qs and vs[:n] == qs[:n] and idx >= 0 and dt in _CODES
+            and k.dtype is dt and v.dtype is dt and k.get_device() == v.get_device() == idx and qs[n] > 0
+            and vs[n] > 0 and vs[n] % qs[n] == 0 and qs[n + 1] in (64, 128) and vs[n + 1] in (64, 128)
+            and vs[n] * vs[n + 1] <= 1 << 22 and q.is_contiguous() and k.is_contiguous() and v.is_contiguous()
+            and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16)
+
+
 def _linear_qkv(q, k, v, lead_dims: int):
     """The rows of q, k [*lead, Hk, K] and v [*lead, Hv, V], read in place where the kernels can, with their strides."""
+    if _dense_qkv(q, k, v, lead_dims):
+        n, qs, vs = lead_dims, q.shape, v.shape
+        qk_ld = qs[n] * qs[n + 1]
+        return (q, qk_ld), (k, qk_ld), (v, vs[n] * vs[n + 1])
     dev = q.device if isinstance(q, torch.Tensor) else None
     ve = 4 if isinstance(q, torch.Tensor) and q.dtype == torch.float32 else 8  # elements in 16 bytes
     q, q_ld = _rows_in_place("q", q, 2, dev, ve, 16)
@@ -1008,11 +1033,11 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
         final_state = torch.empty(n_seqs, Hv, V, K, device=dev, dtype=torch.float32)
     o = torch.empty(B, T, Hv, V, device=dev, dtype=q.dtype)
     code = _CODES[q.dtype]
-    size = int(_native.lib().zlin_attn_workspace_bytes(int(cu_seqlens is not None), n_seqs, T, Hk, Hv, K, V, code))
-    workspace = torch.empty(max(size, 16), device=dev, dtype=torch.uint8)
+    size = _linear_workspace(int(cu_seqlens is not None), n_seqs, T, Hk, Hv, K, V, code)
+    workspace = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
     _call_on(dev, "zlin_attn_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, g.data_ptr(), g_ld,
              g_code, _ptr(initial_state), _ptr(final_state), o.data_ptr(), _ptr(cu_seqlens), n_seqs, B, T, Hk, Hv, K, V,
-             K**-0.5 if scale is None else float(scale), workspace.data_ptr(), workspace.numel(), _stream(dev))
+             K**-0.5 if scale is None else float(scale), _ptr(workspace), size, _stream(dev))
     return o, final_state
 
 
@@ -1050,6 +1075,9 @@ def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
 
 def _matrix_rows(name: str, t, cols: int | None, dev):
     """A bfloat16 matrix with unit column stride on ``dev``, copied where its columns are not beside one another."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.dim() == 2 and t.is_cuda and t.device == dev
+            and t.is_contiguous() and (cols is None or t.shape[1] == cols)):
+        return t, t.shape[1]
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name}: expected a tensor")
     if not t.is_cuda:
@@ -1083,11 +1111,14 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
         _on_gpu("bias", bias, dev)
         if bias.shape != (N,):
             raise RuntimeError(f"bias: expected [{N}], got {tuple(bias.shape)}")
+    y_ld = N
     if out is None:
         out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
     elif not (isinstance(out, torch.Tensor) and out.device == dev and out.shape == (M, N) and out.dtype == torch.bfloat16
               and (N == 1 or out.stride(1) == 1) and (M <= 1 or out.stride(0) >= N)):
         raise RuntimeError(f"out: expected bfloat16 [{M}, {N}] on {dev} with unit column stride and rows apart")
+    else:
+        y_ld = max(out.stride(0), N)
     r_ld = 0
     if residual is not None:
         residual, r_ld = _matrix_rows("residual", residual, N, dev)
@@ -1095,5 +1126,5 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
             raise RuntimeError(f"residual: expected [{M}, {N}], got {tuple(residual.shape)}")
     _call_on(dev, "zlin_gemm_act", x.data_ptr(), x_ld, w.data_ptr(), w_ld, _ptr(bias),
              F32 if bias is None else _code(bias, "bias"), _native.ACTIVATIONS[activation], _ptr(residual), r_ld,
-             out.data_ptr(), max(out.stride(0), N), M, N, K, BF16, _stream(dev))
+             out.data_ptr(), y_ld, M, N, K, BF16, _stream(dev))
     return out

@@ -280,3 +280,26 @@ def test_rows_behind_the_last_sequence_stay(gdn, cuda):
     assert torch.equal(o, o2) and torch.equal(s, s2)
     run([0, 200, 0, 200])
     run([-5, 3, 2, 1])
+
+
+@pytest.mark.parametrize("Hk,Hv,K,V,n,dtype", [(8, 8, 64, 64, 36, BF), (2, 8, 128, 64, 66, BF), (8, 8, 128, 128, 33, BF),
+                                               (4, 8, 64, 128, 70, BF), (3, 6, 128, 64, 48, F32)])
+def test_packed_batches_that_fill_the_device(gdn, cuda, Hk, Hv, K, V, n, dtype):
+    """Enough sequences and heads that one stays whole for many chunks: lengths of one chunk and less, of several, of so
+    many that they are cut all the same; more and fewer than a wave's lanes of sequences; states carried in and out."""
+    announce(f"linear attn batch of {n} {Hk}/{Hv} {K}x{V} {dtype}")
+    gen = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 150, (n,), generator=gen).tolist()
+    lengths[1], lengths[2], lengths[n // 2], lengths[-1] = 1100, 0, 640, 321
+    cu = [0]
+    for length in lengths:
+        cu.append(cu[-1] + length)
+    d = L.inputs((1, cu[-1]), Hk, Hv, K, V, n, dtype, n_states=n, slow=0.2)
+    _check(gdn, cuda, d, cu, msg=f"batch of {n}")
+
+
+@pytest.mark.parametrize("B,T,Hk,Hv,K,V", [(32, 333, 8, 8, 64, 64), (20, 260, 2, 32, 64, 64), (40, 200, 8, 8, 128, 64)])
+def test_padded_batches_that_fill_the_device(gdn, cuda, B, T, Hk, Hv, K, V):
+    """Batches of sequences of several chunks that are not cut."""
+    announce(f"linear attn batch {B} x {T} {Hk}/{Hv} {K}x{V}")
+    _check(gdn, cuda, L.inputs((B, T), Hk, Hv, K, V, B + T, BF, n_states=B, slow=0.2), msg=f"{B} x {T}")

@@ -29,7 +29,9 @@ typedef float lf32x4 __attribute__((ext_vector_type(4)));
 typedef short lshort4 __attribute__((ext_vector_type(4)));
 
 constexpr int ST = 64;  // tokens of a stage of the state pass
+constexpr int CH = 64;  // tokens of a chunk of the walk
 constexpr float G_MIN = -200.f;
+constexpr long CUS = 256;
 
 struct LinArgs {
   const void *q, *k, *v, *g;
@@ -138,6 +140,84 @@ __device__ __forceinline__ void uniform(Piece& p) {
   p.other0 = __builtin_amdgcn_readfirstlane(p.other0);
 }
 
+__device__ __forceinline__ int prefix_count(int x) {  // over the lanes up to this one
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return x;
+}
+
+// The segment that a workgroup of the walk takes, in scalar registers. A sequence of several is cut into equal ones (but for
+// their last chunk). The state pass takes every sequence's but the last, in order. The walk over the outputs takes a packed
+// batch's by length: the longest, one a CU, then the shortest beside them, then the ones between, so that CUs finish
+// together. (Above 64 sequences: in order, there are many to a CU.)
+struct Segment {
+  int seq, bos, slot, first, n;  // slot: of all segments in order; first, n: its tokens in the sequence
+  bool cut, last;                // one of several; the sequence's last
+};
+template <bool OUT>
+__device__ __forceinline__ bool find_segment(const LinArgs& a, int i, int side, Segment& p) {
+  int j, len, n;  // segment of the sequence, the sequence's tokens and segments
+  if (a.cu == nullptr) {
+    n = pieces(a.T, a.run);
+    const int per = OUT ? n : n - 1;
+    p.seq = i / per;
+    j = i - p.seq * per;
+    p.bos = p.seq * a.T;
+    p.slot = p.seq * n + j;
+    len = a.T;
+    if (p.seq >= a.N) return false;
+  } else {
+    const int l = threadIdx.x & 63;
+    int base = 0, taken = 0;
+    bool found = false;
+    for (int s0 = 0; s0 < a.N && !found; s0 += 64) {
+      int bos = 0, eos = 0, mine = 0;
+      if (s0 + l < a.N) {
+        seq_bounds(a.cu, s0 + l, a.T, bos, eos);
+        mine = pieces(eos - bos, a.run);
+      }
+      const int slots = prefix_count(mine);
+      const int counts = OUT ? slots : prefix_count(max(0, mine - 1));
+      const int all = __builtin_amdgcn_readlane(counts, 63);
+      int before = counts - (OUT ? mine : max(0, mine - 1)), at = i - taken;
+      if (OUT && a.N <= 64) {
+        const int size = mine > 0 ? (eos - bos + mine - 1) / mine : 0;
+        before = 0;
+        for (int s = 0; s < a.N; ++s) {
+          const int other = __builtin_amdgcn_readlane(size, s);
+          before += other > size || (other == size && s < l) ? __builtin_amdgcn_readlane(mine, s) : 0;
+        }
+        if (at >= side && at < all) at = at < 2 * side ? all - 1 - (at - side) : at - side;
+        if (i >= all) return false;
+      }
+      const uint64_t here = __ballot(before <= at && at < before + (OUT ? mine : mine - 1));
+      if (here) {
+        const int f = __builtin_ctzll(here);
+        p.seq = s0 + f;
+        p.bos = __builtin_amdgcn_readlane(bos, f);
+        len = __builtin_amdgcn_readlane(eos, f) - p.bos;
+        n = __builtin_amdgcn_readlane(mine, f);
+        j = at - __builtin_amdgcn_readlane(before, f);
+        p.slot = base + __builtin_amdgcn_readlane(slots, f) - n + j;
+        found = true;
+      }
+      base += __builtin_amdgcn_readlane(slots, 63);
+      taken += all;
+    }
+    if (!found) return false;
+  }
+  const int size = (((len + CH - 1) / CH + n - 1) / n) * CH;
+  p.first = j * size;
+  p.n = min(size, len - p.first);
+  p.cut = n > 1;
+  p.last = j == n - 1;
+  return true;
+}
+
 // ---------------------------------------------------------------------------------------------- LDS tiles of rows
 //
 // Rows of ROWB bytes (64 .. 512), 16-byte chunk c of row r at c ^ mask(r): row fragments (16 rows, one chunk each) and
@@ -160,24 +240,45 @@ __device__ __forceinline__ void load_lds(lu32x4 rsrc, uint32_t off, const uint8_
 }
 
 // ROWS rows of ROWB bytes from global memory (row stride ld_bytes, `rows` of them there, zeros behind them) into LDS, by
-// NW waves; each wave instruction fills 1 KiB, so a lane fetches the chunk that belongs at its place.
+// NW waves; each wave instruction fills 1 KiB, so a lane fetches the chunk that belongs at its place. The places in a row
+// repeat every PERIOD instructions of a wave: these byte offsets are kept, the others follow by whole rows.
+template <int ROWB, int NW>
+struct RowsAt {
+  static constexpr int RP = 1024 / ROWB, PERIOD = ROWB >= 256 ? (16 + RP * NW - 1) / (RP * NW) : 1;
+  static_assert(RP * NW * PERIOD % 16 == 0, "the swizzle's period");
+  uint32_t off[PERIOD];
+  __device__ __forceinline__ RowsAt(uint32_t ld_bytes, int wave) {
+    constexpr int n = ROWB / 16;
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < PERIOD; ++i) {
+      const int r = (i * NW + wave) * RP + l / n;
+      off[i] = (uint32_t)(r - i * NW * RP) * ld_bytes + (uint32_t)(chunk_at<ROWB>(r, l % n) - r * ROWB);
+    }
+  }
+  __device__ __forceinline__ void anew() {  // (nothing formed from them is kept across)
+#pragma unroll
+    for (int i = 0; i < PERIOD; ++i) asm volatile("" : "+v"(off[i]));
+  }
+};
+// (instructions i0 .. i1 - 1 of the wave's ROWS ROWB / 1024 / NW)
 template <int ROWB, int ROWS, int NW>
-__device__ __forceinline__ void load_rows(const void* base, uint32_t ld_bytes, int rows, uint8_t* lds, int wave) {
-  constexpr int RP = 1024 / ROWB, P = ROWS / RP;  // rows a piece, pieces
-  static_assert(ROWS % RP == 0 && P % NW == 0, "whole pieces, as many a wave");
+__device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW>& at_row, const void* base, uint32_t ld_bytes, int rows,
+                                          uint8_t* lds, int wave, int i0 = 0, int i1 = ROWS * ROWB / 1024 / NW) {
+  constexpr int RP = 1024 / ROWB;  // rows an instruction
+  static_assert(ROWS % (RP * NW) == 0, "as many a wave");
   const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * ld_bytes + ROWB : 0u;
   const uint64_t at = (uint64_t)(uintptr_t)base;
   const lu32x4 rs = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-  const int l = threadIdx.x & 63;
-  constexpr int n = ROWB / 16;
 #pragma unroll
-  for (int p0 = 0; p0 < P; p0 += NW) {
-    const int p = p0 + wave;
-    const int r = p * RP + l / n, c = l % n;
-    load_lds(rs, (uint32_t)r * ld_bytes + (uint32_t)(chunk_at<ROWB>(r, c) - r * ROWB), lds + 1024 * p);
-  }
+  for (int i = i0; i < i1; ++i)
+    load_lds(rs, at_row.off[i % RowsAt<ROWB, NW>::PERIOD] + (uint32_t)(i * NW * RP) * ld_bytes, lds + 1024 * (i * NW + wave));
+}
+template <int ROWB, int ROWS, int NW>
+__device__ __forceinline__ void load_rows(const void* base, uint32_t ld_bytes, int rows, uint8_t* lds, int wave) {
+  load_rows<ROWB, ROWS, NW>(RowsAt<ROWB, NW>(ld_bytes, wave), base, ld_bytes, rows, lds, wave);
 }
 
 __device__ __forceinline__ uint2 lds_tr(const uint8_t* p) {
@@ -737,93 +838,105 @@ __global__ __launch_bounds__((64 * OutCfg<T, K, V, L>::NW)) void lin_out_kernel(
 
 // ------------------------------------------------------------------------------------------- bf16: a walk over chunks
 //
-// A workgroup walks the 64-token chunks of one piece of a sequence for NH value heads that share a key head (NH V = 64 or
+// A workgroup walks the 64-token chunks of one segment of a sequence for NH value heads that share a key head (NH V = 64 or
 // 128 value columns, 32 a wave). A wave keeps its 32 value rows of S in registers, as transposed tiles [2][K / 16] (D: key
-// 4 g + e; value of lane m and half u: 8 (m / 4) + 4 u + m % 4, so that both halves' rows of an output tile are 8
-// neighbours), which as they stand are an MFMA operand once split into bf16 terms. A chunk:
+// 32 (kt / 2) + 8 g + 4 (kt % 2) + e; value of lane m and half u: 8 (m / 4) + 4 u + m % 4): a pair of key tiles, split into
+// bf16 terms, is an MFMA operand with its keys in memory order, and both halves' rows of an output tile are 8 neighbours.
+// A chunk:
 //   P^T [s, t] = K Q^T, scaled by exp(G_t - G_s) and masked, a few tiles a wave, as two bf16 terms into LDS for all;
 //   O^T [v, t] = exp(G_t) S Q^T + V^T P^T;
 //   S^T = exp(G_end) S^T + K^T V', V' = exp(G_end - G_s) V in three bf16 terms.
-// V^T and K^T are read transposed from LDS. The phases of one workgroup leave each of matrix unit, vector unit and LDS idle
-// in turn: two workgroups run on a CU. OUT false: the state alone.
-
-constexpr int CH = 64;  // tokens of a chunk
+// V^T and K^T are read transposed from LDS. A chunk's 200 MFMAs a wave (16 cycles each) and 700 other vector instructions
+// (4 each) take turns unless they are interleaved: the splits into terms run beside the products of the step before, and
+// two workgroups share a CU. OUT false: the state alone.
 
 template <int K, int V, int NH, bool OUT>
 struct WalkCfg {
   static constexpr int WH = V / 32, NW = NH * WH;  // waves a head, in all
   static constexpr int KB = 2 * K, VB = 2 * NH * V;  // bytes of a row
-  static constexpr int KV_BYTES = CH * (KB + VB);
-  static constexpr int NS = OUT ? 1 : 2;  // stages of k and v
-  static constexpr int AT_Q = NS * KV_BYTES;
+  static constexpr int KI = CH * KB / 1024 / NW, VI = CH * VB / 1024 / NW;  // a wave's load instructions for k (q) and v
   static constexpr int P_TERM = OUT ? 6 * 1024 : 0;  // 16 x 32 blocks of P in fragment order: t tiles 0, 1 one, 2, 3 two
-  static constexpr int AT_P = AT_Q + (OUT ? CH * KB : 0);
   static constexpr int GC = WH;  // chunks whose decays are formed at a time, each by a wave a head
-  static constexpr int G_FLOATS = 3 * CH + 4;
+  static constexpr int G_FLOATS = 3 * CH + 4, G_BYTES = (GC + 1) * NH * G_FLOATS * 4;
+  static constexpr int VS = OUT ? 1 : 2;  // stages of v (and q)
+  static constexpr int REST = VS * CH * VB + (OUT ? CH * KB : 0) + NH * 2 * P_TERM + G_BYTES;
+  static constexpr int KS = REST + 2 * CH * KB <= 80 * 1024 ? 2 : 1;  // stages of k
+  static constexpr int AT_V = KS * CH * KB, AT_Q = AT_V + VS * CH * VB;
+  static constexpr int AT_P = AT_Q + (OUT ? CH * KB : 0);
   static constexpr int AT_G = AT_P + NH * 2 * P_TERM;
-  static constexpr int LDS = AT_G + 2 * GC * NH * G_FLOATS * 4;
-  static_assert(LDS <= 80 * 1024, "two workgroups a CU");
+  static constexpr int LDS = AT_G + G_BYTES;
+  static_assert(LDS <= 80 * 1024 && (OUT || KS == 2), "two workgroups a CU");
+  // P's tiles (s tile i, t tile j, i <= j) by wave of the head, 4 i + j each, a nibble a tile: those of a wave share rows
+  static constexpr uint32_t tiles(int w) {
+    return WH == 4 ? (w == 0 ? 0x73 : w == 1 ? 0xFB : w == 2 ? 0xA62 : 0x051) : (w == 0 ? 0xFB73 : 0x051A62);
+  }
+  static constexpr int count(int w) { return WH == 4 ? (w < 2 ? 2 : 3) : (w == 0 ? 4 : 6); }
 };
 
-template <int K>
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N of the wave's loads outstanding, then a barrier
+  static_assert(N < 64, "counter");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ int walk_row(int u, int m) { return 8 * (m >> 2) + 4 * u + (m & 3); }
 
-// Fragment of V's transpose: the values of half u (of 32 columns from c0) in rows r0 + 4 g + {0..3}, r0 + 16 + 4 g + {0..3}.
-template <int ROWB>
-__device__ __forceinline__ lbf16x8 tr_frag_half(const uint8_t* tile, int r0, int c0, int u) {
-  const int l = threadIdx.x & 63, g = l >> 4, s = l & 15;
-  const int r = r0 + 4 * g + (s >> 2), c = c0 / 8 + (s & 3);
-  const uint2 a = lds_tr(tile + chunk_at<ROWB>(r, c) + 8 * u);
-  const uint2 b = lds_tr(tile + chunk_at<ROWB>(r + 16, c) + 8 * u);
-  return __builtin_bit_cast(lbf16x8, make_uint4(a.x, a.y, b.x, b.y));
+// The scheduler moves nothing across: regions of a few products and the other work that is to run beside them.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+// One product, then N other vector instructions, M times over: the order of a region's.
+template <int M, int N>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, N, 0);
+  }
 }
 
 template <int K, int V, int NH, bool OUT>
 __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk_kernel(LinArgs a) {
   using C = WalkCfg<K, V, NH, OUT>;
-  constexpr int NW = C::NW, WH = C::WH, KT = K / 16;
+  constexpr int NW = C::NW, WH = C::WH, KT = K / 16, KK = K / 32;
   extern __shared__ uint4 lin_lds[];
   uint8_t* lds = reinterpret_cast<uint8_t*>(lin_lds);
   const int groups = a.Hv / NH;
-  const int slot = blockIdx.x / groups, h0 = (blockIdx.x - slot * groups) * NH;
-  const int size = OUT ? a.seg : a.run;
-  Piece p;
-  if (!find_piece(a.cu, a.N, a.T, slot, size, OUT ? a.run : a.seg, p)) return;
-  uniform(p);
-  const int first = p.j * size;
-  const bool last = first + size >= p.len;
-  int n = min(size, p.len - first);  // (0 for an empty sequence)
-  if (!OUT && last) {  // a last run is walked up to its last segment (which has the final state in its outputs' walk)
-    n = max(n - 1, 0) / a.seg * a.seg;
-    if (n == 0) return;
-  }
+  const int index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * NH;
+  Segment p;
+  // (a table whose sequences overlap may name more segments than there are slots)
+  if (!find_segment<OUT>(a, index, max(1, (int)CUS / groups), p) || p.slot >= a.run_slots) return;
+  const int n = p.n;  // (0 for an empty sequence)
   const int wave = wave_id(), l = threadIdx.x & 63, g = l >> 4, m = l & 15;
   const int hh = wave / WH, wl = wave - hh * WH, h = h0 + hh;
-  const size_t row0 = (size_t)p.bos + first;
+  const size_t row0 = (size_t)p.bos + p.first;
   const size_t hk = (size_t)(h0 / (a.Hv / a.Hk)) * K;
   const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + row0 * a.q_ld + hk;
   const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k) + row0 * a.k_ld + hk;
   const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + row0 * a.v_ld + (size_t)h0 * V;
-  float* gb = reinterpret_cast<float*>(lds + C::AT_G) + hh * C::G_FLOATS;  // + NH G_FLOATS a chunk, of 2 GC in turn
+  float* gb = reinterpret_cast<float*>(lds + C::AT_G) + hh * C::G_FLOATS;  // + NH G_FLOATS a chunk, GC + 1 in turn
   uint8_t* pl = lds + C::AT_P + hh * 2 * C::P_TERM + 16 * l;
   const uint8_t* qs = lds + C::AT_Q;
 
   const int chunks = (n + CH - 1) / CH;
   auto rows_of = [&](int c) { return max(0, min(CH, n - c * CH)); };  // (behind the last chunk: none, zeros)
-  auto issue_kv = [&](int c) {
-    uint8_t* at = lds + (C::NS == 2 ? (c & 1) * C::KV_BYTES : 0);
+  RowsAt<C::KB, NW> k_at((uint32_t)a.k_ld * 2u, wave), q_at((uint32_t)a.q_ld * 2u, wave);
+  RowsAt<C::VB, NW> v_at((uint32_t)a.v_ld * 2u, wave);
+  auto issue = [&](const uint16_t* x, long ld, const auto& lanes, auto row_bytes, int at, int c, int i0, int i1) {
     const int rows = rows_of(c);
-    const size_t t = rows > 0 ? (size_t)c * CH : 0;
-    load_rows<C::KB, CH, NW>(kp + t * a.k_ld, (uint32_t)a.k_ld * 2u, rows, at, wave);
-    load_rows<C::VB, CH, NW>(vp + t * a.v_ld, (uint32_t)a.v_ld * 2u, rows, at + CH * C::KB, wave);
+    load_rows<decltype(row_bytes)::value, CH, NW>(lanes, x + (rows > 0 ? (size_t)c * CH : 0) * ld, (uint32_t)ld * 2u, rows,
+                                                  lds + at, wave, i0, i1);
   };
-  auto issue_q = [&](int c) {
-    const int rows = rows_of(c);
-    load_rows<C::KB, CH, NW>(qp + (rows > 0 ? (size_t)c * CH : 0) * a.q_ld, (uint32_t)a.q_ld * 2u, rows, lds + C::AT_Q, wave);
+  auto issue_k = [&](int c, int i0 = 0, int i1 = C::KI) {
+    issue(kp, a.k_ld, k_at, std::integral_constant<int, C::KB>{}, C::KS == 2 ? (c & 1) * CH * C::KB : 0, c, i0, i1);
+  };
+  auto issue_v = [&](int c, int i0 = 0, int i1 = C::VI) {
+    issue(vp, a.v_ld, v_at, std::integral_constant<int, C::VB>{}, C::AT_V + (C::VS == 2 ? (c & 1) * CH * C::VB : 0), c, i0, i1);
+  };
+  auto issue_q = [&](int c, int i0 = 0, int i1 = C::KI) {
+    issue(qp, a.q_ld, q_at, std::integral_constant<int, C::KB>{}, C::AT_Q, c, i0, i1);
   };
   // Log decays, GC chunks at a time, one of them a wave: lane l takes the chunk's tokens l (prefix sums) and 63 - l (suffix
   // sums: lanes in token order from the end).
-  auto g_at = [&](int c) { return gb + (c & (2 * C::GC - 1)) * NH * C::G_FLOATS; };
+  auto g_at = [&](int c) { return gb + (c % (C::GC + 1)) * NH * C::G_FLOATS; };
   struct G2 {
     uint32_t up, down;
   };
@@ -840,162 +953,231 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
     }
     const float s = prefix_sum(g_value(a, x.down)), total = __shfl(s, 63);
     b[2 * CH + 63 - l] = expf(dpp_rows<0x138, 0xF>(s));
-    const Decay d = decay_of(total);
-    if (l == 0) *reinterpret_cast<float4*>(b + 3 * CH) = make_float4(d.add, d.mul, total, 0.f);
+    // S exp(G) as S + S expm1(G): of a slow decay the factor's own rounding, the same at every chunk, would grow with the
+    // length of the memory; of a fast one what is left is off by 2^-25 of what was
+    if (l == 0) *reinterpret_cast<float2*>(b + 3 * CH) = make_float2(expm1f(total), total);
   };
 
   const size_t hs = (size_t)V * K;
   lf32x4 acc[2][KT];
-  auto put = [&](float* dst) {  // [V][K] of the head
+  // a state [V][K] of the head in memory: the lane's tiles are 4 floats each, pairs of them 8
+  const size_t lane_at = (size_t)(32 * wl + walk_row(0, m)) * K + 8 * g;
+  auto state_at = [&](int u, int kt) { return lane_at + 4 * u * K + 32 * (kt >> 1) + 4 * (kt & 1); };
+  auto put = [&](float* dst) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-        *reinterpret_cast<lf32x4*>(dst + (size_t)(32 * wl + walk_row<K>(u, m)) * K + 16 * kt + 4 * g) = acc[u][kt];
-  };
-  auto add_in = [&](const float* src, float f) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const lf32x4 x = *reinterpret_cast<const lf32x4*>(src + (size_t)(32 * wl + walk_row<K>(u, m)) * K + 16 * kt + 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[u][kt][e] = fmaf(x[e], f, acc[u][kt][e]);
-      }
-  };
-
-  float gsum = 0.f;
-  auto write_down = [&](int c) {  // the state before the segment that starts with chunk c of the run
-    const int at = p.other0 + (first + c * CH) / a.seg;
-    if (c == 0 && !(p.j == 0 && p.len <= a.run && a.save_first)) return;
-    if (at >= a.seg_slots) return;  // (only tables whose sequences overlap have so many segments)
-    put(a.ckpt + ((size_t)at * a.Hv + h) * hs);
-    if (wl == 0 && l == 0) a.gcum[(size_t)at * a.Hv + h] = gsum;
+      for (int kt = 0; kt < KT; ++kt) *reinterpret_cast<lf32x4*>(dst + state_at(u, kt)) = acc[u][kt];
   };
 
   G2 gv = g_load(wl);
+  issue_k(0);
   if constexpr (OUT) issue_q(0);
-  issue_kv(0);
+  issue_v(0);
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) acc[u][kt] = lf32x4{0.f, 0.f, 0.f, 0.f};
+  // the state before the segment: carried into it, or the initial one (a sequence of one segment)
+  const float* s_in = nullptr;
   if constexpr (OUT) {
-    // the state before the segment: in a sequence of one run the initial state or what the run's walk wrote down, else the
-    // state carried into the run, decayed, and what the run's walk wrote down
-    const int run = first / a.run, in_run = first - run * a.run;
-    const size_t at = ((size_t)slot * a.Hv + h) * hs;
-    if (p.len <= a.run) {
-      if (in_run > 0 || (a.save_first && !last))
-        add_in(a.ckpt + at, 1.f);
-      else if (a.s_in != nullptr)
-        add_in(a.s_in + ((size_t)p.seq * a.Hv + h) * hs, 1.f);
-    } else {
-      if (in_run > 0) add_in(a.ckpt + at, 1.f);
-      if (p.other0 + run < a.run_slots)
-        add_in(a.ends + ((size_t)(p.other0 + run) * a.Hv + h) * hs, in_run > 0 ? expf(a.gcum[(size_t)slot * a.Hv + h]) : 1.f);
+    s_in = p.cut ? a.ends + ((size_t)p.slot * a.Hv + h) * hs
+           : a.s_in != nullptr ? a.s_in + ((size_t)p.seq * a.Hv + h) * hs
+                               : nullptr;
+    if (s_in != nullptr) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) acc[u][kt] = *reinterpret_cast<const lf32x4*>(s_in + state_at(u, kt));
     }
     // P's tiles above its diagonal blocks of 32 stay zero
     for (int e = wl; e < 2 * C::P_TERM / 1024; e += WH) *reinterpret_cast<uint4*>(pl + 1024 * e) = make_uint4(0, 0, 0, 0);
-  } else if (p.len <= a.run && a.s_in != nullptr) {
-    add_in(a.s_in + ((size_t)p.seq * a.Hv + h) * hs, 1.f);
   }
   g_store(wl, gv);
+  float gsum = 0.f;
 
   // Offsets of the lane's 16-byte chunks in rows of KB bytes: chunk c of the rows of one place mod 16 lies at the offset of
-  // chunk 0 with c's bits flipped. Formed anew each chunk (held, all of them would take 40 registers).
-  int at_row = chunk_at<C::KB>(m, g);                                             // row m, chunk g
-  int at_half = chunk_at<C::KB>(m, g >> 1) + 8 * (g & 1);                         // row m, 8 bytes at 8 g
-  int at_tr = chunk_at<C::KB>(4 * g + (m >> 2), (m & 3) >> 1) + 8 * (m & 1);      // transposing reads, column 0
+  // chunk 0 with c's bits flipped. Formed anew each chunk (held, all of them would take 30 registers).
+  int at_row = chunk_at<C::KB>(m, g);                    // row m, chunk g
+  int at_tr = chunk_at<C::KB>(4 * g + (m >> 2), m & 3);  // transposing reads of rows 4 g ..: a half of each of 4 chunks
   auto flip = [](int at, int c) { return at ^ (c << 4); };
+  const bool keep = p.last && a.s_out != nullptr;  // whether the state behind the last chunk is wanted
 
-  for (int c = 0; c < chunks; ++c) {
-    asm volatile("" : "+v"(at_row), "+v"(at_half), "+v"(at_tr));
-    loads_barrier();  // chunk c is there, and nobody reads what the next loads overwrite
+  // (NT: terms of V')
+  auto chunk = [&](int c, auto terms) {
+    constexpr int NT = decltype(terms)::value;
+    asm volatile("" : "+v"(at_row), "+v"(at_tr));
+    k_at.anew(), v_at.anew();
+    if constexpr (OUT) q_at.anew();
+    // chunk c is there, and nobody reads what the next loads overwrite (the first chunk's state may still be on its way)
+    if (OUT && c == 0 && s_in != nullptr)
+      wait_loads<2 * KT>();
+    else
+      wait_loads<0>();
     const int in_group = c & (C::GC - 1);
     if (in_group == 0 && c + C::GC < chunks) gv = g_load(c + C::GC + wl);
-    if constexpr (!OUT) issue_kv(c + 1);
-    const uint8_t* ks = lds + (C::NS == 2 ? (c & 1) * C::KV_BYTES : 0);
-    const uint8_t* vs = ks + CH * C::KB;
+    if constexpr (!OUT) {
+      issue_k(c + 1);
+      issue_v(c + 1);
+    }
+    const uint8_t* ks = lds + (C::KS == 2 ? (c & 1) * CH * C::KB : 0);
+    const uint8_t* vs = lds + C::AT_V + (C::VS == 2 ? (c & 1) * CH * C::VB : 0);
     const float* b = g_at(c);
     lf32x4 o[2][4];
+    lbf16x8 vf[2][2];  // the wave's columns of V^T: [half][block of 32 tokens]
+    auto read_v = [&] {
+      const int r = 4 * g + (m >> 2), col = (hh * V + 32 * wl) / 8 + (m & 3);
+      const uint8_t* at = vs + chunk_at<C::VB>(r, col);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint2 x = lds_tr(at + 32 * s * C::VB + 8 * u), y = lds_tr(at + (32 * s + 16) * C::VB + 8 * u);
+          vf[u][s] = __builtin_bit_cast(lbf16x8, make_uint4(x.x, x.y, y.x, y.y));
+        }
+    };
+    // V' in terms, a pair of tokens at a time: word i of half u in block s
+    uint32_t vt[2][2][NT][4];  // [block][half][term][word]
+    lf32x4 vw[2][2];          // the weights of a block's tokens (rows 4 g .., 16 + 4 g ..)
+    auto read_weights = [&](int s) {
+      vw[s][0] = *reinterpret_cast<const lf32x4*>(b + 2 * CH + 32 * s + 4 * g);
+      vw[s][1] = *reinterpret_cast<const lf32x4*>(b + 2 * CH + 32 * s + 16 + 4 * g);
+    };
+    auto v_pair = [&](int s, int u, int i) {
+      const uint4 all = __builtin_bit_cast(uint4, vf[u][s]);
+      const uint32_t x = i == 0 ? all.x : i == 1 ? all.y : i == 2 ? all.z : all.w;
+      uint32_t t[NT];
+      split_pair<NT>(lo_f32(x) * vw[s][i >> 1][2 * (i & 1)], hi_f32(x) * vw[s][i >> 1][2 * (i & 1) + 1], t);
+#pragma unroll
+      for (int k = 0; k < NT; ++k) vt[s][u][k][i] = t[k];
+    };
+    static_assert(!OUT || (C::KI + C::VI <= 2 * KK * NT && 4 * KK % C::KI == 0), "regions for the loads");
+    auto v_frag = [&](int s, int u, int k) {
+      return __builtin_bit_cast(lbf16x8, make_uint4(vt[s][u][k][0], vt[s][u][k][1], vt[s][u][k][2], vt[s][u][k][3]));
+    };
+    bool apart = false;
     if constexpr (OUT) {
-      // P^T tiles (s tile i, t tile j, i <= j), in the order 00 01 11 02 12 22 ...
-      constexpr uint64_t TILES = 0xFB73A62510;  // 4 i + j of tile w in its bits 4 w ..
+      // P^T tiles: the wave's all at once
+      auto p_tiles = [&](auto wc) {
+        constexpr int CNT = C::count(decltype(wc)::value);
+        constexpr uint32_t CODE = C::tiles(decltype(wc)::value);
+        lf32x4 d[CNT];
+        lbf16x8 kf[4], qf[4];
 #pragma unroll
-      for (int x = 0; x < (10 + WH - 1) / WH; ++x) {
-        const int w = wl + x * WH;
-        if (w < 10) {
-          const int ij = (int)(TILES >> (4 * w)) & 15, i = ij >> 2, j = ij & 3;
-          lf32x4 d = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < CNT; ++x) d[x] = lf32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kk = 0; kk < K / 32; ++kk) {
-            const lbf16x8 kf = *reinterpret_cast<const lbf16x8*>(ks + 16 * i * C::KB + flip(at_row, 4 * kk));
-            const lbf16x8 qf = *reinterpret_cast<const lbf16x8*>(qs + 16 * j * C::KB + flip(at_row, 4 * kk));
-            d = mfma16(kf, qf, d);
+        for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            bool ki = false, qi = false;
+#pragma unroll
+            for (int x = 0; x < CNT; ++x) {
+              ki |= ((CODE >> (4 * x) & 15) >> 2) == i;
+              qi |= (CODE >> (4 * x) & 3) == i;
+            }
+            if (ki) kf[i] = *reinterpret_cast<const lbf16x8*>(ks + 16 * i * C::KB + flip(at_row, 4 * kk));
+            if (qi) qf[i] = *reinterpret_cast<const lbf16x8*>(qs + 16 * i * C::KB + flip(at_row, 4 * kk));
           }
+#pragma unroll
+          for (int x = 0; x < CNT; ++x) d[x] = mfma16(kf[(CODE >> (4 * x) & 15) >> 2], qf[CODE >> (4 * x) & 3], d[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < CNT; ++x) {
+          const int i = (CODE >> (4 * x) & 15) >> 2, j = CODE >> (4 * x) & 3;
           const lf32x4 gs = *reinterpret_cast<const lf32x4*>(b + 16 * i + 4 * g);
           const float gt = b[16 * j + m];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[e] *= a.scale * __expf(gt - gs[e]);
-          if (i == j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = 4 * g + e <= m ? d[e] : 0.f;
+          for (int e = 0; e < 4; ++e) {
+            d[x][e] *= a.scale * __expf(gt - gs[e]);
+            if (i == j) d[x][e] = 4 * g + e <= m ? d[x][e] : 0.f;
           }
           uint32_t w0[2], w1[2];
-          split_pair<2>(d[0], d[1], w0);
-          split_pair<2>(d[2], d[3], w1);
+          split_pair<2>(d[x][0], d[x][1], w0);
+          split_pair<2>(d[x][2], d[x][3], w1);
           // the block of tile j and tokens 32 (i / 2) .. in fragment order: this very lane's, half i % 2
           const int at = 1024 * (j < 2 ? j : 2 * j - 2 + (i >> 1)) + 8 * (i & 1);
           *reinterpret_cast<uint2*>(pl + at) = make_uint2(w0[0], w1[0]);
           *reinterpret_cast<uint2*>(pl + C::P_TERM + at) = make_uint2(w0[1], w1[1]);
         }
+      };
+      if (wl == 0)
+        p_tiles(std::integral_constant<int, 0>{});
+      else if (wl == 1)
+        p_tiles(std::integral_constant<int, 1>{});
+      else if constexpr (WH == 4) {
+        if (wl == 2)
+          p_tiles(std::integral_constant<int, 2>{});
+        else
+          p_tiles(std::integral_constant<int, 3>{});
       }
-      // O^T = S Q^T, the state in two terms, keys in the order of its tiles
+      // O^T = S Q^T, the state in two terms; beside each step's products the next one's terms and V's of the first block
+      uint32_t st[2][2][2][4];  // [step % 2][half][term][word]
+      lbf16x8 qf[2][4];
+      auto q_read = [&](int kk) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          qf[kk & 1][j] = *reinterpret_cast<const lbf16x8*>(qs + 16 * j * C::KB + flip(at_row, 4 * kk));
+      };
+      auto s_pair = [&](int kk, int u, int i) {
+        uint32_t t[2];
+        const lf32x4 x = acc[u][2 * kk + (i >> 1)];
+        split_pair<2>(x[2 * (i & 1)], x[2 * (i & 1) + 1], t);
+        st[kk & 1][u][0][i] = t[0];
+        st[kk & 1][u][1][i] = t[1];
+      };
+      fence();
+      q_read(0);
+      read_v();
+      read_weights(0);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[u][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < K / 32; ++kk) {
-        lbf16x8 sf[2][2];
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t t[4][2];
+        for (int i = 0; i < 4; ++i) s_pair(0, u, i);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            split_pair<2>(acc[u][2 * kk + i][0], acc[u][2 * kk + i][1], t[2 * i]);
-            split_pair<2>(acc[u][2 * kk + i][2], acc[u][2 * kk + i][3], t[2 * i + 1]);
+      for (int kk = 0; kk < KK; ++kk) {
+        fence();
+        if (kk + 1 < KK) q_read(kk + 1);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // term 1 - r / 2 of half r % 2
+          fence();
+          const int x = 1 - (r >> 1), u = r & 1;
+          const lbf16x8 sf = __builtin_bit_cast(lbf16x8, make_uint4(st[kk & 1][u][x][0], st[kk & 1][u][x][1], st[kk & 1][u][x][2], st[kk & 1][u][x][3]));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[u][j] = mfma16(sf, qf[kk & 1][j], o[u][j]);
+          if (kk + 1 < KK) {
+            s_pair(kk + 1, r >> 1, 2 * (r & 1));
+            s_pair(kk + 1, r >> 1, 2 * (r & 1) + 1);
           }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) sf[u][x] = __builtin_bit_cast(lbf16x8, make_uint4(t[0][x], t[1][x], t[2][x], t[3][x]));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint2 q0 = *reinterpret_cast<const uint2*>(qs + 16 * j * C::KB + flip(at_half, 4 * kk));
-          const uint2 q1 = *reinterpret_cast<const uint2*>(qs + 16 * j * C::KB + flip(at_half, 4 * kk + 2));
-          const lbf16x8 qf = __builtin_bit_cast(lbf16x8, make_uint4(q0.x, q0.y, q1.x, q1.y));
-#pragma unroll
-          for (int u = 0; u < 2; ++u) o[u][j] = mfma16(sf[u][1], qf, o[u][j]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) o[u][j] = mfma16(sf[u][0], qf, o[u][j]);
+          // (the 8 pairs of V' over the 4 KK regions)
+          if constexpr (KK == 4) {
+            if ((r & 1) == 0) v_pair(0, kk >> 1, 2 * (kk & 1) + (r >> 1));
+          } else {
+            v_pair(0, kk, r);
+          }
+          if constexpr (C::KS == 2) {  // the next k's loads, one at a time
+            constexpr int every = 4 * KK / C::KI;
+            if ((4 * kk + r) % every == 0) issue_k(c + 1, (4 * kk + r) / every, (4 * kk + r) / every + 1);
+          }
+          interleave<4, 5>();
         }
       }
+      fence();
+      // (formed here, although only the update needs them)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+          asm volatile("" : "+v"(vt[0][u][k][0]), "+v"(vt[0][u][k][1]), "+v"(vt[0][u][k][2]), "+v"(vt[0][u][k][3]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float f = b[CH + 16 * j + m];
 #pragma unroll
         for (int u = 0; u < 2; ++u) o[u][j] *= f;
       }
-      lds_barrier();  // P is there, and nobody reads q any more
-      issue_q(c + 1);
-    }
-    lbf16x8 vf[2][2];  // [half][block of 32 tokens]
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) vf[u][s] = tr_frag_half<C::VB>(vs, 32 * s, hh * V + 32 * wl, u);
-    if constexpr (OUT) {
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
       u16x2 top = {0, 0};  // the largest magnitude's bits
 #pragma unroll
@@ -1007,20 +1189,33 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu));
         }
+      apart = __ballot(top.x >= 0x7f80 || top.y >= 0x7f80) != 0;
+      lds_barrier();  // P is there, and nobody reads q and v any more
       auto p_frag = [&](int j, int s, int term) {
         return *reinterpret_cast<const lbf16x8*>(pl + term * C::P_TERM + 1024 * (j < 2 ? j : 2 * j - 2 + s));
       };
-      if (__ballot(top.x >= 0x7f80 || top.y >= 0x7f80) == 0) {
+      if (!apart) {
+        lbf16x8 pf[2][4][2];
+        auto p_read = [&](int s) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+          for (int x = 1; x >= 0; --x)
 #pragma unroll
-          for (int j = 2 * s; j < 4; ++j) {
-            const lbf16x8 lo = p_frag(j, s, 1), hi = p_frag(j, s, 0);
+            for (int j = 2 * s; j < 4; ++j) pf[s][j][x] = p_frag(j, s, x);
+        };
+        auto pv = [&](int s, int x) {
+          fence();
 #pragma unroll
-            for (int u = 0; u < 2; ++u) o[u][j] = mfma16(vf[u][s], lo, o[u][j]);
+          for (int j = 2 * s; j < 4; ++j)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) o[u][j] = mfma16(vf[u][s], hi, o[u][j]);
-          }
+            for (int u = 0; u < 2; ++u) o[u][j] = mfma16(vf[u][s], pf[s][j][x], o[u][j]);
+          fence();
+        };
+        p_read(0);
+        pv(0, 1);  // (the small terms first)
+        p_read(1);
+        pv(0, 0);
+        pv(1, 1);
+        pv(1, 0);
       } else {
         // an infinity or a NaN among the values: a masked P is zero, and zero times it NaN. Token by token, each added
         // from its own row on
@@ -1046,7 +1241,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
             }
           }
       }
-      // the lane holds values 8 g .. 8 g + 7 of the wave's, of token 16 j + m (rows behind the piece are dropped)
+      // the lane holds values 8 g .. 8 g + 7 of the wave's, of token 16 j + m (rows behind the segment are dropped)
       const uint32_t lb = (uint32_t)a.Hv * V * 2u;
       const Rsrc rs = raw_rsrc(reinterpret_cast<uint16_t*>(a.o) + ((row0 + (size_t)c * CH) * a.Hv + h) * V,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows_of(c) - 1) * lb + 2 * V)));
@@ -1056,61 +1251,85 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
                           pack_bf16x2(o[1][j][0], o[1][j][1]), pack_bf16x2(o[1][j][2], o[1][j][3])};
         __builtin_amdgcn_raw_buffer_store_b128(w, rs, (uint32_t)(16 * j + m) * lb + 2 * (32 * wl + 8 * g), 0, 0);
       }
-    } else if (c * CH % a.seg == 0) {
-      write_down(c);
-    }
-    const float add = b[3 * CH];
-    gsum += b[3 * CH + 2];
-    if (__builtin_amdgcn_readfirstlane(__float_as_int(b[3 * CH + 1])) != 0) {  // (a slow decay)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[u][kt][e] = fmaf(acc[u][kt][e], add, acc[u][kt][e]);
     } else {
+      read_v();
+      read_weights(0);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) acc[u][kt] *= add;
+        for (int i = 0; i < 4; ++i) v_pair(0, u, i);
     }
+    if (OUT && c + 1 == chunks && !keep) return;
+    // S^T = exp(G_end) S^T + K^T V', a pair of key tiles at a time: beside the first block's products the decay of the next
+    // pair and V' of the second block
+    gsum += b[3 * CH + 1];
+    const float add = b[3 * CH];
+    read_weights(1);
+    lbf16x8 kf[2][2];  // [step % 2][tile of the pair]
+    auto k_read = [&](int x) {  // of step x: pair x % KK of block x / KK
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const float4 w0 = *reinterpret_cast<const float4*>(b + 2 * CH + 32 * s + 4 * g);
-      const float4 w1 = *reinterpret_cast<const float4*>(b + 2 * CH + 32 * s + 16 + 4 * g);
-      uint32_t t[2][4][3];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint4 vw = __builtin_bit_cast(uint4, vf[u][s]);
-        split_pair<3>(lo_f32(vw.x) * w0.x, hi_f32(vw.x) * w0.y, t[u][0]);
-        split_pair<3>(lo_f32(vw.y) * w0.z, hi_f32(vw.y) * w0.w, t[u][1]);
-        split_pair<3>(lo_f32(vw.z) * w1.x, hi_f32(vw.z) * w1.y, t[u][2]);
-        split_pair<3>(lo_f32(vw.w) * w1.z, hi_f32(vw.w) * w1.w, t[u][3]);
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* at = ks + 32 * (x / KK) * C::KB + flip(at_tr, 4 * (x % KK)) + 8 * i;
+        const uint2 y = lds_tr(at), z = lds_tr(at + 16 * C::KB);
+        kf[x & 1][i] = __builtin_bit_cast(lbf16x8, make_uint4(y.x, y.y, z.x, z.y));
       }
+    };
+    auto decay = [&](int kk, int u) {
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const uint2 k0 = lds_tr(ks + 32 * s * C::KB + flip(at_tr, 2 * kt));
-        const uint2 k1 = lds_tr(ks + (32 * s + 16) * C::KB + flip(at_tr, 2 * kt));
-        const lbf16x8 kf = __builtin_bit_cast(lbf16x8, make_uint4(k0.x, k0.y, k1.x, k1.y));
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 2; i >= 0; --i)  // (the small terms first)
+        for (int e = 0; e < 4; ++e) acc[u][2 * kk + i][e] = fmaf(acc[u][2 * kk + i][e], add, acc[u][2 * kk + i][e]);
+    };
+    fence();
+    k_read(0);
+    decay(0, 0);
+    decay(0, 1);
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            acc[u][kt] = mfma16(kf, __builtin_bit_cast(lbf16x8, make_uint4(t[u][0][i], t[u][1][i], t[u][2][i], t[u][3][i])), acc[u][kt]);
+    for (int x = 0; x < 2 * KK; ++x) {
+      const int s = x / KK, kk = x % KK;
+      fence();
+      if (x + 1 < 2 * KK) k_read(x + 1);
+#pragma unroll
+      for (int t = NT - 1; t >= 0; --t) {  // (the small terms first)
+        fence();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const lbf16x8 vfr = v_frag(s, u, t);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[u][2 * kk + i] = mfma16(kf[x & 1][i], vfr, acc[u][2 * kk + i]);
+        }
+        if constexpr (OUT) {  // the next q's and v's loads, one at a time
+          const int i = x * NT + NT - 1 - t;
+          if (i < C::KI)
+            issue_q(c + 1, i, i + 1);
+          else if (i < C::KI + C::VI)
+            issue_v(c + 1, i - C::KI, i - C::KI + 1);
+        }
+        if (s == 0) {
+          if (kk + 1 < KK && t < 2) decay(kk + 1, t);
+          // (the 8 pairs of V' over the NT KK regions)
+          if constexpr (KK == 4) {
+            if (t < 2) v_pair(1, kk >> 1, 2 * (kk & 1) + t);
+          } else {
+            v_pair(1, kk, t);
+            if (t < 4 - NT) v_pair(1, kk, NT + t);
+          }
+          interleave<4, 5>();
+        }
       }
     }
+    fence();
     if (in_group == C::GC - 1 && c + 1 < chunks) g_store(c + 1 + wl, gv);
-    if constexpr (OUT) {
-      lds_barrier();  // nobody reads k and v any more
-      issue_kv(c + 1);
+    if constexpr (C::KS == 1) {
+      lds_barrier();  // nobody reads k any more
+      issue_k(c + 1);
     }
-  }
+  };
+  for (int c = 0; c < chunks; ++c) chunk(c, std::integral_constant<int, 3>{});
   if constexpr (OUT) {
-    if (last && a.s_out != nullptr) put(a.s_out + ((size_t)p.seq * a.Hv + h) * hs);
-  } else if (last) {
-    write_down(chunks);
+    if (keep) put(a.s_out + ((size_t)p.seq * a.Hv + h) * hs);
   } else {
-    const size_t at = (size_t)slot * a.Hv + h;
+    const size_t at = (size_t)p.slot * a.Hv + h;
     put(a.ends + at * hs);
     if (wl == 0 && l == 0) a.gtot[at] = gsum;
   }
@@ -1199,11 +1418,15 @@ Plan make_plan(bool packed, int N, int T, int Hk, int Hv, int K, int V, int dtyp
     return (int)(packed ? T / size + N : N * std::max(1L, (T + size - 1) / size));
   };
   if (walk) {
-    // segments as long as leave two workgroups for every CU
+    // Segments of a CU's share of the chunks. Half as long, two to a CU, costs 7 us at 4096 tokens of 16 heads of 128 x 128
+    // (states 12 us in the join instead of 7, 17 instead of 15 in the state pass, against 1 us less in the outputs) and
+    // gains 2 at 32768. Sequences that fill the CUs uncut are not cut below 1.5 shares: 32 of 64 .. 2048 tokens, 16 heads,
+    // take 180 us so, and 203 cut to 16 chunks (33 in the state pass and 13 in the join against 14 less in the outputs).
     const long rows = packed ? T : (long)N * T, groups = Hv / walk_heads(Hk, Hv, V);
-    const long seg = std::max(1L, (rows * groups / 512 + CH - 1) / CH) * CH;
+    const long share = (rows * groups + CUS * CH - 1) / (CUS * CH);
+    const long seg = std::max(1L, N * groups >= CUS ? share + share / 2 : share) * CH;
     p.seg = (int)std::min(seg, (long)INT32_MAX / 4);
-    p.run = 2 * p.seg;
+    p.run = p.seg;
   } else {
     p.seg = 64;
     const int vg = V / (16 * STATE_NW);
@@ -1213,7 +1436,7 @@ Plan make_plan(bool packed, int N, int T, int Hk, int Hv, int K, int V, int dtyp
   p.run_slots = slots(p.run);
   p.seg_slots = slots(p.seg);
   p.single = T <= p.run;
-  const bool cut = !walk || T > p.seg;
+  const bool cut = !walk;
   const size_t hs = (size_t)K * V * 4;
   auto round = [](size_t x) { return (x + 255) / 256 * 256; };
   p.ckpt = 0;
@@ -1237,8 +1460,9 @@ int launch_walk(const char* fn, const LinArgs& a, const Plan& p, hipStream_t s) 
   if (!lds_ready(lin_walk_kernel<K, V, NH, true>, CO::LDS, so) || !lds_ready(lin_walk_kernel<K, V, NH, false>, CS::LDS, ss))
     return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
   const int groups = a.Hv / NH;
-  if (a.T > p.seg)
-    hipLaunchKernelGGL((lin_walk_kernel<K, V, NH, false>), dim3((unsigned)(p.run_slots * groups)), dim3(64 * CS::NW), CS::LDS, s, a);
+  const int before_last = a.cu != nullptr ? a.T / a.run : a.N * ((a.T + a.run - 1) / a.run - 1);  // segments, at most
+  if (!p.single)
+    hipLaunchKernelGGL((lin_walk_kernel<K, V, NH, false>), dim3((unsigned)(before_last * groups)), dim3(64 * CS::NW), CS::LDS, s, a);
   if (!p.single)
     hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)(a.N * a.Hv * (V * K / 1024))), dim3(256), 0, s, a, V * K);
   hipLaunchKernelGGL((lin_walk_kernel<K, V, NH, true>), dim3((unsigned)(p.seg_slots * groups)), dim3(64 * CO::NW), CO::LDS, s, a);

@@ -2,16 +2,21 @@
 //
 //   S_t = exp(g_t) S_{t-1} + v_t k_t^T,   o_t = S_t (scale q_t)
 //
-// A sequence is cut into segments of L tokens. With S the state before a segment and G the running sum of g in it,
+// With S the state before a chunk of 64 tokens and G the running sum of g in it,
 //   o_t = exp(G_t) S (scale q_t) + sum_{s <= t} exp(G_t - G_s) (scale q_t . k_s) v_s,
-// so the segments' outputs are independent given their start states, which come from sums over the tokens before:
-//   1. lin_state: sequences are also cut into runs of whole segments. A run's state is summed in registers, 64 tokens at a
-//      time, from zeros (a sequence's first run: from its initial state), and written down at each segment's start.
-//   2. lin_carry (where a sequence may have several runs): the state before each run from the runs' end states.
-//   3. lin_out: each segment's outputs from its start state (the written one plus the carried one, decayed) and its rows.
+//   S' = exp(G_end) S + sum_s exp(G_end - G_s) v_s k_s^T.
+// A workgroup walks the chunks of one sequence and head, S in registers. Where there are too few of these for the device a
+// sequence is cut into segments, and then
+//   1. a walk over all segments but the last sums what each adds to the state,
+//   2. the join turns these into the states before the segments,
+//   3. the walk over the segments from there has the outputs (and, last, the final state).
 // Products are bf16 x bf16 with fp32 sums. States stay fp32: where a product takes a state or a weighted value it is
 // split into bf16 terms whose sum has 16 (outputs: two terms) or 24 bits (states: three), so that an output keeps only
 // its own rounding and a state that of fp32 sums. fp32 inputs take the same steps on the fp32 MFMA.
+//
+// Measured (the three kernels, us): 32 packed prompts of 64 .. 2048 tokens, 16 heads of 128 x 128: 5 + 6 + 170; one of 4096:
+// 15 + 7 + 27; one of 32768, 16 heads of 128 x 64 on one key head: 39 + 9 + 92. What bounds it: a chunk's instructions, not
+// its bytes (packed: 569 MB, 104 us at the rate of a copy).
 //
 // The exponents are sums of one sign where all g <= 0: suffix sums to a block's end and prefix sums from its start, not
 // differences of long sums. g is taken as at least -200 (exp(-200) is zero in fp32), so that -inf resets a state.
@@ -28,8 +33,7 @@ typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
 typedef float lf32x4 __attribute__((ext_vector_type(4)));
 typedef short lshort4 __attribute__((ext_vector_type(4)));
 
-constexpr int ST = 64;  // tokens of a stage of the state pass
-constexpr int CH = 64;  // tokens of a chunk of the walk
+constexpr int CH = 64;  // tokens of a chunk
 constexpr float G_MIN = -200.f;
 constexpr long CUS = 256;
 
@@ -43,12 +47,8 @@ struct LinArgs {
   const int32_t* cu;
   int N, T, Hk, Hv;
   float scale;
-  int seg, run;      // tokens of a segment, of a run (a multiple of seg)
-  int seg_slots, run_slots;
-  int direct;        // one run a sequence: its end is the final state
-  int save_first;    // the first segment's start state is written down too (the final state overwrites the initial one)
-  float *ckpt, *gcum;  // [seg_slots][Hv][V * K], [seg_slots][Hv]: state before a segment within its run, log decay from there
-  float *ends, *gtot;  // [run_slots][Hv][V * K], [run_slots][Hv]: a run's end state (then the state before it), log decay
+  int run, run_slots;  // tokens of a segment, at most; segments
+  float *ends, *gtot;  // [run_slots][Hv][V * K], [run_slots][Hv]: what a segment adds (then the state before it), log decay
 };
 
 __device__ __forceinline__ lf32x4 mfma16(lbf16x8 a, lbf16x8 b, lf32x4 c) {
@@ -67,7 +67,6 @@ __device__ __forceinline__ float g_value(const LinArgs& a, uint32_t bits) {
   const float x = __uint_as_float(a.g_bf16 ? bits << 16 : bits);
   return x < G_MIN ? G_MIN : x;  // (a NaN stays)
 }
-__device__ __forceinline__ float load_g(const LinArgs& a, size_t t, int h) { return g_value(a, g_bits(a, t, h)); }
 
 // x exp(G) as x + x expm1(G) for slow decays: the factor's own rounding, the same at every stage, would otherwise grow
 // with the length of the memory.
@@ -84,61 +83,6 @@ __device__ __forceinline__ Decay decay_of(float G) {
 __device__ __forceinline__ float decayed(float x, const Decay& d) { return fmaf(x, d.add, x * d.mul); }
 
 __device__ __forceinline__ int pieces(int len, int size) { return max(1, (len + size - 1) / size); }
-
-// A sequence's piece of `size` tokens by its slot (pieces numbered sequence by sequence, at least one each), with the
-// slot of the sequence's first piece of `other` tokens. Whole waves call it together.
-struct Piece {
-  int seq, j, bos, len, other0;
-};
-__device__ __forceinline__ bool find_piece(const int32_t* cu, int N, int T, int slot, int size, int other, Piece& p) {
-  if (cu == nullptr) {
-    const int per = pieces(T, size);
-    p.seq = slot / per;
-    p.j = slot - p.seq * per;
-    p.bos = p.seq * T;
-    p.len = T;
-    p.other0 = p.seq * pieces(T, other);
-    return p.seq < N;
-  }
-  const int l = threadIdx.x & 63;
-  int base = 0, base2 = 0;
-  for (int s0 = 0; s0 < N; s0 += 64) {
-    int bos = 0, eos = 0, n = 0, n2 = 0;
-    if (s0 + l < N) {
-      seq_bounds(cu, s0 + l, T, bos, eos);
-      n = pieces(eos - bos, size);
-      n2 = pieces(eos - bos, other);
-    }
-    int i = n, i2 = n2;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(i, d), u2 = __shfl_up(i2, d);
-      i += l >= d ? u : 0;
-      i2 += l >= d ? u2 : 0;
-    }
-    const uint64_t past = __ballot(base + i > slot);
-    if (past) {
-      const int f = __builtin_ctzll(past);
-      p.seq = s0 + f;
-      p.j = slot - base - (__shfl(i, f) - __shfl(n, f));
-      p.bos = __shfl(bos, f);
-      p.len = __shfl(eos, f) - p.bos;
-      p.other0 = base2 + __shfl(i2, f) - __shfl(n2, f);
-      return true;
-    }
-    base += __shfl(i, 63);
-    base2 += __shfl(i2, 63);
-  }
-  return false;
-}
-// (the same values in scalar registers: buffer resources are built from them)
-__device__ __forceinline__ void uniform(Piece& p) {
-  p.seq = __builtin_amdgcn_readfirstlane(p.seq);
-  p.j = __builtin_amdgcn_readfirstlane(p.j);
-  p.bos = __builtin_amdgcn_readfirstlane(p.bos);
-  p.len = __builtin_amdgcn_readfirstlane(p.len);
-  p.other0 = __builtin_amdgcn_readfirstlane(p.other0);
-}
 
 __device__ __forceinline__ int prefix_count(int x) {  // over the lanes up to this one
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
@@ -220,13 +164,14 @@ __device__ __forceinline__ bool find_segment(const LinArgs& a, int i, int side, 
 
 // ---------------------------------------------------------------------------------------------- LDS tiles of rows
 //
-// Rows of ROWB bytes (64 .. 512), 16-byte chunk c of row r at c ^ mask(r): row fragments (16 rows, one chunk each) and
+// Rows of ROWB bytes (128 .. 512), 16-byte chunk c of row r at c ^ mask(r): row fragments (16 rows, one chunk each) and
 // transposing reads (4 rows, 32 bytes each, for each group of 16 lanes) then spread over the banks.
 
-template <int ROWB>
+template <int ROWB, typename T = uint16_t>
 __device__ __forceinline__ int chunk_at(int r, int c) {
   constexpr int n = ROWB / 16;
-  const int f = n >= 16 ? (r & 7) << 1 | (r >> 3 & 1) : n == 8 ? (r >> 1) & 7 : (r >> 1) & 3;
+  constexpr bool wide = sizeof(T) == 4;  // (fp32 rows, 256 bytes and more, are read by whole chunks of 16 rows)
+  const int f = wide ? r & 15 : n >= 16 ? (r & 7) << 1 | (r >> 3 & 1) : n == 8 ? (r >> 1) & 7 : (r >> 1) & 3;
   return r * ROWB + ((c ^ f) << 4);
 }
 
@@ -235,14 +180,14 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
 // register; M0 (which these kernels use for nothing else) needs a wait state before the load.
 typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_lds(lu32x4 rsrc, uint32_t off, const uint8_t* lds) {
-  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)lds);
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);  // (an address in LDS: the low half)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc) : "memory");
 }
 
 // ROWS rows of ROWB bytes from global memory (row stride ld_bytes, `rows` of them there, zeros behind them) into LDS, by
 // NW waves; each wave instruction fills 1 KiB, so a lane fetches the chunk that belongs at its place. The places in a row
 // repeat every PERIOD instructions of a wave: these byte offsets are kept, the others follow by whole rows.
-template <int ROWB, int NW>
+template <int ROWB, int NW, typename T = uint16_t>
 struct RowsAt {
   static constexpr int RP = 1024 / ROWB, PERIOD = ROWB >= 256 ? (16 + RP * NW - 1) / (RP * NW) : 1;
   static_assert(RP * NW * PERIOD % 16 == 0, "the swizzle's period");
@@ -253,7 +198,7 @@ struct RowsAt {
 #pragma unroll
     for (int i = 0; i < PERIOD; ++i) {
       const int r = (i * NW + wave) * RP + l / n;
-      off[i] = (uint32_t)(r - i * NW * RP) * ld_bytes + (uint32_t)(chunk_at<ROWB>(r, l % n) - r * ROWB);
+      off[i] = (uint32_t)(r - i * NW * RP) * ld_bytes + (uint32_t)(chunk_at<ROWB, T>(r, l % n) - r * ROWB);
     }
   }
   __device__ __forceinline__ void anew() {  // (nothing formed from them is kept across)
@@ -262,8 +207,8 @@ struct RowsAt {
   }
 };
 // (instructions i0 .. i1 - 1 of the wave's ROWS ROWB / 1024 / NW)
-template <int ROWB, int ROWS, int NW>
-__device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW>& at_row, const void* base, uint32_t ld_bytes, int rows,
+template <int ROWB, int ROWS, int NW, typename T>
+__device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW, T>& at_row, const void* base, uint32_t ld_bytes, int rows,
                                           uint8_t* lds, int wave, int i0 = 0, int i1 = ROWS * ROWB / 1024 / NW) {
   constexpr int RP = 1024 / ROWB;  // rows an instruction
   static_assert(ROWS % (RP * NW) == 0, "as many a wave");
@@ -274,25 +219,10 @@ __device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW>& at_row, const 
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 #pragma unroll
   for (int i = i0; i < i1; ++i)
-    load_lds(rs, at_row.off[i % RowsAt<ROWB, NW>::PERIOD] + (uint32_t)(i * NW * RP) * ld_bytes, lds + 1024 * (i * NW + wave));
+    load_lds(rs, at_row.off[i % RowsAt<ROWB, NW, T>::PERIOD] + (uint32_t)(i * NW * RP) * ld_bytes, lds + 1024 * (i * NW + wave));
 }
-template <int ROWB, int ROWS, int NW>
-__device__ __forceinline__ void load_rows(const void* base, uint32_t ld_bytes, int rows, uint8_t* lds, int wave) {
-  load_rows<ROWB, ROWS, NW>(RowsAt<ROWB, NW>(ld_bytes, wave), base, ld_bytes, rows, lds, wave);
-}
-
 __device__ __forceinline__ uint2 lds_tr(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) lshort4*)p));
-}
-// Fragment of a tile's transpose: column c0 + (lane % 16) of rows r0 + 4 g + {0..3} and r0 + 16 + 4 g + {0..3}
-// (g = lane / 16), the order in which two D tiles below one another hold their rows.
-template <int ROWB>
-__device__ __forceinline__ lbf16x8 tr_frag(const uint8_t* tile, int r0, int c0) {
-  const int l = threadIdx.x & 63, g = l >> 4, s = l & 15;
-  const int r = r0 + 4 * g + (s >> 2), c = c0 / 8 + ((s & 3) >> 1);
-  const uint2 a = lds_tr(tile + chunk_at<ROWB>(r, c) + 8 * (s & 1));
-  const uint2 b = lds_tr(tile + chunk_at<ROWB>(r + 16, c) + 8 * (s & 1));
-  return __builtin_bit_cast(lbf16x8, make_uint4(a.x, a.y, b.x, b.y));
 }
 
 __device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
@@ -310,7 +240,12 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* w) {
 }
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-__device__ __forceinline__ void loads_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N of the wave's loads outstanding, then a barrier
+  static_assert(N < 64, "counter");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 // Sum over the lanes up to this one (DPP: within rows of 16, then rows 0 and 2 on 1 and 3, then the lower half on the upper).
 template <int CTRL, int ROWS>
@@ -327,515 +262,6 @@ __device__ __forceinline__ float prefix_sum(float x) {
   return x;
 }
 
-// Sum over the lanes after this one (suffix, without it) and over all of the wave's.
-__device__ __forceinline__ float suffix_sum(float x, float& total) {
-  const int l = threadIdx.x & 63;
-  float s = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const float u = __shfl_down(s, d);
-    s += l + d < 64 ? u : 0.f;
-  }
-  total = __shfl(s, 0);
-  const float n = __shfl_down(s, 1);
-  return l == 63 ? 0.f : n;
-}
-
-// ------------------------------------------------------------------------------------------------- 1. run states
-//
-// A workgroup of NW waves sums 16 NW value rows of one (run, head); wave w keeps rows 16 w .. of S as the transposed
-// tiles [K / 16] (D: key 4 g + e, value lane % 16). A stage's tokens enter as sum_s K^T (M = key) x weighted V (N = value)
-// over the tokens, both read transposed from LDS; the weights exp(G_end - G_s) go on v, split into three bf16 terms.
-
-template <typename T, int K, int V, int NW>
-struct StateCfg {
-  static constexpr int ES = sizeof(T);
-  static constexpr int KB = K * ES, VB = 16 * NW * ES;  // bytes of a row
-  static constexpr int STAGE = ST * (KB + VB);
-  static constexpr int LDS = 2 * STAGE + NW * ST * 4;
-};
-
-template <int K>
-__device__ __forceinline__ void put_state(float* dst, const lf32x4 (&acc)[K / 16], int v0) {  // dst [V][K] of one head
-  const int l = threadIdx.x & 63, g = l >> 4, m = l & 15;
-#pragma unroll
-  for (int kt = 0; kt < K / 16; ++kt)
-    *reinterpret_cast<lf32x4*>(dst + (size_t)(v0 + m) * K + 16 * kt + 4 * g) = acc[kt];
-}
-
-template <typename T, int K, int V, int NW>
-__global__ __launch_bounds__(64 * NW) void lin_state_kernel(LinArgs a) {
-  using C = StateCfg<T, K, V, NW>;
-  extern __shared__ uint4 lin_lds[];
-  uint8_t* lds = reinterpret_cast<uint8_t*>(lin_lds);
-  constexpr int VG = V / (16 * NW);
-  // units (run, head) one after the other, the VG workgroups of one unit on one XCD (ids equal mod 8)
-  const int id = blockIdx.x, unit = id / (8 * VG) * 8 + id % 8, vg = id / 8 % VG;
-  const int slot = unit / a.Hv, h = unit - slot * a.Hv;
-  if (slot >= a.run_slots) return;
-  Piece p;
-  if (!find_piece(a.cu, a.N, a.T, slot, a.run, a.seg, p)) return;
-  uniform(p);
-  const int wave = wave_id(), l = threadIdx.x & 63, g = l >> 4, m = l & 15;
-  const int first = p.j * a.run, n = min(a.run, p.len - first);  // (n 0 for an empty sequence)
-  const int v0 = 16 * NW * vg + 16 * wave;
-  const size_t row0 = (size_t)p.bos + first;
-  const T* kp = reinterpret_cast<const T*>(a.k) + row0 * a.k_ld + (size_t)(h / (a.Hv / a.Hk)) * K;
-  const T* vp = reinterpret_cast<const T*>(a.v) + row0 * a.v_ld + (size_t)h * V + 16 * NW * vg;
-  const uint32_t k_lb = (uint32_t)a.k_ld * C::ES, v_lb = (uint32_t)a.v_ld * C::ES;
-  float* wts = reinterpret_cast<float*>(lds + 2 * C::STAGE) + wave * ST;  // the wave's own
-
-  auto issue = [&](int s) {
-    uint8_t* at = lds + (s & 1) * C::STAGE;
-    load_rows<C::KB, ST, NW>(kp + (size_t)s * ST * a.k_ld, k_lb, n - s * ST, at, wave);
-    load_rows<C::VB, ST, NW>(vp + (size_t)s * ST * a.v_ld, v_lb, n - s * ST, at + ST * C::KB, wave);
-  };
-  auto g_of = [&](int s) { return s * ST + l < n ? load_g(a, row0 + s * ST + l, h) : 0.f; };
-
-  const int stages = (n + ST - 1) / ST;
-  if (stages > 0) issue(0);
-  float gv = g_of(0), gsum = 0.f;
-
-  lf32x4 acc[K / 16];
-#pragma unroll
-  for (int kt = 0; kt < K / 16; ++kt) acc[kt] = lf32x4{0.f, 0.f, 0.f, 0.f};
-  const size_t hs = (size_t)V * K;
-  if (p.j == 0 && a.s_in != nullptr) {
-    const float* src = a.s_in + ((size_t)p.seq * a.Hv + h) * hs;
-#pragma unroll
-    for (int kt = 0; kt < K / 16; ++kt)
-      acc[kt] = *reinterpret_cast<const lf32x4*>(src + (size_t)(v0 + m) * K + 16 * kt + 4 * g);
-  }
-  // (segments past the slots: only tables whose sequences overlap name so many)
-  if (p.j == 0 && a.save_first && p.other0 < a.seg_slots) put_state<K>(a.ckpt + ((size_t)p.other0 * a.Hv + h) * hs, acc, v0);
-
-  for (int s = 0; s < stages; ++s) {
-    const int at = p.other0 + (first + s * ST) / a.seg;
-    if (s > 0 && s * ST % a.seg == 0 && at < a.seg_slots) {
-      const size_t c = (size_t)at * a.Hv + h;
-      put_state<K>(a.ckpt + c * hs, acc, v0);
-      if (vg == 0 && threadIdx.x == 0) a.gcum[c] = gsum;
-    }
-    loads_barrier();  // stage s is there, and nobody reads the other one any more
-    if (s + 1 < stages) issue(s + 1);
-    float total;
-    const float w = expf(suffix_sum(gv, total));
-    gv = g_of(s + 1);
-    gsum += total;
-    wts[l] = w;
-    const Decay d = decay_of(total);
-#pragma unroll
-    for (int kt = 0; kt < K / 16; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[kt][e] = decayed(acc[kt][e], d);
-    const uint8_t* ks = lds + (s & 1) * C::STAGE;
-    const uint8_t* vs = ks + ST * C::KB;
-    {
-#pragma unroll 1
-      for (int b = 0; b < ST; b += 16) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // tokens b + 4 g + e
-          const int r = b + 4 * g + e;
-          const int cv = 16 * wave + m;
-          const float x = *reinterpret_cast<const float*>(vs + chunk_at<C::VB>(r, cv / 4) + 4 * (cv & 3)) * wts[r];
-#pragma unroll
-          for (int kt = 0; kt < K / 16; ++kt) {
-            const float y = *reinterpret_cast<const float*>(ks + chunk_at<C::KB>(r, 4 * kt + (m >> 2)) + 4 * (m & 3));
-            acc[kt] = mfma4(y, x, acc[kt]);
-          }
-        }
-      }
-    }
-  }
-  if (a.direct) {
-    if (a.s_out != nullptr) put_state<K>(a.s_out + ((size_t)p.seq * a.Hv + h) * hs, acc, v0);
-  } else {
-    const size_t c = (size_t)slot * a.Hv + h;
-    put_state<K>(a.ends + c * hs, acc, v0);
-    if (vg == 0 && threadIdx.x == 0) a.gtot[c] = gsum;
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------- 2. carries
-//
-// The end states of a sequence's runs, in place, become the states carried into them: c_0 = 0 (the first run starts from
-// the initial state itself), c_{j+1} = exp(G_j) c_j + E_j; the last one is the final state. A thread keeps 4 elements.
-
-__global__ __launch_bounds__(256) void lin_carry_kernel(LinArgs a, int hs) {
-  const int per = hs / 1024, unit = blockIdx.x / per, part = blockIdx.x % per;
-  const int seq = unit / a.Hv, h = unit - seq * a.Hv;
-  int slot0 = 0, n = 0;
-  if (a.cu == nullptr) {
-    n = pieces(a.T, a.run);
-    slot0 = seq * n;
-  } else {
-    const int l = threadIdx.x & 63;
-    int sum = 0;
-    for (int s = l; s < seq; s += 64) {
-      int bos, eos;
-      seq_bounds(a.cu, s, a.T, bos, eos);
-      sum += pieces(eos - bos, a.run);
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    slot0 = sum;
-    int bos, eos;
-    seq_bounds(a.cu, seq, a.T, bos, eos);
-    n = pieces(eos - bos, a.run);
-  }
-  n = min(n, a.run_slots - slot0);  // (tables whose sequences overlap may name more runs than there are slots)
-  const size_t at = (size_t)part * 1024 + 4 * threadIdx.x;
-  lf32x4 c = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < n; ++j) {
-    const size_t u = (size_t)(slot0 + j) * a.Hv + h;
-    lf32x4* p = reinterpret_cast<lf32x4*>(a.ends + u * hs + at);
-    const lf32x4 e = *p;
-    const float d = expf(a.gtot[u]);
-    *p = c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = fmaf(c[i], d, e[i]);
-  }
-  if (a.s_out != nullptr) *reinterpret_cast<lf32x4*>(a.s_out + ((size_t)seq * a.Hv + h) * hs + at) = c;
-}
-
-// Whether any of a block's R rows holds an infinity or a NaN (each wave for its own block).
-template <int ROWB, int R>
-__device__ __forceinline__ bool rows_not_finite(const uint8_t* rows, int es) {
-  uint32_t bad = 0;
-#pragma unroll
-  for (int i = 0; i < ROWB * R / 1024; ++i) {
-    const uint4 w = *reinterpret_cast<const uint4*>(rows + 1024 * i + 16 * (threadIdx.x & 63));
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      bad |= (x[e] & 0x7f800000u) == 0x7f800000u;
-      if (es == 2) bad |= (x[e] & 0x7f80u) == 0x7f80u;
-    }
-  }
-  return __ballot(bad) != 0;
-}
-
-// ---------------------------------------------------------------------------------------------------- 3. outputs
-//
-// A workgroup takes one (segment, head); a wave 32 tokens (fp32: 16), which are the columns of its transposed tiles:
-//   O^T [V, t] = S Q^T (rows scaled by exp(G_t)) + V^T P^T,   P^T [s, t] = K Q^T scaled and masked.
-// P^T's D tiles (token s = 4 g + e of 16, t = lane % 16) are the B operand of the second product as they stand, with V^T
-// read transposed from LDS in the same order of s. The start state is split into two bf16 terms in LDS, P into two in
-// registers. exp(G_t - G_s) is exp(prefix_t + blocks between) exp(suffix_s) across blocks of 32 and one exponential an
-// element within a block.
-
-template <typename T, int K, int V, int L>
-struct OutCfg {
-  static constexpr int ES = sizeof(T), TW = ES == 2 ? 32 : 16;  // tokens a wave
-  static constexpr int NW = L / TW;
-  static constexpr int KB = K * ES, VB = V * ES;
-  static constexpr int S_BYTES = V * K * 4;  // two bf16 terms, or fp32
-  static constexpr int AT_K = S_BYTES, AT_V = AT_K + L * KB, AT_W = AT_V + L * VB;
-  static constexpr int LDS = AT_W + 2 * L * 4 + NW * 4 + (ES == 4 ? L * 8 : 0);
-};
-
-template <typename T, int K, int V, int L>
-__global__ __launch_bounds__((64 * OutCfg<T, K, V, L>::NW)) void lin_out_kernel(LinArgs a) {
-  using C = OutCfg<T, K, V, L>;
-  constexpr int TW = C::TW, NW = C::NW, NT = TW / 16;
-  extern __shared__ uint4 lin_lds[];
-  uint8_t* lds = reinterpret_cast<uint8_t*>(lin_lds);
-  uint8_t *kt_ = lds + C::AT_K, *vt_ = lds + C::AT_V;
-  float* wsuf = reinterpret_cast<float*>(lds + C::AT_W);  // exp(suffix) of each token to its block's end
-  float* pre = wsuf + L;                                  // prefix within the block, the token's own g included
-  float* tot = pre + L;                                   // each block's sum
-  const int slot = blockIdx.x / a.Hv, h = blockIdx.x - slot * a.Hv;
-  Piece p;
-  if (!find_piece(a.cu, a.N, a.T, slot, a.seg, a.run, p)) return;
-  uniform(p);
-  const int first = p.j * L, n = min(L, p.len - first);
-  if (n <= 0) return;  // (an empty sequence)
-  const int wave = wave_id(), l = threadIdx.x & 63, g = l >> 4, m = l & 15;
-  const size_t row0 = (size_t)p.bos + first;
-  const size_t hk = (size_t)(h / (a.Hv / a.Hk)) * K;
-  const T* qp = reinterpret_cast<const T*>(a.q) + row0 * a.q_ld + hk;
-  const T* kp = reinterpret_cast<const T*>(a.k) + row0 * a.k_ld + hk;
-  const T* vp = reinterpret_cast<const T*>(a.v) + row0 * a.v_ld + (size_t)h * V;
-
-  // the start state: within the run as written down (or the initial state), and what is carried into the run
-  const int run = first / a.run, in_run = first - run * a.run;
-  const size_t hs = (size_t)V * K;
-  const float* s_loc = in_run > 0 || (p.j == 0 && a.save_first) ? a.ckpt + ((size_t)slot * a.Hv + h) * hs
-                       : p.j == 0 && a.s_in != nullptr          ? a.s_in + ((size_t)p.seq * a.Hv + h) * hs
-                                                                : nullptr;
-  const float* s_car = run > 0 && p.other0 + run < a.run_slots ? a.ends + ((size_t)(p.other0 + run) * a.Hv + h) * hs : nullptr;
-  const bool has_state = s_loc != nullptr || s_car != nullptr;
-  if (has_state) {
-    const float dc = s_car == nullptr ? 0.f : in_run > 0 ? expf(a.gcum[(size_t)slot * a.Hv + h]) : 1.f;
-    constexpr int THREADS = 64 * NW, PER = V * K / 4 / THREADS, BATCH = PER > 16 ? 16 : PER;
-#pragma unroll 1
-    for (int b = 0; b < PER; b += BATCH) {
-      lf32x4 x[BATCH];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const size_t at = 4 * ((size_t)(b + i) * THREADS + threadIdx.x);
-        x[i] = s_loc != nullptr ? *reinterpret_cast<const lf32x4*>(s_loc + at) : lf32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      if (s_car != nullptr) {
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const size_t at = 4 * ((size_t)(b + i) * THREADS + threadIdx.x);
-          const lf32x4 y = *reinterpret_cast<const lf32x4*>(s_car + at);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][e] = fmaf(y[e], dc, x[i][e]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int at = 4 * ((b + i) * THREADS + (int)threadIdx.x), v = at / K, k = at % K;
-        if constexpr (C::ES == 2) {
-          uint32_t w0[2], w1[2];
-          split_pair<2>(x[i][0], x[i][1], w0);
-          split_pair<2>(x[i][2], x[i][3], w1);
-          uint8_t* base = lds + (k / 32) * V * 128;  // rows of 64 bytes of first terms, 64 of second ones
-          const int c = (k % 32) / 8, half = k & 4 ? 8 : 0;
-          *reinterpret_cast<uint2*>(base + chunk_at<128>(v, c) + half) = make_uint2(w0[0], w1[0]);
-          *reinterpret_cast<uint2*>(base + chunk_at<128>(v, 4 + c) + half) = make_uint2(w0[1], w1[1]);
-        } else {
-          *reinterpret_cast<lf32x4*>(lds + chunk_at<K * 4>(v, k / 4)) = x[i];
-        }
-      }
-    }
-  }
-  load_rows<C::KB, L, NW>(kp, (uint32_t)a.k_ld * C::ES, n, kt_, wave);
-  load_rows<C::VB, L, NW>(vp, (uint32_t)a.v_ld * C::ES, n, vt_, wave);
-
-  // the wave's queries: lane's token m of each tile, 16 bytes of keys a step
-  const int t0 = wave * TW;
-  constexpr int QS = C::KB / 64;  // steps of 64 bytes of a row
-  uint4 q[NT][QS];
-  {
-    const uint32_t lb = (uint32_t)a.q_ld * C::ES;
-    const Rsrc rs = raw_rsrc(qp, (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(n - 1) * lb + C::KB)));
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < QS; ++i)
-        q[j][i] = __builtin_bit_cast(
-            uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, (uint32_t)(t0 + 16 * j + m) * lb + 64 * i + 16 * g, 0, 0));
-  }
-  // decays of the wave's own block: lanes 0 .. TW - 1 a token each
-  {
-    const int i = l & (TW - 1), t = t0 + i;
-    const float gv = t < n ? load_g(a, row0 + t, h) : 0.f;
-    float s = gv, u = gv;  // prefix and suffix, inclusive
-    double sd = (double)gv;
-#pragma unroll
-    for (int d = 1; d < TW; d <<= 1) {
-      const float x = __shfl_up(s, d, TW), y = __shfl_down(u, d, TW);
-      s += i >= d ? x : 0.f;
-      u += i + d < TW ? y : 0.f;
-      if constexpr (C::ES == 4) {
-        const double z = __shfl_up(sd, d, TW);
-        sd += i >= d ? z : 0.0;
-      }
-    }
-    const float nx = __shfl_down(u, 1, TW);
-    if (l < TW) {
-      wsuf[t] = expf(i == TW - 1 ? 0.f : nx);
-      pre[t] = s;
-      if constexpr (C::ES == 4) reinterpret_cast<double*>(tot + NW + (NW & 1))[t] = sd;
-      if (i == TW - 1) tot[wave] = s;
-    }
-  }
-  loads_barrier();
-
-  lf32x4 acc[V / 16][NT];
-#pragma unroll
-  for (int v = 0; v < V / 16; ++v)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[v][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
-  float pt[NT];  // the lane's tokens' prefixes
-#pragma unroll
-  for (int j = 0; j < NT; ++j) pt[j] = pre[t0 + 16 * j + m];
-
-  if (has_state) {
-    if constexpr (C::ES == 2) {
-#pragma unroll
-      for (int i = 0; i < K / 32; ++i) {
-        const uint8_t* base = lds + i * V * 128;
-#pragma unroll
-        for (int v = 0; v < V / 16; ++v) {
-          const lbf16x8 hi = *reinterpret_cast<const lbf16x8*>(base + chunk_at<128>(16 * v + m, g));
-          const lbf16x8 lo = *reinterpret_cast<const lbf16x8*>(base + chunk_at<128>(16 * v + m, 4 + g));
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const lbf16x8 b = __builtin_bit_cast(lbf16x8, q[j][i]);
-            acc[v][j] = mfma16(lo, b, acc[v][j]);
-            acc[v][j] = mfma16(hi, b, acc[v][j]);
-          }
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < K / 16; ++i) {
-#pragma unroll
-        for (int v = 0; v < V / 16; ++v) {
-          const lf32x4 x = *reinterpret_cast<const lf32x4*>(lds + chunk_at<K * 4>(16 * v + m, 4 * i + g));
-          lf32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ii = 0; ii < QS; ++ii)
-            if (ii == i) y = __builtin_bit_cast(lf32x4, q[0][ii]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[v][0] = mfma4(x[e], y[e], acc[v][0]);
-        }
-      }
-    }
-    float before = 0.f;
-    for (int b = 0; b < wave; ++b) before += tot[b];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const float f = a.scale * expf(before + pt[j]);
-#pragma unroll
-      for (int v = 0; v < V / 16; ++v) acc[v][j] *= f;
-    }
-  }
-
-  float between = 0.f;  // sum of the blocks between the one at hand and the wave's own
-  for (int sb = wave; sb >= 0; --sb) {
-    const int s0 = sb * TW;
-    lf32x4 pp[NT][NT];  // [s tile][t tile]
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) pp[i][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < QS; ++kk) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(kt_ + chunk_at<C::KB>(s0 + 16 * i + m, 4 * kk + g));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if constexpr (C::ES == 2) {
-            pp[i][j] = mfma16(__builtin_bit_cast(lbf16x8, kf), __builtin_bit_cast(lbf16x8, q[j][kk]), pp[i][j]);
-          } else {
-            const lf32x4 x = __builtin_bit_cast(lf32x4, kf), y = __builtin_bit_cast(lf32x4, q[j][kk]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pp[i][j] = mfma4(x[e], y[e], pp[i][j]);
-          }
-        }
-      }
-    }
-    if (sb == wave) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int s = 16 * i + 4 * g + e, t = 16 * j + m;
-            float d;
-            if constexpr (C::ES == 4) {
-              const double* pd = reinterpret_cast<const double*>(tot + NW + (NW & 1)) + s0;
-              d = (float)(pd[t] - pd[s]);
-            } else {
-              d = pt[j] - pre[s0 + s];
-            }
-            pp[i][j][e] = s <= t ? pp[i][j][e] * (a.scale * expf(d)) : 0.f;
-          }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float f = a.scale * expf(pt[j] + between);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const lf32x4 w = *reinterpret_cast<const lf32x4*>(wsuf + s0 + 16 * i + 4 * g);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pp[i][j][e] *= f * w[e];
-        }
-      }
-      between += tot[sb];
-    }
-    if constexpr (C::ES == 2) {
-      lbf16x8 ph[NT], pl[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint32_t w[4][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          split_pair<2>(pp[i][j][0], pp[i][j][1], w[2 * i]);
-          split_pair<2>(pp[i][j][2], pp[i][j][3], w[2 * i + 1]);
-        }
-        ph[j] = __builtin_bit_cast(lbf16x8, make_uint4(w[0][0], w[1][0], w[2][0], w[3][0]));
-        pl[j] = __builtin_bit_cast(lbf16x8, make_uint4(w[0][1], w[1][1], w[2][1], w[3][1]));
-      }
-      if (sb == wave && rows_not_finite<C::VB, TW>(vt_ + s0 * C::VB, C::ES)) {
-        // a masked P is zero, and zero times such a value is NaN: token by token, each added from its own row on
-        for (int s = 0; s < TW; ++s) {
-          const bool mine = (s >> 2 & 3) == g;  // the lane's fragment holds token s at place s % 4 + 4 (s / 16)
-          const int at = (s & 3) + 4 * (s >> 4);
-#pragma unroll
-          for (int v = 0; v < V / 16; ++v) {
-            uint4 w = __builtin_bit_cast(uint4, tr_frag<C::VB>(vt_, s0, 16 * v));
-            const uint32_t half = mine ? (at & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-            w.x &= at >> 1 == 0 ? half : 0u;
-            w.y &= at >> 1 == 1 ? half : 0u;
-            w.z &= at >> 1 == 2 ? half : 0u;
-            w.w &= at >> 1 == 3 ? half : 0u;
-            const lbf16x8 vf = __builtin_bit_cast(lbf16x8, w);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              lf32x4 x = {0.f, 0.f, 0.f, 0.f};
-              x = mfma16(vf, pl[j], x);
-              x = mfma16(vf, ph[j], x);
-              if (s <= 16 * j + m) acc[v][j] += x;
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < V / 16; ++v) {
-          const lbf16x8 vf = tr_frag<C::VB>(vt_, s0, 16 * v);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            acc[v][j] = mfma16(vf, pl[j], acc[v][j]);
-            acc[v][j] = mfma16(vf, ph[j], acc[v][j]);
-          }
-        }
-      }
-    } else {
-      const bool apart = sb == wave && rows_not_finite<C::VB, TW>(vt_ + s0 * C::VB, C::ES);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = s0 + 4 * g + e;
-#pragma unroll
-        for (int v = 0; v < V / 16; ++v) {
-          const float x = *reinterpret_cast<const float*>(vt_ + chunk_at<C::VB>(r, 4 * v + (m >> 2)) + 4 * (m & 3));
-          if (!apart) {
-            acc[v][0] = mfma4(x, pp[0][0][e], acc[v][0]);
-          } else {  // (as above)
-            for (int gg = 0; gg < 4; ++gg) {
-              const lf32x4 y = mfma4(g == gg ? x : 0.f, pp[0][0][e], lf32x4{0.f, 0.f, 0.f, 0.f});
-              if (4 * gg + e <= m) acc[v][0] += y;
-            }
-          }
-        }
-      }
-    }
-  }
-
-  // the lane holds values 16 v + 4 g .. + 3 of its tokens
-  T* op = reinterpret_cast<T*>(a.o) + (row0 * a.Hv + h) * V;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int t = t0 + 16 * j + m;
-    if (t < n) {
-#pragma unroll
-      for (int v = 0; v < V / 16; ++v) {
-        T* dst = op + (size_t)t * a.Hv * V + 16 * v + 4 * g;
-        if constexpr (C::ES == 2)
-          *reinterpret_cast<uint2*>(dst) =
-              make_uint2(pack_bf16x2(acc[v][j][0], acc[v][j][1]), pack_bf16x2(acc[v][j][2], acc[v][j][3]));
-        else
-          *reinterpret_cast<lf32x4*>(dst) = acc[v][j];
-      }
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------------- bf16: a walk over chunks
 //
 // A workgroup walks the 64-token chunks of one segment of a sequence for NH value heads that share a key head (NH V = 64 or
@@ -846,9 +272,13 @@ __global__ __launch_bounds__((64 * OutCfg<T, K, V, L>::NW)) void lin_out_kernel(
 //   P^T [s, t] = K Q^T, scaled by exp(G_t - G_s) and masked, a few tiles a wave, as two bf16 terms into LDS for all;
 //   O^T [v, t] = exp(G_t) S Q^T + V^T P^T;
 //   S^T = exp(G_end) S^T + K^T V', V' = exp(G_end - G_s) V in three bf16 terms.
-// V^T and K^T are read transposed from LDS. A chunk's 200 MFMAs a wave (16 cycles each) and 700 other vector instructions
-// (4 each) take turns unless they are interleaved: the splits into terms run beside the products of the step before, and
-// two workgroups share a CU. OUT false: the state alone.
+// V^T and K^T are read transposed from LDS. A chunk of 128 x 128 is 200 MFMAs (16 cycles) and 700 other vector instructions
+// a wave; beside an MFMA two of these cost nothing and each further one 4.3 cycles, so the splits into terms run beside the
+// products of the step before, 4600 cycles in all if nothing waited. Measured: 9700 a chunk with one workgroup on the CU,
+// 7500 with two (the rest: P's chain of reads, products, exponentials and writes, 1700; barriers and loads 1000; V^T P^T
+// and stores 1500). The three terms of V' are 32 of the MFMAs and 100 of the others more than two would be; two where a
+// segment's end state is not kept took a second body of the loop and registers it did not have (97 spilled: 27 -> 32 us at
+// 4096 tokens). OUT false: the state alone.
 
 template <int K, int V, int NH, bool OUT>
 struct WalkCfg {
@@ -872,12 +302,6 @@ struct WalkCfg {
   }
   static constexpr int count(int w) { return WH == 4 ? (w < 2 ? 2 : 3) : (w == 0 ? 4 : 6); }
 };
-
-template <int N>
-__device__ __forceinline__ void wait_loads() {  // at most N of the wave's loads outstanding, then a barrier
-  static_assert(N < 64, "counter");
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ int walk_row(int u, int m) { return 8 * (m >> 2) + 4 * u + (m & 3); }
 
@@ -1336,10 +760,323 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads into LDS that nobody reads end before the workgroup does)
 }
 
+// ------------------------------------------------------------------------------------------- fp32: a walk over chunks
+//
+// The same steps on the fp32 MFMA (16 x 16, 4 terms), for one head a workgroup of 4 waves; a wave keeps U = V / 64 tiles of
+// 16 value rows (value of row m and tile u: U m + u of the wave's), all keys. The 4 terms of a product are taken so that a
+// register is an operand as it stands: for S Q^T keys 16 g + 4 i + x of a block of 64 (S^T's tile x holds the block's keys
+// = x mod 4, so a lane's rows 4 g + i are these), for V^T P^T and K^T V' tokens 16 i + 4 g + e, the rows that P's tiles
+// hold; a chunk's values are read once for both. A chunk of 64 x 64 is 216 MFMAs of 32 cycles a wave, 6900 cycles, and takes
+// 13000: 6 prompts of 40 .. 1500 tokens of 8 such heads 11 + 4 + 22 us.
+
+template <int K, int V, bool OUT>
+struct Walk32Cfg {
+  static constexpr int NW = 4, U = V / 64, KB = 4 * K, VB = 4 * V;
+  static constexpr int VS = OUT ? 1 : 2;  // stages of v (and q); k has two
+  static constexpr int AT_V = 2 * CH * KB, AT_Q = AT_V + VS * CH * VB, AT_P = AT_Q + (OUT ? CH * KB : 0);
+  static constexpr int AT_G = AT_P + (OUT ? 10 * 1024 : 0);
+  // a chunk's decays: prefix sums (doubles), scale exp of them, exp of the suffix sums, of all (Decay) and their sum;
+  // formed 4 chunks at a time, one a wave
+  static constexpr int G_FLOATS = 4 * CH + 4, RING = NW + 1;
+  static constexpr int LDS = AT_G + RING * G_FLOATS * 4;
+  static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <int K, int V, bool OUT>
+__global__ __launch_bounds__(256, (K * V > 8192 ? 1 : 2)) void lin_walk_f32_kernel(LinArgs a) {
+  using C = Walk32Cfg<K, V, OUT>;
+  constexpr int NW = C::NW, U = C::U, KH = K / 64;
+  extern __shared__ uint4 lin_lds[];
+  uint8_t* lds = reinterpret_cast<uint8_t*>(lin_lds);
+  const int index = blockIdx.x / a.Hv, h = blockIdx.x - index * a.Hv;
+  Segment p;
+  if (!find_segment<OUT>(a, index, max(1, (int)CUS / a.Hv), p) || p.slot >= a.run_slots) return;  // (as above)
+  const int n = p.n, wave = wave_id(), l = threadIdx.x & 63, g = l >> 4, m = l & 15;
+  const size_t row0 = (size_t)p.bos + p.first, hk = (size_t)(h / (a.Hv / a.Hk)) * K;
+  const float* qp = reinterpret_cast<const float*>(a.q) + row0 * a.q_ld + hk;
+  const float* kp = reinterpret_cast<const float*>(a.k) + row0 * a.k_ld + hk;
+  const float* vp = reinterpret_cast<const float*>(a.v) + row0 * a.v_ld + (size_t)h * V;
+  float* gb = reinterpret_cast<float*>(lds + C::AT_G);
+
+  const int chunks = (n + CH - 1) / CH;
+  RowsAt<C::KB, NW, float> k_at((uint32_t)a.k_ld * 4u, wave), q_at((uint32_t)a.q_ld * 4u, wave);
+  RowsAt<C::VB, NW, float> v_at((uint32_t)a.v_ld * 4u, wave);
+  auto issue = [&](const float* x, long ld, const auto& lanes, auto row_bytes, int at, int c) {
+    const int rows = max(0, min(CH, n - c * CH));  // (behind the last chunk: none, zeros)
+    load_rows<decltype(row_bytes)::value, CH, NW>(lanes, x + (rows > 0 ? (size_t)c * CH : 0) * ld, (uint32_t)ld * 4u, rows, lds + at, wave);
+  };
+  auto issue_k = [&](int c) { issue(kp, a.k_ld, k_at, std::integral_constant<int, C::KB>{}, (c & 1) * CH * C::KB, c); };
+  auto issue_v = [&](int c) {
+    issue(vp, a.v_ld, v_at, std::integral_constant<int, C::VB>{}, C::AT_V + (OUT ? 0 : (c & 1) * CH * C::VB), c);
+  };
+  auto issue_q = [&](int c) { issue(qp, a.q_ld, q_at, std::integral_constant<int, C::KB>{}, C::AT_Q, c); };
+  auto g_at = [&](int c) { return gb + (c % C::RING) * C::G_FLOATS; };
+  auto g_load = [&](int c) {  // lane l: tokens l, and 63 - l for the sums from the end
+    const int t = c * CH + l, u = c * CH + 63 - l;
+    return make_uint2(t < n ? g_bits(a, row0 + t, h) : 0u, u < n ? g_bits(a, row0 + u, h) : 0u);
+  };
+  auto g_store = [&](int c, uint2 x) {
+    float* b = g_at(c);
+    if constexpr (OUT) {
+      double s = g_value(a, x.x);  // (differences of these go into exponents)
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const double y = __shfl_up(s, d);
+        s += l >= d ? y : 0.;
+      }
+      reinterpret_cast<double*>(b)[l] = s;
+      b[2 * CH + l] = a.scale * expf((float)s);
+    }
+    const float s = prefix_sum(g_value(a, x.y)), total = __shfl(s, 63);
+    b[3 * CH + 63 - l] = expf(dpp_rows<0x138, 0xF>(s));
+    const Decay d = decay_of(total);
+    if (l == 0) *reinterpret_cast<lf32x4*>(b + 4 * CH) = lf32x4{d.add, d.mul, total, 0.f};
+  };
+
+  const size_t hs = (size_t)V * K;
+  lf32x4 acc[U][KH][4];  // [tile][block of 64 keys][x]: element i is key 16 g + 4 i + x
+  const int v0 = 16 * U * wave;
+  auto state_at = [&](int u, int kh, int i) { return (size_t)(v0 + U * m + u) * K + 64 * kh + 16 * g + 4 * i; };
+  auto put = [&](float* dst) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<lf32x4*>(dst + state_at(u, kh, i)) =
+              lf32x4{acc[u][kh][0][i], acc[u][kh][1][i], acc[u][kh][2][i], acc[u][kh][3][i]};
+  };
+
+  const uint2 g0 = g_load(wave);
+  issue_k(0);
+  if constexpr (OUT) issue_q(0);
+  issue_v(0);
+  const float* s_in = nullptr;
+  if constexpr (OUT)
+    s_in = p.cut ? a.ends + ((size_t)p.slot * a.Hv + h) * hs
+                 : a.s_in != nullptr ? a.s_in + ((size_t)p.seq * a.Hv + h) * hs : nullptr;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lf32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (OUT && s_in != nullptr) x = *reinterpret_cast<const lf32x4*>(s_in + state_at(u, kh, i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[u][kh][e][i] = x[e];
+      }
+  g_store(wave, g0);
+  uint2 gv = g0;
+  float gsum = 0.f;
+  const bool keep = p.last && a.s_out != nullptr;
+
+  for (int c = 0; c < chunks; ++c) {
+    wait_loads<0>();  // chunk c is there, and nobody reads what the next loads overwrite
+    const int in_group = c % NW;
+    if (in_group == 0 && c + NW < chunks) gv = g_load(c + NW + wave);
+    issue_k(c + 1);
+    if constexpr (!OUT) issue_v(c + 1);
+    const uint8_t* ks = lds + (c & 1) * CH * C::KB;
+    const uint8_t* vs = lds + C::AT_V + (OUT ? 0 : (c & 1) * CH * C::VB);
+    const uint8_t* qs = lds + C::AT_Q;
+    uint8_t* ps = lds + C::AT_P + 16 * l;
+    const float* b = g_at(c);
+    float v[4][4][U];  // tokens 16 i + 4 g + e
+    auto read_v = [&] {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = (v0 + U * m) * 4;  // (a lane's U values lie in one chunk)
+          const uint8_t* src = vs + chunk_at<C::VB, float>(16 * i + 4 * g + e, at >> 4) + (at & 15);
+          if constexpr (U == 2) {
+            const float2 x = *reinterpret_cast<const float2*>(src);
+            v[i][e][0] = x.x, v[i][e][1] = x.y;
+          } else {
+            v[i][e][0] = *reinterpret_cast<const float*>(src);
+          }
+        }
+    };
+    if constexpr (OUT) {
+      // P^T's 10 tiles (s tile i, t tile j, i <= j), wave, wave + 4 and (waves 0, 1) wave + 8
+      lf32x4 d[3];
+      int ti[3], tj[3];
+#pragma unroll
+      for (int x = 0; x < 3; ++x) {
+        const int t = min(wave + 4 * x, 9);
+        tj[x] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
+        ti[x] = t - tj[x] * (tj[x] + 1) / 2;
+        d[x] = lf32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int kk = 0; kk < K / 16; ++kk) {
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+          const lf32x4 kf = *reinterpret_cast<const lf32x4*>(ks + 16 * ti[x] * C::KB + chunk_at<C::KB, float>(m, 4 * kk + g));
+          const lf32x4 qf = *reinterpret_cast<const lf32x4*>(qs + 16 * tj[x] * C::KB + chunk_at<C::KB, float>(m, 4 * kk + g));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[x] = mfma4(kf[e], qf[e], d[x]);
+        }
+      }
+      const double* pd = reinterpret_cast<const double*>(b);
+#pragma unroll
+      for (int x = 0; x < 3; ++x) {
+        const double gt = pd[16 * tj[x] + m];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // (a masked place's exponent may be of any size)
+          const float f = a.scale * __expf((float)(gt - pd[16 * ti[x] + 4 * g + e])) * d[x][e];
+          d[x][e] = 16 * ti[x] + 4 * g + e <= 16 * tj[x] + m ? f : 0.f;
+        }
+        if (x < 2 || wave < 2) *reinterpret_cast<lf32x4*>(ps + 1024 * (wave + 4 * x)) = d[x];
+      }
+      lf32x4 o[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[u][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lf32x4 qf[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            qf[j] = *reinterpret_cast<const lf32x4*>(qs + 16 * j * C::KB + chunk_at<C::KB, float>(m, 16 * kh + 4 * g + i));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int u = 0; u < U; ++u) o[u][j] = mfma4(acc[u][kh][e][i], qf[j][e], o[u][j]);
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = b[2 * CH + 16 * j + m];
+#pragma unroll
+        for (int u = 0; u < U; ++u) o[u][j] *= f;
+      }
+      read_v();
+      bool odd = false;  // (a comparison with a NaN is false)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int u = 0; u < U; ++u) odd |= !(fabsf(v[i][e][u]) < INFINITY);
+      const bool apart = __ballot(odd) != 0;
+      lds_barrier();  // P is there, and nobody reads q and v any more
+      issue_q(c + 1);
+      issue_v(c + 1);
+      auto p_frag = [&](int i, int j) { return *reinterpret_cast<const lf32x4*>(ps + 1024 * (j * (j + 1) / 2 + i)); };
+      if (!apart) {
+        lf32x4 pf[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = i; j < 4; ++j) pf[i][j] = p_frag(i, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = i; j < 4; ++j)
+#pragma unroll
+              for (int u = 0; u < U; ++u) o[u][j] = mfma4(v[i][e][u], pf[i][j][e], o[u][j]);
+      } else {
+        // an infinity or a NaN among the values: a masked P is zero, and zero times it NaN. Token by token, each added
+        // from its own row on
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i <= j; ++i) {
+            const lf32x4 pf = p_frag(i, j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int u = 0; u < U; ++u)
+#pragma unroll 1
+                for (int gg = 0; gg < 4; ++gg) {
+                  const lf32x4 y = mfma4(g == gg ? v[i][e][u] : 0.f, pf[e], lf32x4{0.f, 0.f, 0.f, 0.f});
+                  if (16 * i + 4 * gg + e <= 16 * j + m) o[u][j] += y;
+                }
+          }
+      }
+      // the lane holds values 4 U g .. + 4 U - 1 of the wave's, of token 16 j + m (rows behind the segment are dropped)
+      const uint32_t lb = (uint32_t)a.Hv * V * 4u;
+      const int rows = min(CH, n - c * CH);
+      const Rsrc rs = raw_rsrc(reinterpret_cast<float*>(a.o) + ((row0 + (size_t)c * CH) * a.Hv + h) * V,
+                               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows - 1) * lb + 4 * V)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+          lf32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = U == 2 ? o[e & 1][j][2 * y + (e >> 1)] : o[0][j][e];
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(lu32x4, w), rs,
+                                                 (uint32_t)(16 * j + m) * lb + 4 * (v0 + 4 * U * g + 4 * y), 0, 0);
+        }
+      if (c + 1 == chunks && !keep) break;
+    } else {
+      read_v();
+    }
+    const lf32x4 decay = *reinterpret_cast<const lf32x4*>(b + 4 * CH);
+    const Decay dc = {decay[0], decay[1]};
+    gsum += decay[2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[u][kh][x][i] = decayed(acc[u][kh][x][i], dc);
+    lf32x4 kf[2][KH];  // k's fragments, read one step ahead
+    auto k_read = [&](int x) {
+#pragma unroll
+      for (int kh = 0; kh < KH; ++kh)
+        kf[x & 1][kh] = *reinterpret_cast<const lf32x4*>(ks + chunk_at<C::KB, float>(16 * (x >> 2) + 4 * g + (x & 3), 16 * kh + m));
+    };
+    k_read(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const lf32x4 w = *reinterpret_cast<const lf32x4*>(b + 3 * CH + 16 * i + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[i][e][u] *= w[e];
+    }
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      fence();
+      if (x + 1 < 16) k_read(x + 1);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[u][kh][y] = mfma4(kf[x & 1][kh][y], v[x >> 2][x & 3][u], acc[u][kh][y]);
+    }
+    fence();
+    if (in_group == NW - 1 && c + 1 < chunks) g_store(c + 1 + wave, gv);
+  }
+  if constexpr (OUT) {
+    if (keep) put(a.s_out + ((size_t)p.seq * a.Hv + h) * hs);
+  } else {
+    const size_t at = (size_t)p.slot * a.Hv + h;
+    put(a.ends + at * hs);
+    if (wave == 0 && l == 0) a.gtot[at] = gsum;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (as above)
+}
+
 // The states before a sequence's runs, in place of what the runs add: c_0 the initial state, c_{j+1} = exp(G_j) c_j + E_j.
 // A thread keeps 4 elements, 8 runs loaded ahead.
 __global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a, int hs) {
-  const int per = hs / 1024, unit = blockIdx.x / per, part = blockIdx.x % per;
+  const int unit = blockIdx.x, part = blockIdx.y;
   const int seq = unit / a.Hv, h = unit - seq * a.Hv;
   int slot0 = 0, n = 0;
   if (a.cu == nullptr) {
@@ -1401,11 +1138,9 @@ bool lds_ready(F kernel, int bytes, std::atomic<signed char>* state) {
   return ok;
 }
 
-constexpr int STATE_NW = 4;  // waves (of 16 value rows) a workgroup of the state pass
-
 struct Plan {
-  int seg, run, seg_slots, run_slots, single;
-  size_t ckpt, gcum, ends, gtot, total;  // offsets into the workspace, its size
+  int run, run_slots, single;
+  size_t gtot, total;  // offset into the workspace (behind the segments' states), its size
 };
 
 // Value heads that a workgroup of the bf16 walk takes together: two of 64 columns where they share a key head.
@@ -1413,37 +1148,18 @@ int walk_heads(int Hk, int Hv, int V) { return V == 64 && Hv / Hk % 2 == 0 ? 2 :
 
 Plan make_plan(bool packed, int N, int T, int Hk, int Hv, int K, int V, int dtype) {
   Plan p;
-  const bool walk = dtype == ZGDN_BF16;
-  auto slots = [&](long size) {  // at most: a packed batch's sequences are not known here
-    return (int)(packed ? T / size + N : N * std::max(1L, (T + size - 1) / size));
-  };
-  if (walk) {
-    // Segments of a CU's share of the chunks. Half as long, two to a CU, costs 7 us at 4096 tokens of 16 heads of 128 x 128
-    // (states 12 us in the join instead of 7, 17 instead of 15 in the state pass, against 1 us less in the outputs) and
-    // gains 2 at 32768. Sequences that fill the CUs uncut are not cut below 1.5 shares: 32 of 64 .. 2048 tokens, 16 heads,
-    // take 180 us so, and 203 cut to 16 chunks (33 in the state pass and 13 in the join against 14 less in the outputs).
-    const long rows = packed ? T : (long)N * T, groups = Hv / walk_heads(Hk, Hv, V);
-    const long share = (rows * groups + CUS * CH - 1) / (CUS * CH);
-    const long seg = std::max(1L, N * groups >= CUS ? share + share / 2 : share) * CH;
-    p.seg = (int)std::min(seg, (long)INT32_MAX / 4);
-    p.run = p.seg;
-  } else {
-    p.seg = 64;
-    const int vg = V / (16 * STATE_NW);
-    p.run = (int)std::min((long)INT32_MAX / 128 * 64, std::max(1L, (T + 63L) / 64) * 64);
-    while (p.run > 4 * p.seg && (long)slots(p.run) * Hv * vg < 256) p.run = (p.run / p.seg + 1) / 2 * p.seg;
-  }
-  p.run_slots = slots(p.run);
-  p.seg_slots = slots(p.seg);
+  // Segments of a CU's share of the chunks. Half as long, two to a CU, costs 7 us at 4096 tokens of 16 heads of 128 x 128
+  // (states 12 us in the join instead of 7, 17 instead of 15 in the state pass, against 1 us less in the outputs) and
+  // gains 2 at 32768. Sequences that fill the CUs uncut are not cut below 1.5 shares: 32 of 64 .. 2048 tokens, 16 heads,
+  // take 180 us so, and 203 cut to 16 chunks (33 in the state pass and 13 in the join against 14 less in the outputs).
+  const long rows = packed ? T : (long)N * T, groups = dtype == ZGDN_BF16 ? Hv / walk_heads(Hk, Hv, V) : Hv;
+  const long share = (rows * groups + CUS * CH - 1) / (CUS * CH);
+  p.run = (int)std::min(std::max(1L, N * groups >= CUS ? share + share / 2 : share) * CH, (long)INT32_MAX / 4);
+  // (at most: a packed batch's sequences are not known here)
+  p.run_slots = (int)(packed ? T / p.run + (long)N : N * std::max(1L, ((long)T + p.run - 1) / p.run));
   p.single = T <= p.run;
-  const bool cut = !walk;
-  const size_t hs = (size_t)K * V * 4;
-  auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-  p.ckpt = 0;
-  p.gcum = p.ckpt + (cut ? (size_t)p.seg_slots * Hv * hs : 0);
-  p.ends = p.gcum + (cut ? round((size_t)p.seg_slots * Hv * 4) : 0);
-  p.gtot = p.ends + (p.single ? 0 : (size_t)p.run_slots * Hv * hs);
-  p.total = p.gtot + (p.single ? 0 : round((size_t)p.run_slots * Hv * 4));
+  p.gtot = p.single ? 0 : (size_t)p.run_slots * Hv * K * V * 4;
+  p.total = p.gtot + (p.single ? 0 : ((size_t)p.run_slots * Hv * 4 + 255) / 256 * 256);
   return p;
 }
 
@@ -1452,53 +1168,46 @@ bool sizes_ok(int Hk, int Hv, int K, int V, int dtype) {
          (dtype == ZGDN_F32 || dtype == ZGDN_BF16);
 }
 
-template <int K, int V, int NH>
-int launch_walk(const char* fn, const LinArgs& a, const Plan& p, hipStream_t s) {
-  using CO = WalkCfg<K, V, NH, true>;
-  using CS = WalkCfg<K, V, NH, false>;
-  static std::atomic<signed char> so[64], ss[64];
-  if (!lds_ready(lin_walk_kernel<K, V, NH, true>, CO::LDS, so) || !lds_ready(lin_walk_kernel<K, V, NH, false>, CS::LDS, ss))
+// The state pass over all segments but a sequence's last, the join, the walk over the outputs.
+template <typename FS, typename FO>
+int launch_walks(const char* fn, const LinArgs& a, const Plan& p, FS states, int states_lds, FO outputs, int outputs_lds,
+                 std::atomic<signed char>* ready, int groups, int threads, int state_size, hipStream_t s) {
+  if (!lds_ready(outputs, outputs_lds, ready) || !lds_ready(states, states_lds, ready + 64))
     return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
-  const int groups = a.Hv / NH;
-  const int before_last = a.cu != nullptr ? a.T / a.run : a.N * ((a.T + a.run - 1) / a.run - 1);  // segments, at most
-  if (!p.single)
-    hipLaunchKernelGGL((lin_walk_kernel<K, V, NH, false>), dim3((unsigned)(before_last * groups)), dim3(64 * CS::NW), CS::LDS, s, a);
-  if (!p.single)
-    hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)(a.N * a.Hv * (V * K / 1024))), dim3(256), 0, s, a, V * K);
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, NH, true>), dim3((unsigned)(p.seg_slots * groups)), dim3(64 * CO::NW), CO::LDS, s, a);
+  if (!p.single) {
+    const int before_last = a.cu != nullptr ? a.T / a.run : a.N * ((a.T + a.run - 1) / a.run - 1);  // segments, at most
+    hipLaunchKernelGGL(states, dim3((unsigned)(before_last * groups)), dim3(threads), states_lds, s, a);
+    hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)(a.N * a.Hv), (unsigned)(state_size / 1024)), dim3(256), 0, s, a, state_size);
+  }
+  hipLaunchKernelGGL(outputs, dim3((unsigned)(p.run_slots * groups)), dim3(threads), outputs_lds, s, a);
   return ZGDN_OK;
 }
 
-template <int K, int V>
+template <int K, int V, int NH>
 int launch_bf16(const char* fn, const LinArgs& a, const Plan& p, hipStream_t s) {
-  if constexpr (V == 64) {
-    if (walk_heads(a.Hk, a.Hv, V) == 2) return launch_walk<K, V, 2>(fn, a, p, s);
-  }
-  return launch_walk<K, V, 1>(fn, a, p, s);
+  using CO = WalkCfg<K, V, NH, true>;
+  using CS = WalkCfg<K, V, NH, false>;
+  static std::atomic<signed char> ready[128];
+  return launch_walks(fn, a, p, lin_walk_kernel<K, V, NH, false>, CS::LDS, lin_walk_kernel<K, V, NH, true>, CO::LDS, ready,
+                      a.Hv / NH, 64 * CO::NW, K * V, s);
 }
 
 template <int K, int V>
 int launch_f32(const char* fn, const LinArgs& a, const Plan& p, hipStream_t s) {
-  constexpr int NW = STATE_NW, VG = V / (16 * NW);
-  using CS = StateCfg<float, K, V, NW>;
-  using CO = OutCfg<float, K, V, 64>;
-  static std::atomic<signed char> so[64], ss[64];
-  if (!lds_ready(lin_out_kernel<float, K, V, 64>, CO::LDS, so) || !lds_ready(lin_state_kernel<float, K, V, NW>, CS::LDS, ss))
-    return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
-  if (a.s_out != nullptr || a.T > p.seg) {
-    const int units = p.run_slots * a.Hv;
-    hipLaunchKernelGGL((lin_state_kernel<float, K, V, NW>), dim3((unsigned)((units + 7) / 8 * 8 * VG)), dim3(64 * NW), CS::LDS, s, a);
-  }
-  if (!p.single)
-    hipLaunchKernelGGL(lin_carry_kernel, dim3((unsigned)(a.N * a.Hv * (V * K / 1024))), dim3(256), 0, s, a, V * K);
-  if (a.T > 0)
-    hipLaunchKernelGGL((lin_out_kernel<float, K, V, 64>), dim3((unsigned)(a.seg_slots * a.Hv)), dim3(64 * CO::NW), CO::LDS, s, a);
-  return ZGDN_OK;
+  using CO = Walk32Cfg<K, V, true>;
+  using CS = Walk32Cfg<K, V, false>;
+  static std::atomic<signed char> ready[128];
+  return launch_walks(fn, a, p, lin_walk_f32_kernel<K, V, false>, CS::LDS, lin_walk_f32_kernel<K, V, true>, CO::LDS, ready,
+                      a.Hv, 64 * CO::NW, K * V, s);
 }
 
 template <int K, int V>
 int launch_all(const char* fn, const LinArgs& a, const Plan& p, int dtype, hipStream_t s) {
-  return dtype == ZGDN_F32 ? launch_f32<K, V>(fn, a, p, s) : launch_bf16<K, V>(fn, a, p, s);
+  if (dtype == ZGDN_F32) return launch_f32<K, V>(fn, a, p, s);
+  if constexpr (V == 64) {
+    if (walk_heads(a.Hk, a.Hv, V) == 2) return launch_bf16<K, V, 2>(fn, a, p, s);
+  }
+  return launch_bf16<K, V, 1>(fn, a, p, s);
 }
 
 }  // namespace
@@ -1542,7 +1251,8 @@ extern "C" int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld,
     return fail(ZGDN_EINVAL, "%s: initial_state and final_state overlap without being the same", fn);
   if ((long)B * T > INT32_MAX) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x T=%d rows", fn, B, T);
   const Plan p = make_plan(cu_seqlens != nullptr, N, T, Hk, Hv, K, V, dtype);
-  if ((long)p.seg_slots * Hv > INT32_MAX / 16) return fail(ZGDN_EUNSUPPORTED, "%s: %d segments of %d heads", fn, p.seg_slots, Hv);
+  if ((long)p.run_slots * Hv >= 1 << 24)  // (a grid has 2^32 threads; slots: at least one a sequence)
+    return fail(ZGDN_EUNSUPPORTED, "%s: %d segments of %d heads", fn, p.run_slots, Hv);
   if (workspace_bytes < p.total || (workspace == nullptr && p.total > 0))
     return fail(ZGDN_EINVAL, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, p.total);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
@@ -1552,10 +1262,8 @@ extern "C" int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld,
   a.g_bf16 = g_dtype == ZGDN_BF16;
   a.s_in = initial_state, a.s_out = final_state, a.o = o, a.cu = cu_seqlens;
   a.N = N, a.T = T, a.Hk = Hk, a.Hv = Hv, a.scale = scale;
-  a.seg = p.seg, a.run = p.run, a.seg_slots = p.seg_slots, a.run_slots = p.run_slots;
-  a.direct = p.single;
-  a.save_first = initial_state != nullptr && initial_state == final_state;
-  a.ckpt = (float*)(ws + p.ckpt), a.gcum = (float*)(ws + p.gcum), a.ends = (float*)(ws + p.ends), a.gtot = (float*)(ws + p.gtot);
+  a.run = p.run, a.run_slots = p.run_slots;
+  a.ends = (float*)ws, a.gtot = (float*)(ws + p.gtot);
   hipStream_t hs = (hipStream_t)stream;
   const int st = K == 128 ? (V == 128 ? launch_all<128, 128>(fn, a, p, dtype, hs) : launch_all<128, 64>(fn, a, p, dtype, hs))
                           : (V == 128 ? launch_all<64, 128>(fn, a, p, dtype, hs) : launch_all<64, 64>(fn, a, p, dtype, hs));

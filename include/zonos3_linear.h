@@ -35,7 +35,7 @@ size_t zlin_attn_workspace_bytes(int packed, int n_seqs, int T, int Hk, int Hv, 
  *   aligned bases; at most 2^22). o is dense.
  *   g: g_ld == 0: float32 [Hv], one log decay a head. Else [B, T, Hv] in g_dtype, g_ld elements between tokens.
  *   initial_state [N, Hv, V, K] float32 or NULL (zeros); final_state likewise or NULL (not written). final_state may
- *   be initial_state itself (in place); they may not overlap otherwise.
+ *   be initial_state itself (in place). Otherwise o, final_state and the workspace may overlap no operand.
  *   cu_seqlens: int32 [n_seqs + 1] with B == 1, or NULL. Rows that belong to no sequence are left as they were.
  */
 int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
@@ -49,6 +49,7 @@ int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld, const void
  *   [B, Hv] in g_dtype, g_ld elements between streams.
  *   state [n_slots, Hv, V, K] float32. slots: NULL (stream b's state is row b; n_slots == B), or int64 [B]. A stream
  *   whose slot lies outside the table, or that an earlier stream of the call has, gets zeros in o and touches no state.
+ *   o and state may overlap no other operand.
  */
 int zlin_attn_step(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
                    const void* g, long g_ld, int g_dtype, float* state, const int64_t* slots, int n_slots, void* o,
@@ -58,7 +59,7 @@ int zlin_attn_step(const void* q, long q_ld, const void* k, long k_ld, const voi
  * y = act(x w^T + bias) + residual: x [M, K], w [N, K] (both bf16, rows x_ld and w_ld elements apart), bias [N] in
  * bias_dtype or NULL, residual [M, N] bf16 or NULL, y [M, N] bf16; products summed and the epilogue computed in float32,
  * rounded once. Any M, N, K and strides; rows that start on 16-byte boundaries take wide loads. y may be the residual
- * itself (same pointer and stride), and may overlap no other operand.
+ * itself (same pointer and stride); it may share no memory with another operand, but rows with it (columns beside its own).
  */
 int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld, const void* bias, int bias_dtype, int act,
                   const void* residual, long r_ld, void* y, long y_ld, int M, int N, int K, int dtype, void* stream);

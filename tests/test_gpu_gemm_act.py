@@ -173,3 +173,19 @@ def test_a_layer_of_linear_attention(gdn, cuda):
     err, mixer = (got.cpu().double() - want).norm(), (want - x.double()).norm()
     print(f"[errors] {float(err / mixer):.2e} of the mixer's part")
     assert float(err) <= 4 * 2.0**-7 * float(mixer) + 2.0**-8 * float(want.norm())
+
+
+def test_columns_beside_one_another(gdn, cuda):
+    """x, the residual and y as columns of one buffer's rows; the same columns are refused."""
+    announce("gemm_act columns of one buffer")
+    M, N, K = 70, 64, 128
+    x, w, b, r = _data(cuda, M, N, K, 9)
+    buf = torch.cat([x, r, torch.zeros_like(r)], 1)
+    y = buf[:, K + N:]
+    gdn.ops.gemm_act(buf[:, :K], w, bias=b, activation="silu", residual=buf[:, K: K + N], out=y)
+    torch.cuda.synchronize()
+    assert torch.equal(y, gdn.ops.gemm_act(x, w, bias=b, activation="silu", residual=r))
+    assert torch.equal(buf[:, :K], x) and torch.equal(buf[:, K: K + N], r)
+    for bad in (buf[:, :N], buf[:, K - 8: K - 8 + N], buf[:, K + 8: K + 8 + N]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            gdn.ops.gemm_act(buf[:, :K], w, residual=buf[:, K: K + N], out=bad)

@@ -167,3 +167,27 @@ def test_host_layer_refuses(gdn, cuda):
     refused("out", gemm, x, w, out=z(4, 16)[:, ::2])
     refused("out", gemm, x, w, out=z(4, 9))
     refused("w: expected", gemm, x, z(8, 17))
+
+
+def test_overlapping_operands_are_refused(native):
+    """Outputs that share memory with an input: refused, before any launch."""
+    at = lambda n: ctypes.c_void_p((1 << 24) + n)  # noqa: E731
+    MB = 1 << 20
+    need = native.lib().zlin_attn_workspace_bytes(0, 1, 300, 4, 4, 128, 128, 1)
+    fwd = dict(q=at(0), q_ld=512, k=at(MB), k_ld=512, v=at(2 * MB), v_ld=512, dtype=1, g=at(3 * MB), g_ld=4, g_dtype=0,
+               s_in=at(4 * MB), s_out=at(5 * MB), o=at(6 * MB), cu=None, n_seqs=0, B=1, T=300, Hk=4, Hv=4, K=128, V=128,
+               scale=1.0, ws=at(16 * MB), ws_bytes=need, stream=None)
+    _refused(native, "zlin_attn_fwd", fwd, [
+        (dict(o=at(2 * MB)), "overlap"), (dict(o=at(299 * 1024)), "overlap"), (dict(o=at(3 * MB + 16)), "overlap"),
+        (dict(o=at(5 * MB + 4 * 128 * 128 * 4 - 16)), "overlap"), (dict(s_out=at(MB)), "overlap"),
+        (dict(ws=at(2 * MB + 16)), "overlap"), (dict(o=at(4 * MB)), "overlap")])
+    step = dict(q=at(0), q_ld=512, k=at(MB), k_ld=512, v=at(2 * MB), v_ld=512, dtype=1, g=at(3 * MB), g_ld=0, g_dtype=0,
+                state=at(8 * MB), slots=None, n_slots=3, o=at(4 * MB), B=3, Hk=4, Hv=4, K=128, V=128, scale=1.0, stream=None)
+    _refused(native, "zlin_attn_step", step, [
+        (dict(o=at(2 * MB + 1024)), "overlap"), (dict(o=at(8 * MB)), "overlap"), (dict(state=at(MB - 16)), "overlap"),
+        (dict(slots=at(8 * MB + 8)), "overlap")])
+    gemm = dict(x=at(0), x_ld=512, w=at(MB), w_ld=256, bias=at(2 * MB), bias_dtype=0, act=2, res=at(3 * MB), r_ld=64,
+                y=at(4 * MB), y_ld=64, M=4, N=64, K=256, dtype=1, stream=None)
+    _refused(native, "zlin_gemm_act", gemm, [
+        (dict(y=at(0)), "overlap"), (dict(y=at(512), y_ld=512, K=257, w_ld=257), "overlap"), (dict(y=at(2 * MB - 2)), "overlap"),
+        (dict(y=at(3 * MB + 2)), "overlap"), (dict(y=at(3 * MB), y_ld=72), "overlap"), (dict(y=at(MB + 2 * 255)), "overlap")])

@@ -229,6 +229,21 @@ namespace zgdn {
 // Records a message for zgdn_last_error() and returns `code`.
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
+
+// Rows of `row` bytes, `ld` bytes apart.
+struct Region {
+  const void* at;
+  size_t rows, row, ld;
+};
+// Whether two of them meet in memory. Columns beside one another in rows of one stride do not.
+inline bool regions_meet(const Region& a, const Region& b) {
+  if (a.at == nullptr || b.at == nullptr || a.rows == 0 || b.rows == 0) return false;
+  const uintptr_t pa = (uintptr_t)a.at, pb = (uintptr_t)b.at;
+  if (pa + (a.rows - 1) * a.ld + a.row <= pb || pb + (b.rows - 1) * b.ld + b.row <= pa) return false;
+  if (a.ld != b.ld || a.row > a.ld || b.row > b.ld) return true;
+  const size_t d = (size_t)(pb >= pa ? (pb - pa) % a.ld : (a.ld - (pa - pb) % a.ld) % a.ld);  // b's column in a's rows
+  return d < a.row || d + b.row > a.ld;
+}
 // CUs of the current device (256 when it cannot be asked), asked once per device.
 int device_cus();
 

@@ -615,6 +615,12 @@ extern "C" int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld,
   if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 2048 ||
       (long)((M + 63) / 64) * ((N + 63) / 64) > INT32_MAX / 64)
     return fail(ZGDN_EUNSUPPORTED, "%s: M=%d N=%d K=%d", fn, M, N, K);
+  const Region ry = {y, (size_t)M, (size_t)N * 2, (size_t)y_ld * 2};
+  const size_t bias_bytes = (size_t)N * (bias_dtype == ZGDN_F32 ? 4 : 2);
+  if (regions_meet(ry, {x, (size_t)M, (size_t)K * 2, (size_t)x_ld * 2}) || regions_meet(ry, {w, (size_t)N, (size_t)K * 2, (size_t)w_ld * 2}) ||
+      regions_meet(ry, {bias, 1, bias_bytes, bias_bytes}) ||
+      (!(residual == y && r_ld == y_ld) && regions_meet(ry, {residual, (size_t)M, (size_t)N * 2, (size_t)r_ld * 2})))
+    return fail(ZGDN_EINVAL, "%s: y overlaps another operand (it may only be the residual itself)", fn);
   ActArgs a{(const uint16_t*)x, (const uint16_t*)w, x_ld, w_ld, bias, bias_dtype == ZGDN_BF16, act,
             (const uint16_t*)residual, residual != nullptr ? r_ld : 0, (uint16_t*)y, y_ld, M, N, K, 1, 0, 0};
   auto takes = [&](int n) {  // accesses of n elements of y and the residual

@@ -1255,6 +1255,16 @@ extern "C" int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld,
     return fail(ZGDN_EUNSUPPORTED, "%s: %d segments of %d heads", fn, p.run_slots, Hv);
   if (workspace_bytes < p.total || (workspace == nullptr && p.total > 0))
     return fail(ZGDN_EINVAL, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, p.total);
+  const size_t es = dtype == ZGDN_F32 ? 4 : 2, ge = g_dtype == ZGDN_F32 ? 4 : 2, rows = (size_t)B * T;
+  const Region out = {o, rows, (size_t)Hv * V * es, (size_t)Hv * V * es}, end = {final_state, 1, n_state * 4, n_state * 4},
+               work = {workspace, 1, p.total, p.total};
+  const Region in[] = {{q, rows, (size_t)Hk * K * es, q_ld * es}, {k, rows, (size_t)Hk * K * es, k_ld * es},
+                       {v, rows, (size_t)Hv * V * es, v_ld * es}, {g, g_ld == 0 ? 1 : rows, Hv * ge, g_ld == 0 ? Hv * ge : g_ld * ge},
+                       {cu_seqlens, 1, (size_t)(N + 1) * 4, (size_t)(N + 1) * 4}, {initial_state, 1, n_state * 4, n_state * 4}};
+  bool meet = regions_meet(out, end) || regions_meet(out, work) || regions_meet(end, work);
+  for (const Region& r : in)
+    meet = meet || regions_meet(out, r) || regions_meet(work, r) || (r.at != initial_state && regions_meet(end, r));
+  if (meet) return fail(ZGDN_EINVAL, "%s: o, final_state or the workspace overlap another operand", fn);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   LinArgs a{};
   a.q = q, a.k = k, a.v = v, a.g = g;

@@ -182,6 +182,15 @@ extern "C" int zlin_attn_step(const void* q, long q_ld, const void* k, long k_ld
     return fail(ZGDN_EINVAL, "%s: q, k, v, o and state need 16-byte aligned bases", fn);
   if ((long)B * Hv * V >= INT32_MAX) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Hv=%d x V=%d rows", fn, B, Hv, V);
   if (B == 0) return ZGDN_OK;
+  const size_t es = dtype == ZGDN_F32 ? 4 : 2, ge = g_dtype == ZGDN_F32 ? 4 : 2, n = (size_t)B;
+  const size_t table = (size_t)n_slots * Hv * V * K * 4;
+  const Region out = {o, n, (size_t)Hv * V * es, (size_t)Hv * V * es}, st = {state, 1, table, table};
+  const Region in[] = {{q, n, (size_t)Hk * K * es, q_ld * es}, {k, n, (size_t)Hk * K * es, k_ld * es},
+                       {v, n, (size_t)Hv * V * es, v_ld * es}, {g, g_ld == 0 ? 1 : n, Hv * ge, g_ld == 0 ? Hv * ge : g_ld * ge},
+                       {slots, 1, n * 8, n * 8}};
+  bool meet = regions_meet(out, st);
+  for (const Region& r : in) meet = meet || regions_meet(out, r) || regions_meet(st, r);
+  if (meet) return fail(ZGDN_EINVAL, "%s: o or state overlap another operand", fn);
   StepArgs a{q, k, v, g, q_ld, k_ld, v_ld, g_ld, g_dtype == ZGDN_BF16, state, slots, n_slots, o, B, Hk, Hv, V, 0, scale};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == ZGDN_F32)

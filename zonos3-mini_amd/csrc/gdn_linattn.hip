@@ -15,7 +15,7 @@
 // its own rounding and a state that of fp32 sums. fp32 inputs take the same steps on the fp32 MFMA.
 //
 // Measured (the three kernels, us): 32 packed prompts of 64 .. 2048 tokens, 16 heads of 128 x 128: 5 + 6 + 170; one of 4096:
-// 15 + 7 + 27; one of 32768, 16 heads of 128 x 64 on one key head: 39 + 9 + 92. What bounds it: a chunk's instructions, not
+// 14 + 8 + 25; one of 32768, 16 heads of 128 x 64 on one key head: 39 + 9 + 86. What bounds it: a chunk's instructions, not
 // its bytes (packed: 569 MB, 104 us at the rate of a copy).
 //
 // The exponents are sums of one sign where all g <= 0: suffix sums to a block's end and prefix sums from its start, not
@@ -178,6 +178,7 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
 // 16 bytes a lane from a buffer straight into LDS, lane i at lds + 16 i. In assembly, since the compiler waits for every such
 // load ahead of a transposing LDS read, whatever it reads: here the kernels' own waits are in charge. Nothing is written to a
 // register; M0 (which these kernels use for nothing else) needs a wait state before the load.
+typedef uint32_t lu32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_lds(lu32x4 rsrc, uint32_t off, const uint8_t* lds) {
   const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);  // (an address in LDS: the low half)
@@ -265,9 +266,10 @@ __device__ __forceinline__ float prefix_sum(float x) {
 // ------------------------------------------------------------------------------------------- bf16: a walk over chunks
 //
 // A workgroup walks the 64-token chunks of one segment of a sequence for NH value heads that share a key head (NH V = 64 or
-// 128 value columns, 32 a wave). A wave keeps its 32 value rows of S in registers, as transposed tiles [2][K / 16] (D: key
-// 32 (kt / 2) + 8 g + 4 (kt % 2) + e; value of lane m and half u: 8 (m / 4) + 4 u + m % 4): a pair of key tiles, split into
-// bf16 terms, is an MFMA operand with its keys in memory order, and both halves' rows of an output tile are 8 neighbours.
+// 128 value columns, 16 U a wave). A wave keeps its U halves of 16 value rows of S in registers, as transposed tiles
+// [U][K / 16] (D: key 32 (kt / 2) + 8 g + 4 (kt % 2) + e; value of lane m and half u: 8 (m / 4) + 4 u + m % 4, of one half m):
+// a pair of key tiles, split into bf16 terms, is an MFMA operand with its keys in memory order, and the halves' rows of an
+// output tile are 4 U neighbours.
 // A chunk:
 //   P^T [s, t] = K Q^T, scaled by exp(G_t - G_s) and masked, a few tiles a wave, as two bf16 terms into LDS for all;
 //   O^T [v, t] = exp(G_t) S Q^T + V^T P^T;
@@ -279,10 +281,13 @@ __device__ __forceinline__ float prefix_sum(float x) {
 // and stores 1500). The three terms of V' are 32 of the MFMAs and 100 of the others more than two would be; two where a
 // segment's end state is not kept took a second body of the loop and registers it did not have (97 spilled: 27 -> 32 us at
 // 4096 tokens). OUT false: the state alone.
+// U = 2 where workgroups share CUs, U = 1 where none has to: the same work by 8 waves, two on each SIMD, one of which computes
+// while the other waits (the three kernels, us, U 2 / 1: one prompt of 64 tokens 10.5 / 10.0, of 4096, 16 heads 50 / 48; two
+// workgroups of 8 waves would not fit a CU's registers).
 
-template <int K, int V, int NH, bool OUT>
+template <int K, int V, int NH, int U, bool OUT>
 struct WalkCfg {
-  static constexpr int WH = V / 32, NW = NH * WH;  // waves a head, in all
+  static constexpr int WH = V / (16 * U), NW = NH * WH;  // waves a head, in all
   static constexpr int KB = 2 * K, VB = 2 * NH * V;  // bytes of a row
   static constexpr int KI = CH * KB / 1024 / NW, VI = CH * VB / 1024 / NW;  // a wave's load instructions for k (q) and v
   static constexpr int P_TERM = OUT ? 6 * 1024 : 0;  // 16 x 32 blocks of P in fragment order: t tiles 0, 1 one, 2, 3 two
@@ -290,20 +295,28 @@ struct WalkCfg {
   static constexpr int G_FLOATS = 3 * CH + 4, G_BYTES = (GC + 1) * NH * G_FLOATS * 4;
   static constexpr int VS = OUT ? 1 : 2;  // stages of v (and q)
   static constexpr int REST = VS * CH * VB + (OUT ? CH * KB : 0) + NH * 2 * P_TERM + G_BYTES;
-  static constexpr int KS = REST + 2 * CH * KB <= 80 * 1024 ? 2 : 1;  // stages of k
+  static constexpr int LDS_MAX = (NW == 8 ? 160 : 80) * 1024;  // 8 waves a CU, in one workgroup or two
+  static constexpr int KS = REST + 2 * CH * KB <= LDS_MAX ? 2 : 1;  // stages of k
   static constexpr int AT_V = KS * CH * KB, AT_Q = AT_V + VS * CH * VB;
   static constexpr int AT_P = AT_Q + (OUT ? CH * KB : 0);
   static constexpr int AT_G = AT_P + NH * 2 * P_TERM;
   static constexpr int LDS = AT_G + G_BYTES;
-  static_assert(LDS <= 80 * 1024 && (OUT || KS == 2), "two workgroups a CU");
-  // P's tiles (s tile i, t tile j, i <= j) by wave of the head, 4 i + j each, a nibble a tile: those of a wave share rows
+  static_assert(LDS <= LDS_MAX && (OUT || KS == 2), "LDS");
+  // P's tiles (s tile i, t tile j, i <= j) by wave of the head, 4 i + j each, a nibble a tile, those of a wave in one row or
+  // column where they can be
+  static constexpr int MOST = WH == 8 ? 2 : WH == 4 ? 3 : 6;
   static constexpr uint32_t tiles(int w) {
-    return WH == 4 ? (w == 0 ? 0x73 : w == 1 ? 0xFB : w == 2 ? 0xA62 : 0x051) : (w == 0 ? 0xFB73 : 0x051A62);
+    return WH == 8 ? (w == 0 ? 0x0 : w == 1 ? 0x2 : w == 2 ? 0x3 : w == 3 ? 0x7 : w == 4 ? 0xB : w == 5 ? 0xF : w == 6 ? 0x51 : 0xA6)
+         : WH == 4 ? (w == 0 ? 0x73 : w == 1 ? 0xFB : w == 2 ? 0xA62 : 0x051)
+                   : (w == 0 ? 0xFB73 : 0x051A62);
   }
-  static constexpr int count(int w) { return WH == 4 ? (w < 2 ? 2 : 3) : (w == 0 ? 4 : 6); }
+  static constexpr int count(int w) { return WH == 8 ? (w < 6 ? 1 : 2) : WH == 4 ? (w < 2 ? 2 : 3) : (w == 0 ? 4 : 6); }
 };
 
-__device__ __forceinline__ int walk_row(int u, int m) { return 8 * (m >> 2) + 4 * u + (m & 3); }
+template <int U>
+__device__ __forceinline__ int walk_row(int u, int m) {
+  return U == 2 ? 8 * (m >> 2) + 4 * u + (m & 3) : m;
+}
 
 // The scheduler moves nothing across: regions of a few products and the other work that is to run beside them.
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
@@ -317,9 +330,9 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-template <int K, int V, int NH, bool OUT>
-__global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk_kernel(LinArgs a) {
-  using C = WalkCfg<K, V, NH, OUT>;
+template <int K, int V, int NH, int U, bool OUT>
+__global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_walk_kernel(LinArgs a) {
+  using C = WalkCfg<K, V, NH, U, OUT>;
   constexpr int NW = C::NW, WH = C::WH, KT = K / 16, KK = K / 32;
   extern __shared__ uint4 lin_lds[];
   uint8_t* lds = reinterpret_cast<uint8_t*>(lin_lds);
@@ -383,13 +396,13 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
   };
 
   const size_t hs = (size_t)V * K;
-  lf32x4 acc[2][KT];
+  lf32x4 acc[U][KT];
   // a state [V][K] of the head in memory: the lane's tiles are 4 floats each, pairs of them 8
-  const size_t lane_at = (size_t)(32 * wl + walk_row(0, m)) * K + 8 * g;
+  const size_t lane_at = (size_t)(16 * U * wl + walk_row<U>(0, m)) * K + 8 * g;
   auto state_at = [&](int u, int kt) { return lane_at + 4 * u * K + 32 * (kt >> 1) + 4 * (kt & 1); };
   auto put = [&](float* dst) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) *reinterpret_cast<lf32x4*>(dst + state_at(u, kt)) = acc[u][kt];
   };
@@ -399,7 +412,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
   if constexpr (OUT) issue_q(0);
   issue_v(0);
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) acc[u][kt] = lf32x4{0.f, 0.f, 0.f, 0.f};
   // the state before the segment: carried into it, or the initial one (a sequence of one segment)
@@ -410,7 +423,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
                                : nullptr;
     if (s_in != nullptr) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) acc[u][kt] = *reinterpret_cast<const lf32x4*>(s_in + state_at(u, kt));
     }
@@ -435,7 +448,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
     if constexpr (OUT) q_at.anew();
     // chunk c is there, and nobody reads what the next loads overwrite (the first chunk's state may still be on its way)
     if (OUT && c == 0 && s_in != nullptr)
-      wait_loads<2 * KT>();
+      wait_loads<U * KT>();
     else
       wait_loads<0>();
     const int in_group = c & (C::GC - 1);
@@ -447,21 +460,21 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
     const uint8_t* ks = lds + (C::KS == 2 ? (c & 1) * CH * C::KB : 0);
     const uint8_t* vs = lds + C::AT_V + (C::VS == 2 ? (c & 1) * CH * C::VB : 0);
     const float* b = g_at(c);
-    lf32x4 o[2][4];
-    lbf16x8 vf[2][2];  // the wave's columns of V^T: [half][block of 32 tokens]
+    lf32x4 o[U][4];
+    lbf16x8 vf[U][2];  // the wave's columns of V^T: [half][block of 32 tokens]
     auto read_v = [&] {
-      const int r = 4 * g + (m >> 2), col = (hh * V + 32 * wl) / 8 + (m & 3);
-      const uint8_t* at = vs + chunk_at<C::VB>(r, col);
+      const int r = 4 * g + (m >> 2), col = (hh * V + 16 * U * wl) / 8 + (U == 2 ? m & 3 : (m & 3) >> 1);
+      const uint8_t* at = vs + chunk_at<C::VB>(r, col) + (U == 2 ? 0 : 8 * (m & 1));
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
           const uint2 x = lds_tr(at + 32 * s * C::VB + 8 * u), y = lds_tr(at + (32 * s + 16) * C::VB + 8 * u);
           vf[u][s] = __builtin_bit_cast(lbf16x8, make_uint4(x.x, x.y, y.x, y.y));
         }
     };
     // V' in terms, a pair of tokens at a time: word i of half u in block s
-    uint32_t vt[2][2][NT][4];  // [block][half][term][word]
+    uint32_t vt[2][U][NT][4];  // [block][half][term][word]
     lf32x4 vw[2][2];          // the weights of a block's tokens (rows 4 g .., 16 + 4 g ..)
     auto read_weights = [&](int s) {
       vw[s][0] = *reinterpret_cast<const lf32x4*>(b + 2 * CH + 32 * s + 4 * g);
@@ -475,7 +488,9 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
 #pragma unroll
       for (int k = 0; k < NT; ++k) vt[s][u][k][i] = t[k];
     };
-    static_assert(!OUT || (C::KI + C::VI <= 2 * KK * NT && 4 * KK % C::KI == 0), "regions for the loads");
+    constexpr int SR = 2 * U;                   // regions of a step of S Q^T: a term of a half each
+    constexpr int XS = 3 - U, GX = 2 * KK / XS;  // the update's steps: pairs of key tiles at a time, steps in all
+    static_assert(!OUT || (C::KI + C::VI <= GX * NT && SR * KK % C::KI == 0), "regions for the loads");
     auto v_frag = [&](int s, int u, int k) {
       return __builtin_bit_cast(lbf16x8, make_uint4(vt[s][u][k][0], vt[s][u][k][1], vt[s][u][k][2], vt[s][u][k][3]));
     };
@@ -524,18 +539,29 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
           *reinterpret_cast<uint2*>(pl + C::P_TERM + at) = make_uint2(w0[1], w1[1]);
         }
       };
-      if (wl == 0)
-        p_tiles(std::integral_constant<int, 0>{});
-      else if (wl == 1)
-        p_tiles(std::integral_constant<int, 1>{});
-      else if constexpr (WH == 4) {
-        if (wl == 2)
-          p_tiles(std::integral_constant<int, 2>{});
-        else
-          p_tiles(std::integral_constant<int, 3>{});
+      switch (wl) {
+        case 0: p_tiles(std::integral_constant<int, 0>{}); break;
+        case 1: p_tiles(std::integral_constant<int, 1>{}); break;
+        case 2:
+          if constexpr (WH > 2) p_tiles(std::integral_constant<int, 2>{});
+          break;
+        case 3:
+          if constexpr (WH > 2) p_tiles(std::integral_constant<int, 3>{});
+          break;
+        case 4:
+          if constexpr (WH > 4) p_tiles(std::integral_constant<int, 4>{});
+          break;
+        case 5:
+          if constexpr (WH > 4) p_tiles(std::integral_constant<int, 5>{});
+          break;
+        case 6:
+          if constexpr (WH > 4) p_tiles(std::integral_constant<int, 6>{});
+          break;
+        default:
+          if constexpr (WH > 4) p_tiles(std::integral_constant<int, 7>{});
       }
       // O^T = S Q^T, the state in two terms; beside each step's products the next one's terms and V's of the first block
-      uint32_t st[2][2][2][4];  // [step % 2][half][term][word]
+      uint32_t st[2][U][2][4];  // [step % 2][half][term][word]
       lbf16x8 qf[2][4];
       auto q_read = [&](int kk) {
 #pragma unroll
@@ -554,11 +580,11 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
       read_v();
       read_weights(0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[u][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s_pair(0, u, i);
 #pragma unroll
@@ -566,9 +592,9 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
         fence();
         if (kk + 1 < KK) q_read(kk + 1);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {  // term 1 - r / 2 of half r % 2
+        for (int r = 0; r < SR; ++r) {  // term 1 - r / U of half r % U
           fence();
-          const int x = 1 - (r >> 1), u = r & 1;
+          const int x = 1 - r / U, u = r % U;
           const lbf16x8 sf = __builtin_bit_cast(lbf16x8, make_uint4(st[kk & 1][u][x][0], st[kk & 1][u][x][1], st[kk & 1][u][x][2], st[kk & 1][u][x][3]));
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[u][j] = mfma16(sf, qf[kk & 1][j], o[u][j]);
@@ -576,15 +602,11 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
             s_pair(kk + 1, r >> 1, 2 * (r & 1));
             s_pair(kk + 1, r >> 1, 2 * (r & 1) + 1);
           }
-          // (the 8 pairs of V' over the 4 KK regions)
-          if constexpr (KK == 4) {
-            if ((r & 1) == 0) v_pair(0, kk >> 1, 2 * (kk & 1) + (r >> 1));
-          } else {
-            v_pair(0, kk, r);
-          }
+          const int at = SR * kk + r;  // (the 4 U pairs of V' over the SR KK regions)
+          if (at * 2 % KK == 0) v_pair(0, at * 2 / KK >> 2, at * 2 / KK & 3);
           if constexpr (C::KS == 2) {  // the next k's loads, one at a time
-            constexpr int every = 4 * KK / C::KI;
-            if ((4 * kk + r) % every == 0) issue_k(c + 1, (4 * kk + r) / every, (4 * kk + r) / every + 1);
+            constexpr int every = SR * KK / C::KI;
+            if (at % every == 0) issue_k(c + 1, at / every, at / every + 1);
           }
           interleave<4, 5>();
         }
@@ -592,7 +614,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
       fence();
       // (formed here, although only the update needs them)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < NT; ++k)
           asm volatile("" : "+v"(vt[0][u][k][0]), "+v"(vt[0][u][k][1]), "+v"(vt[0][u][k][2]), "+v"(vt[0][u][k][3]));
@@ -600,12 +622,12 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
       for (int j = 0; j < 4; ++j) {
         const float f = b[CH + 16 * j + m];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) o[u][j] *= f;
+        for (int u = 0; u < U; ++u) o[u][j] *= f;
       }
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
       u16x2 top = {0, 0};  // the largest magnitude's bits
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const uint4 w = __builtin_bit_cast(uint4, vf[u][s]);
@@ -631,20 +653,29 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
 #pragma unroll
           for (int j = 2 * s; j < 4; ++j)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) o[u][j] = mfma16(vf[u][s], pf[s][j][x], o[u][j]);
+            for (int u = 0; u < U; ++u) o[u][j] = mfma16(vf[u][s], pf[s][j][x], o[u][j]);
           fence();
         };
         p_read(0);
+        if constexpr (U == 1) {
+          fence();
+          issue_q(c + 1, 0, C::KI);
+          issue_v(c + 1, 0, C::VI);
+        }
         pv(0, 1);  // (the small terms first)
         p_read(1);
         pv(0, 0);
         pv(1, 1);
         pv(1, 0);
       } else {
+        if constexpr (U == 1) {
+          issue_q(c + 1, 0, C::KI);
+          issue_v(c + 1, 0, C::VI);
+        }
         // an infinity or a NaN among the values: a masked P is zero, and zero times it NaN. Token by token, each added
         // from its own row on
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const uint4 all = __builtin_bit_cast(uint4, vf[u][s]);
@@ -665,21 +696,25 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
             }
           }
       }
-      // the lane holds values 8 g .. 8 g + 7 of the wave's, of token 16 j + m (rows behind the segment are dropped)
+      // the lane holds values 4 U g .. of the wave's, of token 16 j + m (rows behind the segment are dropped)
       const uint32_t lb = (uint32_t)a.Hv * V * 2u;
       const Rsrc rs = raw_rsrc(reinterpret_cast<uint16_t*>(a.o) + ((row0 + (size_t)c * CH) * a.Hv + h) * V,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows_of(c) - 1) * lb + 2 * V)));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const lu32x4 w = {pack_bf16x2(o[0][j][0], o[0][j][1]), pack_bf16x2(o[0][j][2], o[0][j][3]),
-                          pack_bf16x2(o[1][j][0], o[1][j][1]), pack_bf16x2(o[1][j][2], o[1][j][3])};
-        __builtin_amdgcn_raw_buffer_store_b128(w, rs, (uint32_t)(16 * j + m) * lb + 2 * (32 * wl + 8 * g), 0, 0);
+        const uint32_t at = (uint32_t)(16 * j + m) * lb + 2 * (16 * U * wl + 4 * U * g);
+        const uint32_t w0 = pack_bf16x2(o[0][j][0], o[0][j][1]), w1 = pack_bf16x2(o[0][j][2], o[0][j][3]);
+        if constexpr (U == 2)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              lu32x4{w0, w1, pack_bf16x2(o[1][j][0], o[1][j][1]), pack_bf16x2(o[1][j][2], o[1][j][3])}, rs, at, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b64(lu32x2{w0, w1}, rs, at, 0, 0);
       }
     } else {
       read_v();
       read_weights(0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v_pair(0, u, i);
     }
@@ -689,55 +724,59 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, OUT>::NW), 2) void lin_walk
     gsum += b[3 * CH + 1];
     const float add = b[3 * CH];
     read_weights(1);
-    lbf16x8 kf[2][2];  // [step % 2][tile of the pair]
-    auto k_read = [&](int x) {  // of step x: pair x % KK of block x / KK
+    lbf16x8 kf[2][XS][2];  // [step % 2][pair][tile of the pair]
+    auto k_read = [&](int x) {  // pair x of 2 KK: pair x % KK of block x / KK
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint8_t* at = ks + 32 * (x / KK) * C::KB + flip(at_tr, 4 * (x % KK)) + 8 * i;
         const uint2 y = lds_tr(at), z = lds_tr(at + 16 * C::KB);
-        kf[x & 1][i] = __builtin_bit_cast(lbf16x8, make_uint4(y.x, y.y, z.x, z.y));
+        kf[x / XS & 1][x % XS][i] = __builtin_bit_cast(lbf16x8, make_uint4(y.x, y.y, z.x, z.y));
       }
     };
-    auto decay = [&](int kk, int u) {
+    auto decay = [&](int y, int part) {  // of the tiles of step y, by halves
+      const int kk = XS * y + (U == 2 ? 0 : part), u = U == 2 ? part : 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[u][2 * kk + i][e] = fmaf(acc[u][2 * kk + i][e], add, acc[u][2 * kk + i][e]);
     };
     fence();
-    k_read(0);
+#pragma unroll
+    for (int x = 0; x < XS; ++x) k_read(x);
     decay(0, 0);
     decay(0, 1);
 #pragma unroll
-    for (int x = 0; x < 2 * KK; ++x) {
-      const int s = x / KK, kk = x % KK;
+    for (int y = 0; y < GX; ++y) {
+      const int s = 2 * y / GX;
       fence();
-      if (x + 1 < 2 * KK) k_read(x + 1);
+      if (y + 1 < GX) {
+#pragma unroll
+        for (int x = 0; x < XS; ++x) k_read(XS * (y + 1) + x);
+      }
 #pragma unroll
       for (int t = NT - 1; t >= 0; --t) {  // (the small terms first)
         fence();
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const lbf16x8 vfr = v_frag(s, u, t);
+        for (int x = 0; x < XS; ++x)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) acc[u][2 * kk + i] = mfma16(kf[x & 1][i], vfr, acc[u][2 * kk + i]);
-        }
-        if constexpr (OUT) {  // the next q's and v's loads, one at a time
-          const int i = x * NT + NT - 1 - t;
+          for (int u = 0; u < U; ++u) {
+            const lbf16x8 vfr = v_frag(s, u, t);
+            const int kk = (XS * y + x) % KK;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[u][2 * kk + i] = mfma16(kf[y & 1][x][i], vfr, acc[u][2 * kk + i]);
+          }
+        if constexpr (OUT && U == 2) {  // the next q's and v's loads, one at a time
+          const int i = y * NT + NT - 1 - t;
           if (i < C::KI)
             issue_q(c + 1, i, i + 1);
           else if (i < C::KI + C::VI)
             issue_v(c + 1, i - C::KI, i - C::KI + 1);
         }
         if (s == 0) {
-          if (kk + 1 < KK && t < 2) decay(kk + 1, t);
-          // (the 8 pairs of V' over the NT KK regions)
-          if constexpr (KK == 4) {
-            if (t < 2) v_pair(1, kk >> 1, 2 * (kk & 1) + t);
-          } else {
-            v_pair(1, kk, t);
-            if (t < 4 - NT) v_pair(1, kk, NT + t);
-          }
+          if (2 * (y + 1) < GX && t < 2) decay(y + 1, t);
+          constexpr int PER = 8 * U / GX;  // pairs of V' a step
+#pragma unroll
+          for (int q = t; q < PER; q += NT) v_pair(1, (PER * y + q) >> 2, (PER * y + q) & 3);
           interleave<4, 5>();
         }
       }
@@ -1183,12 +1222,12 @@ int launch_walks(const char* fn, const LinArgs& a, const Plan& p, FS states, int
   return ZGDN_OK;
 }
 
-template <int K, int V, int NH>
+template <int K, int V, int NH, int U>
 int launch_bf16(const char* fn, const LinArgs& a, const Plan& p, hipStream_t s) {
-  using CO = WalkCfg<K, V, NH, true>;
-  using CS = WalkCfg<K, V, NH, false>;
+  using CO = WalkCfg<K, V, NH, U, true>;
+  using CS = WalkCfg<K, V, NH, U, false>;
   static std::atomic<signed char> ready[128];
-  return launch_walks(fn, a, p, lin_walk_kernel<K, V, NH, false>, CS::LDS, lin_walk_kernel<K, V, NH, true>, CO::LDS, ready,
+  return launch_walks(fn, a, p, lin_walk_kernel<K, V, NH, U, false>, CS::LDS, lin_walk_kernel<K, V, NH, U, true>, CO::LDS, ready,
                       a.Hv / NH, 64 * CO::NW, K * V, s);
 }
 
@@ -1205,9 +1244,10 @@ template <int K, int V>
 int launch_all(const char* fn, const LinArgs& a, const Plan& p, int dtype, hipStream_t s) {
   if (dtype == ZGDN_F32) return launch_f32<K, V>(fn, a, p, s);
   if constexpr (V == 64) {
-    if (walk_heads(a.Hk, a.Hv, V) == 2) return launch_bf16<K, V, 2>(fn, a, p, s);
+    if (walk_heads(a.Hk, a.Hv, V) == 2)
+      return (long)p.run_slots * (a.Hv / 2) <= CUS ? launch_bf16<K, V, 2, 1>(fn, a, p, s) : launch_bf16<K, V, 2, 2>(fn, a, p, s);
   }
-  return launch_bf16<K, V, 1>(fn, a, p, s);
+  return (long)p.run_slots * a.Hv <= CUS ? launch_bf16<K, V, 1, 1>(fn, a, p, s) : launch_bf16<K, V, 1, 2>(fn, a, p, s);
 }
 
 }  // namespace

@@ -284,18 +284,21 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS, FOLD>::PER_CU)) v
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows - 1) * (uint32_t)a.y_ld * 2u + (uint32_t)a.N * 2u)));
       const Rsrc rr = raw_rsrc(a.res + (size_t)m0 * a.r_ld,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(rows - 1) * (uint32_t)a.r_ld * 2u + (uint32_t)a.N * 2u)));
+      au32x4 r[TN][TM];  // (all of a lane's, ahead of the first store: one wait for memory; 30526 x 1024 x 2048: 135 us half by half, 132 so)
+      if (a.res != nullptr) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j)
+            r[i][j] = __builtin_amdgcn_raw_buffer_load_b128(
+                rr, (uint32_t)(wm + 16 * j + m) * (uint32_t)a.r_ld * 2u + 2u * (n0 + wn + 32 * i + 8 * g), 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
         const int n = n0 + wn + 32 * i + 8 * g;
         float b[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) b[e] = a.bias != nullptr ? bias_at(a, n + e) : 0.f;
-        au32x4 r[TM];
-        if (a.res != nullptr) {
-#pragma unroll
-          for (int j = 0; j < TM; ++j)
-            r[j] = __builtin_amdgcn_raw_buffer_load_b128(rr, (uint32_t)(wm + 16 * j + m) * (uint32_t)a.r_ld * 2u + 2u * n, 0, 0);
-        }
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
           float c[8];
@@ -304,8 +307,8 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS, FOLD>::PER_CU)) v
           if (a.res != nullptr) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-              c[e] += __uint_as_float(r[j][e / 2] << 16);
-              c[e + 1] += __uint_as_float(r[j][e / 2] & 0xffff0000u);
+              c[e] += __uint_as_float(r[i][j][e / 2] << 16);
+              c[e + 1] += __uint_as_float(r[i][j][e / 2] & 0xffff0000u);
             }
           }
           const au32x4 y = {pack_bf16x2(c[0], c[1]), pack_bf16x2(c[2], c[3]), pack_bf16x2(c[4], c[5]), pack_bf16x2(c[6], c[7])};

@@ -189,3 +189,15 @@ def test_columns_beside_one_another(gdn, cuda):
     for bad in (buf[:, :N], buf[:, K - 8: K - 8 + N], buf[:, K + 8: K + 8 + N]):
         with pytest.raises(RuntimeError, match="overlap"):
             gdn.ops.gemm_act(buf[:, :K], w, residual=buf[:, K: K + N], out=bad)
+
+
+@pytest.mark.parametrize("M,N,K", [(1100, 17, 264), (1100, 17, 261), (2000, 8, 512), (900, 72, 520), (513, 130, 333), (40, 3, 2050),
+                                   (70, 600, 130), (129, 300, 190)])
+def test_few_columns_and_odd_rows(gdn, cuda, M, N, K):
+    """Tall products of few columns (fewer column tiles than XCDs), rows off 16-byte boundaries, K behind its last block."""
+    announce(f"gemm_act tall {M}x{N}x{K}")
+    x, w, b, r = _data(cuda, M, N, K, M + N + K)
+    _check(gdn.ops.gemm_act(x, w, bias=b, activation="relu", residual=r), x, w, b, "relu", r)
+    wide = torch.full((M, K + 3), float("nan"), dtype=BF, device=cuda)  # rows 2 bytes off, beside values that nobody may use
+    wide[:, 1: 1 + K] = x
+    _check(gdn.ops.gemm_act(wide[:, 1: 1 + K], w), x, w, None, None, None)

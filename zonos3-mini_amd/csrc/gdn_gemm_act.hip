@@ -349,7 +349,8 @@ __global__ __launch_bounds__(512, (2 * TileCfg<BM, BN, WM, NS, FOLD>::PER_CU)) v
 // SL = 128 / R elements, slice q to wave q % 8: such a call is the weights' way from memory and a few round trips, so each
 // wave keeps two slices of both operands on their way (direct-to-LDS, whole runs of 256 / R bytes of a row; chunk c of a
 // row at c ^ f(row)) and waits for nobody before its products. The 8 partial tiles are added in LDS in wave order. The row
-// tiles of one column tile run on one XCD and share its copy of the weights.
+// tiles of one column tile run on one XCD where they can, and share its copy of the weights (whole column tiles by XCD leave
+// most of the XCDs idle where there are fewer than 8: 21614 x 17 x 5168 307 us, 56 in runs of tiles).
 
 constexpr int RW = 8;  // waves
 template <int R>
@@ -363,18 +364,16 @@ struct SplitCfg {
 struct __attribute__((packed, aligned(2))) Packed8 {
   uint32_t w[4];
 };
-// 8 elements of a row from k on, wherever the row starts: zeros behind the rows and behind K.
-__device__ __forceinline__ uint4 fetch8(const uint16_t* base, long ld, int row, int rows, int k, int K) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (row >= rows || k >= K) return v;
-  const uint16_t* p = base + (size_t)row * ld + k;
-  if (k + 8 <= K) {
-    const Packed8 x = *reinterpret_cast<const Packed8*>(p);
-    return make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
-  }
+// 8 elements from p on, wherever that is; of these only `n` (zeros behind them).
+__device__ __forceinline__ uint4 fetch8(const uint16_t* p) {
+  const Packed8 x = *reinterpret_cast<const Packed8*>(p);
+  return make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+}
+__device__ __forceinline__ uint4 fetch8_upto(const uint16_t* p, int n) {
+  if (n >= 8) return fetch8(p);
   uint32_t u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = k + i < K ? p[i] : 0u;
+  for (int i = 0; i < 8; ++i) u[i] = i < n ? p[i] : 0u;
   return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
 }
 
@@ -384,9 +383,10 @@ __global__ __launch_bounds__(64 * RW) void gemm_act_split_kernel(ActArgs a) {
   using C = SplitCfg<R>;
   extern __shared__ uint4 act_lds[];
   uint8_t* lds = reinterpret_cast<uint8_t*>(act_lds);
-  const int grp = blockIdx.x / (8 * a.tiles_m), in = blockIdx.x - grp * 8 * a.tiles_m;
-  const int tn = grp * 8 + (in & 7), tm = in >> 3;
-  if (tn >= a.tiles_n) return;
+  // each XCD (workgroups go round-robin over the 8) takes a run of tiles, column tile by column tile
+  const int total = a.tiles_m * a.tiles_n, per = (total + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t >= total) return;
+  const int tn = t / a.tiles_m, tm = t - tn * a.tiles_m;
   const int wave = wave_id(), l = threadIdx.x & 63, m = l & 15, g = l >> 4;
   const int m0 = __builtin_amdgcn_readfirstlane(16 * R * tm), n0 = __builtin_amdgcn_readfirstlane(16 * R * tn);
   const au32x4 rx = rows_rsrc(a.x + (size_t)m0 * a.x_ld, a.x_ld, min(16 * R, a.M - m0), a.K);
@@ -400,8 +400,9 @@ __global__ __launch_bounds__(64 * RW) void gemm_act_split_kernel(ActArgs a) {
     for (int p = 0; p < 4; ++p) {  // 1 KiB: 64 / CH rows
       const int r = p * (64 / C::CH) + l / C::CH, c = (l % C::CH) ^ C::f(r);
       if constexpr (!WIDE) {
-        vw[p] = fetch8(a.w, a.w_ld, n0 + r, a.N, k0 + 8 * c, a.K);
-        vx[p] = fetch8(a.x, a.x_ld, m0 + r, a.M, k0 + 8 * c, a.K);
+        // (rows behind the last: the last, whose products nobody stores)
+        vw[p] = fetch8_upto(a.w + (size_t)min(n0 + r, a.N - 1) * a.w_ld + k0 + 8 * c, a.K - k0 - 8 * c);
+        vx[p] = fetch8_upto(a.x + (size_t)min(m0 + r, a.M - 1) * a.x_ld + k0 + 8 * c, a.K - k0 - 8 * c);
         continue;
       }
       const bool there = k0 + 8 * c < a.K;
@@ -472,14 +473,17 @@ __global__ __launch_bounds__(64 * RW) void gemm_act_split_kernel(ActArgs a) {
   }
 }
 
-// Any sizes and alignments: T x T tiles, 4 waves of T / 2 x T / 2, blocks of 64 of K through registers (loaded under the
-// products of the block before: 8 elements of a row at a time from wherever it starts, one by one at the end of K) into
-// LDS (128-byte rows, 16-byte chunks swizzled by row).
+// Any sizes and alignments: T x T tiles, 4 waves of T / 2 x T / 2, blocks of 64 of K through registers (loaded two blocks
+// ahead: 8 elements of a row at a time from wherever it starts, one by one at the end of K; rows behind the last: the last,
+// whose products nobody stores) into two stages of LDS (128-byte rows, 16-byte chunks swizzled by row).
 template <int T>
 __global__ __launch_bounds__(256) void gemm_act_any_kernel(ActArgs a) {
   constexpr int W = T / 32, L = T / 32;  // 16-row tiles a wave and side; 8-element pieces a thread and operand
-  __shared__ uint4 sx[T * 8], sw[T * 8];
-  const int n0 = (blockIdx.x % a.tiles_n) * T, m0 = (blockIdx.x / a.tiles_n) * T;
+  __shared__ uint4 sx[2][T * 8], sw[2][T * 8];
+  // each XCD takes a run of tiles, row tile by row tile
+  const int total = a.tiles_m * a.tiles_n, per = (total + 7) / 8, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (at >= total) return;
+  const int n0 = (at % a.tiles_n) * T, m0 = (at / a.tiles_n) * T;
   const int wave = wave_id(), l = threadIdx.x & 63, m = l & 15, g = l >> 4;
   const int wm = (wave & 1) * (T / 2), wn = (wave >> 1) * (T / 2);
   af32x4 acc[W][W];
@@ -487,39 +491,59 @@ __global__ __launch_bounds__(256) void gemm_act_any_kernel(ActArgs a) {
   for (int i = 0; i < W; ++i)
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[i][j] = af32x4{0.f, 0.f, 0.f, 0.f};
-  uint4 px[L], pw[L];
-  auto load = [&](int k0) {
+  const int c = threadIdx.x & 7;
+  const uint16_t *xp[L], *wp[L];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int e = threadIdx.x + 256 * i, r = e >> 3, c = e & 7;
-      px[i] = fetch8(a.x, a.x_ld, m0 + r, a.M, k0 + 8 * c, a.K);
-      pw[i] = fetch8(a.w, a.w_ld, n0 + r, a.N, k0 + 8 * c, a.K);
+  for (int i = 0; i < L; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i;
+    xp[i] = a.x + (size_t)min(m0 + r, a.M - 1) * a.x_ld + 8 * c;
+    wp[i] = a.w + (size_t)min(n0 + r, a.N - 1) * a.w_ld + 8 * c;
+  }
+  uint4 px[2][L], pw[2][L];
+  auto load = [&](int kb, int s) {
+    if (64 * kb + 64 <= a.K) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        px[s][i] = fetch8(xp[i] + 64 * kb);
+        pw[s][i] = fetch8(wp[i] + 64 * kb);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        px[s][i] = fetch8_upto(xp[i] + 64 * kb, a.K - 64 * kb - 8 * c);
+        pw[s][i] = fetch8_upto(wp[i] + 64 * kb, a.K - 64 * kb - 8 * c);
+      }
     }
   };
-  load(0);
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    __syncthreads();
+  const int nk = (a.K + 63) / 64;
+  auto block = [&](int kb, int s) {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const int e = threadIdx.x + 256 * i, r = e >> 3, c = e & 7;
-      sx[r * 8 + (c ^ fx(r))] = px[i];
-      sw[r * 8 + (c ^ fx(r))] = pw[i];
+      const int r = (threadIdx.x >> 3) + 32 * i;
+      sx[s][r * 8 + (c ^ fx(r))] = px[s][i];
+      sw[s][r * 8 + (c ^ fx(r))] = pw[s][i];
     }
-    __syncthreads();
-    if (k0 + 64 < a.K) load(k0 + 64);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the block is there, the other stage read by everybody
+    if (kb + 2 < nk) load(kb + 2, s);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int t = 0; t < 2; ++t) {
       abf16x8 fa[W], fb[W];
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        fa[i] = __builtin_bit_cast(abf16x8, sw[(wn + 16 * i + m) * 8 + ((4 * s + g) ^ fx(m))]);
-        fb[i] = __builtin_bit_cast(abf16x8, sx[(wm + 16 * i + m) * 8 + ((4 * s + g) ^ fx(m))]);
+        fa[i] = __builtin_bit_cast(abf16x8, sw[s][(wn + 16 * i + m) * 8 + ((4 * t + g) ^ fx(m))]);
+        fb[i] = __builtin_bit_cast(abf16x8, sx[s][(wm + 16 * i + m) * 8 + ((4 * t + g) ^ fx(m))]);
       }
 #pragma unroll
       for (int i = 0; i < W; ++i)
 #pragma unroll
         for (int j = 0; j < W; ++j) acc[i][j] = amfma(fa[i], fb[j], acc[i][j]);
     }
+  };
+  load(0, 0);
+  if (nk > 1) load(1, 1);
+  for (int kb = 0; kb < nk; kb += 2) {
+    block(kb, 0);
+    if (kb + 1 < nk) block(kb + 1, 1);
   }
   with_act(a.act, [&](auto act) {
 #pragma unroll
@@ -559,14 +583,14 @@ int launch_split(const char* fn, ActArgs a, hipStream_t s) {
   static std::atomic<signed char> state[64];
   if (!lds_ready(gemm_act_split_kernel<R, WIDE>, C::LDS, state)) return fail(ZGDN_EHIP, "%s: the device refused the LDS", fn);
   a.tiles_m = (a.M + 16 * R - 1) / (16 * R), a.tiles_n = (a.N + 16 * R - 1) / (16 * R);
-  hipLaunchKernelGGL((gemm_act_split_kernel<R, WIDE>), dim3((unsigned)((a.tiles_n + 7) / 8 * 8) * a.tiles_m), dim3(64 * RW), C::LDS, s, a);
+  hipLaunchKernelGGL((gemm_act_split_kernel<R, WIDE>), dim3((unsigned)(((long)a.tiles_m * a.tiles_n + 7) / 8 * 8)), dim3(64 * RW), C::LDS, s, a);
   return ZGDN_OK;
 }
 
 template <int T>
 int launch_any(ActArgs a, hipStream_t s) {
   a.tiles_m = (a.M + T - 1) / T, a.tiles_n = (a.N + T - 1) / T;
-  hipLaunchKernelGGL(gemm_act_any_kernel<T>, dim3((unsigned)a.tiles_m * a.tiles_n), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(gemm_act_any_kernel<T>, dim3((unsigned)(((long)a.tiles_m * a.tiles_n + 7) / 8 * 8)), dim3(256), 0, s, a);
   return ZGDN_OK;
 }
 

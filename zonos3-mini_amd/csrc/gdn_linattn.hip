@@ -280,7 +280,7 @@ __device__ __forceinline__ float prefix_sum(float x) {
 // 7500 with two (the rest: P's chain of reads, products, exponentials and writes, 1700; barriers and loads 1000; V^T P^T
 // and stores 1500). The three terms of V' are 32 of the MFMAs and 100 of the others more than two would be; two where a
 // segment's end state is not kept took a second body of the loop and registers it did not have (97 spilled: 27 -> 32 us at
-// 4096 tokens). OUT false: the state alone.
+// 4096 tokens; with U = 1, below, there was room and nothing gained). OUT false: the state alone.
 // U = 2 where workgroups share CUs, U = 1 where none has to: the same work by 8 waves, two on each SIMD, one of which computes
 // while the other waits (the three kernels, us, U 2 / 1: one prompt of 64 tokens 10.5 / 10.0, of 4096, 16 heads 50 / 48; two
 // workgroups of 8 waves would not fit a CU's registers).

@@ -303,3 +303,31 @@ def test_padded_batches_that_fill_the_device(gdn, cuda, B, T, Hk, Hv, K, V):
     """Batches of sequences of several chunks that are not cut."""
     announce(f"linear attn batch {B} x {T} {Hk}/{Hv} {K}x{V}")
     _check(gdn, cuda, L.inputs((B, T), Hk, Hv, K, V, B + T, BF, n_states=B, slow=0.2), msg=f"{B} x {T}")
+
+
+@pytest.mark.parametrize("K,V,Hk", [(64, 64, 8), (128, 128, 8), (128, 64, 4)])
+def test_nothing_leaks_in_batches_that_fill_the_device(gdn, cuda, K, V, Hk):
+    """Infinities and NaN in q, k and v of a few tokens of a large batch: what does not see them keeps its bits."""
+    announce(f"linear attn non-finite in a batch {Hk}/8 {K}x{V}")
+    B, T, Hv = 40, 170, 8
+    d = L.inputs((B, T), Hk, Hv, K, V, 5, BF, slow=0.1)
+    x = {n: d[n].to(cuda) for n in ("q", "k", "v", "g")}
+    o, s = gdn.ops.linear_attn_fwd(*x.values())
+    seen = torch.zeros(B, T, Hv, dtype=torch.bool, device=cuda)
+    y = {n: t.clone() for n, t in x.items()}
+    y["v"][3, 150, 2, 5] = math.inf
+    seen[3, 150:, 2] = True
+    y["v"][4, 64, 7] = math.nan
+    seen[4, 64:, 7] = True
+    y["k"][5, 100, 0, 1] = math.nan
+    seen[5, 100:, : Hv // Hk] = True
+    y["q"][7, 20, 1] = math.inf
+    seen[7, 20, Hv // Hk: 2 * (Hv // Hk)] = True
+    o2, s2 = gdn.ops.linear_attn_fwd(*y.values())
+    torch.cuda.synchronize()
+    assert torch.equal(o[~seen], o2[~seen]) and bool(torch.isfinite(o2[~seen].float()).all())
+    touched = torch.zeros(B, Hv, dtype=torch.bool, device=cuda)
+    touched[3, 2] = touched[4, 7] = True
+    touched[5, : Hv // Hk] = True
+    assert torch.equal(s[~touched], s2[~touched])
+    assert not bool(torch.isfinite(o2[4, 64:, 7].float()).any()) and not bool(torch.isfinite(o2[3, 150:, 2, 5].float()).any())

@@ -18,8 +18,10 @@
 // 14 + 8 + 25; one of 32768, 16 heads of 128 x 64 on one key head: 39 + 9 + 86. What bounds it: a chunk's instructions, not
 // its bytes (packed: 569 MB, 104 us at the rate of a copy).
 //
-// The exponents are sums of one sign where all g <= 0: suffix sums to a block's end and prefix sums from its start, not
-// differences of long sums. g is taken as at least -200 (exp(-200) is zero in fp32), so that -inf resets a state.
+// The exponents are sums within a chunk, prefix sums from its start and suffix sums to its end, of one sign where all g <= 0;
+// P's are differences of the prefix sums (fp32: formed in doubles; bf16: off by up to 2^-24 of the chunk's sum, which is
+// 2^-13 of a P, a thirtieth of an output's rounding, behind 10 resets in one chunk). g is taken as at least -200 (exp(-200) is
+// zero in fp32), so that -inf resets a state.
 #include <algorithm>
 #include <atomic>
 

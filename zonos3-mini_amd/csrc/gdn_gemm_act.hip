@@ -111,11 +111,6 @@ __device__ __forceinline__ au32x4 rows_rsrc(const uint16_t* p, long ld, int rows
                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 
-// 16 bytes a lane from a buffer straight into LDS (lane i at lds + 16 i), `k` bytes on from the lane's offset. In assembly:
-// the kernels' own waits count these loads. M0, which they use for nothing else, needs a wait state before the load.
-__device__ __forceinline__ void load_lds(au32x4 rsrc, uint32_t off, uint32_t k, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(rsrc), "s"(k) : "memory");
-}
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
 }

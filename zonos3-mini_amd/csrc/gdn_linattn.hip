@@ -177,15 +177,8 @@ __device__ __forceinline__ int chunk_at(int r, int c) {
   return r * ROWB + ((c ^ f) << 4);
 }
 
-// 16 bytes a lane from a buffer straight into LDS, lane i at lds + 16 i. In assembly, since the compiler waits for every such
-// load ahead of a transposing LDS read, whatever it reads: here the kernels' own waits are in charge. Nothing is written to a
-// register; M0 (which these kernels use for nothing else) needs a wait state before the load.
 typedef uint32_t lu32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void load_lds(lu32x4 rsrc, uint32_t off, const uint8_t* lds) {
-  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);  // (an address in LDS: the low half)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc) : "memory");
-}
 
 // ROWS rows of ROWB bytes from global memory (row stride ld_bytes, `rows` of them there, zeros behind them) into LDS, by
 // NW waves; each wave instruction fills 1 KiB, so a lane fetches the chunk that belongs at its place. The places in a row
@@ -222,7 +215,8 @@ __device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW, T>& at_row, con
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 #pragma unroll
   for (int i = i0; i < i1; ++i)
-    load_lds(rs, at_row.off[i % RowsAt<ROWB, NW, T>::PERIOD] + (uint32_t)(i * NW * RP) * ld_bytes, lds + 1024 * (i * NW + wave));
+    load_lds(rs, at_row.off[i % RowsAt<ROWB, NW, T>::PERIOD] + (uint32_t)(i * NW * RP) * ld_bytes,
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds + 1024 * (i * NW + wave))));  // (in LDS: the low half)
 }
 __device__ __forceinline__ uint2 lds_tr(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) lshort4*)p));

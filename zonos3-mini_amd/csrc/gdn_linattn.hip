@@ -386,9 +386,8 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
     }
     const float s = prefix_sum(g_value(a, x.down)), total = __shfl(s, 63);
     b[2 * CH + 63 - l] = expf(dpp_rows<0x138, 0xF>(s));
-    // S exp(G) as S + S expm1(G): of a slow decay the factor's own rounding, the same at every chunk, would grow with the
-    // length of the memory; of a fast one what is left is off by 2^-25 of what was
-    if (l == 0) *reinterpret_cast<float2*>(b + 3 * CH) = make_float2(expm1f(total), total);
+    const Decay d = decay_of(total);
+    if (l == 0) *reinterpret_cast<lf32x4*>(b + 3 * CH) = lf32x4{d.add, d.mul, total, 0.f};
   };
 
   const size_t hs = (size_t)V * K;
@@ -717,8 +716,9 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
     if (OUT && c + 1 == chunks && !keep) return;
     // S^T = exp(G_end) S^T + K^T V', a pair of key tiles at a time: beside the first block's products the decay of the next
     // pair and V' of the second block
-    gsum += b[3 * CH + 1];
-    const float add = b[3 * CH];
+    const lf32x4 all = *reinterpret_cast<const lf32x4*>(b + 3 * CH);
+    gsum += all[2];
+    const Decay dc = {all[0], all[1]};
     read_weights(1);
     lbf16x8 kf[2][XS][2];  // [step % 2][pair][tile of the pair]
     auto k_read = [&](int x) {  // pair x of 2 KK: pair x % KK of block x / KK
@@ -734,7 +734,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[u][2 * kk + i][e] = fmaf(acc[u][2 * kk + i][e], add, acc[u][2 * kk + i][e]);
+        for (int e = 0; e < 4; ++e) acc[u][2 * kk + i][e] = decayed(acc[u][2 * kk + i][e], dc);
     };
     fence();
 #pragma unroll

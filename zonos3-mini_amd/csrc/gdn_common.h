@@ -132,16 +132,17 @@ __device__ __forceinline__ Rsrc raw_rsrc(const void* p, uint32_t bytes) {
 // 16 bytes a lane from a buffer straight into LDS, lane i at lds + 16 i (rsrc: the words of a buffer resource; lds: an
 // address within LDS, wave-uniform). In assembly, since the compiler waits for every such load ahead of an LDS read it
 // cannot tell from it, whatever that reads: the waits of a kernel that uses this count these loads. Nothing is written to a
-// register. The compiler puts the address into M0, but it does not look into the text, so the wait states stand here: a
-// memory instruction reads a scalar five wait states after a vector instruction (a readfirstlane of the resource, right
-// before, perhaps) wrote it, and M0 one after a scalar one.
+// register. The compiler puts the address into M0, but it does not look into the text, where wait states are the author's:
+// one behind M0's move stands here. A scalar that a vector instruction wrote (readfirstlane) needs five: the callers form
+// resources from scalars alone, or long before (five states in every load: 1 % of the kernels' time), and a test reads the
+// built library's disassembly for any that are too near.
 typedef uint32_t RsrcWords __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_lds(RsrcWords rsrc, uint32_t off, uint32_t lds) {
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 // (`k` bytes on from the lane's offset, wave-uniform)
 __device__ __forceinline__ void load_lds(RsrcWords rsrc, uint32_t off, uint32_t k, uint32_t lds) {
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc), "s"(k), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc), "s"(k), "{m0}"(lds) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------ chunked prefill

@@ -208,6 +208,7 @@ __device__ __forceinline__ void load_rows(const RowsAt<ROWB, NW, T>& at_row, con
                                           uint8_t* lds, int wave, int i0 = 0, int i1 = ROWS * ROWB / 1024 / NW) {
   constexpr int RP = 1024 / ROWB;  // rows an instruction
   static_assert(ROWS % (RP * NW) == 0, "as many a wave");
+  // (formed by scalar instructions; a clamp of the rows to 0 .. 64 would be a vector one, with five wait states behind it)
   const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * ld_bytes + ROWB : 0u;
   const uint64_t at = (uint64_t)(uintptr_t)base;
   const lu32x4 rs = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
@@ -350,7 +351,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
   const uint8_t* qs = lds + C::AT_Q;
 
   const int chunks = (n + CH - 1) / CH;
-  auto rows_of = [&](int c) { return max(0, min(CH, n - c * CH)); };  // (behind the last chunk: none, zeros)
+  auto rows_of = [&](int c) { return min(CH, n - c * CH); };  // (behind the last chunk 0 and less: zeros)
   RowsAt<C::KB, NW> k_at((uint32_t)a.k_ld * 2u, wave), q_at((uint32_t)a.q_ld * 2u, wave);
   RowsAt<C::VB, NW> v_at((uint32_t)a.v_ld * 2u, wave);
   auto issue = [&](const uint16_t* x, long ld, const auto& lanes, auto row_bytes, int at, int c, int i0, int i1) {
@@ -837,7 +838,7 @@ __global__ __launch_bounds__(256, (K * V > 8192 ? 1 : 2)) void lin_walk_f32_kern
   RowsAt<C::KB, NW, float> k_at((uint32_t)a.k_ld * 4u, wave), q_at((uint32_t)a.q_ld * 4u, wave);
   RowsAt<C::VB, NW, float> v_at((uint32_t)a.v_ld * 4u, wave);
   auto issue = [&](const float* x, long ld, const auto& lanes, auto row_bytes, int at, int c) {
-    const int rows = max(0, min(CH, n - c * CH));  // (behind the last chunk: none, zeros)
+    const int rows = min(CH, n - c * CH);  // (behind the last chunk 0 and less: zeros)
     load_rows<decltype(row_bytes)::value, CH, NW>(lanes, x + (rows > 0 ? (size_t)c * CH : 0) * ld, (uint32_t)ld * 4u, rows, lds + at, wave);
   };
   auto issue_k = [&](int c) { issue(kp, a.k_ld, k_at, std::integral_constant<int, C::KB>{}, (c & 1) * CH * C::KB, c); };

@@ -27,6 +27,21 @@ def _quiet(B, T, Hk, Hv, K, V, seed, dtype):
     return d
 
 
+SMALLEST = 2.0**-126  # fp32's least normal number: exp(-150) times anything of a test's size lies below, and below it a
+# value has no 24 bits (and a matrix product may take it as zero): nothing smaller is held to a relative bound
+
+
+def _hold(gdn, cuda, d, dtype):
+    T, K = d["q"].shape[1], d["q"].shape[3]
+    o, s = gdn.ops.linear_attn_fwd(*(d[n].to(cuda) for n in ("q", "k", "v", "g")))
+    torch.cuda.synchronize()
+    o_ref, s_ref, o_mag, s_mag = L.tokens(d["q"], d["k"], d["v"], d["g"])
+    eo = L.within(o, o_ref, L.out_bound(o_ref, o_mag, dtype, T, K) + SMALLEST)
+    es = L.within(s, s_ref, L.state_bound(s_mag, T) + SMALLEST)
+    print(f"[errors] outputs {eo:.3f}, states {es:.3f} of their bounds")
+    assert eo <= 1 and es <= 1, (eo, es)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("B,T,Hk,Hv,K,V", [(32, 192, 8, 8, 64, 64), (40, 192, 8, 8, 128, 64), (2, 200, 2, 8, 128, 128),
                                            (1, 1280, 8, 64, 64, 128)])
@@ -34,12 +49,7 @@ def test_what_is_left_behind_strong_decays(gdn, cuda, B, T, Hk, Hv, K, V, dtype)
     """Sequences walked whole by 8 and by 4 waves, in segments of one chunk and of five."""
     announce(f"linear attn quiet tail {B} x {T} {Hk}/{Hv} {K}x{V} {dtype}")
     d = _quiet(B, T, Hk, Hv, K, V, B + T, dtype)
-    o, s = gdn.ops.linear_attn_fwd(*(d[n].to(cuda) for n in ("q", "k", "v", "g")))
-    torch.cuda.synchronize()
-    o_ref, s_ref, o_mag, s_mag = L.tokens(d["q"], d["k"], d["v"], d["g"])
-    eo, es = L.within(o, o_ref, L.out_bound(o_ref, o_mag, dtype, T, K)), L.within(s, s_ref, L.state_bound(s_mag, T))
-    print(f"[errors] outputs {eo:.3f}, states {es:.3f} of their bounds")
-    assert eo <= 1 and es <= 1, (eo, es)
+    _hold(gdn, cuda, d, dtype)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -55,3 +65,20 @@ def test_a_quiet_prompt_and_quiet_steps_agree(gdn, cuda, dtype):
     torch.cuda.synchronize()
     mag = L.tokens(*(d[n] for n in ("q", "k", "v", "g")))[3]
     assert L.within(s, at.double().cpu(), 2 * L.state_bound(mag, T)) <= 1
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,H", [(2, 150, 2), (40, 128, 8)])
+@pytest.mark.parametrize("low", [float("-inf"), -150.0, -20.0])
+def test_slow_tokens_behind_many_fast_ones(gdn, cuda, low, B, T, H, dtype):
+    """Dozens of resets, or of decays nearly as strong, in a chunk and a run of slow tokens behind them: the weights of those
+    among one another are as exact as anywhere. Keys and queries near one direction, so that every token has its part in an
+    output, values of both signs, so that outputs are smaller than their parts."""
+    announce(f"linear attn {low} and slow, {B} x {T} {H} {dtype}")
+    d = L.inputs((B, T), H, H, 64, 64, 17, dtype)
+    one = torch.nn.functional.normalize(torch.randn(64, generator=torch.Generator().manual_seed(1)), dim=0)
+    for n in ("q", "k"):
+        d[n] = torch.nn.functional.normalize(one + 0.3 * d[n].float(), dim=-1).to(dtype)
+    at = torch.arange(T) % 64
+    d["g"] = torch.where((at < 48)[None, :, None], torch.full((), low), 0.05 * d["g"])
+    _hold(gdn, cuda, d, dtype)

@@ -19,9 +19,10 @@
 // its bytes (packed: 569 MB, 104 us at the rate of a copy).
 //
 // The exponents are sums within a chunk, prefix sums from its start and suffix sums to its end, of one sign where all g <= 0;
-// P's are differences of the prefix sums (fp32: formed in doubles; bf16: off by up to 2^-24 of the chunk's sum, which is
-// 2^-13 of a P, a thirtieth of an output's rounding, behind 10 resets in one chunk). g is taken as at least -200 (exp(-200) is
-// zero in fp32), so that -inf resets a state.
+// P's are differences of the prefix sums. These are held so that many strong decays do not cost the slow ones behind
+// them their digits: in doubles for fp32, for bf16 as sums of whole numbers (exact) and of what is left of each decay (at
+// most 32 in all: a difference is off by 2^-18 at most; as plain fp32 sums 48 resets left 2^-11, outputs up to 10 times their
+// bound off). g is taken as at least -200 (exp(-200) is zero in fp32), so that -inf resets a state.
 #include <algorithm>
 #include <atomic>
 
@@ -380,10 +381,10 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
   };
   auto g_store = [&](int c, const G2& x) {
     float* b = g_at(c);
-    if constexpr (OUT) {
-      const float s = prefix_sum(g_value(a, x.up));
-      b[l] = s;
-      b[CH + l] = a.scale * expf(s);
+    if constexpr (OUT) {  // (whole numbers and what is left of them: sums of the first are exact, those of the second small)
+      const float up = g_value(a, x.up), whole = rintf(up);
+      b[l] = prefix_sum(whole);
+      b[CH + l] = prefix_sum(up - whole);
     }
     const float s = prefix_sum(g_value(a, x.down)), total = __shfl(s, 63);
     b[2 * CH + 63 - l] = expf(dpp_rows<0x138, 0xF>(s));
@@ -519,11 +520,11 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
 #pragma unroll
         for (int x = 0; x < CNT; ++x) {
           const int i = (CODE >> (4 * x) & 15) >> 2, j = CODE >> (4 * x) & 3;
-          const lf32x4 gs = *reinterpret_cast<const lf32x4*>(b + 16 * i + 4 * g);
-          const float gt = b[16 * j + m];
+          const lf32x4 ws = *reinterpret_cast<const lf32x4*>(b + 16 * i + 4 * g), rs = *reinterpret_cast<const lf32x4*>(b + CH + 16 * i + 4 * g);
+          const float wt = b[16 * j + m], rt = b[CH + 16 * j + m];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            d[x][e] *= a.scale * __expf(gt - gs[e]);
+            d[x][e] *= a.scale * __expf((wt - ws[e]) + (rt - rs[e]));
             if (i == j) d[x][e] = 4 * g + e <= m ? d[x][e] : 0.f;
           }
           uint32_t w0[2], w1[2];
@@ -616,7 +617,7 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
           asm volatile("" : "+v"(vt[0][u][k][0]), "+v"(vt[0][u][k][1]), "+v"(vt[0][u][k][2]), "+v"(vt[0][u][k][3]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float f = b[CH + 16 * j + m];
+        const float f = a.scale * __expf(b[16 * j + m] + b[CH + 16 * j + m]);
 #pragma unroll
         for (int u = 0; u < U; ++u) o[u][j] *= f;
       }

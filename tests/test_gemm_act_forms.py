@@ -1,0 +1,55 @@
+"""Which kernel ``gemm_act`` takes for a product (the library's own query; without a GPU the rule counts 256 CUs), on the CPU."""
+
+from __future__ import annotations
+
+import ctypes
+import importlib
+import random
+
+import pytest
+
+# The forms' codes, with their tiles' rows and columns and a workgroup's threads.
+FORMS = {1: (16, 16, 512), 2: (32, 32, 512), 3: (64, 128, 512), 4: (128, 128, 512), 5: (128, 128, 512), 6: (128, 256, 512),
+         7: (256, 256, 512), 8: (64, 64, 256), 9: (128, 128, 256)}
+
+
+@pytest.fixture(scope="module")
+def native():
+    return importlib.import_module("zonos3-mini_amd._native")
+
+
+def form(native, M, N, K, wide=True):
+    """(form, workgroups)."""
+    groups = ctypes.c_int64(-1)
+    return native.lib().zgdn_gemm_act_form(M, N, K, int(wide), ctypes.byref(groups)), groups.value
+
+
+@pytest.mark.parametrize("wide", [True, False])
+def test_grids_hold_their_tiles(native, wide):
+    """Products of any size: a grid of fewer than 2^32 threads that holds every tile, or no form at all."""
+    rng = random.Random(5)
+    sizes = [(2**29, 8, 8), (2**30, 1, 8), (2**31 - 257, 1, 1), (8, 2**29, 8), (1, 2**31 - 257, 16), (2**20, 2**16, 8),
+             (2**25, 2**10, 64), (2**18, 2**18, 2**15), (2**30, 2**30, 8)]
+    sizes += [tuple(int(2 ** rng.uniform(0, 30.9)) for _ in range(3)) for _ in range(2000)]
+    refused = 0
+    for M, N, K in sizes:
+        f, groups = form(native, M, N, K, wide)
+        if f == 0:
+            refused += 1
+            assert -(-M // 64) * -(-N // 64) > 2**23  # (fewer always fit)
+            continue
+        rows, cols, threads = FORMS[f]
+        assert wide == (f < 8) or f <= 2
+        assert groups * threads < 2**32 and groups % 8 == 0
+        tiles = -(-M // rows) * (N // cols if f == 5 else -(-N // cols))
+        assert 0 <= groups - tiles < 8, (M, N, K, f, groups)
+        if f == 5:
+            assert 0 < N % 128 <= 16 and N // 128 >= 8
+    assert 0 < refused < len(sizes)
+    assert form(native, 2**29, 8, 8, wide)[0] and form(native, 2**30, 1, 8, wide)[0]
+
+
+def test_products_without_a_form_are_refused(native):
+    at = [ctypes.c_void_p(1 << n) for n in (20, 40, 60)]  # never read
+    with pytest.raises(RuntimeError, match="more tiles than a grid holds"):
+        native.call("zlin_gemm_act", at[0], 8, at[1], 8, None, 0, 0, None, 0, at[2], 1 << 30, 1 << 30, 1 << 30, 8, 1, None)

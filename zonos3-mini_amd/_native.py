@@ -111,6 +111,7 @@ LINEAR: dict[str, tuple] = {
 INTERNAL: dict[str, tuple] = {
     "zgdn_chunk32_slices": (c_int, [c_int, c_int, c_int, c_int]),
     "zgdn_gemm_rows": (c_int, [_P, c_long, _P, _P, c_long, c_int, c_int, c_int, c_int, _P]),
+    "zgdn_gemm_act_form": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(ctypes.c_int64)]),
     "zgdn_serving_gather": (
         c_int, [_P, _P, c_int, c_int, _P, c_int, c_int, c_int, c_int, c_int, _P, _P]),
     "zgdn_serving_extend_workspace": (c_size_t, [c_int, c_int, c_int]),

@@ -589,18 +589,6 @@ int launch_any(ActArgs a, hipStream_t s) {
   return ZGDN_OK;
 }
 
-// Which form takes the least time, by what each was measured to take (us, MI355X, graph replays): a fixed part and, a round
-// of workgroups over the CUs, a part for each block of K. `one`, `all`: with one workgroup a CU, with all that fit.
-struct Form {
-  int bm, bn, bk, per_cu;
-  double fixed, round, one, all;
-};
-double form_us(const Form& f, long M, long N, long K, long n_cu) {
-  const long tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn), blocks = (K + f.bk - 1) / f.bk;
-  const long rounds = (tiles + n_cu * f.per_cu - 1) / (n_cu * f.per_cu);
-  return f.fixed + rounds * f.round + blocks * (tiles <= n_cu ? f.one : rounds * f.all);
-}
-
 template <int BM, int BN, int WM, int NS, bool FOLD = false>
 int launch_tiles(const char* fn, ActArgs a, hipStream_t s) {
   using C = TileCfg<BM, BN, WM, NS, FOLD>;
@@ -611,6 +599,60 @@ int launch_tiles(const char* fn, ActArgs a, hipStream_t s) {
   const long per = ((long)a.tiles_m * a.tiles_n + 7) / 8;
   hipLaunchKernelGGL((gemm_act_tile_kernel<BM, BN, WM, NS, FOLD>), dim3((unsigned)(8 * per)), dim3(512), C::LDS, s, a);
   return ZGDN_OK;
+}
+
+// Which form takes the least time, by what each was measured to take (us, MI355X, graph replays): a fixed part and, a round
+// of workgroups over the CUs, a part for each block of K. `one`, `all`: with one workgroup a CU, with all that fit.
+struct Form {
+  int bm, bn, bk, per_cu, threads;
+  double fixed, round, one, all;
+};
+enum FormCode { F_NONE, F_SPLIT16, F_SPLIT32, F_TILE64, F_TILE128, F_FOLD, F_WIDE, F_TILE256, F_ANY64, F_ANY128, F_COUNT };
+// The fit's points (M x N x K, us), the form taken and the next best: 4 x 2056 x 1024 3.4 split 1, 4.0 split 2;
+// 64 x 1024 x 2048 4.4 split 1, 4.9 split 2; 64 x 2056 x 1024 4.1 split 2, 6.1 split 1; 200 x 1024 x 2048 5.5 split 2,
+// 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 2; 1000 x 2056 x 1024 12.4 tile 64 x 128, 13.9 128 x
+// 128; 4096 x 2056 x 1024 23.8 tile 128 x 128 (its last 8 columns folded), 29.6 256 x 256; 30526 x 1024 x 2048 113
+// tile 256 x 256, 134 128 x 128 and 128 x 256.
+constexpr Form FORMS[F_COUNT] = {
+    {},
+    {16, 16, 1024, 1, 512, 1.5, 1.0, 0.6, 0.6},
+    {32, 32, 512, 1, 512, 1.5, 1.0, 0.7, 0.7},
+    {64, 128, 64, 2, 512, 3.0, 0.0, 0.275, 0.52},
+    {128, 128, 64, 2, 512, 3.0, 0.0, 0.66, 1.15},
+    {128, 128, 64, 2, 512, 3.0, 0.0, 0.66, 1.15},
+    {128, 256, 64, 1, 512, 3.0, 0.0, 0.96, 0.98},
+    {256, 256, 64, 1, 512, 3.0, 0.0, 1.62, 1.65},
+    {64, 64, 64, 2, 256, 3.0, 0.0, 0.75, 1.0},
+    {128, 128, 64, 1, 256, 3.0, 0.0, 1.2, 1.2},
+};
+constexpr double NEVER = 1e300;
+
+// Columns behind the last whole tile of 128 that the tiles before them form as well (see gemm_act_tile_kernel); else 0.
+int folded(int N) {
+  const int over = N % 128;
+  return over <= 16 && N / 128 >= 8 ? over : 0;
+}
+long workgroups(const Form& f, long M, long cols) {  // (whole rounds over the 8 XCDs)
+  return (((M + f.bm - 1) / f.bm) * ((cols + f.bn - 1) / f.bn) + 7) / 8 * 8;
+}
+double form_us(const Form& f, long M, long cols, long K, long n_cu) {
+  if (workgroups(f, M, cols) * f.threads >= 1L << 32) return NEVER;  // (a grid has fewer than 2^32 threads)
+  const long tiles = ((M + f.bm - 1) / f.bm) * ((cols + f.bn - 1) / f.bn), blocks = (K + f.bk - 1) / f.bk;
+  const long rounds = (tiles + n_cu * f.per_cu - 1) / (n_cu * f.per_cu);
+  return f.fixed + rounds * f.round + blocks * (tiles <= n_cu ? f.one : rounds * f.all);
+}
+// The form of a product, F_NONE where none fits a grid. wide: rows on 16-byte boundaries (the forms with direct loads).
+int choose(int M, int N, int K, bool wide, long n_cu) {
+  int best = F_NONE;
+  double least = NEVER;
+  for (int f = F_SPLIT16; f < F_COUNT; ++f) {
+    const bool split = f <= F_SPLIT32;
+    if (f == F_FOLD ? !folded(N) : f == F_TILE128 && folded(N)) continue;
+    if (!split && wide != (f < F_ANY64)) continue;
+    const double us = (split && !wide ? 2.1 : 1.0) * form_us(FORMS[f], M, f == F_FOLD ? N - folded(N) : N, K, n_cu);
+    if (us < least) least = us, best = f;
+  }
+  return best;
 }
 
 }  // namespace
@@ -634,8 +676,7 @@ extern "C" int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld,
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)residual) % 2 ||
       (uintptr_t)bias % (bias_dtype == ZGDN_F32 ? 4 : 2))
     return fail(ZGDN_EINVAL, "%s: pointers off their element's boundary", fn);
-  if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 2048 ||
-      (long)((M + 63) / 64) * ((N + 63) / 64) > INT32_MAX / 64)
+  if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 2048)
     return fail(ZGDN_EUNSUPPORTED, "%s: M=%d N=%d K=%d", fn, M, N, K);
   const Region ry = {y, (size_t)M, (size_t)N * 2, (size_t)y_ld * 2};
   const size_t bias_bytes = (size_t)N * (bias_dtype == ZGDN_F32 ? 4 : 2);
@@ -655,35 +696,27 @@ extern "C" int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld,
   if (y_ld >= (1 << 21) || r_ld >= (1 << 21)) a.vec = std::min(a.vec, 4);  // (likewise for the whole tiles' stores)
   hipStream_t s = (hipStream_t)stream;
   int st = ZGDN_OK;
-  // The fit's points (M x N x K, us), the form taken and the next best: 4 x 2056 x 1024 3.4 split 1, 4.0 split 2;
-  // 64 x 1024 x 2048 4.4 split 1, 4.9 split 2; 64 x 2056 x 1024 4.1 split 2, 6.1 split 1; 200 x 1024 x 2048 5.5 split 2,
-  // 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 2; 1000 x 2056 x 1024 12.4 tile 64 x 128, 13.9 128 x
-  // 128; 4096 x 2056 x 1024 23.8 tile 128 x 128 (its last 8 columns folded), 29.6 256 x 256; 30526 x 1024 x 2048 113
-  // tile 256 x 256, 134 128 x 128 and 128 x 256.
-  static const Form split1 = {16, 16, 1024, 1, 1.5, 1.0, 0.6, 0.6}, split2 = {32, 32, 512, 1, 1.5, 1.0, 0.7, 0.7};
-  static const Form t64 = {64, 128, 64, 2, 3.0, 0.0, 0.275, 0.52}, t128 = {128, 128, 64, 2, 3.0, 0.0, 0.66, 1.15};
-  static const Form t128w = {128, 256, 64, 1, 3.0, 0.0, 0.96, 0.98}, t256 = {256, 256, 64, 1, 3.0, 0.0, 1.62, 1.65};
-  static const Form any64 = {64, 64, 64, 2, 3.0, 0.0, 0.75, 1.0}, any128 = {128, 128, 64, 1, 3.0, 0.0, 1.2, 1.2};
-  const long n_cu = device_cus();
-  auto us = [&](const Form& f, long cols) { return form_us(f, M, cols, K, n_cu); };
-  const double s1 = us(split1, N), s2 = us(split2, N);
-  if (!wide) {
-    const double u1 = 2.1 * s1, u2 = 2.1 * s2, u3 = us(any64, N), u4 = us(any128, N), best = std::min(std::min(u1, u2), std::min(u3, u4));
-    st = best == u1   ? launch_split<1, false>(fn, a, s)
-         : best == u2 ? launch_split<2, false>(fn, a, s)
-         : best == u3 ? launch_any<64>(a, s)
-                      : launch_any<128>(a, s);
-  } else {
-    const int over = N % 128;  // columns behind the last whole tile of 128
-    const bool fold = over > 0 && over <= 16 && N / 128 >= 8;
-    const double u3 = us(t64, N), u4 = us(t128, fold ? N - over : N), u5 = us(t128w, N), u6 = us(t256, N);
-    const double best = std::min(std::min(std::min(s1, s2), std::min(u3, u4)), std::min(u5, u6));
-    st = best == s1   ? launch_split<1, true>(fn, a, s)
-         : best == s2 ? launch_split<2, true>(fn, a, s)
-         : best == u3 ? launch_tiles<64, 128, 2, 3>(fn, a, s)
-         : best == u4 ? (fold ? launch_tiles<128, 128, 2, 2, true>(fn, a, s) : launch_tiles<128, 128, 2, 2>(fn, a, s))
-         : best == u5 ? launch_tiles<128, 256, 2, 3>(fn, a, s)
-                      : launch_tiles<256, 256, 2, 2>(fn, a, s);
+  switch (choose(M, N, K, wide, device_cus())) {
+    case F_SPLIT16: st = wide ? launch_split<1, true>(fn, a, s) : launch_split<1, false>(fn, a, s); break;
+    case F_SPLIT32: st = wide ? launch_split<2, true>(fn, a, s) : launch_split<2, false>(fn, a, s); break;
+    case F_TILE64: st = launch_tiles<64, 128, 2, 3>(fn, a, s); break;
+    case F_TILE128: st = launch_tiles<128, 128, 2, 2>(fn, a, s); break;
+    case F_FOLD: st = launch_tiles<128, 128, 2, 2, true>(fn, a, s); break;
+    case F_WIDE: st = launch_tiles<128, 256, 2, 3>(fn, a, s); break;
+    case F_TILE256: st = launch_tiles<256, 256, 2, 2>(fn, a, s); break;
+    case F_ANY64: st = launch_any<64>(a, s); break;
+    case F_ANY128: st = launch_any<128>(a, s); break;
+    default: return fail(ZGDN_EUNSUPPORTED, "%s: M=%d N=%d K=%d: more tiles than a grid holds", fn, M, N, K);
   }
   return st != ZGDN_OK ? st : check_launch(fn);
+}
+
+// Host layer and tests (not part of the public header): the form that a product of these sizes takes and, where `groups` is
+// not NULL, the workgroups of its launch. 0: none, the product is refused.
+extern "C" int zgdn_gemm_act_form(int M, int N, int K, int wide, int64_t* groups) {
+  using namespace zgdn;
+  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 2048) return F_NONE;
+  const int f = choose(M, N, K, wide != 0, device_cus());
+  if (groups != nullptr) *groups = f == F_NONE ? 0 : workgroups(FORMS[f], M, f == F_FOLD ? N - folded(N) : N);
+  return f;
 }

@@ -9,8 +9,9 @@ import random
 import pytest
 
 # The forms' codes, with their tiles' rows and columns and a workgroup's threads.
-FORMS = {1: (16, 16, 512), 2: (32, 32, 512), 3: (64, 128, 512), 4: (128, 128, 512), 5: (128, 128, 512), 6: (128, 256, 512),
-         7: (256, 256, 512), 8: (64, 64, 256), 9: (128, 128, 256)}
+SPLIT16, SPLIT32, TILE64, FOLD, WIDE, TILE256, ANY64, ANY128 = range(1, 9)
+FORMS = {SPLIT16: (16, 16, 512), SPLIT32: (32, 32, 512), TILE64: (64, 128, 512), FOLD: (128, 128, 512), WIDE: (128, 256, 512),
+         TILE256: (256, 256, 512), ANY64: (64, 64, 256), ANY128: (128, 128, 256)}
 
 
 @pytest.fixture(scope="module")
@@ -39,11 +40,11 @@ def test_grids_hold_their_tiles(native, wide):
             assert -(-M // 64) * -(-N // 64) > 2**23  # (fewer always fit)
             continue
         rows, cols, threads = FORMS[f]
-        assert wide == (f < 8) or f <= 2
+        assert wide == (f < ANY64) or f <= SPLIT32
         assert groups * threads < 2**32 and groups % 8 == 0
-        tiles = -(-M // rows) * (N // cols if f == 5 else -(-N // cols))
+        tiles = -(-M // rows) * (N // cols if f == FOLD else -(-N // cols))
         assert 0 <= groups - tiles < 8, (M, N, K, f, groups)
-        if f == 5:
+        if f == FOLD:
             assert 0 < N % 128 <= 16 and N // 128 >= 8
     assert 0 < refused < len(sizes)
     assert form(native, 2**29, 8, 8, wide)[0] and form(native, 2**30, 1, 8, wide)[0]
@@ -53,3 +54,16 @@ def test_products_without_a_form_are_refused(native):
     at = [ctypes.c_void_p(1 << n) for n in (20, 40, 60)]  # never read
     with pytest.raises(RuntimeError, match="more tiles than a grid holds"):
         native.call("zlin_gemm_act", at[0], 8, at[1], 8, None, 0, 0, None, 0, at[2], 1 << 30, 1 << 30, 1 << 30, 8, 1, None)
+
+
+def test_every_form_is_taken(native):
+    """No form of the table that no product of a model's sizes takes."""
+    rng = random.Random(2)
+    taken = set()
+    for _ in range(20000):
+        M, N, K = (int(2 ** rng.uniform(0, b)) for b in (16, 13, 13))
+        if rng.random() < 0.3:
+            N = 128 * rng.randint(8, 40) + rng.randint(1, 16)
+        for wide in (True, False):
+            taken.add(form(native, M, N, K, wide)[0])
+    assert taken == set(FORMS)

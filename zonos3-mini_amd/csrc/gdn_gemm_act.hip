@@ -607,7 +607,8 @@ struct Form {
   int bm, bn, bk, per_cu, threads;
   double fixed, round, one, all;
 };
-enum FormCode { F_NONE, F_SPLIT16, F_SPLIT32, F_TILE64, F_TILE128, F_FOLD, F_WIDE, F_TILE256, F_ANY64, F_ANY128, F_COUNT };
+// (Tiles of 128 x 128 without folded columns have no place: twice as many of 64 x 128 take less at every size.)
+enum FormCode { F_NONE, F_SPLIT16, F_SPLIT32, F_TILE64, F_FOLD, F_WIDE, F_TILE256, F_ANY64, F_ANY128, F_COUNT };
 // The fit's points (M x N x K, us), the form taken and the next best: 4 x 2056 x 1024 3.4 split 1, 4.0 split 2;
 // 64 x 1024 x 2048 4.4 split 1, 4.9 split 2; 64 x 2056 x 1024 4.1 split 2, 6.1 split 1; 200 x 1024 x 2048 5.5 split 2,
 // 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 2; 1000 x 2056 x 1024 12.4 tile 64 x 128, 13.9 128 x
@@ -618,7 +619,6 @@ constexpr Form FORMS[F_COUNT] = {
     {16, 16, 1024, 1, 512, 1.5, 1.0, 0.6, 0.6},
     {32, 32, 512, 1, 512, 1.5, 1.0, 0.7, 0.7},
     {64, 128, 64, 2, 512, 3.0, 0.0, 0.275, 0.52},
-    {128, 128, 64, 2, 512, 3.0, 0.0, 0.66, 1.15},
     {128, 128, 64, 2, 512, 3.0, 0.0, 0.66, 1.15},
     {128, 256, 64, 1, 512, 3.0, 0.0, 0.96, 0.98},
     {256, 256, 64, 1, 512, 3.0, 0.0, 1.62, 1.65},
@@ -647,7 +647,7 @@ int choose(int M, int N, int K, bool wide, long n_cu) {
   double least = NEVER;
   for (int f = F_SPLIT16; f < F_COUNT; ++f) {
     const bool split = f <= F_SPLIT32;
-    if (f == F_FOLD ? !folded(N) : f == F_TILE128 && folded(N)) continue;
+    if (f == F_FOLD && !folded(N)) continue;
     if (!split && wide != (f < F_ANY64)) continue;
     const double us = (split && !wide ? 2.1 : 1.0) * form_us(FORMS[f], M, f == F_FOLD ? N - folded(N) : N, K, n_cu);
     if (us < least) least = us, best = f;
@@ -700,7 +700,6 @@ extern "C" int zlin_gemm_act(const void* x, long x_ld, const void* w, long w_ld,
     case F_SPLIT16: st = wide ? launch_split<1, true>(fn, a, s) : launch_split<1, false>(fn, a, s); break;
     case F_SPLIT32: st = wide ? launch_split<2, true>(fn, a, s) : launch_split<2, false>(fn, a, s); break;
     case F_TILE64: st = launch_tiles<64, 128, 2, 3>(fn, a, s); break;
-    case F_TILE128: st = launch_tiles<128, 128, 2, 2>(fn, a, s); break;
     case F_FOLD: st = launch_tiles<128, 128, 2, 2, true>(fn, a, s); break;
     case F_WIDE: st = launch_tiles<128, 256, 2, 3>(fn, a, s); break;
     case F_TILE256: st = launch_tiles<256, 256, 2, 2>(fn, a, s); break;

@@ -36,7 +36,9 @@ size_t zlin_attn_workspace_bytes(int packed, int n_seqs, int T, int Hk, int Hv, 
  *   g: g_ld == 0: float32 [Hv], one log decay a head. Else [B, T, Hv] in g_dtype, g_ld elements between tokens.
  *   initial_state [N, Hv, V, K] float32 or NULL (zeros); final_state likewise or NULL (not written). final_state may
  *   be initial_state itself (in place). Otherwise o, final_state and the workspace may overlap no operand.
- *   cu_seqlens: int32 [n_seqs + 1] with B == 1, or NULL. Rows that belong to no sequence are left as they were.
+ *   cu_seqlens: int32 [n_seqs + 1] with B == 1, or NULL. Rows that belong to no sequence are left as they were. Bounds are
+ *   clamped to the rows 0 .. T and to the bound before; where sequences overlap even so (a table that decreases), what
+ *   their rows and states get is not specified, and nothing else is written.
  */
 int zlin_attn_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
                   const void* g, long g_ld, int g_dtype, const float* initial_state, float* final_state, void* o,

@@ -191,3 +191,33 @@ def test_overlapping_operands_are_refused(native):
     _refused(native, "zlin_gemm_act", gemm, [
         (dict(y=at(0)), "overlap"), (dict(y=at(512), y_ld=512, K=257, w_ld=257), "overlap"), (dict(y=at(2 * MB - 2)), "overlap"),
         (dict(y=at(3 * MB + 2)), "overlap"), (dict(y=at(3 * MB), y_ld=72), "overlap"), (dict(y=at(MB + 2 * 255)), "overlap")])
+
+
+@pytest.mark.gpu
+def test_results_that_autograd_records_refuse_their_backward(gdn, cuda):
+    """Direct calls and registered operators on inputs that require a gradient: the values of the plain call, and a
+    backward that raises in place of gradients that are silently missing. Nothing is recorded without such inputs, under
+    no_grad, into ``out`` or into a state."""
+    gen = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(cuda)  # noqa: E731
+    x, w, q, v, a = r(5, 64), r(24, 64), r(1, 70, 2, 64), r(1, 70, 2, 64), -r(1, 70, 2).abs()
+    st = torch.zeros(70, 2, 64, 64, device=cuda)
+    z = torch.ops.zgdn
+    fwd = lambda f: lambda p: f(q, q, p, a)[0]  # noqa: E731
+    step = lambda f: lambda p: f(q[0], q[0], p, a[0], st.clone())  # noqa: E731
+    for call, p in ((lambda p: gdn.gemm_act(x, p), w), (lambda p: z.gemm_act(x, p), w), (fwd(gdn.linear_attn_fwd), v),
+                    (fwd(z.linear_attn_fwd), v), (step(gdn.linear_attn_step), v[0]), (step(z.linear_attn_step), v[0])):
+        want = call(p)
+        assert not want.requires_grad
+        p = p.clone().requires_grad_()
+        got = call(p)
+        assert got.requires_grad and torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="no backward|no autograd formula"):
+            got.float().sum().backward()
+        with torch.no_grad():
+            assert not call(p).requires_grad
+    p, out = w.clone().requires_grad_(), torch.zeros(5, 24, dtype=torch.bfloat16, device=cuda)
+    assert gdn.gemm_act(x, p, out=out) is out and not out.requires_grad and torch.equal(out, gdn.gemm_act(x, w))
+    _, s = gdn.linear_attn_fwd(q, q, v.clone().requires_grad_(), a)
+    gdn.linear_attn_step(q[0], q[0], v[0].clone().requires_grad_(), a[0], st)
+    assert not s.requires_grad and not st.requires_grad

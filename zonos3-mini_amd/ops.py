@@ -929,6 +929,28 @@ def _call_on(dev, name: str, *args) -> None:
             _native.call(name, *args)
 
 
+class _NoBackward(torch.autograd.Function):
+    """A new result of a call whose inputs autograd records: it stays in the graph, and its backward raises (as that of the
+    registered operators does) where a plain result would pass for a constant."""
+
+    @staticmethod
+    def forward(ctx, name, result, *inputs):
+        ctx.name = name
+        ctx.mark_dirty(result)
+        return result
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name}: no backward pass (inference only)")
+
+
+def _recorded(name: str, result, *inputs):
+    """``result``, in the graph where autograd records one of the inputs."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        return _NoBackward.apply(name, result, *inputs)
+    return result
+
+
 def _linear_decay(g, lead: tuple, Hv: int, dev):
     """(g, row stride, dtype code) of the log decays: float32 [Hv] (stride 0), or [*lead, Hv] read in place."""
     if not isinstance(g, torch.Tensor):
@@ -1007,7 +1029,8 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
     copied). initial_state [N, Hv, V, K] float32 or None (zeros). ``final_state`` may name an existing float32 tensor to
     write (it may be ``initial_state`` itself: in place). q, k, v, g may be column slices of wider rows. ``scale``
     defaults to ``K ** -0.5``. Returns (o [B, T, Hv, V] in q's dtype, final state or None); rows that no sequence of a
-    device table holds are not written."""
+    device table holds are not written. There is no backward pass: one through o raises, states are not recorded."""
+    inputs = (q, k, v, g, initial_state)
     (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 2)
     dev = q.device
     B, T, Hk, K = q.shape
@@ -1038,7 +1061,7 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
     _call_on(dev, "zlin_attn_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, g.data_ptr(), g_ld,
              g_code, _ptr(initial_state), _ptr(final_state), o.data_ptr(), _ptr(cu_seqlens), n_seqs, B, T, Hk, Hv, K, V,
              K**-0.5 if scale is None else float(scale), _ptr(workspace), size, _stream(dev))
-    return o, final_state
+    return _recorded("linear_attn_fwd", o, *inputs), final_state
 
 
 def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
@@ -1048,7 +1071,9 @@ def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
     q, k [B, Hk, K], v [B, Hv, V] (rows may be slices of a projection's), g float32 [Hv] or float32 / bfloat16 [B, Hv].
     state [B, Hv, V, K] float32; with ``slots`` (int64 [B]) a table [n_slots, Hv, V, K] of which stream b has row
     ``slots[b]``: a stream whose slot lies outside the table, or that an earlier stream of the call names, gets zeros and
-    touches no state. Returns o [B, Hv, V] in v's dtype."""
+    touches no state. Returns o [B, Hv, V] in v's dtype. There is no backward pass: one through o raises, states are not
+    recorded."""
+    inputs = (q, k, v, g, state)
     (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 1)
     dev = q.device
     B, Hk, K = q.shape
@@ -1070,7 +1095,7 @@ def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
     _call_on(dev, "zlin_attn_step", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, _CODES[q.dtype],
              g.data_ptr(), g_ld, g_code, state.data_ptr(), _ptr(slots), n_slots, o.data_ptr(), B, Hk, Hv, K, V,
              K**-0.5 if scale is None else float(scale), _stream(dev))
-    return o
+    return _recorded("linear_attn_step", o, *inputs)
 
 
 def _matrix_rows(name: str, t, cols: int | None, dev):
@@ -1097,7 +1122,9 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
 
     x [M, K], w [N, K] bfloat16 (any sizes; rows may be strided), bias [N] bfloat16 or float32, ``activation`` None,
     "relu", "silu", "gelu" (erf) or "gelu_tanh", residual [M, N] bfloat16. Returns y [M, N] bfloat16: ``out`` when given
-    (unit column stride; it may be ``residual`` itself, and may overlap no other operand)."""
+    (unit column stride; it may be ``residual`` itself, and may overlap no other operand). There is no backward pass: one
+    through a new y raises, an ``out`` is not recorded."""
+    inputs = (x, w, bias, residual) if out is None else ()
     dev = x.device if isinstance(x, torch.Tensor) else None
     x, x_ld = _matrix_rows("x", x, None, dev)
     M, K = x.shape
@@ -1127,4 +1154,4 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
     _call_on(dev, "zlin_gemm_act", x.data_ptr(), x_ld, w.data_ptr(), w_ld, _ptr(bias),
              F32 if bias is None else _code(bias, "bias"), _native.ACTIVATIONS[activation], _ptr(residual), r_ld,
              out.data_ptr(), y_ld, M, N, K, BF16, _stream(dev))
-    return out
+    return _recorded("gemm_act", out, *inputs)

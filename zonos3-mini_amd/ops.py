@@ -945,10 +945,8 @@ class _NoBackward(torch.autograd.Function):
 
 
 def _recorded(name: str, result, *inputs):
-    """``result``, in the graph where autograd records one of the inputs."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return _NoBackward.apply(name, result, *inputs)
-    return result
+    """``result`` of a call of which an input requires a gradient."""
+    return _NoBackward.apply(name, result, *inputs) if torch.is_grad_enabled() else result
 
 
 def _linear_decay(g, lead: tuple, Hv: int, dev):
@@ -1030,7 +1028,6 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
     write (it may be ``initial_state`` itself: in place). q, k, v, g may be column slices of wider rows. ``scale``
     defaults to ``K ** -0.5``. Returns (o [B, T, Hv, V] in q's dtype, final state or None); rows that no sequence of a
     device table holds are not written. There is no backward pass: one through o raises, states are not recorded."""
-    inputs = (q, k, v, g, initial_state)
     (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 2)
     dev = q.device
     B, T, Hk, K = q.shape
@@ -1061,7 +1058,10 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
     _call_on(dev, "zlin_attn_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, g.data_ptr(), g_ld,
              g_code, _ptr(initial_state), _ptr(final_state), o.data_ptr(), _ptr(cu_seqlens), n_seqs, B, T, Hk, Hv, K, V,
              K**-0.5 if scale is None else float(scale), _ptr(workspace), size, _stream(dev))
-    return _recorded("linear_attn_fwd", o, *inputs), final_state
+    if q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or (
+            initial_state is not None and initial_state.requires_grad):
+        o = _recorded("linear_attn_fwd", o, q, k, v, g, initial_state)
+    return o, final_state
 
 
 def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
@@ -1073,7 +1073,6 @@ def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
     ``slots[b]``: a stream whose slot lies outside the table, or that an earlier stream of the call names, gets zeros and
     touches no state. Returns o [B, Hv, V] in v's dtype. There is no backward pass: one through o raises, states are not
     recorded."""
-    inputs = (q, k, v, g, state)
     (q, q_ld), (k, k_ld), (v, v_ld) = _linear_qkv(q, k, v, 1)
     dev = q.device
     B, Hk, K = q.shape
@@ -1095,7 +1094,9 @@ def linear_attn_step(q, k, v, g, state, scale=None, slots=None):
     _call_on(dev, "zlin_attn_step", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, _CODES[q.dtype],
              g.data_ptr(), g_ld, g_code, state.data_ptr(), _ptr(slots), n_slots, o.data_ptr(), B, Hk, Hv, K, V,
              K**-0.5 if scale is None else float(scale), _stream(dev))
-    return _recorded("linear_attn_step", o, *inputs)
+    if q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or state.requires_grad:
+        o = _recorded("linear_attn_step", o, q, k, v, g, state)
+    return o
 
 
 def _matrix_rows(name: str, t, cols: int | None, dev):
@@ -1124,7 +1125,6 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
     "relu", "silu", "gelu" (erf) or "gelu_tanh", residual [M, N] bfloat16. Returns y [M, N] bfloat16: ``out`` when given
     (unit column stride; it may be ``residual`` itself, and may overlap no other operand). There is no backward pass: one
     through a new y raises, an ``out`` is not recorded."""
-    inputs = (x, w, bias, residual) if out is None else ()
     dev = x.device if isinstance(x, torch.Tensor) else None
     x, x_ld = _matrix_rows("x", x, None, dev)
     M, K = x.shape
@@ -1138,8 +1138,8 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
         _on_gpu("bias", bias, dev)
         if bias.shape != (N,):
             raise RuntimeError(f"bias: expected [{N}], got {tuple(bias.shape)}")
-    y_ld = N
-    if out is None:
+    y_ld, new = N, out is None
+    if new:
         out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
     elif not (isinstance(out, torch.Tensor) and out.device == dev and out.shape == (M, N) and out.dtype == torch.bfloat16
               and (N == 1 or out.stride(1) == 1) and (M <= 1 or out.stride(0) >= N)):
@@ -1154,4 +1154,7 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
     _call_on(dev, "zlin_gemm_act", x.data_ptr(), x_ld, w.data_ptr(), w_ld, _ptr(bias),
              F32 if bias is None else _code(bias, "bias"), _native.ACTIVATIONS[activation], _ptr(residual), r_ld,
              out.data_ptr(), y_ld, M, N, K, BF16, _stream(dev))
-    return _recorded("gemm_act", out, *inputs)
+    if new and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)
+                or (residual is not None and residual.requires_grad)):
+        out = _recorded("gemm_act", out, x, w, bias, residual)
+    return out

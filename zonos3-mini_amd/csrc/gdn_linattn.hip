@@ -576,6 +576,9 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
       q_read(0);
       read_v();
       read_weights(0);
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = a.scale * __expf(b[16 * j + m] + b[CH + 16 * j + m]);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -616,11 +619,9 @@ __global__ __launch_bounds__((64 * WalkCfg<K, V, NH, U, OUT>::NW), 2) void lin_w
         for (int k = 0; k < NT; ++k)
           asm volatile("" : "+v"(vt[0][u][k][0]), "+v"(vt[0][u][k][1]), "+v"(vt[0][u][k][2]), "+v"(vt[0][u][k][3]));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float f = a.scale * __expf(b[16 * j + m] + b[CH + 16 * j + m]);
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int u = 0; u < U; ++u) o[u][j] *= f;
-      }
+        for (int u = 0; u < U; ++u) o[u][j] *= f[j];
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
       u16x2 top = {0, 0};  // the largest magnitude's bits
 #pragma unroll

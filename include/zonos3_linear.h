@@ -8,7 +8,8 @@
  *
  * The recurrence, for each sequence and value head, over the state S [V, K] (float32, value-major):
  *   S_t = exp(g_t) S_{t-1} + v_t k_t^T,   o_t = S_t (scale q_t)
- * Value head h reads key head h / (Hv / Hk). g is a log decay; -inf (exp = 0) forgets all that was before.
+ * Value head h reads key head h / (Hv / Hk). g is a log decay; -inf (exp = 0) forgets all that was before, but for what is
+ * not finite: infinities and NaN leave an infinity or a NaN in every output and state that depends on them, and in no other.
  */
 #ifndef ZONOS3_LINEAR_H
 #define ZONOS3_LINEAR_H

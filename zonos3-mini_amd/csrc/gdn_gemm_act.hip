@@ -126,11 +126,13 @@ __device__ __forceinline__ void wait_and_meet() {  // at most N of the wave's lo
 // 8 waves, WM of them along the rows of x: BM x BN tiles, a wave BM / WM x BN / WN of it. Blocks of BK = 64 of K in NS
 // stages of LDS (128-byte rows, 16-byte chunk c of row r at c ^ f(r)): block kb computes while the next ones land. The
 // fragments of a block's second half are read under the products of its first, those of the next block's first half under
-// the products of its second: read when needed, LDS and matrix unit wait for each other (8192 x 4096 x 4096: 213 us read when needed, 211 so; the matrix unit runs at 85 % of the rate of the library's product, 178).
+// the products of its second (read right before their own products they cost the same within noise: 8192 x 4096 x 4096 221 us
+// either way, 4096 x 2056 x 1024 22.9 and 22.7; the library's product of the first takes 178).
 // Fragment reads touch 16 rows, one chunk each: f spreads rows 0 .. 15 (x) and rows 8 a + b, b < 4 (w, whose fragments
 // interleave) over all 16 places of 256 bytes.
 // FOLD: the at most 16 columns behind the last full tile are formed by the tiles (row block tm, column tile tn: rows
-// 16 tn .. of its block), not by a column of tiles of their own (4096 x 2056 x 1024: 30.4 us, 24.9 so).
+// 16 tn .. of its block), not by a column of tiles of their own (4096 x 2056 x 1024 with bias
+// and SiLU, whole calls: 30.9 us, 22.7 so).
 
 constexpr int BK = 64;
 
@@ -607,13 +609,25 @@ struct Form {
   int bm, bn, bk, per_cu, threads;
   double fixed, round, one, all;
 };
-// (Tiles of 128 x 128 without folded columns have no place: twice as many of 64 x 128 take less at every size.)
 enum FormCode { F_NONE, F_SPLIT16, F_SPLIT32, F_TILE64, F_FOLD, F_WIDE, F_TILE256, F_ANY64, F_ANY128, F_COUNT };
-// The fit's points (M x N x K, us), the form taken and the next best: 4 x 2056 x 1024 3.4 split 1, 4.0 split 2;
-// 64 x 1024 x 2048 4.4 split 1, 4.9 split 2; 64 x 2056 x 1024 4.1 split 2, 6.1 split 1; 200 x 1024 x 2048 5.5 split 2,
-// 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 2; 1000 x 2056 x 1024 12.4 tile 64 x 128, 13.9 128 x
-// 128; 4096 x 2056 x 1024 23.8 tile 128 x 128 (its last 8 columns folded), 29.6 256 x 256; 30526 x 1024 x 2048 113
-// tile 256 x 256, 134 128 x 128 and 128 x 256.
+// The fit's points (M x N x K, us in graph replays), the form taken and the next best: 4 x 2056 x 1024 3.4 split 16, 4.0
+// split 32; 64 x 1024 x 2048 4.4 split 16, 4.9 split 32; 64 x 2056 x 1024 4.1 split 32, 6.1 split 16; 200 x 1024 x 2048 5.5
+// split 32, 11.9 tile 64 x 128; 400 x 2056 x 1024 8.0 tile 64 x 128, 11.5 split 32; 1000 x 2056 x 1024 12.4 tile 64 x 128,
+// 13.9 128 x 128; 4096 x 2056 x 1024 23.8 tile 128 x 128 (its last 8 columns folded), 29.6 256 x 256; 30526 x 1024 x 2048
+// 113 tile 256 x 256, 134 128 x 128 and 128 x 256. (128 x 128 without folded columns is no form: twice as many tiles of
+// 64 x 128 take less at every size.) Between them the rule is off by up to a quarter where columns are few (us of calls, taken
+// / best): 30000 x 32 x 1024 19.5 split 32 / 15.7 tile 64 x 128, 5104 x 72 x 2176 14.2 split 32 / 12.8 tile 64 x 128; it is
+// right at 21614 x 17 x 5168 (56 split 32, 67) and 8192 x 64 x 4096 (25 split 32, 29).
+// Rows off 16-byte boundaries, where the split forms go through registers at 2.1 times their figures (us of calls; the form
+// taken in brackets):
+//                          split 16   split 32   any 64   any 128
+//   4 x 2056 x 1025          [6.8]       7.6      13.2     24.5
+//   512 x 64 x 8193         [13.6]      23.4      74.6    149
+//   64 x 2056 x 1025         14.4       [7.2]     13.0     25.9
+//   1260 x 362 x 1869        50.5      [19.8]     22.1     43.3
+//   3000 x 300 x 300         52.3       18.9      [6.8]    12.4
+//   5836 x 1038 x 1501      562        185        68.7    [51.7]
+//   20000 x 1000 x 1001    1209        412       122      [98.3]
 constexpr Form FORMS[F_COUNT] = {
     {},
     {16, 16, 1024, 1, 512, 1.5, 1.0, 0.6, 0.6},

@@ -14,8 +14,8 @@
 // split into bf16 terms whose sum has 16 (outputs: two terms) or 24 bits (states: three), so that an output keeps only
 // its own rounding and a state that of fp32 sums. fp32 inputs take the same steps on the fp32 MFMA.
 //
-// Measured (the three kernels, us): 32 packed prompts of 64 .. 2048 tokens, 16 heads of 128 x 128: 5 + 6 + 170; one of 4096:
-// 14 + 8 + 25; one of 32768, 16 heads of 128 x 64 on one key head: 39 + 9 + 86. What bounds it: a chunk's instructions, not
+// Measured (the three kernels, us): 32 packed prompts of 64 .. 2048 tokens, 16 heads of 128 x 128: 5 + 5 + 173; one of 4096:
+// 15 + 7 + 25; one of 32768, 16 heads of 128 x 64 on one key head: 40 + 9 + 88. What bounds it: a chunk's instructions, not
 // its bytes (packed: 569 MB, 104 us at the rate of a copy).
 //
 // The exponents are sums within a chunk, prefix sums from its start and suffix sums to its end, of one sign where all g <= 0;
@@ -280,7 +280,8 @@ __device__ __forceinline__ float prefix_sum(float x) {
 // segment's end state is not kept took a second body of the loop and registers it did not have (97 spilled: 27 -> 32 us at
 // 4096 tokens; with U = 1, below, there was room and nothing gained). OUT false: the state alone.
 // U = 2 where workgroups share CUs, U = 1 where none has to: the same work by 8 waves, two on each SIMD, one of which computes
-// while the other waits (the three kernels, us, U 2 / 1: one prompt of 64 tokens 10.5 / 10.0, of 4096, 16 heads 50 / 48; two
+// while the other waits (U 2 / 1: the kernel of two prompts of 64 tokens 10.5 / 10.0 us, whole calls of one prompt of 4096,
+// 16 heads, 48.3 / 46.2, of 32768 on one key head 136 / 126; two
 // workgroups of 8 waves would not fit a CU's registers).
 
 template <int K, int V, int NH, int U, bool OUT>
@@ -1186,10 +1187,10 @@ int walk_heads(int Hk, int Hv, int V) { return V == 64 && Hv / Hk % 2 == 0 ? 2 :
 
 Plan make_plan(bool packed, int N, int T, int Hk, int Hv, int K, int V, int dtype) {
   Plan p;
-  // Segments of a CU's share of the chunks. Half as long, two to a CU, costs 7 us at 4096 tokens of 16 heads of 128 x 128
-  // (states 12 us in the join instead of 7, 17 instead of 15 in the state pass, against 1 us less in the outputs) and
-  // gains 2 at 32768. Sequences that fill the CUs uncut are not cut below 1.5 shares: 32 of 64 .. 2048 tokens, 16 heads,
-  // take 180 us so, and 203 cut to 16 chunks (33 in the state pass and 13 in the join against 14 less in the outputs).
+  // Segments of a CU's share of the chunks. Half as long, two to a CU, 4096 tokens of 16 heads of 128 x 128 take 53.3 us
+  // instead of 46.2 (more states through the join and the state pass) and 32768 on one key head the same 127. Sequences that
+  // fill the CUs uncut are not cut below 1.5 shares: 32 of 64 .. 2048 tokens, 16 heads, take 173 us so, and 198 cut to 16
+  // chunks.
   const long rows = packed ? T : (long)N * T, groups = dtype == ZGDN_BF16 ? Hv / walk_heads(Hk, Hv, V) : Hv;
   const long share = (rows * groups + CUS * CH - 1) / (CUS * CH);
   p.run = (int)std::min(std::max(1L, N * groups >= CUS ? share + share / 2 : share) * CH, (long)INT32_MAX / 4);

@@ -2,8 +2,10 @@
 //
 // HBM-bound: the state is read and written once, 8 V K bytes a stream and head, next to which the rest is nothing. A row
 // of K state entries is held by K / 8 lanes (two 16-byte pieces each), so that a wave's load covers whole rows; o is one
-// reduction a row over those lanes. Waves walk tiles of 16 passes (a pass: 64 / (K / 8) rows) of one stream and head,
-// with the next tile's loads issued before the current one is updated and stored.
+// reduction a row over those lanes. A pass of a wave is 64 / (K / 8) rows of one stream and head (4 at K = 128, 8 at 64).
+// Where there is work for three workgroups a CU, waves walk tiles of 4 passes with the next tile's loads issued before the
+// current one is updated and stored; below, a tile is one pass and a wave has one (64 streams of 16 heads of 128 x 128:
+// 20.8 us; one stream of 4 heads: 3.3).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -1022,7 +1022,7 @@ def linear_attn_fwd(q, k, v, g, scale=None, initial_state=None, output_final_sta
 
     q, k [B, T, Hk, K], v [B, T, Hv, V], all bfloat16 or all float32, K and V each 64 or 128; value head h reads key head
     ``h // (Hv / Hk)``. g: log decays, float32 [Hv] (one a head) or float32 / bfloat16 [B, T, Hv] (-inf forgets all that
-    was before; values below -200 count as -200, whose exponential is zero in float32). Packed sequences: B == 1 and
+    was before, if it was finite; values below -200 count as -200, whose exponential is zero in float32). Packed sequences: B == 1 and
     ``cu_seqlens`` int32 [N + 1] (a device table is not read on the host; a list or CPU tensor is checked, then
     copied). initial_state [N, Hv, V, K] float32 or None (zeros). ``final_state`` may name an existing float32 tensor to
     write (it may be ``initial_state`` itself: in place). q, k, v, g may be column slices of wider rows. ``scale``

@@ -272,9 +272,9 @@ __device__ __forceinline__ float prefix_sum(float x) {
 //   P^T [s, t] = K Q^T, scaled by exp(G_t - G_s) and masked, a few tiles a wave, as two bf16 terms into LDS for all;
 //   O^T [v, t] = exp(G_t) S Q^T + V^T P^T;
 //   S^T = exp(G_end) S^T + K^T V', V' = exp(G_end - G_s) V in three bf16 terms.
-// V^T and K^T are read transposed from LDS. A chunk of 128 x 128 is 200 MFMAs (16 cycles) and 700 other vector instructions
+// V^T and K^T are read transposed from LDS. A chunk of 128 x 128 is 200 MFMAs (16 cycles) and 780 other vector instructions
 // a wave; beside an MFMA two of these cost nothing and each further one 4.3 cycles, so the splits into terms run beside the
-// products of the step before, 4600 cycles in all if nothing waited. Measured: 9700 a chunk with one workgroup on the CU,
+// products of the step before, 4900 cycles in all if nothing waited. Measured: 9700 a chunk with one workgroup on the CU,
 // 7500 with two (the rest: P's chain of reads, products, exponentials and writes, 1700; barriers and loads 1000; V^T P^T
 // and stores 1500). The three terms of V' are 32 of the MFMAs and 100 of the others more than two would be; two where a
 // segment's end state is not kept took a second body of the loop and registers it did not have (97 spilled: 27 -> 32 us at

@@ -1,5 +1,5 @@
-"""ctypes binding of ``libzonos3_gdn.so`` (the C ABI declared in ``include/zonos3_gdn.h`` and
-``include/zonos3_linear.h``).
+"""ctypes binding of ``libzonos3_gdn.so`` (the C ABI declared in ``include/zonos3_gdn.h``,
+``include/zonos3_linear.h`` and ``include/zonos3_attn.h``).
 
 The library is loaded after ``torch`` so that it binds to the HIP runtime torch already loaded (both carry
 the soname ``libamdhip64.so.7``); device pointers and streams then come straight from torch tensors.
@@ -107,6 +107,26 @@ LINEAR: dict[str, tuple] = {
     ),
 }
 
+# Entry points of include/zonos3_attn.h (the same library): name -> (restype, argtypes).
+ATTN: dict[str, tuple] = {
+    "zattn_qk_norm_rope": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_long, c_int, _P, c_int, _P, c_int, _P, _P, c_int, c_float, c_int, _P, _P, _P, c_long,
+         _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
+    ),
+    "zattn_window_fwd": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_long, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+         c_int, c_float, _P],
+    ),
+    "zattn_window_step_workspace_bytes": (c_size_t, [c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "zattn_window_step": (
+        c_int,
+        [_P, c_long, _P, c_long, _P, c_long, c_int, _P, _P, c_int, c_int, c_long, _P, c_int, c_int, c_int, c_int, c_int,
+         c_int, c_float, _P, c_size_t, _P],
+    ),
+}
+
 # Entry points of this package's own host layer, outside the published header: name -> (restype, argtypes).
 INTERNAL: dict[str, tuple] = {
     "zgdn_chunk32_slices": (c_int, [c_int, c_int, c_int, c_int]),
@@ -139,7 +159,7 @@ def lib() -> ctypes.CDLL:
             handle = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
         except OSError as exc:
             raise RuntimeError(f"cannot load {LIB_PATH}: {exc}") from exc
-        for name, (res, args) in (SIGNATURES | LINEAR | INTERNAL).items():
+        for name, (res, args) in (SIGNATURES | LINEAR | ATTN | INTERNAL).items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

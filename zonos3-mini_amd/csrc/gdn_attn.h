@@ -1,0 +1,78 @@
+// What the attention kernels share: tiles of K and V rows in LDS, loads straight into them, MFMA fragments.
+#pragma once
+
+#include "gdn_common.h"
+
+namespace zgdn {
+
+typedef __bf16 abf16x8 __attribute__((ext_vector_type(8)));
+typedef float af32x4 __attribute__((ext_vector_type(4)));
+typedef float af32x16 __attribute__((ext_vector_type(16)));
+typedef short ashort4 __attribute__((ext_vector_type(4)));
+
+// Rows of ROWB bytes (128, 256 or 512) in LDS, 16-byte chunk c of row r at place c ^ mask(r). What is read at a time then
+// spreads over the banks: for row fragments 16 rows at one chunk, for transposing reads 4 neighbouring rows at two chunks
+// beside one another (bf16), or, for single floats, 4 rows 4 apart at four chunks (fp32).
+template <int ROWB, typename T>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+  constexpr int n = ROWB / 16;
+  return sizeof(T) == 4 ? r & 15 : n == 16 ? (r & 7) << 1 | (r >> 3 & 1) : (r >> 1) & 7;
+}
+template <int ROWB, typename T>
+__device__ __forceinline__ int row_chunk(int r, int c) {
+  return r * ROWB + ((c ^ swizzle<ROWB, T>(r)) << 4);
+}
+
+// Four rows by 16 columns of 16-bit entries, transposed: in each group of 16 lanes, lane s gives the address of 4 entries of
+// row s / 4, columns 4 (s % 4) .., and gets the 4 rows' entries of column s.
+__device__ __forceinline__ uint2 lds_transposed(const uint8_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ashort4*)p));
+}
+
+// 16 bytes a lane from its own address straight into LDS, lane i at lds + 16 i (lds: an address within LDS, wave-uniform).
+// As for load_lds (gdn_common.h): in assembly, so that the kernel's own waits count it; a wait state behind M0's move.
+__device__ __forceinline__ void load_lds_from(const void* p, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+}
+// At most N of the wave's own loads still on their way.
+template <int N>
+__device__ __forceinline__ void wait_own_loads() {
+  static_assert(N < 64, "counter");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Position-aligned tiles of TILE keys that the queries at positions first .. last see at most: those of the sinks, then those
+// from the window's start on.
+struct KeyTiles {
+  int sinks, from, n;  // tiles of the sinks, the first of the window's, all
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : from + (i - sinks); }
+};
+template <int TILE>
+__device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, int sinks) {
+  KeyTiles t;
+  const int lo = window > 0 ? max(0, first - window + 1) : 0;
+  t.from = lo / TILE;
+  t.sinks = min((min(sinks, lo) + TILE - 1) / TILE, t.from);
+  t.n = last < 0 ? 0 : t.sinks + last / TILE + 1 - t.from;
+  return t;
+}
+
+// Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum.
+__device__ __forceinline__ float max_over_groups(float x) {
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // (one instruction; below 2^-126: 0)
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+}  // namespace zgdn

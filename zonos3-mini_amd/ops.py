@@ -1158,3 +1158,259 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
                 or (residual is not None and residual.requires_grad)):
         out = _recorded("gemm_act", out, x, w, bias, residual)
     return out
+
+
+# --------------------------------------------------------- the attention sublayer between gated-delta-rule layers
+
+
+def _head_vectors(name: str, t, lead: tuple | None, heads: int | None, D: int | None, dtype, dev):
+    """(t, row stride) of vectors [*lead, heads, D] whose rows the kernels read in place, else of a copy."""
+    ve = 4 if dtype is torch.float32 else 8  # elements in 16 bytes
+    if (isinstance(t, torch.Tensor) and t.dim() >= 2 and t.is_cuda and (dev is None or t.device == dev) and t.is_contiguous()
+            and not t.data_ptr() % 16):
+        ld = t.shape[-1] * t.shape[-2]
+    else:
+        t, ld = _rows_in_place(name, t, 2, dev, ve, 16)
+    shape = t.shape
+    if (len(shape) < 3 or (lead is not None and shape[:-2] != lead) or (heads is not None and shape[-2] != heads)
+            or (D is not None and shape[-1] != D)):
+        want = "*rows" if lead is None else ", ".join(map(str, lead))
+        raise RuntimeError(f"{name}: expected [{want}, {'heads' if heads is None else heads}, {'D' if D is None else D}], "
+                           f"got {tuple(shape)}")
+    if t.dtype is not dtype:
+        raise RuntimeError(f"{name}: {t.dtype}, expected {dtype} as the queries")
+    if ld > 1 << 22:  # rows further apart than the kernels' 32-bit offsets reach
+        t, ld = t.contiguous(), shape[-1] * shape[-2]
+    return t, ld
+
+
+def _cache_rows(name: str, t, heads: int, D: int, dtype, dev):
+    """The row stride of a cache [pages, page size, heads, D], read and written in place: never copied."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: must be a GPU tensor (got device {t.device}); there is no CPU path")
+    if t.device != dev:
+        raise RuntimeError(f"{name}: on {t.device}, expected {dev}")
+    if not (t.dim() == 4 and t.shape[2:] == (heads, D) and t.dtype is dtype):
+        raise RuntimeError(f"{name}: expected {dtype} [pages, page size, {heads}, {D}], got {t.dtype} {tuple(t.shape)}")
+    ld = _row_stride(t, 2)
+    if ld is None or ld % (4 if dtype is torch.float32 else 8) or t.data_ptr() % 16 or ld > 1 << 22:
+        raise RuntimeError(f"{name}: rows at one stride of whole 16 bytes from a 16-byte boundary, at most 2^22 elements "
+                           f"apart, expected; got strides {t.stride()}")
+    return ld
+
+
+def _window(window, sinks) -> tuple[int, int]:
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise RuntimeError(f"window: {window} keys (at least 1, or None)")
+    if sinks < 0:
+        raise RuntimeError(f"sinks: {sinks}")
+    return min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, v=None, k_cache=None,
+                 v_cache=None, rows=None, output_k=True):
+    """Norms of queries and keys for each head and the position rotation in one pass (C ABI ``zattn_qk_norm_rope``):
+    ``y = x * rsqrt(mean(x^2) + eps) * weight``, then the first R entries of a head turned by pairs through
+    ``position * inv_freq``.
+
+    q [*lead, Hq, D], k [*lead, Hk, D], both bfloat16 or both float32, D 64 or 128 (may be column slices of a projection's
+    rows). positions [*lead] int64 or int32. inv_freq [R / 2] float64 or float32, R a multiple of 16, at most D (the other
+    entries are only normalised); angles are formed in float64. Pairs are entries i and i + R / 2, or 2 i and 2 i + 1 where
+    ``interleaved``. q_weight, k_weight [D] float32 or bfloat16 (one type for both) or None.
+    With ``rows`` (int64 [*lead]), k_cache [pages, page size, Hk, D] gets each token's key at its row ``page * page size +
+    place``, and v_cache the values v [*lead, Hk, D] as they are; rows outside the cache are not written, and a row that two
+    tokens name holds pieces of either. Returns (q, k), k None where not ``output_k``. There is no backward pass: one through
+    them raises, what is written into a cache is not recorded."""
+    if not isinstance(q, torch.Tensor):
+        raise RuntimeError("q: expected a tensor")
+    code = _code(q, "q")
+    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    dev, lead, (Hq, D) = q.device, q.shape[:-2], q.shape[-2:]
+    k, k_ld = _head_vectors("k", k, lead, None, D, q.dtype, dev)
+    Hk = k.shape[-2]
+    if D not in (64, 128):
+        raise RuntimeError(f"head dim D={D}; queries and keys take 64 or 128")
+    if Hq < 1 or Hk < 1:
+        raise RuntimeError(f"heads: {Hq} of queries, {Hk} of keys")
+    n = 1
+    for x in lead:
+        n *= x
+    _on_gpu("positions", positions, dev)
+    if not (positions.shape == lead and positions.dtype in (torch.int64, torch.int32)):
+        raise RuntimeError(f"positions: expected int64 or int32 {list(lead)}, got {positions.dtype} {tuple(positions.shape)}")
+    _on_gpu("inv_freq", inv_freq, dev)
+    if not (inv_freq.dim() == 1 and inv_freq.dtype in (torch.float64, torch.float32)):
+        raise RuntimeError(f"inv_freq: expected float64 or float32 [R / 2], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    R = 2 * inv_freq.shape[0]
+    if R % 16 or R > D:
+        raise RuntimeError(f"inv_freq: turns {R} entries of a head (a multiple of 16, at most {D})")
+    w_code = F32
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            _on_gpu(name, t, dev)
+            if t.shape != (D,):
+                raise RuntimeError(f"{name}: expected [{D}], got {tuple(t.shape)}")
+            w_code = _code(t, name)
+            if t.data_ptr() % 16:
+                raise RuntimeError(f"{name}: not on a 16-byte boundary")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise RuntimeError("q_weight, k_weight: must share a dtype")
+    v_ld = kc_ld = vc_ld = n_rows = 0
+    if rows is None:
+        if k_cache is not None or v_cache is not None or v is not None:
+            raise RuntimeError("k_cache, v and v_cache need rows")
+        if not output_k:
+            raise RuntimeError("output_k: k has nowhere to go without a cache")
+    else:
+        _on_gpu("rows", rows, dev)
+        if not (rows.dtype == torch.int64 and rows.shape == lead):
+            raise RuntimeError(f"rows: expected int64 {list(lead)}, got {rows.dtype} {tuple(rows.shape)}")
+        if k_cache is None or (v is None) != (v_cache is None):
+            raise RuntimeError("rows need k_cache, and v and v_cache go together")
+        kc_ld = _cache_rows("k_cache", k_cache, Hk, D, q.dtype, dev)
+        n_rows = k_cache.shape[0] * k_cache.shape[1]
+        if v is not None:
+            v, v_ld = _head_vectors("v", v, lead, Hk, D, q.dtype, dev)
+            vc_ld = _cache_rows("v_cache", v_cache, Hk, D, q.dtype, dev)
+            if v_cache.shape != k_cache.shape:
+                raise RuntimeError(f"v_cache: {tuple(v_cache.shape)}, expected {tuple(k_cache.shape)} as k_cache")
+    q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    k_out = torch.empty(k.shape, device=dev, dtype=q.dtype) if output_k else None
+    if n:
+        _call_on(dev, "zattn_qk_norm_rope", q.data_ptr(), q_ld, k.data_ptr(), k_ld, _ptr(v), v_ld, code,
+                 positions.data_ptr(), int(positions.dtype is torch.int32), inv_freq.data_ptr(),
+                 int(inv_freq.dtype is torch.float32), _ptr(q_weight), _ptr(k_weight), w_code, float(eps), int(interleaved),
+                 q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), kc_ld, _ptr(v_cache), vc_ld, _ptr(rows), n_rows, n, Hq, Hk, D,
+                 R, _stream(dev))
+    inputs = (q, k, inv_freq, q_weight, k_weight)
+    if any(t is not None and t.requires_grad for t in inputs):
+        q_out = _recorded("qk_norm_rope", q_out, *inputs)
+        if k_out is not None:
+            k_out = _recorded("qk_norm_rope", k_out, *inputs)
+    return q_out, k_out
+
+
+def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, cu_seqlens_k=None):
+    """Causal attention over whole sequences with a sliding window and first tokens that stay visible (C ABI
+    ``zattn_window_fwd``): the query at position p sees the keys j <= p with ``p - j < window`` or ``j < sinks``.
+
+    q [B, Tq, Hq, D], k and v [B, Tk, Hk, D], all bfloat16 or all float32, D 64 or 128; query head h reads key head
+    ``h // (Hq / Hk)``. A sequence's last query stands at its last key (Tk > Tq: keys of earlier calls before them; queries
+    before the first key, and no others, see nothing and get zeros). ``window`` None: all keys up to the query. Packed
+    sequences: B == 1 and ``cu_seqlens`` int32 [N + 1] over the rows of q, ``cu_seqlens_k`` over those of k and v (None: the
+    same); a device table is not read on the host, a list or CPU tensor is checked, then copied. q, k and v may be column
+    slices of wider rows. ``scale`` defaults to ``D ** -0.5``. Returns o [B, Tq, Hq, D]; rows that no sequence of a device
+    table holds are not written. There is no backward pass: one through o raises."""
+    if not isinstance(q, torch.Tensor):
+        raise RuntimeError("q: expected a tensor")
+    code = _code(q, "q")
+    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    if q.dim() != 4:
+        raise RuntimeError(f"q: expected [B, Tq, Hq, D], got {tuple(q.shape)}")
+    dev, (B, Tq, Hq, D) = q.device, q.shape
+    k, k_ld = _head_vectors("k", k, None, None, D, q.dtype, dev)
+    if k.dim() != 4 or k.shape[0] != B:
+        raise RuntimeError(f"k: expected [{B}, Tk, Hk, {D}], got {tuple(k.shape)}")
+    Tk, Hk = k.shape[1], k.shape[2]
+    v, v_ld = _head_vectors("v", v, (B, Tk), Hk, D, q.dtype, dev)
+    if D not in (64, 128):
+        raise RuntimeError(f"head dim D={D}; attention takes 64 or 128")
+    if B < 1:
+        raise RuntimeError("q: no batch (B == 0)")
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise RuntimeError(f"query heads ({Hq}) must be a multiple of key heads ({Hk})")
+    window, sinks = _window(window, sinks)
+    n_seqs = B
+    if cu_seqlens is None:
+        if cu_seqlens_k is not None:
+            raise RuntimeError("cu_seqlens_k needs cu_seqlens")
+    else:
+        if B != 1:
+            raise RuntimeError("cu_seqlens: packed sequences need B == 1")
+        cu_seqlens = _bounds_table(cu_seqlens, Tq, dev)
+        if cu_seqlens_k is None:
+            if Tk != Tq:
+                raise RuntimeError(f"cu_seqlens_k: needed for {Tk} keys of {Tq} queries")
+            cu_seqlens_k = cu_seqlens
+        else:
+            cu_seqlens_k = _bounds_table(cu_seqlens_k, Tk, dev)
+        n_seqs = cu_seqlens.numel() - 1
+        if cu_seqlens_k.numel() != n_seqs + 1:
+            raise RuntimeError(f"cu_seqlens_k: {cu_seqlens_k.numel()} entries, expected {n_seqs + 1} as cu_seqlens")
+    o = torch.empty(B, Tq, Hq, D, device=dev, dtype=q.dtype)
+    _call_on(dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
+             _ptr(cu_seqlens), _ptr(cu_seqlens_k), n_seqs, B, Tq, Tk, Hq, Hk, D, window, sinks,
+             D**-0.5 if scale is None else float(scale), _stream(dev))
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        o = _recorded("window_attn_fwd", o, q, k, v)
+    return o
+
+
+def _bounds_table(cu, total: int, dev):
+    """A packed batch's bounds on the device: a host table is checked, then copied."""
+    if _on_host(cu):
+        cu = cu.tolist() if isinstance(cu, torch.Tensor) else [int(x) for x in cu]
+        check_cu_seqlens(cu, total)
+        cu = torch.tensor(cu, dtype=torch.int32).to(dev)
+    _cu_check(cu, total, dev)
+    return cu
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_step_workspace(*sizes: int) -> int:
+    return int(_native.lib().zattn_window_step_workspace_bytes(*sizes))
+
+
+def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=None, pages=None):
+    """One token of ``window_attn_fwd`` for each of B streams over a cache (C ABI ``zattn_window_step``): stream b's query
+    stands at position ``lengths[b] - 1``, whose key and value the cache holds already.
+
+    q [B, Hq, D] bfloat16 or float32, D 64 or 128; k_cache and v_cache of one shape [n, page size, Hk, D] in q's dtype (rows at
+    one stride, so slices of a joint cache qualify). lengths int32 [B]. ``pages`` int32 [B, P]: position p of stream b lies in
+    row ``p % page size`` of page ``pages[b, p // page size]``, the page size a power of two; None: n == B, the stream's
+    own. Lengths are clamped to the positions there are; positions on a page outside the cache are not seen. A stream that
+    sees nothing gets zeros. Returns o [B, Hq, D]. There is no backward pass: one through o raises."""
+    if not isinstance(q, torch.Tensor):
+        raise RuntimeError("q: expected a tensor")
+    code = _code(q, "q")
+    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    if q.dim() != 3:
+        raise RuntimeError(f"q: expected [B, Hq, D], got {tuple(q.shape)}")
+    dev, (B, Hq, D) = q.device, q.shape
+    if D not in (64, 128):
+        raise RuntimeError(f"head dim D={D}; attention takes 64 or 128")
+    Hk = k_cache.shape[2] if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 1
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise RuntimeError(f"query heads ({Hq}) must be a multiple of key heads ({Hk})")
+    kc_ld = _cache_rows("k_cache", k_cache, Hk, D, q.dtype, dev)
+    vc_ld = _cache_rows("v_cache", v_cache, Hk, D, q.dtype, dev)
+    if v_cache.shape != k_cache.shape:
+        raise RuntimeError(f"v_cache: {tuple(v_cache.shape)}, expected {tuple(k_cache.shape)} as k_cache")
+    _on_gpu("lengths", lengths, dev)
+    if not (lengths.dtype == torch.int32 and lengths.shape == (B,)):
+        raise RuntimeError(f"lengths: expected int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+    n, page_size = k_cache.shape[:2]
+    n_pages = 1
+    if pages is not None:
+        _on_gpu("pages", pages, dev)
+        if not (pages.dtype == torch.int32 and pages.dim() == 2 and pages.shape[0] == B):
+            raise RuntimeError(f"pages: expected int32 [{B}, pages a stream], got {pages.dtype} {tuple(pages.shape)}")
+        if page_size < 1 or page_size & (page_size - 1):
+            raise RuntimeError(f"k_cache: pages of {page_size} rows (a power of two with a page table)")
+        n_pages = pages.shape[1]
+    elif n != B:
+        raise RuntimeError(f"k_cache: {n} streams' rows for {B} streams (pages name them)")
+    window, sinks = _window(window, sinks)
+    o = torch.empty(B, Hq, D, device=dev, dtype=q.dtype)
+    size = _window_step_workspace(B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
+    workspace = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+    _call_on(dev, "zattn_window_step", q.data_ptr(), q_ld, k_cache.data_ptr(), kc_ld, v_cache.data_ptr(), vc_ld, code,
+             lengths.data_ptr(), _ptr(pages), page_size, n_pages, n * page_size, o.data_ptr(), B, Hq, Hk, D, window, sinks,
+             D**-0.5 if scale is None else float(scale), _ptr(workspace), size, _stream(dev))
+    if q.requires_grad or k_cache.requires_grad or v_cache.requires_grad:
+        o = _recorded("window_attn_step", o, q, k_cache, v_cache)
+    return o

@@ -236,6 +236,56 @@ def _(x, w, bias=None, activation=None, residual=None):
     return x.new_empty(x.shape[0], w.shape[0])
 
 
+# --------------------------------------------------------- the attention sublayer between gated-delta-rule layers
+
+
+@torch.library.custom_op(f"{NS}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, q_weight: Optional[Tensor] = None,
+                 k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    return ops.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(f"{NS}::qk_norm_rope_cache", mutates_args=("k_cache", "v_cache"))
+def qk_norm_rope_cache(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Tensor, k_cache: Tensor, v_cache: Tensor,
+                       rows: Tensor, q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
+                       eps: float = 1e-6, interleaved: bool = False) -> Tensor:
+    return ops.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, v, k_cache, v_cache, rows,
+                            output_k=False)[0]
+
+
+@qk_norm_rope_cache.register_fake
+def _(q, k, v, positions, inv_freq, k_cache, v_cache, rows, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NS}::window_attn_fwd", mutates_args=())
+def window_attn_fwd(q: Tensor, k: Tensor, v: Tensor, window: Optional[int] = None, sinks: int = 0,
+                    scale: Optional[float] = None, cu_seqlens: Optional[Tensor] = None,
+                    cu_seqlens_k: Optional[Tensor] = None) -> Tensor:
+    return ops.window_attn_fwd(q, k, v, window, sinks, scale, cu_seqlens, cu_seqlens_k)
+
+
+@window_attn_fwd.register_fake
+def _(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, cu_seqlens_k=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NS}::window_attn_step", mutates_args=())
+def window_attn_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, window: Optional[int] = None,
+                     sinks: int = 0, scale: Optional[float] = None, pages: Optional[Tensor] = None) -> Tensor:
+    return ops.window_attn_step(q, k_cache, v_cache, lengths, window, sinks, scale, pages)
+
+
+@window_attn_step.register_fake
+def _(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=None, pages=None):
+    return q.new_empty(q.shape)
+
+
 OPERATORS = ("recurrent_fwd", "decode_step", "chunk_fwd", "fused_decode_step", "serving_decode_step",
              "attnres_route", "accent_shift", "causal_conv1d", "l2norm", "sigmoid", "gated_rmsnorm", "linear_attn_fwd",
-             "linear_attn_step", "gemm_act")
+             "linear_attn_step", "gemm_act", "qk_norm_rope", "qk_norm_rope_cache", "window_attn_fwd", "window_attn_step")

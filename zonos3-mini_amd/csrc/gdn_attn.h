@@ -29,10 +29,14 @@ __device__ __forceinline__ uint2 lds_transposed(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ashort4*)p));
 }
 
-// 16 bytes a lane from its own address straight into LDS, lane i at lds + 16 i (lds: an address within LDS, wave-uniform).
-// As for load_lds (gdn_common.h): in assembly, so that the kernel's own waits count it; a wait state behind M0's move.
+// 16 bytes a lane straight into LDS, lane i at lds + 16 i (lds: an address within LDS, wave-uniform), from the lane's own
+// address, or from a uniform one and the lane's offset. As for load_lds (gdn_common.h): in assembly, so that the kernel's own
+// waits count it; a wait state behind M0's move. `nt`: the rows of a cache are not read again before others of their size.
 __device__ __forceinline__ void load_lds_from(const void* p, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void load_lds_from(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 // At most N of the wave's own loads still on their way.
 template <int N>

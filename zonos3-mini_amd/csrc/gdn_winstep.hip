@@ -4,7 +4,7 @@
 //
 // HBM-bound: the visible rows of K and V are read once for all the query heads that share them. A workgroup takes one stream,
 // key head and chunk of tiles (position-aligned, TILE keys), its waves the chunk's tiles in turn, each for itself: a wave
-// has its own two stages in LDS, filled by loads straight into it (K and V of a tile, 16 KiB at D = 128) while the tile before
+// has its own stages in LDS, filled by loads straight into it (K and V of a tile, 16 KiB at D = 128) while the tile before
 // is computed. S^T = K Q^T has a query a lane (16 columns, as many as heads share the key head), so that its softmax is
 // within a lane but for one exchange over the lane groups, and S^T's own layout is the second operand of
 // O^T = V^T P^T: keys in the order that S^T leaves them, V read transposed in the same order. The waves' parts (running
@@ -18,7 +18,8 @@
 namespace zgdn {
 namespace {
 
-constexpr int WS_NW = 4;        // waves a workgroup
+constexpr int WS_NW = 2, WS_WIDE = 8;  // waves a workgroup
+constexpr long WS_PER_CU = 2;           // workgroups a CU
 constexpr int WS_KEYS = 1024;   // keys of a chunk, at most
 constexpr long MOST_ROOM = 1L << 30;  // positions of a stream
 constexpr int WS_Q = 16;        // query heads of a workgroup, at most
@@ -55,48 +56,27 @@ __device__ __forceinline__ KeyTiles stream_tiles(const WinStepArgs& a, int b, in
   return key_tiles<TILE>(n - 1, n - 1, a.window, a.sinks);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
+// NW waves of RING stages each: two waves of two, so that two workgroups (four and more at D = 64) share a CU and the start of
+// one is hidden behind the others' loads; or, for a few short streams, eight waves that need no second kernel to join them.
+template <typename T, int D, int NW, int RING>
+__global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int TILE = WsCfg<T>::TILE, ROWB = D * (int)sizeof(T), CH = ROWB / 16, RP = 64 / CH;
   constexpr int LI = TILE * ROWB / 1024;  // load instructions for a tile of K (and of V)
   constexpr int STAGE = 2 * TILE * ROWB;
   constexpr int DT = D / 16;
-  __shared__ __align__(1024) uint8_t ring[WS_NW][2][STAGE];
+  __shared__ __align__(1024) uint8_t ring[NW][RING][STAGE];
   __shared__ int32_t page_of[WS_KEYS];
-  static_assert(WS_NW * 2 * STAGE >= WS_NW * WS_Q * (D + 2) * 4, "the waves' parts");
+  static_assert(RING * STAGE >= WS_Q * (D + 2) * 4, "the waves' parts");
   const int lane = threadIdx.x & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
-  const int qg = unit % a.q_groups, bh = unit / a.q_groups, b = bh / a.Hk, hk = bh - b * a.Hk;
+  // (the key heads of one stream's chunk beside one another: a row of the cache is all of them)
+  const int per_chunk = a.Hk * a.q_groups, bs = blockIdx.x / per_chunk, b = bs / a.splits, split = bs - b * a.splits;
+  const int unit = b * per_chunk + (blockIdx.x - bs * per_chunk), hk = (unit - b * per_chunk) / a.q_groups;
+  const int qg = unit - b * per_chunk - hk * a.q_groups;
   int n, lo;
   const KeyTiles tiles = stream_tiles<TILE>(a, b, n, lo);
   const int first = split * a.chunk, count = min(a.chunk, tiles.n - first);  // the chunk's tiles
   const int G = a.Hq / a.Hk, h0 = hk * G + qg * a.gq, heads = min(a.gq, G - qg * a.gq);
-  if (count <= 0) {
-    if (a.splits == 1)  // nothing is seen
-      for (int i = threadIdx.x; i < heads * D; i += 64 * WS_NW)
-        io<T>::store(reinterpret_cast<T*>(a.o) + ((size_t)b * a.Hq + h0) * D + i, 0.f);
-    return;
-  }
-  const int sink_end = min(a.sinks, lo);
-  // the pages of the chunk's positions, one entry for each run of `gran` of them; -1 for one that is not in the cache
-  const int gran = a.pages == nullptr ? TILE : min(a.page_size, TILE), per_tile = TILE / gran;
-  bool missing = false;
-  if (a.pages != nullptr) {
-    for (int i = threadIdx.x; i < count * per_tile; i += 64 * WS_NW) {
-      const int p = tiles.at(first + i / per_tile) * TILE + (i % per_tile) * gran;
-      int32_t page = -1;
-      if (p < n) {
-        page = a.pages[(size_t)b * a.n_pages + (p >> a.page_shift)];
-        if (page < 0 || page >= a.cache_pages) {
-          page = -1;
-          missing = true;
-        }
-      }
-      page_of[i] = page;
-    }
-    missing = __syncthreads_or(missing);
-  }
 
   // queries as the second operand: column m, entries k of the lane's group
   uint4 qf[BF ? D / 32 : D / 16];
@@ -108,7 +88,31 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
       qf[t] = *reinterpret_cast<const uint4*>(src + (BF ? 32 * t + 8 * g : 16 * t + 4 * g));
     }
   }
-
+  // the pages of the chunk's positions, one entry for each run of `gran` of them; -1 for one that is not in the cache. (Without
+  // a window the positions do not depend on the length: the pages are read while it is.)
+  const int gran = a.pages == nullptr ? TILE : min(a.page_size, TILE), per_tile = TILE / gran;
+  bool missing = false;
+  if (a.pages != nullptr) {
+    const int room = a.page_size * a.n_pages;
+    for (int i = threadIdx.x; i < a.chunk * per_tile; i += 64 * NW) {
+      const int tile = a.window > 0 ? tiles.at(first + i / per_tile) : first + i / per_tile;
+      const int p = tile * TILE + (i % per_tile) * gran;
+      int32_t page = p < room ? a.pages[(size_t)b * a.n_pages + (p >> a.page_shift)] : -1;
+      if (page < 0 || page >= a.cache_pages) {
+        page = -1;
+        missing = missing || p < n;
+      }
+      page_of[i] = page;
+    }
+    missing = __syncthreads_or(missing);
+  }
+  if (count <= 0) {
+    if (a.splits == 1)  // nothing is seen
+      for (int i = threadIdx.x; i < heads * D; i += 64 * NW)
+        io<T>::store(reinterpret_cast<T*>(a.o) + ((size_t)b * a.Hq + h0) * D + i, 0.f);
+    return;
+  }
+  const int sink_end = min(a.sinks, lo);
 #pragma unroll
   for (int t = 0; t < (int)(sizeof(qf) / 16); ++t) asm volatile("" : "+v"(qf[t].x));  // (awaited here, not in the loop)
 
@@ -120,26 +124,40 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
   const uint8_t* kb = reinterpret_cast<const uint8_t*>(a.kc) + (size_t)hk * ROWB;
   const uint8_t* vb = reinterpret_cast<const uint8_t*>(a.vc) + (size_t)hk * ROWB;
   const size_t kl = (size_t)a.kc_ld * sizeof(T), vl = (size_t)a.vc_ld * sizeof(T);
+  uint32_t koff[LI], voff[LI];  // of a tile whose rows follow one another: the lane's pieces from its first row on
+#pragma unroll
+  for (int j = 0; j < LI; ++j) {
+    const int r = j * RP + lane / CH;
+    const uint32_t c = (uint32_t)((lane % CH) ^ swizzle<ROWB, T>(r)) << 4;
+    koff[j] = (uint32_t)r * (uint32_t)kl + c;
+    voff[j] = (uint32_t)r * (uint32_t)vl + c;
+  }
+  auto whole_tile = [&](int p0) { return !missing && p0 + TILE <= n && (p0 >= lo || p0 + TILE <= sink_end); };
   auto issue = [&](int i, int stage) {  // tile i of the chunk
     const int p0 = tiles.at(first + i) * TILE;
-    const uint32_t at = (uint32_t)(uintptr_t)&ring[wave][stage][0];
-    const void *kp[LI], *vp[LI];
+    const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)&ring[wave][stage][0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what the stage held before has been read
+    if (gran == TILE && whole_tile(p0)) {
+      const size_t row = a.pages == nullptr ? (size_t)b * a.page_size + p0
+                                            : (size_t)__builtin_amdgcn_readfirstlane(page_of[i]) * a.page_size +
+                                                  (p0 & (a.page_size - 1));
+      const uint8_t *kt = kb + row * kl, *vt = vb + row * vl;
+#pragma unroll
+      for (int j = 0; j < LI; ++j) load_lds_from(kt, koff[j], at + 1024 * j);
+#pragma unroll
+      for (int j = 0; j < LI; ++j) load_lds_from(vt, voff[j], at + TILE * ROWB + 1024 * j);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < LI; ++j) {
       const int r = j * RP + lane / CH, p = p0 + r;
       const size_t c = (size_t)(((lane % CH) ^ swizzle<ROWB, T>(r)) << 4);
-      const size_t row = a.pages == nullptr ? (size_t)b * a.page_size + p
-                                            : (size_t)page_of[i * per_tile + r / gran] * a.page_size + (p & (a.page_size - 1));
       const bool s = seen(i, p);
-      kp[j] = s ? (const void*)(kb + row * kl + c) : (const void*)zeros16;
-      vp[j] = s ? (const void*)(vb + row * vl + c) : (const void*)zeros16;
+      size_t row = (size_t)b * a.page_size + p;
+      if (a.pages != nullptr) row = (size_t)page_of[i * per_tile + r / gran] * a.page_size + (p & (a.page_size - 1));
+      load_lds_from(s ? (const void*)(kb + row * kl + c) : (const void*)zeros16, at + 1024 * j);
+      load_lds_from(s ? (const void*)(vb + row * vl + c) : (const void*)zeros16, at + TILE * ROWB + 1024 * j);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what the stage held before has been read
-#pragma unroll
-    for (int j = 0; j < LI; ++j) load_lds_from(kp[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(at + 1024 * j)));
-#pragma unroll
-    for (int j = 0; j < LI; ++j)
-      load_lds_from(vp[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(at + TILE * ROWB + 1024 * j)));
   };
 
   af32x4 o[DT] = {};
@@ -166,7 +184,7 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
         }
       }
     }
-    const bool whole = !missing && p0 + TILE <= n && (p0 >= lo || p0 + TILE <= sink_end);
+    const bool whole = whole_tile(p0);
     float best = -INFINITY;
 #pragma unroll
     for (int t = 0; t < ST; ++t)
@@ -224,15 +242,23 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
   };
 
   wait_own_loads<0>();
-  if (wave < count) issue(wave, 0);
-  for (int i = wave, stage = 0; i < count; i += WS_NW, stage ^= 1) {
-    if (i + WS_NW < count) {
-      issue(i + WS_NW, stage ^ 1);
-      wait_own_loads<2 * LI>();
-    } else {
+  if constexpr (RING == 1) {
+    for (int i = wave; i < count; i += NW) {
+      issue(i, 0);
       wait_own_loads<0>();
+      compute(i, 0);
     }
-    compute(i, stage);
+  } else {
+    if (wave < count) issue(wave, 0);
+    for (int i = wave, stage = 0; i < count; i += NW, stage ^= 1) {
+      if (i + NW < count) {
+        issue(i + NW, stage ^ 1);
+        wait_own_loads<2 * LI>();
+      } else {
+        wait_own_loads<0>();
+      }
+      compute(i, stage);
+    }
   }
 
   // the waves' parts, joined in LDS: [wave][query][D + 2]
@@ -252,16 +278,16 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
   }
   __syncthreads();
   const float* parts = reinterpret_cast<const float*>(&ring[0][0][0]);
-  for (int i = threadIdx.x; i < heads * D; i += 64 * WS_NW) {
+  for (int i = threadIdx.x; i < heads * D; i += 64 * NW) {
     const int h = i / D, d = i - h * D;
     float best = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WS_NW; ++w) best = fmaxf(best, parts[(w * WS_Q + h) * (D + 2) + D]);
+    for (int w = 0; w < NW; ++w) best = fmaxf(best, parts[(w * WS_Q + h) * (D + 2) + D]);
     const float base = best == -INFINITY ? 0.f : best;
     float x = 0.f, l = 0.f;
     bool saw = false;
 #pragma unroll
-    for (int w = 0; w < WS_NW; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float* p = parts + (w * WS_Q + h) * (D + 2);
       if (p[D + 1] < 0.f) continue;
       const float f = exp2_of(p[D] - base);
@@ -282,38 +308,64 @@ __global__ __launch_bounds__(64 * WS_NW) void win_step_kernel(WinStepArgs a) {
   }
 }
 
-// A workgroup of D threads for each stream and query head: its chunks' parts, in order.
+// A workgroup for each stream and query head joins its chunks' parts: JG groups of D threads, every JG-th chunk each, in order,
+// with a running maximum (so that a part's statistics and values are read at one time), then the groups' sums.
+constexpr int WS_JOIN = 512;  // threads
+struct Joined {
+  float top = -INFINITY, sum = 0.f, x = 0.f;
+  bool any = false;
+  __device__ __forceinline__ void add(float t, float l, float v) {  // (l below zero: the part saw nothing)
+    const bool saw = !(l < 0.f);
+    const float next = saw ? fmaxf(top, t) : top, base = next == -INFINITY ? 0.f : next, keep = exp2_of(top - base);
+    const float f = exp2_of(t - base);
+    top = next;
+    sum = fmaf(sum, keep, saw ? l * f : 0.f);
+    x = fmaf(x, keep, saw ? v * f : 0.f);
+    any = any || saw;
+  }
+};
 template <typename T, int D>
-__global__ __launch_bounds__(D) void win_step_join_kernel(WinStepArgs a) {
+__global__ __launch_bounds__(WS_JOIN) void win_step_join_kernel(WinStepArgs a) {
+  constexpr int JG = WS_JOIN / D;
+  __shared__ float x_of[JG][D], top_of[JG], sum_of[JG];
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq, G = a.Hq / a.Hk, hk = h / G, qg = (h - hk * G) / a.gq;
+  const size_t unit = ((size_t)b * a.Hk + hk) * a.q_groups + qg;
+  const size_t at = unit * a.splits * a.gq + (h - hk * G - qg * a.gq);
   int n, lo;
   const KeyTiles tiles = stream_tiles<WsCfg<T>::TILE>(a, b, n, lo);
   const int used = (tiles.n + a.chunk - 1) / a.chunk;
-  const size_t unit = ((size_t)b * a.Hk + hk) * a.q_groups + qg;
-  const size_t at = unit * a.splits * a.gq + (h - hk * G - qg * a.gq);
-  float best = -INFINITY;
-  for (int i = 0; i < used; ++i) best = fmaxf(best, a.part_ml[2 * (at + (size_t)i * a.gq)]);
-  const float base = best == -INFINITY ? 0.f : best;
-  float x = 0.f, l = 0.f;
-  bool saw = false;
-#pragma unroll 4
-  for (int i = 0; i < used; ++i) {
-    const size_t p = at + (size_t)i * a.gq;
-    const float pl = a.part_ml[2 * p + 1], po = a.part_o[p * D + threadIdx.x];
-    const float f = exp2_of(a.part_ml[2 * p] - base);
-    if (!(pl < 0.f)) {
-      x = fmaf(po, f, x);
-      l = fmaf(pl, f, l);
-      saw = true;
+  const int d = threadIdx.x % D, jg = threadIdx.x / D;
+  Joined j;
+  constexpr int AT = 8;  // parts read at a time
+  for (int i0 = jg; i0 < used; i0 += JG * AT) {
+    float2 ml[AT];
+    float x[AT];
+#pragma unroll
+    for (int e = 0; e < AT; ++e) {
+      const size_t p = at + (size_t)min(i0 + e * JG, used - 1) * a.gq;
+      ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+      x[e] = a.part_o[p * D + d];
     }
+#pragma unroll
+    for (int e = 0; e < AT; ++e) j.add(ml[e].x, i0 + e * JG < used ? ml[e].y : -1.f, x[e]);
   }
-  io<T>::store(reinterpret_cast<T*>(a.o) + (size_t)blockIdx.x * D + threadIdx.x, saw ? x / l : 0.f);
+  x_of[jg][d] = j.x;
+  if (d == 0) {
+    top_of[jg] = j.top;
+    sum_of[jg] = j.any ? j.sum : -1.f;
+  }
+  __syncthreads();
+  if (jg != 0) return;
+#pragma unroll
+  for (int i = 1; i < JG; ++i) j.add(top_of[i], sum_of[i], x_of[i][d]);
+  io<T>::store(reinterpret_cast<T*>(a.o) + (size_t)blockIdx.x * D + d, j.any ? j.x / j.sum : 0.f);
 }
 
 // How a call is cut: chunks of at most WS_KEYS keys, of at least a tile for each wave, two workgroups for each CU where the
-// streams' visible positions have that many.
+// streams' visible positions have that many. Up to WS_KEYS keys of streams and key heads that a CU each can take are not cut.
 struct StepPlan {
   int q_groups, gq, chunk, splits;
+  bool wide;
 };
 StepPlan step_plan(int B, long room, int Hq, int Hk, int window, int sinks, int dtype) {
   StepPlan p;
@@ -324,10 +376,18 @@ StepPlan step_plan(int B, long room, int Hq, int Hk, int window, int sinks, int 
   long tiles = std::max(1L, (room + tile - 1) / tile);
   if (window > 0) tiles = std::min(tiles, (window + tile - 2) / tile + 1 + (sinks + tile - 1) / tile);
   const long units = (long)B * Hk * p.q_groups;
-  long chunk = (tiles * units + 2 * device_cus() - 1) / (2 * device_cus());
-  chunk = (std::min(std::max(chunk, (long)WS_NW), WS_KEYS / tile) + WS_NW - 1) / WS_NW * WS_NW;
-  p.chunk = (int)chunk;
+  p.wide = tiles <= WS_KEYS / tile && units <= device_cus();
+  if (p.wide) {
+    p.chunk = (int)tiles;
+    p.splits = 1;
+    return p;
+  }
+  const long want = (WS_PER_CU * device_cus() + units - 1) / units;  // chunks of a stream
+  long chunk = std::min(std::max((tiles + want - 1) / want, (long)WS_NW), WS_KEYS / tile);
   p.splits = (int)((tiles + chunk - 1) / chunk);
+  chunk = (tiles + p.splits - 1) / p.splits;  // (of equal size)
+  p.chunk = (int)(chunk + WS_NW - 1) / WS_NW * WS_NW;
+  p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
   return p;
 }
 size_t step_bytes(const StepPlan& p, int B, int Hk, int D) {
@@ -335,10 +395,14 @@ size_t step_bytes(const StepPlan& p, int B, int Hk, int D) {
 }
 
 template <typename T, int D>
-void launch_win_step(const WinStepArgs& a, hipStream_t s) {
+void launch_win_step(const WinStepArgs& a, bool wide, hipStream_t s) {
   const unsigned units = (unsigned)(a.B * a.Hk * a.q_groups);
-  hipLaunchKernelGGL((win_step_kernel<T, D>), dim3(units * a.splits), dim3(64 * WS_NW), 0, s, a);
-  if (a.splits > 1) hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(D), 0, s, a);
+  if (wide) {
+    hipLaunchKernelGGL((win_step_kernel<T, D, WS_WIDE, 128 / D>), dim3(units), dim3(64 * WS_WIDE), 0, s, a);
+    return;
+  }
+  hipLaunchKernelGGL((win_step_kernel<T, D, WS_NW, 2>), dim3(units * a.splits), dim3(64 * WS_NW), 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(WS_JOIN), 0, s, a);
 }
 
 bool step_sizes(int B, long room, int Hq, int Hk, int D, int window, int sinks, int dtype) {
@@ -386,7 +450,7 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
     return fail(ZGDN_EINVAL, "%s: q, caches, o and workspace need 16-byte aligned bases", fn);
   if (((uintptr_t)lengths | (uintptr_t)pages) % 4) return fail(ZGDN_EINVAL, "%s: lengths, pages not on 4-byte boundaries", fn);
   const StepPlan p = step_plan(B, room, Hq, Hk, window, sinks, dtype);
-  if ((long)B * Hk * p.q_groups * p.splits > (1L << 32) / (64 * WS_NW) - 1 || (long)B * Hq > (1L << 32) / D - 1)
+  if ((long)B * Hk * p.q_groups * p.splits > (1L << 32) / (64 * WS_NW) - 1 || (long)B * Hq > (1L << 32) / WS_JOIN - 1)
     return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Hq=%d x %d chunks", fn, B, Hq, p.splits);
   const size_t need = step_bytes(p, B, Hk, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
@@ -407,8 +471,8 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
                 need ? part + rows * D : nullptr};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == ZGDN_F32)
-    D == 128 ? launch_win_step<float, 128>(a, s) : launch_win_step<float, 64>(a, s);
+    D == 128 ? launch_win_step<float, 128>(a, p.wide, s) : launch_win_step<float, 64>(a, p.wide, s);
   else
-    D == 128 ? launch_win_step<bf16, 128>(a, s) : launch_win_step<bf16, 64>(a, s);
+    D == 128 ? launch_win_step<bf16, 128>(a, p.wide, s) : launch_win_step<bf16, 64>(a, p.wide, s);
   return check_launch(fn);
 }

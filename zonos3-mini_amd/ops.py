@@ -1161,16 +1161,32 @@ def gemm_act(x, w, bias=None, activation=None, residual=None, out=None):
 
 
 # --------------------------------------------------------- the attention sublayer between gated-delta-rule layers
+#
+# Small calls are bound by the host: what most of them hand over passes one expression (``_heads_ld``, ``_plain``), and only
+# what does not is looked at check by check (``_head_vectors``, ``_on_gpu``), copied or refused.
+
+
+def _heads_ld(t, dtype, index: int) -> int:
+    """Elements between the tokens of vectors [*lead, heads, D] that the kernels read in place as they are, else 0."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        return 0
+    z, s = t.shape, t.stride()
+    if len(z) == 3:
+        ld = s[0] if z[0] != 1 else z[1] * z[2]
+    elif len(z) == 4 and z[1] != 1 and (z[0] == 1 or s[0] == z[1] * s[1]):
+        ld = s[1]
+    else:
+        return 0
+    if (s[-1] != 1 or (s[-2] != z[-1] and z[-2] != 1) or ld < z[-1] * z[-2] or ld % (4 if dtype is torch.float32 else 8)
+            or ld > 1 << 22 or t.data_ptr() % 16):
+        return 0
+    return ld
 
 
 def _head_vectors(name: str, t, lead: tuple | None, heads: int | None, D: int | None, dtype, dev):
     """(t, row stride) of vectors [*lead, heads, D] whose rows the kernels read in place, else of a copy."""
     ve = 4 if dtype is torch.float32 else 8  # elements in 16 bytes
-    if (isinstance(t, torch.Tensor) and t.dim() >= 2 and t.is_cuda and (dev is None or t.device == dev) and t.is_contiguous()
-            and not t.data_ptr() % 16):
-        ld = t.shape[-1] * t.shape[-2]
-    else:
-        t, ld = _rows_in_place(name, t, 2, dev, ve, 16)
+    t, ld = _rows_in_place(name, t, 2, dev, ve, 16)
     shape = t.shape
     if (len(shape) < 3 or (lead is not None and shape[:-2] != lead) or (heads is not None and shape[-2] != heads)
             or (D is not None and shape[-1] != D)):
@@ -1184,8 +1200,30 @@ def _head_vectors(name: str, t, lead: tuple | None, heads: int | None, D: int | 
     return t, ld
 
 
-def _cache_rows(name: str, t, heads: int, D: int, dtype, dev):
+def _queries(q):
+    """(q, row stride, dtype code, device, its index)."""
+    if not isinstance(q, torch.Tensor):
+        raise RuntimeError("q: expected a tensor")
+    code, index = _code(q, "q"), q.get_device()
+    ld = _heads_ld(q, q.dtype, index) if index >= 0 else 0
+    if not ld:
+        q, ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    if q.shape[-1] not in (64, 128):
+        raise RuntimeError(f"head dim D={q.shape[-1]}; attention takes 64 or 128")
+    return q, ld, code, q.device, index
+
+
+def _plain(name: str, t, index: int, dev) -> None:
+    """A dense tensor on the queries' GPU, or an error that says what is wrong with it."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.is_contiguous()):
+        _on_gpu(name, t, dev)
+
+
+def _cache_ld(name: str, t, heads: int, D: int, dtype, index: int, dev) -> int:
     """The row stride of a cache [pages, page size, heads, D], read and written in place: never copied."""
+    if (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.dim() == 4 and t.is_contiguous()
+            and t.shape[2] == heads and t.shape[3] == D and not t.data_ptr() % 16 and heads * D <= 1 << 22):
+        return heads * D
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name}: expected a tensor")
     if not t.is_cuda:
@@ -1211,6 +1249,16 @@ def _window(window, sinks) -> tuple[int, int]:
     return min(int(window), 1 << 30), min(int(sinks), 1 << 30)
 
 
+def _launch(index: int, dev, name: str, *args) -> None:
+    """``_native.call`` on the current stream of device ``index``, which is the current device meanwhile."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        _native.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _native.call(name, *args, stream)
+
+
 def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, v=None, k_cache=None,
                  v_cache=None, rows=None, output_k=True):
     """Norms of queries and keys for each head and the position rotation in one pass (C ABI ``zattn_qk_norm_rope``):
@@ -1225,25 +1273,22 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     place``, and v_cache the values v [*lead, Hk, D] as they are; rows outside the cache are not written, and a row that two
     tokens name holds pieces of either. Returns (q, k), k None where not ``output_k``. There is no backward pass: one through
     them raises, what is written into a cache is not recorded."""
-    if not isinstance(q, torch.Tensor):
-        raise RuntimeError("q: expected a tensor")
-    code = _code(q, "q")
-    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
-    dev, lead, (Hq, D) = q.device, q.shape[:-2], q.shape[-2:]
-    k, k_ld = _head_vectors("k", k, lead, None, D, q.dtype, dev)
+    q, q_ld, code, dev, index = _queries(q)
+    dtype, shape = q.dtype, q.shape
+    lead, Hq, D = shape[:-2], shape[-2], shape[-1]
+    k_ld = _heads_ld(k, dtype, index)
+    if not k_ld or k.shape[:-2] != lead or k.shape[-1] != D:
+        k, k_ld = _head_vectors("k", k, lead, None, D, dtype, dev)
     Hk = k.shape[-2]
-    if D not in (64, 128):
-        raise RuntimeError(f"head dim D={D}; queries and keys take 64 or 128")
     if Hq < 1 or Hk < 1:
         raise RuntimeError(f"heads: {Hq} of queries, {Hk} of keys")
-    n = 1
-    for x in lead:
-        n *= x
-    _on_gpu("positions", positions, dev)
-    if not (positions.shape == lead and positions.dtype in (torch.int64, torch.int32)):
+    _plain("positions", positions, index, dev)
+    p32 = positions.dtype is torch.int32
+    if positions.shape != lead or not (p32 or positions.dtype is torch.int64):
         raise RuntimeError(f"positions: expected int64 or int32 {list(lead)}, got {positions.dtype} {tuple(positions.shape)}")
-    _on_gpu("inv_freq", inv_freq, dev)
-    if not (inv_freq.dim() == 1 and inv_freq.dtype in (torch.float64, torch.float32)):
+    _plain("inv_freq", inv_freq, index, dev)
+    f32 = inv_freq.dtype is torch.float32
+    if inv_freq.dim() != 1 or not (f32 or inv_freq.dtype is torch.float64):
         raise RuntimeError(f"inv_freq: expected float64 or float32 [R / 2], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     R = 2 * inv_freq.shape[0]
     if R % 16 or R > D:
@@ -1251,13 +1296,13 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     w_code = F32
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         if t is not None:
-            _on_gpu(name, t, dev)
-            if t.shape != (D,):
+            _plain(name, t, index, dev)
+            if t.dim() != 1 or t.shape[0] != D:
                 raise RuntimeError(f"{name}: expected [{D}], got {tuple(t.shape)}")
             w_code = _code(t, name)
             if t.data_ptr() % 16:
                 raise RuntimeError(f"{name}: not on a 16-byte boundary")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
         raise RuntimeError("q_weight, k_weight: must share a dtype")
     v_ld = kc_ld = vc_ld = n_rows = 0
     if rows is None:
@@ -1266,28 +1311,30 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
         if not output_k:
             raise RuntimeError("output_k: k has nowhere to go without a cache")
     else:
-        _on_gpu("rows", rows, dev)
-        if not (rows.dtype == torch.int64 and rows.shape == lead):
+        _plain("rows", rows, index, dev)
+        if not (rows.dtype is torch.int64 and rows.shape == lead):
             raise RuntimeError(f"rows: expected int64 {list(lead)}, got {rows.dtype} {tuple(rows.shape)}")
         if k_cache is None or (v is None) != (v_cache is None):
             raise RuntimeError("rows need k_cache, and v and v_cache go together")
-        kc_ld = _cache_rows("k_cache", k_cache, Hk, D, q.dtype, dev)
+        kc_ld = _cache_ld("k_cache", k_cache, Hk, D, dtype, index, dev)
         n_rows = k_cache.shape[0] * k_cache.shape[1]
         if v is not None:
-            v, v_ld = _head_vectors("v", v, lead, Hk, D, q.dtype, dev)
-            vc_ld = _cache_rows("v_cache", v_cache, Hk, D, q.dtype, dev)
+            v_ld = _heads_ld(v, dtype, index)
+            if not v_ld or v.shape != k.shape:
+                v, v_ld = _head_vectors("v", v, lead, Hk, D, dtype, dev)
+            vc_ld = _cache_ld("v_cache", v_cache, Hk, D, dtype, index, dev)
             if v_cache.shape != k_cache.shape:
                 raise RuntimeError(f"v_cache: {tuple(v_cache.shape)}, expected {tuple(k_cache.shape)} as k_cache")
-    q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    k_out = torch.empty(k.shape, device=dev, dtype=q.dtype) if output_k else None
+    q_out = q.new_empty(shape)
+    k_out = k.new_empty(k.shape) if output_k else None
+    n = positions.numel()
     if n:
-        _call_on(dev, "zattn_qk_norm_rope", q.data_ptr(), q_ld, k.data_ptr(), k_ld, _ptr(v), v_ld, code,
-                 positions.data_ptr(), int(positions.dtype is torch.int32), inv_freq.data_ptr(),
-                 int(inv_freq.dtype is torch.float32), _ptr(q_weight), _ptr(k_weight), w_code, float(eps), int(interleaved),
-                 q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), kc_ld, _ptr(v_cache), vc_ld, _ptr(rows), n_rows, n, Hq, Hk, D,
-                 R, _stream(dev))
-    inputs = (q, k, inv_freq, q_weight, k_weight)
-    if any(t is not None and t.requires_grad for t in inputs):
+        _launch(index, dev, "zattn_qk_norm_rope", q.data_ptr(), q_ld, k.data_ptr(), k_ld, _ptr(v), v_ld, code,
+                positions.data_ptr(), p32, inv_freq.data_ptr(), f32, _ptr(q_weight), _ptr(k_weight), w_code, eps, interleaved,
+                q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), kc_ld, _ptr(v_cache), vc_ld, _ptr(rows), n_rows, n, Hq, Hk, D, R)
+    if (q.requires_grad or k.requires_grad or inv_freq.requires_grad or (q_weight is not None and q_weight.requires_grad)
+            or (k_weight is not None and k_weight.requires_grad)):
+        inputs = (q, k, inv_freq, q_weight, k_weight)
         q_out = _recorded("qk_norm_rope", q_out, *inputs)
         if k_out is not None:
             k_out = _recorded("qk_norm_rope", k_out, *inputs)
@@ -1305,20 +1352,19 @@ def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, 
     same); a device table is not read on the host, a list or CPU tensor is checked, then copied. q, k and v may be column
     slices of wider rows. ``scale`` defaults to ``D ** -0.5``. Returns o [B, Tq, Hq, D]; rows that no sequence of a device
     table holds are not written. There is no backward pass: one through o raises."""
-    if not isinstance(q, torch.Tensor):
-        raise RuntimeError("q: expected a tensor")
-    code = _code(q, "q")
-    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    q, q_ld, code, dev, index = _queries(q)
     if q.dim() != 4:
         raise RuntimeError(f"q: expected [B, Tq, Hq, D], got {tuple(q.shape)}")
-    dev, (B, Tq, Hq, D) = q.device, q.shape
-    k, k_ld = _head_vectors("k", k, None, None, D, q.dtype, dev)
+    dtype, (B, Tq, Hq, D) = q.dtype, q.shape
+    k_ld = _heads_ld(k, dtype, index)
+    if not k_ld or k.shape[-1] != D:
+        k, k_ld = _head_vectors("k", k, None, None, D, dtype, dev)
     if k.dim() != 4 or k.shape[0] != B:
         raise RuntimeError(f"k: expected [{B}, Tk, Hk, {D}], got {tuple(k.shape)}")
     Tk, Hk = k.shape[1], k.shape[2]
-    v, v_ld = _head_vectors("v", v, (B, Tk), Hk, D, q.dtype, dev)
-    if D not in (64, 128):
-        raise RuntimeError(f"head dim D={D}; attention takes 64 or 128")
+    v_ld = _heads_ld(v, dtype, index)
+    if not v_ld or v.shape != k.shape:
+        v, v_ld = _head_vectors("v", v, (B, Tk), Hk, D, dtype, dev)
     if B < 1:
         raise RuntimeError("q: no batch (B == 0)")
     if Hk < 1 or Hq < 1 or Hq % Hk:
@@ -1341,10 +1387,10 @@ def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, 
         n_seqs = cu_seqlens.numel() - 1
         if cu_seqlens_k.numel() != n_seqs + 1:
             raise RuntimeError(f"cu_seqlens_k: {cu_seqlens_k.numel()} entries, expected {n_seqs + 1} as cu_seqlens")
-    o = torch.empty(B, Tq, Hq, D, device=dev, dtype=q.dtype)
-    _call_on(dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
-             _ptr(cu_seqlens), _ptr(cu_seqlens_k), n_seqs, B, Tq, Tk, Hq, Hk, D, window, sinks,
-             D**-0.5 if scale is None else float(scale), _stream(dev))
+    o = q.new_empty(q.shape)
+    _launch(index, dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
+            _ptr(cu_seqlens), _ptr(cu_seqlens_k), n_seqs, B, Tq, Tk, Hq, Hk, D, window, sinks,
+            D**-0.5 if scale is None else scale)
     if q.requires_grad or k.requires_grad or v.requires_grad:
         o = _recorded("window_attn_fwd", o, q, k, v)
     return o
@@ -1374,30 +1420,25 @@ def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=N
     row ``p % page size`` of page ``pages[b, p // page size]``, the page size a power of two; None: n == B, the stream's
     own. Lengths are clamped to the positions there are; positions on a page outside the cache are not seen. A stream that
     sees nothing gets zeros. Returns o [B, Hq, D]. There is no backward pass: one through o raises."""
-    if not isinstance(q, torch.Tensor):
-        raise RuntimeError("q: expected a tensor")
-    code = _code(q, "q")
-    q, q_ld = _head_vectors("q", q, None, None, None, q.dtype, None)
+    q, q_ld, code, dev, index = _queries(q)
     if q.dim() != 3:
         raise RuntimeError(f"q: expected [B, Hq, D], got {tuple(q.shape)}")
-    dev, (B, Hq, D) = q.device, q.shape
-    if D not in (64, 128):
-        raise RuntimeError(f"head dim D={D}; attention takes 64 or 128")
+    dtype, (B, Hq, D) = q.dtype, q.shape
     Hk = k_cache.shape[2] if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 1
     if Hk < 1 or Hq < 1 or Hq % Hk:
         raise RuntimeError(f"query heads ({Hq}) must be a multiple of key heads ({Hk})")
-    kc_ld = _cache_rows("k_cache", k_cache, Hk, D, q.dtype, dev)
-    vc_ld = _cache_rows("v_cache", v_cache, Hk, D, q.dtype, dev)
+    kc_ld = _cache_ld("k_cache", k_cache, Hk, D, dtype, index, dev)
+    vc_ld = _cache_ld("v_cache", v_cache, Hk, D, dtype, index, dev)
     if v_cache.shape != k_cache.shape:
         raise RuntimeError(f"v_cache: {tuple(v_cache.shape)}, expected {tuple(k_cache.shape)} as k_cache")
-    _on_gpu("lengths", lengths, dev)
-    if not (lengths.dtype == torch.int32 and lengths.shape == (B,)):
+    _plain("lengths", lengths, index, dev)
+    if not (lengths.dtype is torch.int32 and lengths.dim() == 1 and lengths.shape[0] == B):
         raise RuntimeError(f"lengths: expected int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
-    n, page_size = k_cache.shape[:2]
+    n, page_size = k_cache.shape[0], k_cache.shape[1]
     n_pages = 1
     if pages is not None:
-        _on_gpu("pages", pages, dev)
-        if not (pages.dtype == torch.int32 and pages.dim() == 2 and pages.shape[0] == B):
+        _plain("pages", pages, index, dev)
+        if not (pages.dtype is torch.int32 and pages.dim() == 2 and pages.shape[0] == B):
             raise RuntimeError(f"pages: expected int32 [{B}, pages a stream], got {pages.dtype} {tuple(pages.shape)}")
         if page_size < 1 or page_size & (page_size - 1):
             raise RuntimeError(f"k_cache: pages of {page_size} rows (a power of two with a page table)")
@@ -1405,12 +1446,12 @@ def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=N
     elif n != B:
         raise RuntimeError(f"k_cache: {n} streams' rows for {B} streams (pages name them)")
     window, sinks = _window(window, sinks)
-    o = torch.empty(B, Hq, D, device=dev, dtype=q.dtype)
+    o = q.new_empty(q.shape)
     size = _window_step_workspace(B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
-    workspace = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
-    _call_on(dev, "zattn_window_step", q.data_ptr(), q_ld, k_cache.data_ptr(), kc_ld, v_cache.data_ptr(), vc_ld, code,
-             lengths.data_ptr(), _ptr(pages), page_size, n_pages, n * page_size, o.data_ptr(), B, Hq, Hk, D, window, sinks,
-             D**-0.5 if scale is None else float(scale), _ptr(workspace), size, _stream(dev))
+    workspace = o.new_empty(size, dtype=torch.uint8) if size else None
+    _launch(index, dev, "zattn_window_step", q.data_ptr(), q_ld, k_cache.data_ptr(), kc_ld, v_cache.data_ptr(), vc_ld, code,
+            lengths.data_ptr(), _ptr(pages), page_size, n_pages, n * page_size, o.data_ptr(), B, Hq, Hk, D, window, sinks,
+            D**-0.5 if scale is None else scale, _ptr(workspace), size)
     if q.requires_grad or k_cache.requires_grad or v_cache.requires_grad:
         o = _recorded("window_attn_step", o, q, k_cache, v_cache)
     return o

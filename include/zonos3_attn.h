@@ -40,16 +40,23 @@ int zattn_qk_norm_rope(const void* q, long q_ld, const void* k, long k_ld, const
                        long n_cache_rows, int n_tokens, int Hq, int Hk, int D, int R, void* stream);
 
 /*
+ * Bytes of workspace that zattn_window_fwd needs for the same sizes (0 for sizes that it refuses, and where it needs none).
+ * packed: 1 where cu_q and cu_k are given (n_seqs sequences in Tq and Tk rows), else 0 (n_seqs = B).
+ */
+size_t zattn_window_fwd_workspace_bytes(int packed, int n_seqs, int Tq, int Tk, int Hq, int Hk, int D, int window, int sinks,
+                                        int dtype);
+
+/*
  * Attention over whole sequences: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that i sees.
  *   q, o [B, Tq, Hq, D], k, v [B, Tk, Hk, D] in `dtype`; o is dense. Query i of a sequence of nq queries and nk keys stands at
  *   position nk - nq + i (negative: it sees nothing).
  *   cu_q, cu_k: int32 [n_seqs + 1] with B == 1, or both NULL (n_seqs is not read). Rows that belong to no sequence are left as
  *   they were. Bounds are clamped to the rows and to the bound before; where sequences overlap even so, what their rows get is
- *   not specified, and nothing else is written. o overlaps no operand.
+ *   not specified, and nothing else is written. o and the workspace overlap no other operand.
  */
 int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype, void* o,
                      const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int B, int Tq, int Tk, int Hq, int Hk, int D,
-                     int window, int sinks, float scale, void* stream);
+                     int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Bytes of workspace that zattn_window_step needs for the same sizes (0 for sizes that it refuses, and where it needs none).

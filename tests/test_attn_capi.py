@@ -66,7 +66,7 @@ def test_qk_norm_rope_refuses(native):
 
 def test_window_fwd_refuses(native):
     args = dict(q=P, q_ld=1024, k=_at(1), k_ld=256, v=_at(2), v_ld=256, dtype=1, o=_at(3), cu_q=None, cu_k=None, n_seqs=0, B=2,
-                Tq=100, Tk=130, Hq=8, Hk=2, D=128, window=64, sinks=4, scale=1.0, stream=None)
+                Tq=100, Tk=130, Hq=8, Hk=2, D=128, window=64, sinks=4, scale=1.0, ws=None, ws_bytes=0, stream=None)
     _refused(native, "zattn_window_fwd", args, [
         (dict(B=0), "bad sizes"), (dict(Tq=-1), "bad sizes"), (dict(window=-1), "bad sizes"), (dict(sinks=-1), "bad sizes"),
         (dict(Hk=3), "multiple"), (dict(D=256), "D=256"), (dict(dtype=5), "dtype code 5"), (dict(cu_q=_at(4)), "go together"),

@@ -117,8 +117,9 @@ ATTN: dict[str, tuple] = {
     "zattn_window_fwd": (
         c_int,
         [_P, c_long, _P, c_long, _P, c_long, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-         c_int, c_float, _P],
+         c_int, c_float, _P, c_size_t, _P],
     ),
+    "zattn_window_fwd_workspace_bytes": (c_size_t, [c_int] * 10),
     "zattn_window_step_workspace_bytes": (c_size_t, [c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_int]),
     "zattn_window_step": (
         c_int,

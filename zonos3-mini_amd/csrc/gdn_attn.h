@@ -8,19 +8,23 @@ namespace zgdn {
 typedef __bf16 abf16x8 __attribute__((ext_vector_type(8)));
 typedef float af32x4 __attribute__((ext_vector_type(4)));
 typedef float af32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 abf16x2 __attribute__((ext_vector_type(2)));
 typedef short ashort4 __attribute__((ext_vector_type(4)));
 
-// Rows of ROWB bytes (128, 256 or 512) in LDS, 16-byte chunk c of row r at place c ^ mask(r). What is read at a time then
-// spreads over the banks: for row fragments 16 rows at one chunk, for transposing reads 4 neighbouring rows at two chunks
-// beside one another (bf16), or, for single floats, 4 rows 4 apart at four chunks (fp32).
-template <int ROWB, typename T>
+// Rows of ROWB bytes (128, 256 or 512) in LDS, 16-byte chunk c of row r at place c ^ mask(r), so that what is read at a time
+// spreads over the banks (256 bytes). Row fragments: 16 rows at one chunk; all masks give 16 neighbouring rows different
+// places. Values, for products of M x M tiles: bf16, transposing reads, by 32 lanes 8 rows by 2 chunks (M = 16) or 4 rows by 4
+// chunks (M = 32); fp32, single floats, 4 rows 4 apart by 4 chunks (M = 16) or 2 rows 4 apart by 8 chunks (M = 32).
+template <int ROWB, typename T, int M>
 __device__ __forceinline__ constexpr int swizzle(int r) {
   constexpr int n = ROWB / 16;
-  return sizeof(T) == 4 ? r & 15 : n == 16 ? (r & 7) << 1 | (r >> 3 & 1) : (r >> 1) & 7;
+  if (sizeof(T) == 4) return M == 16 ? r & 15 : (r & 3) | (r >> 3 & 1) << 2 | (r >> 2 & 1) << 3;
+  if (M == 16) return n == 16 ? (r & 7) << 1 | (r >> 3 & 1) : (r >> 1) & 7;
+  return n == 16 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3);
 }
-template <int ROWB, typename T>
+template <int ROWB, typename T, int M>
 __device__ __forceinline__ int row_chunk(int r, int c) {
-  return r * ROWB + ((c ^ swizzle<ROWB, T>(r)) << 4);
+  return r * ROWB + ((c ^ swizzle<ROWB, T, M>(r)) << 4);
 }
 
 // Four rows by 16 columns of 16-bit entries, transposed: in each group of 16 lanes, lane s gives the address of 4 entries of
@@ -38,27 +42,12 @@ __device__ __forceinline__ void load_lds_from(const void* p, uint32_t lds) {
 __device__ __forceinline__ void load_lds_from(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
+static __device__ __attribute__((aligned(16))) const uint32_t zeros16[4] = {0, 0, 0, 0};  // where loads of no row go
 // At most N of the wave's own loads still on their way.
 template <int N>
 __device__ __forceinline__ void wait_own_loads() {
   static_assert(N < 64, "counter");
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// Position-aligned tiles of TILE keys that the queries at positions first .. last see at most: those of the sinks, then those
-// from the window's start on.
-struct KeyTiles {
-  int sinks, from, n;  // tiles of the sinks, the first of the window's, all
-  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : from + (i - sinks); }
-};
-template <int TILE>
-__device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, int sinks) {
-  KeyTiles t;
-  const int lo = window > 0 ? max(0, first - window + 1) : 0;
-  t.from = lo / TILE;
-  t.sinks = min((min(sinks, lo) + TILE - 1) / TILE, t.from);
-  t.n = last < 0 ? 0 : t.sinks + last / TILE + 1 - t.from;
-  return t;
 }
 
 // Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum.

@@ -27,8 +27,11 @@ struct WinArgs {
   void* o;
   const int32_t *cu_q, *cu_k;
   int N, Tq, Tk, Hq, Hk, window, sinks;
-  float c;    // scale log2(e)
+  float c;    // |scale| log2(e)
+  int flip;   // scale below zero: the queries change their signs
   int tiles;  // of rows a key head, at most
+  int splits;               // workgroups that share a tile of 32 rows
+  float *part_o, *part_ml;  // [workgroup][32][D], [workgroup][32][2]
 };
 
 __device__ __forceinline__ int prefix_count(int x) {  // over the lanes up to this one
@@ -125,251 +128,621 @@ __device__ __noinline__ void win_row(const T* q, const T* k, long k_ld, const T*
   for (int d = 0; d < D / 64; ++d) io<T>::store(o + 64 * d + lane, acc[d] / sum);
 }
 
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW) void win_attn_kernel(WinArgs a) {
-  constexpr bool BF = sizeof(T) == 2;
-  constexpr int ES = (int)sizeof(T), ROWB = D * ES, CH = ROWB / 16, RP = 64 / CH;
-  constexpr int KT = BF ? 64 : 32, ST = KT / 32;  // keys of a tile
-  constexpr int LW = KT * ROWB / 1024 / NW;       // a wave's load instructions for a tile of K (and of V)
-  constexpr int STAGE = 2 * KT * ROWB, DT = D / 32, QF = D * ES / 32;
-  constexpr int ROWS = 32 * NW;
-  __shared__ __align__(1024) uint8_t lds[2][STAGE];
-  __shared__ int dirty;  // something of V was zeroed
-  const int lane = threadIdx.x & 63, wave = wave_id(), m = lane & 31, h = lane >> 5;
-  const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
-  RowTile rt;
-  if (!find_rows<ROWS>(a, blockIdx.x / a.Hk, rt)) return;
-  const uint32_t rows = (uint32_t)rt.nq * G, r0 = (uint32_t)rt.tile * ROWS, rw = r0 + 32 * wave;
-  const bool real = rw + m < rows;
-  const uint32_t row = min(rw + m, rows - 1);  // (lanes behind the last row: as that one, without its stores)
-  const int past = rt.nk - rt.nq;
-  const int qi = (int)(row / G), hq = hk * G + (int)(row - (uint32_t)qi * G);
-  const int p = past + qi;  // the lane's position
-  // positions of the workgroup's and of the wave's rows
-  const int first = past + (int)(r0 / G), last = past + (int)((min(rows, r0 + ROWS) - 1) / G);
-  const int wfirst = past + (int)(min(rows - 1, rw) / G), wlast = past + (int)((min(rows, rw + 32) - 1) / G);
-  const KeyTiles tiles = key_tiles<KT>(first, last, a.window, a.sinks);
+// The same for query qi of a workgroup's sequence, head hq.
+template <typename T, int D>
+__device__ __forceinline__ void redo_row(const WinArgs& a, const RowTile& t, const T* k, const T* v, int qi, int hq) {
+  win_row<T, D>(reinterpret_cast<const T*>(a.q) + (size_t)(t.q0 + qi) * a.q_ld + (size_t)hq * D, k, a.k_ld, v, a.v_ld,
+                reinterpret_cast<T*>(a.o) + ((size_t)(t.q0 + qi) * a.Hq + hq) * D, t.nk - t.nq + qi, a.window, a.sinks,
+                a.flip ? -a.c : a.c);
+}
+// The keys that the rows at positions first .. last see, as a list of places: the sinks ahead of the window's start, then all
+// from there on. Place u is position u, or u + shift behind the sinks.
+struct KeyList {
+  int s, shift, sunk, n;  // places of sinks; positions left out; places below sunk are seen whatever the window; tiles
+  __device__ __forceinline__ int position(int u) const { return u < s ? u : u + shift; }
+};
+template <int KT>
+__device__ __forceinline__ KeyList key_list(const WinArgs& a, int first, int last) {
+  KeyList k;
+  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+  k.s = min(a.sinks, lo);
+  k.shift = lo - k.s;
+  k.sunk = max(k.s, a.sinks - k.shift);
+  k.n = last < 0 ? 0 : (last - k.shift) / KT + 1;
+  return k;
+}
 
-  const T* qrow = reinterpret_cast<const T*>(a.q) + (size_t)(rt.q0 + qi) * a.q_ld + (size_t)hq * D;
-  uint4 qf[QF];
-#pragma unroll
-  for (int t = 0; t < QF; ++t) qf[t] = *reinterpret_cast<const uint4*>(qrow + (BF ? 16 * t + 8 * h : 8 * t + 4 * h));
-#pragma unroll
-  for (int t = 0; t < QF; ++t) asm volatile("" : "+v"(qf[t].x));  // (awaited here, not in the loop)
-
-  const T* kbase = reinterpret_cast<const T*>(a.k) + (size_t)rt.k0 * a.k_ld + (size_t)hk * D;
-  const T* vbase = reinterpret_cast<const T*>(a.v) + (size_t)rt.k0 * a.v_ld + (size_t)hk * D;
-  const uint32_t k_row = (uint32_t)a.k_ld * ES, v_row = (uint32_t)a.v_ld * ES;
-  uint32_t koff[LW], voff[LW];
-#pragma unroll
-  for (int j = 0; j < LW; ++j) {
-    const int r = (wave * LW + j) * RP + lane / CH;
-    const uint32_t c = (uint32_t)((lane % CH) ^ swizzle<ROWB, T>(r)) << 4;
-    koff[j] = (uint32_t)r * k_row + c;
-    voff[j] = (uint32_t)r * v_row + c;
+// A workgroup's rows of a sequence and key head, and their keys. Positions, from here on, are places of the list's second part
+// (p - shift): differences and bounds are the same.
+template <int ROWS, int KT>
+struct Rows {
+  RowTile t;
+  uint32_t rows, r0;
+  int G, hk, past, first, last;  // past: position of query 0; first, last: places of the first and last row
+  KeyList keys;
+  __device__ __forceinline__ bool find(const WinArgs& a, int i, int key_head) {
+    if (!find_rows<ROWS>(a, i, t)) return false;
+    G = a.Hq / a.Hk;
+    hk = key_head;
+    rows = (uint32_t)t.nq * G;
+    r0 = (uint32_t)t.tile * ROWS;
+    past = t.nk - t.nq;
+    first = past + (int)(r0 / G);
+    last = past + (int)((min(rows, r0 + ROWS) - 1) / G);
+    keys = key_list<KT>(a, first, last);
+    first -= keys.shift;
+    last -= keys.shift;
+    return true;
   }
-  auto rsrc = [&](const T* base, long ld, uint32_t row_bytes, int p0) {
-    const uint64_t at = (uint64_t)(uintptr_t)(base + (size_t)p0 * ld);
-    const int there = min(KT, rt.nk - p0);
-    return RsrcWords{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(there - 1) * row_bytes + ROWB)), 0x00020000u};
-  };
-  auto issue = [&](int i, int stage) {
-    const int p0 = tiles.at(i) * KT;
-    const uint32_t at = (uint32_t)(uintptr_t)&lds[stage][0] + 1024 * LW * wave;
-    const RsrcWords kr = rsrc(kbase, a.k_ld, k_row, p0), vr = rsrc(vbase, a.v_ld, v_row, p0);
-#pragma unroll
-    for (int j = 0; j < LW; ++j) load_lds(kr, koff[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(at + 1024 * j)));
-#pragma unroll
-    for (int j = 0; j < LW; ++j)
-      load_lds(vr, voff[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(at + KT * ROWB + 1024 * j)));
-  };
+  // Do rows at places f .. l all see the whole tile at place p0?
+  __device__ __forceinline__ bool whole(const WinArgs& a, int p0, int f, int l) const {
+    return p0 + KT - 1 <= f && (a.window == 0 || l - max(p0, keys.sunk) < a.window || p0 + KT <= keys.sunk);
+  }
+  __device__ __forceinline__ bool sees(const WinArgs& a, int p, int u) const {
+    return u <= p && (a.window == 0 || p - u < a.window || u < keys.sunk);
+  }
+};
 
-  af32x16 o[DT] = {};
-  float top = -INFINITY, sum = 0.f;  // of the lane's row; sum: of the lane's keys
-  auto edge = [&](int p0) {  // is there a row that does not see all of the tile
-    return !(p0 + KT - 1 <= first && (a.window == 0 || last - p0 < a.window || p0 + KT <= a.sinks));
-  };
-  auto clean = [&](int stage) {  // zeros for what is not finite in V
-    uint8_t* vs = &lds[stage][KT * ROWB];
+// Loads of a tile's rows of K or V straight into LDS by N instructions of a wave, the first at row r0 of the tile.
+template <typename T, int D, int KT, int N>
+struct TileLoad {
+  static constexpr int ES = (int)sizeof(T), ROWB = D * ES, CH = ROWB / 16, RP = 64 / CH;
+  const T* base;  // the sequence's first row
+  long ld;
+  uint32_t row_bytes, off[N];
+  int at;  // the first instruction's row of the tile
+  __device__ __forceinline__ TileLoad(const void* p, long row_ld, int k0, int hk, int r0) {
+    base = reinterpret_cast<const T*>(p) + (size_t)k0 * row_ld + (size_t)hk * D;
+    ld = row_ld;
+    row_bytes = (uint32_t)row_ld * ES;
+    at = r0;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < LW; ++j) {
-      uint4* at = reinterpret_cast<uint4*>(vs + 1024 * (LW * wave + j) + 16 * lane);
-      uint4 w = *at;
-      if (clear_odd<T>(w)) {
-        *at = w;
-        dirty = 1;
+    for (int j = 0; j < N; ++j) {
+      const int r = r0 + j * RP + lane / CH;
+      off[j] = (uint32_t)r * row_bytes + ((uint32_t)((lane % CH) ^ swizzle<ROWB, T, 32>(r)) << 4);
+    }
+  }
+  // The tile at place p0 of a sequence of nk keys, to LDS address `to`. Rows behind the last key are zeros.
+  __device__ __forceinline__ void issue(const KeyList& k, int nk, int p0, uint32_t to) const {
+    if (p0 >= k.s || k.shift == 0 || p0 + KT <= k.s) {  // rows that follow one another
+      const int row = k.position(p0);
+      const uint64_t from = (uint64_t)(uintptr_t)(base + (size_t)row * ld);
+      const RsrcWords rs = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)from),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(from >> 32) & 0xffffu)),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(min(KT, nk - row) - 1) * row_bytes + ROWB)),
+                            0x00020000u};
+#pragma unroll
+      for (int j = 0; j < N; ++j) load_lds(rs, off[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(to + 1024 * j)));
+    } else {  // the last sinks and the window's first keys
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));  // (nothing of this is kept across a loop)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int r = at + j * RP + lane / CH, row = k.position(p0 + r), c = (lane % CH) ^ swizzle<ROWB, T, 32>(r);
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(base + (size_t)row * ld) + 16 * c;
+        load_lds_from(row < nk ? (const void*)from : (const void*)zeros16,
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)(to + 1024 * j)));
       }
     }
+  }
+};
+
+// Zeros for what is not finite in the pieces of V that TileLoad's N instructions brought to `at`; whether there was anything.
+template <typename T, int N>
+__device__ __forceinline__ bool clean_tile(uint8_t* at) {
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    uint4* p = reinterpret_cast<uint4*>(at + 1024 * j + 16 * (threadIdx.x & 63));
+    uint4 w = *p;
+    if (clear_odd<T>(w)) {
+      *p = w;
+      any = true;
+    }
+  }
+  return any;
+}
+
+// One wave's 32 rows, a row a lane and its partner (lane ^ 32).
+template <typename T, int D, int KT>
+struct RowWave {
+  static constexpr bool BF = sizeof(T) == 2;
+  static constexpr int ES = (int)sizeof(T), ROWB = D * ES, ST = KT / 32, DT = D / 32, QF = D * ES / 32;
+  struct Scores {
+    af32x16 t[ST];
   };
-  auto compute = [&](int i, int stage) {
-    const int p0 = tiles.at(i) * KT;
-    // does a row of the wave see any of the tile, do all see all of it
-    if (p0 > wlast || (a.window > 0 && p0 + KT <= wfirst - a.window + 1 && p0 >= a.sinks)) return;
-    const bool whole = p0 + KT - 1 <= wfirst && (a.window == 0 || wlast - p0 < a.window || p0 + KT <= a.sinks);
-    const uint8_t *ks = &lds[stage][0], *vs = ks + KT * ROWB;
-    af32x16 st[ST] = {};
+  uint4 qf[QF];      // the query as the second operand: entries k of the lane's half
+  af32x16 o[DT];     // O^T
+  float top, sum;    // of the row; of the lane's keys
+  float c, lag;      // lag: how far the maximum may lag behind (weights up to 2^8)
+  int m, h, l, l4;   // row, half, lane of 16, group of 16 of the half
+
+  __device__ __forceinline__ void start(const WinArgs& a, const T* q) {
+    const int lane = threadIdx.x & 63;
+    m = lane & 31, h = lane >> 5, l = lane & 15, l4 = (lane >> 4) & 1;
+    c = a.c, lag = 8.f / a.c, top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < QF; ++t) qf[t] = *reinterpret_cast<const uint4*>(q + (BF ? 16 * t + 8 * h : 8 * t + 4 * h));
+    if (a.flip) {
+      constexpr uint32_t signs = BF ? 0x80008000u : 0x80000000u;
+#pragma unroll
+      for (int t = 0; t < QF; ++t) qf[t] = make_uint4(qf[t].x ^ signs, qf[t].y ^ signs, qf[t].z ^ signs, qf[t].w ^ signs);
+    }
+#pragma unroll
+    for (int t = 0; t < QF; ++t) asm volatile("" : "+v"(qf[t].x));  // (awaited here, not in the loop)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = af32x16{};
+  }
+  __device__ __forceinline__ uint4 key_frag(const uint8_t* ks, int t, int kk) const {
+    return *reinterpret_cast<const uint4*>(ks + row_chunk<ROWB, T, 32>(32 * t + m, 2 * kk + h));
+  }
+  __device__ __forceinline__ af32x16 score_step(const uint4& kf, int kk, af32x16 x) const {
+    if constexpr (BF) {
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8, kf), __builtin_bit_cast(abf16x8, qf[kk]), x, 0, 0, 0);
+    } else {
+      const uint32_t kw[4] = {kf.x, kf.y, kf.z, kf.w}, qw[4] = {qf[kk].x, qf[kk].y, qf[kk].z, qf[kk].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), x, 0, 0, 0);
+      return x;
+    }
+  }
+  // S^T: place 32 t + 8 (e / 4) + 4 h + e % 4 of the tile in t[t][e].
+  __device__ __forceinline__ void scores(const uint8_t* ks, Scores& s) const {
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      s.t[t] = af32x16{};
+#pragma unroll
+      for (int kk = 0; kk < QF; ++kk) s.t[t] = score_step(key_frag(ks, t, kk), kk, s.t[t]);
+    }
+  }
+  static __device__ __forceinline__ float largest(const Scores& s) {  // of the lane's
+    float best = s.t[0][0];
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(ks + row_chunk<ROWB, T>(32 * t + m, 2 * kk + h));
-        if constexpr (BF) {
-          st[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8, kf), __builtin_bit_cast(abf16x8, qf[kk]),
-                                                          st[t], 0, 0, 0);
-        } else {
-          const uint32_t kw[4] = {kf.x, kf.y, kf.z, kf.w}, qw[4] = {qf[kk].x, qf[kk].y, qf[kk].z, qf[kk].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            st[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), st[t], 0, 0, 0);
-        }
-      }
-    float best = -INFINITY;
+      for (int e = t == 0; e + 1 < 16; e += 2) best = fmaxf(fmaxf(best, s.t[t][e]), s.t[t][e + 1]);
+    return fmaxf(best, s.t[0][15]);
+  }
+  // What the row at place p does not see of the tile at p0; the lane's largest of the rest.
+  __device__ __forceinline__ float mask(const WinArgs& a, const KeyList& k, int p, int p0, Scores& s) const {
+    // (bounds on the lane's places, formed here: kept across a loop they took 64 registers)
+    int upto = p - p0 - 4 * h, sunk = k.sunk - p0 - 4 * h;
+    asm volatile("" : "+v"(upto), "+v"(sunk));
+    const int behind = a.window > 0 ? upto - a.window : -0x7fffffff;
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float x = st[t][e] * a.c;
-        if (!whole) {
-          const int j = p0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-          x = j <= p && (a.window == 0 || p - j < a.window || j < a.sinks) ? x : -INFINITY;
-        }
-        st[t][e] = x;
-        best = fmaxf(best, x);
+        const int j = 32 * t + 8 * (e >> 2) + (e & 3);
+        s.t[t][e] = j <= upto && (j > behind || j < sunk) ? s.t[t][e] : -INFINITY;
       }
+    return largest(s);
+  }
+  // The running maximum, and what goes by it, where it is more than `lag` behind.
+  __device__ __forceinline__ void settle(float best) {
     const auto pair = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
     const float next = fmaxf(top, fmaxf(__uint_as_float(pair[0]), __uint_as_float(pair[1])));
-    const float base = next == -INFINITY ? 0.f : next, keep = exp2_of(top - base);
-    top = next;
-    float add = 0.f;
-#pragma unroll
-    for (int t = 0; t < ST; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        st[t][e] = exp2_of(st[t][e] - base);
-        add += st[t][e];
-      }
-    sum = fmaf(sum, keep, add);
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][e] *= keep;
-    const int s = lane & 15;
-    if constexpr (BF) {
-#pragma unroll
-      for (int t = 0; t < ST; ++t)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {  // 16 keys
-          const abf16x8 pf = __builtin_bit_cast(
-              abf16x8, make_uint4(pack_bf16x2(st[t][8 * u], st[t][8 * u + 1]), pack_bf16x2(st[t][8 * u + 2], st[t][8 * u + 3]),
-                                  pack_bf16x2(st[t][8 * u + 4], st[t][8 * u + 5]), pack_bf16x2(st[t][8 * u + 6], st[t][8 * u + 7])));
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const int r = 32 * t + 16 * u + 4 * h + (s >> 2), c = 4 * d + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
-            const uint2 v0 = lds_transposed(vs + row_chunk<ROWB, T>(r, c) + 8 * (s & 1));
-            const uint2 v1 = lds_transposed(vs + row_chunk<ROWB, T>(r + 8, c) + 8 * (s & 1));
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8, make_uint4(v0.x, v0.y, v1.x, v1.y)), pf,
-                                                           o[d], 0, 0, 0);
-          }
-        }
-    } else {
+    if (__any(next > top + lag)) {
+      const float keep = exp2_of((top - (next == -INFINITY ? 0.f : next)) * c);
+      top = next;
+      sum *= keep;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = 8 * (e >> 2) + 4 * h + (e & 3);
-          const float v = *reinterpret_cast<const float*>(vs + row_chunk<ROWB, T>(r, 8 * d + (m >> 2)) + 4 * (m & 3));
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, st[0][e], o[d], 0, 0, 0);
-        }
+        for (int e = 0; e < 16; ++e) o[d][e] *= keep;
     }
-  };
-
-  if (threadIdx.x == 0) dirty = 0;
-  if (tiles.n > 0) issue(0, 0);
-  for (int i = 0; i < tiles.n; ++i) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the tile is there, the other stage read
-    if (i + 1 < tiles.n) issue(i + 1, (i + 1) & 1);
-    if (edge(tiles.at(i) * KT)) {
-      clean(i & 1);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    compute(i, i & 1);
   }
-
-  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-  sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-  const float inv = p < 0 ? 0.f : 1.f / sum;
+  __device__ __forceinline__ uint4 value_frag(const uint8_t* vs, int u, int d) const {  // bf16: 16 keys u, 32 columns d
+    const int r = 16 * u + 4 * h + (l >> 2), cc = 4 * d + 2 * l4 + ((l & 3) >> 1);
+    const uint2 v0 = lds_transposed(vs + row_chunk<ROWB, T, 32>(r, cc) + 8 * (l & 1));
+    const uint2 v1 = lds_transposed(vs + row_chunk<ROWB, T, 32>(r + 8, cc) + 8 * (l & 1));
+    return make_uint4(v0.x, v0.y, v1.x, v1.y);
+  }
+  // O^T + V^T P^T. AHEAD: beside it the scores of the next tile and the lane's largest of them, given out over the weights.
+  template <bool AHEAD>
+  __device__ __forceinline__ void add(const uint8_t* vs, Scores& s, const uint8_t* next_ks, Scores& ahead, float& best) {
+    const float base = top == -INFINITY ? 0.f : top * c;
+    if constexpr (BF) {
+      uint32_t w[2 * ST][4];
+      auto weigh = [&](int n) {  // two weights, rounded and summed (the sum of what the product takes)
+        const af32x16& x = s.t[n / 8];
+        const uint32_t y = pack_bf16x2(exp2_of(fmaf(x[2 * (n % 8)], c, -base)), exp2_of(fmaf(x[2 * (n % 8) + 1], c, -base)));
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(abf16x2, y), __builtin_bit_cast(abf16x2, 0x3f803f80u), sum, false);
+        w[n / 4][n % 4] = y;
+      };
+      constexpr int LATE = AHEAD ? 4 : 0;  // weights of the last 8 keys of the lane's, beside the product's first steps
+      if constexpr (AHEAD) {
+        uint4 kf[2][ST];
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+        for (int t = 0; t < ST; ++t) ahead.t[t] = af32x16{}, kf[0][t] = key_frag(next_ks, t, 0);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] *= inv;
-  uint32_t again = 0;  // the wave's rows that see what was zeroed
-  if (tiles.n > 0 && dirty) {
-    for (int i = 0; i < tiles.n; ++i) {
-      const int p0 = tiles.at(i) * KT, j = p0 + lane;
-      if (!edge(p0)) continue;
-      bool bad = false;
-      if (lane < KT && j < rt.nk)
-        for (int c = 0; c < CH; ++c) {
-          uint4 w = *reinterpret_cast<const uint4*>(vbase + (size_t)j * a.v_ld + c * (16 / ES));
-          bad = clear_odd<T>(w) || bad;
+        for (int kk = 0; kk < QF; ++kk) {
+          if (kk + 1 < QF)
+#pragma unroll
+            for (int t = 0; t < ST; ++t) kf[(kk + 1) & 1][t] = key_frag(next_ks, t, kk + 1);
+#pragma unroll
+          for (int t = 0; t < ST; ++t) ahead.t[t] = score_step(kf[kk & 1][t], kk, ahead.t[t]);
+#pragma unroll
+          for (int n = (8 * ST - LATE) * kk / QF; n < (8 * ST - LATE) * (kk + 1) / QF; ++n) weigh(n);
         }
-      if (__ballot(bad) == 0) continue;
-      for (int l = 0; l < 32; ++l) {
-        const int rp = __builtin_amdgcn_readlane(p, l);
-        if (__ballot(bad && j <= rp && (a.window == 0 || rp - j < a.window || j < a.sinks))) again |= 1u << l;
+      } else {
+#pragma unroll
+        for (int n = 0; n < 8 * ST; ++n) weigh(n);
+      }
+      uint4 vf[2][DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vf[0][d] = value_frag(vs, 0, d);
+#pragma unroll
+      for (int u = 0; u < 2 * ST; ++u) {
+        if (u + 1 < 2 * ST)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) vf[(u + 1) & 1][d] = value_frag(vs, u + 1, d);
+        const abf16x8 pf = __builtin_bit_cast(abf16x8, make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]));
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf16x8, vf[u & 1][d]), pf, o[d], 0, 0, 0);
+        if constexpr (AHEAD) {
+          if (u < 2) weigh(8 * ST - LATE + 2 * u), weigh(8 * ST - LATE + 2 * u + 1);
+          if (u == 2) best = largest(ahead);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s.t[0][e] = exp2_of(fmaf(s.t[0][e], c, -base));
+        sum += s.t[0][e];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+          const float v = *reinterpret_cast<const float*>(vs + row_chunk<ROWB, T, 32>(r, 8 * d + (m >> 2)) + 4 * (m & 3));
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s.t[0][e], o[d], 0, 0, 0);
+        }
+      if constexpr (AHEAD) {
+        scores(next_ks, ahead);
+        best = largest(ahead);
       }
     }
+  }
+  // The row's sum over both halves.
+  __device__ __forceinline__ float whole_sum() const {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  }
+};
+
+// Those of the wave's 32 rows (places p, a lane each) that see a value that is not finite in the tile at place p0. (Rare: from
+// global memory, a key a lane.)
+template <typename T, int D, typename R, int KT>
+__device__ __forceinline__ uint32_t rows_that_see_odd(const WinArgs& a, const R& r, const T* v, int p, int p0) {
+  const int lane = threadIdx.x & 63, u = p0 + lane, j = r.keys.position(u);
+  bool bad = false;
+  if (lane < KT && j < r.t.nk)
+    for (int c = 0; c < D * (int)sizeof(T) / 16; ++c) {
+      uint4 w = *reinterpret_cast<const uint4*>(v + (size_t)j * a.v_ld + c * (16 / (int)sizeof(T)));
+      bad = clear_odd<T>(w) || bad;
+    }
+  uint32_t found = 0;
+  if (__ballot(bad) != 0)
+    for (int l = 0; l < 32; ++l)
+      if (__ballot(bad && r.sees(a, __builtin_amdgcn_readlane(p, l), u))) found |= 1u << l;
+  return found;
+}
+
+// Many rows: a wave for each 32 of a workgroup's, all on the same tiles. The scores of a tile are formed beside the product of
+// the one before, so that matrix and vector instructions have each other to run beside; K is loaded a tile further ahead than V.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || D == 64 ? 2 : 1) void win_attn_kernel(WinArgs a) {
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32, ROWB = D * (int)sizeof(T), LW = KT * ROWB / 1024 / NW, ROWS = 32 * NW;
+  using Wave = RowWave<T, D, KT>;
+  using R = Rows<ROWS, KT>;
+  __shared__ __align__(1024) uint8_t k_lds[2][KT * ROWB], v_lds[2][KT * ROWB];
+  __shared__ int dirty;  // something of V was zeroed
+  const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+  R r;
+  if (!r.find(a, blockIdx.x / a.Hk, blockIdx.x % a.Hk)) return;
+  const uint32_t rw = r.r0 + 32 * wave, row = min(rw + m, r.rows - 1);  // (lanes behind the last row: as that one, without stores)
+  const bool real = rw + m < r.rows;
+  const int qi = (int)(row / r.G), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
+  const int shift = r.keys.shift, n = r.keys.n, p = r.past + qi - shift;
+  const int wfirst = r.past + (int)(min(r.rows - 1, rw) / r.G) - shift;
+  const int wlast = r.past + (int)((min(r.rows, rw + 32) - 1) / r.G) - shift;
+  constexpr int RP = 1024 / ROWB;
+  const TileLoad<T, D, KT, LW> load_k(a.k, a.k_ld, r.t.k0, r.hk, wave * LW * RP), load_v(a.v, a.v_ld, r.t.k0, r.hk, wave * LW * RP);
+  auto issue_k = [&](int i) { load_k.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&k_lds[i & 1][0] + 1024 * LW * wave); };
+  auto issue_v = [&](int i) { load_v.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&v_lds[i & 1][0] + 1024 * LW * wave); };
+
+  if (threadIdx.x == 0) dirty = 0;
+  if (n > 0) issue_k(0);
+  Wave w;
+  w.start(a, reinterpret_cast<const T*>(a.q) + (size_t)(r.t.q0 + qi) * a.q_ld + (size_t)hq * D);
+  using Scores = typename Wave::Scores;
+  auto settle = [&](int i, Scores& s, float best) {
+    if (!r.whole(a, KT * i, wfirst, wlast)) best = w.mask(a, r.keys, p, KT * i, s);
+    w.settle(best);
+  };
+  if (n > 0) {
+    if (n > 1) issue_k(1);
+    issue_v(0);
+    asm volatile("s_barrier" ::: "memory");  // (K of tile 0 is there: each wave has waited for its loads, with those of q)
+    Scores one, two;
+    w.scores(k_lds[0], one);
+    settle(0, one, w.largest(one));
+    // (the tile behind the last one is scored too, on what its stage holds, and not used)
+    auto step = [&](int i, Scores& s, Scores& ahead) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // V of tile i and K of the next are there
+      if (i + 2 < n) issue_k(i + 2);
+      if (i + 1 < n) issue_v(i + 1);
+      if (!r.whole(a, KT * i, r.first, r.last)) {
+        if (clean_tile<T, LW>(&v_lds[i & 1][1024 * LW * wave])) dirty = 1;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      float best;
+      w.template add<true>(v_lds[i & 1], s, k_lds[(i + 1) & 1], ahead, best);
+      if (i + 1 < n) settle(i + 1, ahead, best);
+    };
+    for (int i = 0;;) {
+      step(i, one, two);
+      if (++i >= n) break;
+      step(i, two, one);
+      if (++i >= n) break;
+    }
+  }
+
+  const float inv = p + shift < 0 ? 0.f : 1.f / w.whole_sum();
+  uint32_t again = 0;  // the wave's rows that see what was zeroed
+  if (n > 0 && dirty) {
+    for (int i = 0; i < n; ++i)
+      if (!r.whole(a, KT * i, r.first, r.last)) again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
     again &= (uint32_t)__ballot(real);
   }
   if (real && !(again >> m & 1)) {
-    T* orow = reinterpret_cast<T*>(a.o) + ((size_t)(rt.q0 + qi) * a.Hq + hq) * D;
+    T* orow = reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + qi) * a.Hq + hq) * D;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < Wave::DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        io<T>::store4(orow + 32 * d + 2 * e + 4 * h, make_float4(o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]));
+        io<T>::store4(orow + 32 * d + 2 * e + 4 * h,
+                      make_float4(w.o[d][e] * inv, w.o[d][e + 1] * inv, w.o[d][e + 2] * inv, w.o[d][e + 3] * inv));
   }
   while (again != 0) {
-    const int l = __builtin_ctz(again);
+    const int x = __builtin_ctz(again);
     again &= again - 1;
-    const int lq = __builtin_amdgcn_readlane(qi, l), lh = __builtin_amdgcn_readlane(hq, l), lp = __builtin_amdgcn_readlane(p, l);
-    win_row<T, D>(reinterpret_cast<const T*>(a.q) + (size_t)(rt.q0 + lq) * a.q_ld + (size_t)lh * D, kbase, a.k_ld, vbase,
-                  a.v_ld, reinterpret_cast<T*>(a.o) + ((size_t)(rt.q0 + lq) * a.Hq + lh) * D, lp, a.window, a.sinks, a.c);
+    redo_row<T, D>(a, r.t, load_k.base, load_v.base, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x));
   }
 }
 
-template <int ROWS>
-long row_tiles(const WinArgs& a) {
-  const int G = a.Hq / a.Hk;
-  if (a.cu_q == nullptr) return a.N * (((long)a.Tq * G + ROWS - 1) / ROWS);
-  return ((long)a.Tq * G + ROWS - 1) / ROWS + a.N;  // (each sequence may leave a part of a tile)
+// Few rows: a workgroup for 32 rows and a share of their tiles (a.splits), whose waves take them in turn, each with stages of
+// its own and no barrier; the waves' parts (maximum, sum, O) are joined in LDS, those of several workgroups by a second
+// kernel, in order.
+constexpr int FEW_NW = 4, FEW_KT = 32;
+template <typename T, int D>
+struct FewCfg {
+  static constexpr int TILE = 2 * FEW_KT * D * (int)sizeof(T);  // bytes of K and V
+  static constexpr int RING = TILE <= 16384 ? 2 : 1, PART = D + 4;
+  static_assert(RING * TILE >= 32 * PART * 4, "the waves' parts");
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
+  constexpr int KT = FEW_KT, ROWB = D * (int)sizeof(T), LI = KT * ROWB / 1024, RING = FewCfg<T, D>::RING, PART = FewCfg<T, D>::PART;
+  using Wave = RowWave<T, D, KT>;
+  using R = Rows<32, KT>;
+  __shared__ __align__(1024) uint8_t ring[FEW_NW][RING][2][KT * ROWB];
+  __shared__ float top_of[FEW_NW][32], sum_of[FEW_NW][32];
+  __shared__ uint32_t odd_of[FEW_NW];  // rows that see a value that is not finite in a tile with a mask
+  const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+  const int ts = blockIdx.x / a.Hk, split = ts % a.splits;
+  R r;
+  if (!r.find(a, ts / a.splits, blockIdx.x % a.Hk)) return;
+  const uint32_t row = min(r.r0 + m, r.rows - 1);
+  const int qi = (int)(row / r.G), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
+  const int p = r.past + qi - r.keys.shift;
+  const int t0 = (int)((long)r.keys.n * split / a.splits), t1 = (int)((long)r.keys.n * (split + 1) / a.splits);
+  const TileLoad<T, D, KT, LI> load_k(a.k, a.k_ld, r.t.k0, r.hk, 0), load_v(a.v, a.v_ld, r.t.k0, r.hk, 0);
+  auto issue = [&](int i, int stage) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what the stage held before has been read
+    load_k.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&ring[wave][stage][0][0]);
+    load_v.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&ring[wave][stage][1][0]);
+  };
+  if (t0 + wave < t1) issue(t0 + wave, 0);
+  Wave w;
+  w.start(a, reinterpret_cast<const T*>(a.q) + (size_t)(r.t.q0 + qi) * a.q_ld + (size_t)hq * D);
+  uint32_t again = 0;
+  auto compute = [&](int i, int stage) {
+    typename Wave::Scores s;
+    float best;
+    w.scores(ring[wave][stage][0], s);
+    if (r.whole(a, KT * i, r.first, r.last)) {
+      best = w.largest(s);
+    } else {
+      if (__ballot(clean_tile<T, LI>(ring[wave][stage][1])) != 0)
+        again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
+      best = w.mask(a, r.keys, p, KT * i, s);
+    }
+    w.settle(best);
+    w.template add<false>(ring[wave][stage][1], s, nullptr, s, best);
+  };
+  for (int i = t0 + wave, stage = 0; i < t1; i += FEW_NW, stage ^= RING - 1) {
+    if (RING == 2 && i + FEW_NW < t1) {
+      issue(i + FEW_NW, stage ^ 1);
+      wait_own_loads<2 * LI>();
+    } else {
+      wait_own_loads<0>();
+    }
+    compute(i, stage);
+    if (RING == 1 && i + FEW_NW < t1) issue(i + FEW_NW, 0);
+  }
+
+  const float sum = w.whole_sum();
+  __syncthreads();
+  float* mine = reinterpret_cast<float*>(&ring[wave][0][0][0]) + m * PART;
+#pragma unroll
+  for (int d = 0; d < Wave::DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4*>(mine + 32 * d + 2 * e + 4 * h) = make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+  if (h == 0) {
+    top_of[wave][m] = w.top;
+    sum_of[wave][m] = sum;
+  }
+  if ((threadIdx.x & 63) == 0) odd_of[wave] = again;
+  __syncthreads();
+  uint32_t odd = 0;
+#pragma unroll
+  for (int x = 0; x < FEW_NW; ++x) odd |= odd_of[x];
+  for (int i = threadIdx.x; i < 32 * D / 4; i += 64 * FEW_NW) {
+    const int x = i / (D / 4), d = i % (D / 4) * 4;
+    if (r.r0 + x >= r.rows) continue;
+    float best = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < FEW_NW; ++y) best = fmaxf(best, top_of[y][x]);
+    const float base = best == -INFINITY ? 0.f : best;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float all = 0.f;
+#pragma unroll
+    for (int y = 0; y < FEW_NW; ++y) {
+      const float f = exp2_of((top_of[y][x] - base) * a.c);
+      const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&ring[y][0][0][0]) + x * PART + d);
+      v = make_float4(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w));
+      all = fmaf(sum_of[y][x], f, all);
+    }
+    if (a.splits > 1) {
+      const size_t at = (size_t)blockIdx.x * 32 + x;
+      *reinterpret_cast<float4*>(a.part_o + at * D + d) = v;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(best, odd >> x & 1 ? -1.f : all);
+    } else if (!(odd >> x & 1)) {
+      const uint32_t rr = r.r0 + x;
+      const int q = (int)(rr / r.G), hh = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
+      const float inv = r.past + q < 0 ? 0.f : 1.f / all;
+      io<T>::store4(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + q) * a.Hq + hh) * D + d,
+                    make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
+  }
+  if (a.splits > 1) return;
+  for (int x = wave; x < 32; x += FEW_NW)
+    if ((odd >> x & 1) && r.r0 + x < r.rows)
+      redo_row<T, D>(a, r.t, load_k.base, load_v.base, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x));
 }
 
-template <typename T, int D, int NW>
-bool launch_win_rows(WinArgs a, hipStream_t s) {
-  const long tiles = row_tiles<32 * NW>(a);
-  if (tiles * a.Hk > (1L << 32) / (64 * NW) - 1) return false;
-  a.tiles = (int)tiles;
-  hipLaunchKernelGGL((win_attn_kernel<T, D, NW>), dim3((unsigned)(tiles * a.Hk)), dim3(64 * NW), 0, s, a);
-  return true;
-}
-// Rows of a workgroup: as many as leave one for every CU.
+// A workgroup joins the parts of 8 rows, D / 4 lanes each.
 template <typename T, int D>
-bool launch_win(const WinArgs& a, hipStream_t s) {
+__global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
+  using R = Rows<32, FEW_KT>;
+  const int t8 = blockIdx.x / a.Hk, tile = t8 / 4;
+  R r;
+  if (!r.find(a, tile, blockIdx.x % a.Hk)) return;
+  const int x = (t8 & 3) * 8 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const bool real = r.r0 + x < r.rows;
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool odd = false;
+  constexpr int AT = 4;  // parts read at a time
+  for (int i0 = 0; i0 < a.splits; i0 += AT) {
+    float2 ml[AT];
+    float4 u[AT];
+#pragma unroll
+    for (int e = 0; e < AT; ++e) {
+      const size_t at = ((size_t)(tile * a.splits + min(i0 + e, a.splits - 1)) * a.Hk + r.hk) * 32 + (real ? x : 0);
+      ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+      u[e] = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
+    }
+#pragma unroll
+    for (int e = 0; e < AT; ++e)
+      if (i0 + e < a.splits) {
+        const float next = fmaxf(top, ml[e].x), base = next == -INFINITY ? 0.f : next;
+        const float keep = exp2_of((top - base) * a.c), f = exp2_of((ml[e].x - base) * a.c);
+        top = next;
+        odd = odd || ml[e].y < 0.f;
+        sum = fmaf(sum, keep, ml[e].y * f);
+        v = make_float4(fmaf(v.x, keep, u[e].x * f), fmaf(v.y, keep, u[e].y * f), fmaf(v.z, keep, u[e].z * f),
+                        fmaf(v.w, keep, u[e].w * f));
+      }
+  }
+  const uint32_t rr = min(r.r0 + x, r.rows - 1);
+  const int q = (int)(rr / r.G), hq = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
+  odd = odd && real;
+  if (real && !odd) {
+    const float inv = r.past + q < 0 ? 0.f : 1.f / sum;
+    io<T>::store4(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + q) * a.Hq + hq) * D + d,
+                  make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+  }
+  const T* kb = reinterpret_cast<const T*>(a.k) + (size_t)r.t.k0 * a.k_ld + (size_t)r.hk * D;
+  const T* vb = reinterpret_cast<const T*>(a.v) + (size_t)r.t.k0 * a.v_ld + (size_t)r.hk * D;
+  for (uint64_t left = __ballot(odd && d == 0); left != 0; left &= left - 1) {  // (a row's lanes are of one wave)
+    const int lane = __builtin_ctzll(left);
+    redo_row<T, D>(a, r.t, kb, vb, __builtin_amdgcn_readlane(q, lane), __builtin_amdgcn_readlane(hq, lane));
+  }
+}
+
+// How a call is cut. Where 128 rows a workgroup leave CUs without any, 32 rows and a share of the keys: as many shares as
+// there are CUs for, of two tiles for each wave at least.
+struct WinPlan {
+  long tiles;  // of rows a key head
+  int rows, splits;
+};
+long row_tiles(const WinArgs& a, int rows) {
+  const long all = (long)a.Tq * (a.Hq / a.Hk);
+  if (a.cu_q == nullptr) return a.N * ((all + rows - 1) / rows);
+  return (all + rows - 1) / rows + a.N;  // (each sequence may leave a part of a tile)
+}
+WinPlan win_plan(const WinArgs& a) {
+  WinPlan p;
   const long cus = device_cus();
-  if (row_tiles<256>(a) * a.Hk >= cus) return launch_win_rows<T, D, 8>(a, s);
-  if (row_tiles<128>(a) * a.Hk >= cus) return launch_win_rows<T, D, 4>(a, s);
-  return launch_win_rows<T, D, 2>(a, s);
+  p.rows = 128, p.splits = 1;
+  p.tiles = row_tiles(a, 128);
+  if (p.tiles * a.Hk >= cus) return p;
+  p.rows = 32;
+  p.tiles = row_tiles(a, 32);
+  long keys = a.Tk;
+  if (a.window > 0) keys = std::min(keys, (long)a.window + 32 + a.sinks);
+  const long most = std::max(1L, keys / (2 * FEW_NW * FEW_KT));
+  p.splits = (int)std::max(1L, std::min(most, cus / (p.tiles * a.Hk)));
+  return p;
+}
+size_t win_bytes(const WinPlan& p, const WinArgs& a, int D) {
+  return p.splits == 1 ? 0 : (size_t)p.tiles * a.Hk * p.splits * 32 * (D + 2) * sizeof(float);
+}
+
+template <typename T, int D>
+void launch_win(WinArgs a, const WinPlan& p, hipStream_t s) {
+  a.tiles = (int)p.tiles;
+  a.splits = p.splits;
+  const unsigned n = (unsigned)(p.tiles * a.Hk);
+  if (p.rows == 128) {
+    hipLaunchKernelGGL((win_attn_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, a);
+    return;
+  }
+  hipLaunchKernelGGL((win_few_kernel<T, D>), dim3(n * p.splits), dim3(64 * FEW_NW), 0, s, a);
+  if (p.splits > 1) hipLaunchKernelGGL((win_few_join_kernel<T, D>), dim3(4 * n), dim3(2 * D), 0, s, a);
+}
+
+bool win_sizes(int B, int Tq, int Tk, int Hq, int Hk, int D, int window, int sinks, int dtype) {
+  return B >= 1 && Tq >= 0 && Tk >= 0 && Hq >= 1 && Hk >= 1 && Hq % Hk == 0 && (D == 64 || D == 128) && window >= 0 &&
+         sinks >= 0 && (dtype == ZGDN_F32 || dtype == ZGDN_BF16) && (long)B * Tq <= 1L << 30 && (long)B * Tk <= 1L << 30 &&
+         (long)B * Tq * Hq <= 1L << 31;
 }
 
 }  // namespace
 }  // namespace zgdn
 
+extern "C" size_t zattn_window_fwd_workspace_bytes(int packed, int n_seqs, int Tq, int Tk, int Hq, int Hk, int D, int window,
+                                                   int sinks, int dtype) {
+  using namespace zgdn;
+  if (n_seqs < 1 || !win_sizes(packed ? 1 : n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, dtype) || Tq == 0) return 0;
+  WinArgs a{};
+  const int32_t bounds = 0;  // (told from none by its address alone)
+  a.cu_q = packed ? &bounds : nullptr;
+  a.N = n_seqs, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hk = Hk, a.window = window, a.sinks = sinks;
+  return win_bytes(win_plan(a), a, D);
+}
+
 extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
                                 void* o, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int B, int Tq, int Tk, int Hq,
-                                int Hk, int D, int window, int sinks, float scale, void* stream) {
+                                int Hk, int D, int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace zgdn;
   const char* fn = "zattn_window_fwd";
   if (B < 1 || Tq < 0 || Tk < 0 || Hq < 1 || Hk < 1 || window < 0 || sinks < 0)
@@ -392,20 +765,30 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
     return fail(ZGDN_EINVAL, "%s: row strides q=%ld k=%ld v=%ld (multiples of %d elements, at least a row, at most 2^22)", fn,
                 q_ld, k_ld, v_ld, ve);
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 16)
-    return fail(ZGDN_EINVAL, "%s: q, k, v and o need 16-byte aligned bases", fn);
+    return fail(ZGDN_EINVAL, "%s: q, k, v, o and workspace need 16-byte aligned bases", fn);
   if (((uintptr_t)cu_q | (uintptr_t)cu_k) % 4) return fail(ZGDN_EINVAL, "%s: cu_q, cu_k not on 4-byte boundaries", fn);
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
-  const Region out = {o, nq, wq * es, wq * es};
+  WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
+            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 1, nullptr, nullptr};
+  const WinPlan p = win_plan(a);
+  if (p.tiles * p.splits * Hk > (1L << 32) / 256 - 1) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
+  const size_t need = win_bytes(p, a, D);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(ZGDN_EINVAL, "%s: workspace of %zu bytes, %zu needed", fn, workspace == nullptr ? 0 : workspace_bytes, need);
+  const Region out = {o, nq, wq * es, wq * es}, ws = {need ? workspace : nullptr, 1, need, need};
   const Region in[] = {{q, nq, wq * es, q_ld * es}, {k, nk, wk * es, k_ld * es}, {v, nk, wk * es, v_ld * es},
                        {cu_q, 1, cu, cu}, {cu_k, 1, cu, cu}};
-  bool meet = false;
-  for (const Region& r : in) meet = meet || regions_meet(out, r);
-  if (meet) return fail(ZGDN_EINVAL, "%s: o overlaps another operand", fn);
-  WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
-            scale * LOG2E, 0};
+  bool meet = regions_meet(out, ws);
+  for (const Region& r : in) meet = meet || regions_meet(out, r) || regions_meet(ws, r);
+  if (meet) return fail(ZGDN_EINVAL, "%s: o or the workspace overlaps another operand", fn);
+  if (need > 0) {
+    a.part_o = reinterpret_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)p.tiles * Hk * p.splits * 32 * D;
+  }
   hipStream_t s = (hipStream_t)stream;
-  const bool ok = dtype == ZGDN_F32 ? (D == 128 ? launch_win<float, 128>(a, s) : launch_win<float, 64>(a, s))
-                                    : (D == 128 ? launch_win<bf16, 128>(a, s) : launch_win<bf16, 64>(a, s));
-  if (!ok) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
+  if (dtype == ZGDN_F32)
+    D == 128 ? launch_win<float, 128>(a, p, s) : launch_win<float, 64>(a, p, s);
+  else
+    D == 128 ? launch_win<bf16, 128>(a, p, s) : launch_win<bf16, 64>(a, p, s);
   return check_launch(fn);
 }

@@ -40,20 +40,33 @@ struct WinStepArgs {
   float *part_o, *part_ml;  // [unit][split][gq][D], [unit][split][gq][2]
 };
 
-__device__ __attribute__((aligned(16))) const uint32_t zeros16[4] = {0, 0, 0, 0};
-
 template <typename T>
 struct WsCfg {
   static constexpr int TILE = sizeof(T) == 2 ? 32 : 16;
 };
 
-// The positions that stream b's query sees, in tiles.
+// Position-aligned tiles of TILE keys that the query at position `at` sees: those of the sinks, then those from the window's
+// start on.
+struct KeyTiles {
+  int sinks, from, n;  // tiles of the sinks, the first of the window's, all
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : from + (i - sinks); }
+};
+template <int TILE>
+__device__ __forceinline__ KeyTiles key_tiles(int at, int window, int sinks) {
+  KeyTiles t;
+  const int lo = window > 0 ? max(0, at - window + 1) : 0;
+  t.from = lo / TILE;
+  t.sinks = min((min(sinks, lo) + TILE - 1) / TILE, t.from);
+  t.n = at < 0 ? 0 : t.sinks + at / TILE + 1 - t.from;
+  return t;
+}
+// Those of stream b.
 template <int TILE>
 __device__ __forceinline__ KeyTiles stream_tiles(const WinStepArgs& a, int b, int& n, int& lo) {
   const long room = (long)a.page_size * a.n_pages;
   n = (int)max(0L, min((long)a.lengths[b], room));
   lo = a.window > 0 ? max(0, n - a.window) : 0;
-  return key_tiles<TILE>(n - 1, n - 1, a.window, a.sinks);
+  return key_tiles<TILE>(n - 1, a.window, a.sinks);
 }
 
 // NW waves of RING stages each: two waves of two, so that two workgroups (four and more at D = 64) share a CU and the start of
@@ -128,7 +141,7 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
 #pragma unroll
   for (int j = 0; j < LI; ++j) {
     const int r = j * RP + lane / CH;
-    const uint32_t c = (uint32_t)((lane % CH) ^ swizzle<ROWB, T>(r)) << 4;
+    const uint32_t c = (uint32_t)((lane % CH) ^ swizzle<ROWB, T, 16>(r)) << 4;
     koff[j] = (uint32_t)r * (uint32_t)kl + c;
     voff[j] = (uint32_t)r * (uint32_t)vl + c;
   }
@@ -151,7 +164,7 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
 #pragma unroll
     for (int j = 0; j < LI; ++j) {
       const int r = j * RP + lane / CH, p = p0 + r;
-      const size_t c = (size_t)(((lane % CH) ^ swizzle<ROWB, T>(r)) << 4);
+      const size_t c = (size_t)(((lane % CH) ^ swizzle<ROWB, T, 16>(r)) << 4);
       const bool s = seen(i, p);
       size_t row = (size_t)b * a.page_size + p;
       if (a.pages != nullptr) row = (size_t)page_of[i * per_tile + r / gran] * a.page_size + (p & (a.page_size - 1));
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
     for (int t = 0; t < ST; ++t) {
 #pragma unroll
       for (int kk = 0; kk < (int)(sizeof(qf) / 16); ++kk) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(ks + row_chunk<ROWB, T>(16 * t + m, 4 * kk + g));
+        const uint4 kf = *reinterpret_cast<const uint4*>(ks + row_chunk<ROWB, T, 16>(16 * t + m, 4 * kk + g));
         if constexpr (BF) {
           st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(abf16x8, kf), __builtin_bit_cast(abf16x8, qf[kk]),
                                                           st[t], 0, 0, 0);
@@ -225,8 +238,8 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const int r = 4 * g + (s >> 2), c = 2 * d + ((s & 3) >> 1), low = 8 * (s & 1);
-        const uint2 v0 = lds_transposed(vs + row_chunk<ROWB, T>(r, c) + low);
-        const uint2 v1 = lds_transposed(vs + row_chunk<ROWB, T>(r + 16, c) + low);
+        const uint2 v0 = lds_transposed(vs + row_chunk<ROWB, T, 16>(r, c) + low);
+        const uint2 v1 = lds_transposed(vs + row_chunk<ROWB, T, 16>(r + 16, c) + low);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(abf16x8, make_uint4(v0.x, v0.y, v1.x, v1.y)), pf,
                                                        o[d], 0, 0, 0);
       }
@@ -235,7 +248,7 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = *reinterpret_cast<const float*>(vs + row_chunk<ROWB, T>(4 * g + e, 4 * d + (s >> 2)) + 4 * (s & 3));
+          const float v = *reinterpret_cast<const float*>(vs + row_chunk<ROWB, T, 16>(4 * g + e, 4 * d + (s >> 2)) + 4 * (s & 3));
           o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, st[0][e], o[d], 0, 0, 0);
         }
     }

@@ -1388,9 +1388,11 @@ def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, 
         if cu_seqlens_k.numel() != n_seqs + 1:
             raise RuntimeError(f"cu_seqlens_k: {cu_seqlens_k.numel()} entries, expected {n_seqs + 1} as cu_seqlens")
     o = q.new_empty(q.shape)
+    size = _window_fwd_workspace(int(cu_seqlens is not None), n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, code)
+    workspace = o.new_empty(size, dtype=torch.uint8) if size else None
     _launch(index, dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
             _ptr(cu_seqlens), _ptr(cu_seqlens_k), n_seqs, B, Tq, Tk, Hq, Hk, D, window, sinks,
-            D**-0.5 if scale is None else scale)
+            D**-0.5 if scale is None else scale, _ptr(workspace), size)
     if q.requires_grad or k.requires_grad or v.requires_grad:
         o = _recorded("window_attn_fwd", o, q, k, v)
     return o
@@ -1404,6 +1406,11 @@ def _bounds_table(cu, total: int, dev):
         cu = torch.tensor(cu, dtype=torch.int32).to(dev)
     _cu_check(cu, total, dev)
     return cu
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_fwd_workspace(*sizes: int) -> int:
+    return int(_native.lib().zattn_window_fwd_workspace_bytes(*sizes))
 
 
 @functools.lru_cache(maxsize=1024)

@@ -1,6 +1,8 @@
 // What the attention kernels share: tiles of K and V rows in LDS, loads straight into them, MFMA fragments.
 #pragma once
 
+#include <atomic>
+
 #include "gdn_common.h"
 
 namespace zgdn {
@@ -31,6 +33,17 @@ __device__ __forceinline__ int row_chunk(int r, int c) {
 // row s / 4, columns 4 (s % 4) .., and gets the 4 rows' entries of column s.
 __device__ __forceinline__ uint2 lds_transposed(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ashort4*)p));
+}
+
+// Reads by an address within LDS.
+typedef uint32_t au32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const au32x4* LdsPieces;
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)p; }  // (the low half)
+__device__ __forceinline__ uint4 lds_piece(uint32_t at) {
+  return __builtin_bit_cast(uint4, *(LdsPieces)(uintptr_t)at);
+}
+__device__ __forceinline__ uint2 lds_transposed(uint32_t at) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ashort4*)(uintptr_t)at));
 }
 
 // 16 bytes a lane straight into LDS, lane i at lds + 16 i (lds: an address within LDS, wave-uniform), from the lane's own
@@ -65,6 +78,19 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // (one instruction; below 2^-126: 0)
+
+// Lets `kernel` have `bytes` of dynamic LDS on the current device, once a device; false where the device refuses.
+constexpr int MAX_DEVICES = 64;
+inline bool lds_ready(const void* kernel, int bytes, std::atomic<signed char>* ready) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return false;
+  const signed char was = ready[dev].load(std::memory_order_acquire);
+  if (was != 0) return was > 0;
+  const bool ok = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+  if (!ok) (void)hipGetLastError();
+  ready[dev].store(ok ? 1 : -1, std::memory_order_release);
+  return ok;
+}
 
 constexpr float LOG2E = 1.44269504088896340736f;
 

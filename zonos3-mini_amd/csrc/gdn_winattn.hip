@@ -10,10 +10,12 @@
 // Tiles of K and V are loaded straight into LDS, a tile ahead. Tiles that no row sees are left out, tiles that all rows of a
 // wave see whole have no mask.
 // Scores, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
-// A masked weight is 0, but 0 times an infinity or a NaN of V is a NaN: in tiles that a row of the workgroup does not see
-// whole, such entries are zeroed in LDS ahead of the product, and the rows that see one of them are computed again in the end,
-// key by key (win_row).
+// A masked weight is 0, but 0 times an infinity or a NaN of V is a NaN. A workgroup with an output that is not finite computes
+// its rows once more, and in tiles that a row of it does not see whole zeroes such entries in LDS ahead of the product; the
+// rows that see one of them are then computed again key by key (win_row). (Cleaned at once, with a barrier more, such tiles cost
+// 32768 tokens through a window of 1024 9 us of 329.)
 #include <algorithm>
+#include <atomic>
 
 #include "gdn_attn.h"
 #include "zonos3_attn.h"
@@ -30,6 +32,7 @@ struct WinArgs {
   float c;    // |scale| log2(e)
   int flip;   // scale below zero: the queries change their signs
   int tiles;  // of rows a key head, at most
+  int paired;               // two workgroups a CU hold the whole call
   int splits;               // workgroups that share a tile of 32 rows
   float *part_o, *part_ml;  // [workgroup][32][D], [workgroup][32][2]
 };
@@ -44,7 +47,9 @@ __device__ __forceinline__ int prefix_count(int x) {  // over the lanes up to th
   return x;
 }
 
-// The rows that a workgroup takes: tile `tile` of a sequence's nq G rows, the last tiles first (they have the most keys).
+// The rows that a workgroup takes: tile `tile` of a sequence's nq G rows, the last tiles first (they have the most keys). Where
+// all workgroups are on the device at one time (paired), the first tiles come second, so that CUs have one of many keys and one
+// of few (4096 tokens, 16 heads: 93 -> 88 us; 8192 tokens, 8 heads 176 -> 167).
 struct RowTile {
   int q0, nq, k0, nk, tile;  // (q0, k0: the sequence's first row of q and of k)
 };
@@ -53,7 +58,8 @@ __device__ __forceinline__ bool find_rows(const WinArgs& a, int i, RowTile& t) {
   const int G = a.Hq / a.Hk;
   if (a.cu_q == nullptr) {
     const int per = a.tiles / a.N, s = i % a.N;
-    t = {s * a.Tq, a.Tq, s * a.Tk, a.Tk, per - 1 - i / a.N};
+    const int j = i / a.N;
+    t = {s * a.Tq, a.Tq, s * a.Tk, a.Tk, a.paired && 2 * j >= per ? j - (per + 1) / 2 : per - 1 - j};
     return true;
   }
   const int l = threadIdx.x & 63;
@@ -152,6 +158,11 @@ __device__ __forceinline__ KeyList key_list(const WinArgs& a, int first, int las
   return k;
 }
 
+struct WholeTiles {
+  int to, from, sunk;  // those below `to` from `from` on, or below `sunk`
+  __device__ __forceinline__ bool has(int i) const { return i < to && (i >= from || i < sunk); }
+};
+
 // A workgroup's rows of a sequence and key head, and their keys. Positions, from here on, are places of the list's second part
 // (p - shift): differences and bounds are the same.
 template <int ROWS, int KT>
@@ -174,25 +185,32 @@ struct Rows {
     last -= keys.shift;
     return true;
   }
-  // Do rows at places f .. l all see the whole tile at place p0?
-  __device__ __forceinline__ bool whole(const WinArgs& a, int p0, int f, int l) const {
-    return p0 + KT - 1 <= f && (a.window == 0 || l - max(p0, keys.sunk) < a.window || p0 + KT <= keys.sunk);
+  // The tiles that rows at places f .. l all see whole.
+  __device__ __forceinline__ WholeTiles whole(const WinArgs& a, int f, int l) const {
+    WholeTiles w;
+    w.to = f < 0 ? 0 : (f + 1) / KT;
+    w.from = a.window == 0 || keys.sunk > l - a.window ? 0 : (l - a.window) / KT + 1;
+    w.sunk = keys.sunk / KT;
+    return w;
   }
   __device__ __forceinline__ bool sees(const WinArgs& a, int p, int u) const {
     return u <= p && (a.window == 0 || p - u < a.window || u < keys.sunk);
   }
 };
 
-// Loads of a tile's rows of K or V straight into LDS by N instructions of a wave, the first at row r0 of the tile.
+// Loads of the tiles of K or of V straight into LDS, one after the other, by N instructions of a wave each, the first at row
+// `at` of a tile. (What a tile costs in scalar instructions counts: a wave issues one instruction in four or five cycles.)
 template <typename T, int D, int KT, int N>
-struct TileLoad {
+struct TileLoads {
   static constexpr int ES = (int)sizeof(T), ROWB = D * ES, CH = ROWB / 16, RP = 64 / CH;
   const T* base;  // the sequence's first row
   long ld;
   uint32_t row_bytes, off[N];
-  int at;  // the first instruction's row of the tile
-  __device__ __forceinline__ TileLoad(const void* p, long row_ld, int k0, int hk, int r0) {
-    base = reinterpret_cast<const T*>(p) + (size_t)k0 * row_ld + (size_t)hk * D;
+  int at, next, last, split;    // the next tile; the last one; the one where the list's parts meet
+  uint64_t from;                // of the next tile's first row
+  uint32_t tile_bytes, last_bytes;
+  __device__ __forceinline__ TileLoads(const void* p, long row_ld, const RowTile& t, int hk, int r0) {
+    base = reinterpret_cast<const T*>(p) + (size_t)t.k0 * row_ld + (size_t)hk * D;
     ld = row_ld;
     row_bytes = (uint32_t)row_ld * ES;
     at = r0;
@@ -203,15 +221,20 @@ struct TileLoad {
       off[j] = (uint32_t)r * row_bytes + ((uint32_t)((lane % CH) ^ swizzle<ROWB, T, 32>(r)) << 4);
     }
   }
-  // The tile at place p0 of a sequence of nk keys, to LDS address `to`. Rows behind the last key are zeros.
-  __device__ __forceinline__ void issue(const KeyList& k, int nk, int p0, uint32_t to) const {
-    if (p0 >= k.s || k.shift == 0 || p0 + KT <= k.s) {  // rows that follow one another
-      const int row = k.position(p0);
-      const uint64_t from = (uint64_t)(uintptr_t)(base + (size_t)row * ld);
+  // From tile i on. Rows behind the last of nk keys are zeros.
+  __device__ __forceinline__ void start(const KeyList& k, int nk, int i) {
+    next = i;
+    last = k.n - 1;
+    split = k.s > 0 && k.shift > 0 ? k.s / KT : -1;
+    tile_bytes = (KT - 1) * row_bytes + ROWB;
+    last_bytes = (uint32_t)(min(KT, nk - (KT * last + k.shift)) - 1) * row_bytes + ROWB;  // (where the parts do not meet in it)
+    from = (uint64_t)(uintptr_t)(base + (size_t)(KT * i + (i > split ? k.shift : 0)) * ld);
+  }
+  __device__ __forceinline__ void issue(const KeyList& k, int nk, uint32_t to) {
+    if (next != split) {
       const RsrcWords rs = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)from),
                             (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(from >> 32) & 0xffffu)),
-                            (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(min(KT, nk - row) - 1) * row_bytes + ROWB)),
-                            0x00020000u};
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)(next == last ? last_bytes : tile_bytes)), 0x00020000u};
 #pragma unroll
       for (int j = 0; j < N; ++j) load_lds(rs, off[j], (uint32_t)__builtin_amdgcn_readfirstlane((int)(to + 1024 * j)));
     } else {  // the last sinks and the window's first keys
@@ -219,12 +242,15 @@ struct TileLoad {
       asm volatile("" : "+v"(lane));  // (nothing of this is kept across a loop)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int r = at + j * RP + lane / CH, row = k.position(p0 + r), c = (lane % CH) ^ swizzle<ROWB, T, 32>(r);
-        const uint8_t* from = reinterpret_cast<const uint8_t*>(base + (size_t)row * ld) + 16 * c;
-        load_lds_from(row < nk ? (const void*)from : (const void*)zeros16,
+        const int r = at + j * RP + lane / CH, row = k.position(KT * next + r), c = (lane % CH) ^ swizzle<ROWB, T, 32>(r);
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(base + (size_t)row * ld) + 16 * c;
+        load_lds_from(row < nk ? (const void*)p : (const void*)zeros16,
                       (uint32_t)__builtin_amdgcn_readfirstlane((int)(to + 1024 * j)));
       }
+      from += (uint64_t)k.shift * row_bytes;
     }
+    from += (uint64_t)KT * row_bytes;
+    ++next;
   }
 };
 
@@ -271,11 +297,34 @@ struct RowWave {
     }
 #pragma unroll
     for (int t = 0; t < QF; ++t) asm volatile("" : "+v"(qf[t].x));  // (awaited here, not in the loop)
+    float zero = 0.f;
+    asm volatile("" : "+v"(zero));  // (a constant tuple would be kept in registers for the next start)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = af32x16{};
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = zero;
   }
-  __device__ __forceinline__ uint4 key_frag(const uint8_t* ks, int t, int kk) const {
-    return *reinterpret_cast<const uint4*>(ks + row_chunk<ROWB, T, 32>(32 * t + m, 2 * kk + h));
+  // Where a stage's fragments are for the lane. Those of the other steps differ in some bits of the address alone (rows 32
+  // apart have one mask, rows 8 apart masks that differ in one bit). Formed for each stage anew: the addresses of all steps,
+  // kept across a loop, took 16 registers.
+  __device__ __forceinline__ uint32_t key_at(const uint8_t* ks) const {
+    uint32_t at = lds_address(ks) + row_chunk<ROWB, T, 32>(m, h);
+    asm volatile("" : "+v"(at));
+    return at;
+  }
+  static __device__ __forceinline__ uint4 key_frag(uint32_t at, int t, int kk) {  // rows 32 t + m, piece 2 kk + h
+    return lds_piece((at ^ (kk << 5)) + 32 * t * ROWB);
+  }
+  __device__ __forceinline__ uint32_t value_at(const uint8_t* vs) const {
+    uint32_t at = lds_address(vs) + row_chunk<ROWB, T, 32>(4 * h + (l >> 2), 2 * l4 + ((l & 3) >> 1)) + 8 * (l & 1);
+    asm volatile("" : "+v"(at));
+    return at;
+  }
+  static __device__ __forceinline__ uint4 value_frag(uint32_t at, int u, int d) {  // bf16: 16 keys u, 32 columns d
+    constexpr int FLIP = (swizzle<ROWB, T, 32>(0) ^ swizzle<ROWB, T, 32>(8)) << 4;
+    const uint2 v0 = lds_transposed((at ^ (d << 6)) + 16 * u * ROWB);
+    const uint2 v1 = lds_transposed((at ^ (d << 6) ^ FLIP) + (16 * u + 8) * ROWB);
+    return make_uint4(v0.x, v0.y, v1.x, v1.y);
   }
   __device__ __forceinline__ af32x16 score_step(const uint4& kf, int kk, af32x16 x) const {
     if constexpr (BF) {
@@ -289,11 +338,23 @@ struct RowWave {
   }
   // S^T: place 32 t + 8 (e / 4) + 4 h + e % 4 of the tile in t[t][e].
   __device__ __forceinline__ void scores(const uint8_t* ks, Scores& s) const {
+    const uint32_t at = key_at(ks);
+    if constexpr (BF) {
 #pragma unroll
-    for (int t = 0; t < ST; ++t) {
-      s.t[t] = af32x16{};
+      for (int t = 0; t < ST; ++t) {
+        s.t[t] = af32x16{};
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) s.t[t] = score_step(key_frag(ks, t, kk), kk, s.t[t]);
+        for (int kk = 0; kk < QF; ++kk) s.t[t] = score_step(key_frag(at, t, kk), kk, s.t[t]);
+      }
+    } else {  // (fragments read a step ahead, so that a step's four products wait for none)
+      uint4 kf[2] = {key_frag(at, 0, 0)};
+      s.t[0] = af32x16{};
+#pragma unroll
+      for (int kk = 0; kk < QF; ++kk) {
+        if (kk + 1 < QF) kf[(kk + 1) & 1] = key_frag(at, 0, kk + 1);
+        s.t[0] = score_step(kf[kk & 1], kk, s.t[0]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   static __device__ __forceinline__ float largest(const Scores& s) {  // of the lane's
@@ -304,18 +365,23 @@ struct RowWave {
       for (int e = t == 0; e + 1 < 16; e += 2) best = fmaxf(fmaxf(best, s.t[t][e]), s.t[t][e + 1]);
     return fmaxf(best, s.t[0][15]);
   }
-  // What the row at place p does not see of the tile at p0; the lane's largest of the rest.
+  // Which of the lane's places, a bit each, lie below place x of the tile.
+  static __device__ __forceinline__ uint32_t places_below(int x) {
+    x = min(max(x, 0), KT);
+    const int n = (x >> 3) * 4 + min(x & 7, 4);
+    return n >= 32 ? ~0u : (1u << n) - 1u;
+  }
+  // -inf for what the row at place p does not see of the tile at p0; the lane's largest of the rest.
   __device__ __forceinline__ float mask(const WinArgs& a, const KeyList& k, int p, int p0, Scores& s) const {
-    // (bounds on the lane's places, formed here: kept across a loop they took 64 registers)
-    int upto = p - p0 - 4 * h, sunk = k.sunk - p0 - 4 * h;
-    asm volatile("" : "+v"(upto), "+v"(sunk));
-    const int behind = a.window > 0 ? upto - a.window : -0x7fffffff;
+    const int at = p0 + 4 * h;
+    uint32_t seen = a.window > 0 ? ~places_below(p - a.window + 1 - at) : ~0u;
+    seen = places_below(p + 1 - at) & (seen | places_below(k.sunk - at));
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int j = 32 * t + 8 * (e >> 2) + (e & 3);
-        s.t[t][e] = j <= upto && (j > behind || j < sunk) ? s.t[t][e] : -INFINITY;
+        const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, 16 * t + e, 1);  // all ones or none
+        s.t[t][e] = __uint_as_float((__float_as_uint(s.t[t][e]) & keep) | (0xff800000u & ~keep));
       }
     return largest(s);
   }
@@ -333,12 +399,6 @@ struct RowWave {
         for (int e = 0; e < 16; ++e) o[d][e] *= keep;
     }
   }
-  __device__ __forceinline__ uint4 value_frag(const uint8_t* vs, int u, int d) const {  // bf16: 16 keys u, 32 columns d
-    const int r = 16 * u + 4 * h + (l >> 2), cc = 4 * d + 2 * l4 + ((l & 3) >> 1);
-    const uint2 v0 = lds_transposed(vs + row_chunk<ROWB, T, 32>(r, cc) + 8 * (l & 1));
-    const uint2 v1 = lds_transposed(vs + row_chunk<ROWB, T, 32>(r + 8, cc) + 8 * (l & 1));
-    return make_uint4(v0.x, v0.y, v1.x, v1.y);
-  }
   // O^T + V^T P^T. AHEAD: beside it the scores of the next tile and the lane's largest of them, given out over the weights.
   template <bool AHEAD>
   __device__ __forceinline__ void add(const uint8_t* vs, Scores& s, const uint8_t* next_ks, Scores& ahead, float& best) {
@@ -353,16 +413,22 @@ struct RowWave {
       };
       constexpr int LATE = AHEAD ? 4 : 0;  // weights of the last 8 keys of the lane's, beside the product's first steps
       if constexpr (AHEAD) {
-        uint4 kf[2][ST];
+        const uint32_t kat = key_at(next_ks);
+        constexpr int PF = D == 128 ? 2 : 1;  // steps that a fragment is read ahead (as many as registers allow)
+        uint4 kf[PF + 1][ST];
 #pragma unroll
-        for (int t = 0; t < ST; ++t) ahead.t[t] = af32x16{}, kf[0][t] = key_frag(next_ks, t, 0);
+        for (int t = 0; t < ST; ++t) ahead.t[t] = af32x16{};
+#pragma unroll
+        for (int kk = 0; kk < PF; ++kk)
+#pragma unroll
+          for (int t = 0; t < ST; ++t) kf[kk][t] = key_frag(kat, t, kk);
 #pragma unroll
         for (int kk = 0; kk < QF; ++kk) {
-          if (kk + 1 < QF)
+          if (kk + PF < QF)
 #pragma unroll
-            for (int t = 0; t < ST; ++t) kf[(kk + 1) & 1][t] = key_frag(next_ks, t, kk + 1);
+            for (int t = 0; t < ST; ++t) kf[(kk + PF) % (PF + 1)][t] = key_frag(kat, t, kk + PF);
 #pragma unroll
-          for (int t = 0; t < ST; ++t) ahead.t[t] = score_step(kf[kk & 1][t], kk, ahead.t[t]);
+          for (int t = 0; t < ST; ++t) ahead.t[t] = score_step(kf[kk % (PF + 1)][t], kk, ahead.t[t]);
 #pragma unroll
           for (int n = (8 * ST - LATE) * kk / QF; n < (8 * ST - LATE) * (kk + 1) / QF; ++n) weigh(n);
         }
@@ -370,14 +436,15 @@ struct RowWave {
 #pragma unroll
         for (int n = 0; n < 8 * ST; ++n) weigh(n);
       }
+      const uint32_t vat = value_at(vs);
       uint4 vf[2][DT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vf[0][d] = value_frag(vs, 0, d);
+      for (int d = 0; d < DT; ++d) vf[0][d] = value_frag(vat, 0, d);
 #pragma unroll
       for (int u = 0; u < 2 * ST; ++u) {
         if (u + 1 < 2 * ST)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) vf[(u + 1) & 1][d] = value_frag(vs, u + 1, d);
+          for (int d = 0; d < DT; ++d) vf[(u + 1) & 1][d] = value_frag(vat, u + 1, d);
         const abf16x8 pf = __builtin_bit_cast(abf16x8, make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]));
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -393,19 +460,55 @@ struct RowWave {
         s.t[0][e] = exp2_of(fmaf(s.t[0][e], c, -base));
         sum += s.t[0][e];
       }
+      float v[2][DT];
+      auto values = [&](int e) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+        for (int d = 0; d < DT; ++d)
+          v[e & 1][d] = *reinterpret_cast<const float*>(
+              vs + row_chunk<ROWB, T, 32>(8 * (e >> 2) + 4 * h + (e & 3), 8 * d + (m >> 2)) + 4 * (m & 3));
+      };
+      values(0);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const int r = 8 * (e >> 2) + 4 * h + (e & 3);
-          const float v = *reinterpret_cast<const float*>(vs + row_chunk<ROWB, T, 32>(r, 8 * d + (m >> 2)) + 4 * (m & 3));
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s.t[0][e], o[d], 0, 0, 0);
-        }
+      for (int e = 0; e < 16; ++e) {
+        if (e + 1 < 16) values(e + 1);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e & 1][d], s.t[0][e], o[d], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if constexpr (AHEAD) {
         scores(next_ks, ahead);
         best = largest(ahead);
       }
     }
+  }
+  // Is an entry of O's row not finite?
+  __device__ __forceinline__ bool odd() const {
+    float x = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = fmaf(o[d][e], 0.f, x);
+    return x != 0.f;
+  }
+  // O's row times `by`, 16 bytes a lane: of two groups of four entries a half has every other one, so the halves exchange them.
+  __device__ __forceinline__ void store(T* row, float by) const {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = o[d][e + i] * by;
+        T* at = row + 32 * d + 2 * e + 8 * h;
+        if constexpr (BF) {
+          const auto u = __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[4], x[5]), false, false);
+          const auto v = __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[2], x[3]), pack_bf16x2(x[6], x[7]), false, false);
+          *reinterpret_cast<uint4*>(at) = make_uint4(u[0], v[0], u[1], v[1]);
+        } else {
+          *reinterpret_cast<float4*>(row + 32 * d + 2 * e + 4 * h) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(row + 32 * d + 2 * e + 8 + 4 * h) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
   }
   // The row's sum over both halves.
   __device__ __forceinline__ float whole_sum() const {
@@ -435,13 +538,15 @@ __device__ __forceinline__ uint32_t rows_that_see_odd(const WinArgs& a, const R&
 // Many rows: a wave for each 32 of a workgroup's, all on the same tiles. The scores of a tile are formed beside the product of
 // the one before, so that matrix and vector instructions have each other to run beside; K is loaded a tile further ahead than V.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || D == 64 ? 2 : 1) void win_attn_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : sizeof(T) == 2 ? 2 : 1) void win_attn_kernel(WinArgs a) {
   constexpr int KT = sizeof(T) == 2 ? 64 : 32, ROWB = D * (int)sizeof(T), LW = KT * ROWB / 1024 / NW, ROWS = 32 * NW;
   using Wave = RowWave<T, D, KT>;
   using R = Rows<ROWS, KT>;
-  __shared__ __align__(1024) uint8_t k_lds[2][KT * ROWB], v_lds[2][KT * ROWB];
+  __shared__ __align__(1024) uint8_t stages[4][KT * ROWB];
   __shared__ int dirty;  // something of V was zeroed
-  const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+  auto k_lds = [&](int i) { return stages[i & 1]; };
+  auto v_lds = [&](int i) { return stages[2 + (i & 1)]; };
+  const int wave = wave_id(), m = threadIdx.x & 31;
   R r;
   if (!r.find(a, blockIdx.x / a.Hk, blockIdx.x % a.Hk)) return;
   const uint32_t rw = r.r0 + 32 * wave, row = min(rw + m, r.rows - 1);  // (lanes behind the last row: as that one, without stores)
@@ -451,63 +556,69 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 || D == 64 ? 2 : 1) void wi
   const int wfirst = r.past + (int)(min(r.rows - 1, rw) / r.G) - shift;
   const int wlast = r.past + (int)((min(r.rows, rw + 32) - 1) / r.G) - shift;
   constexpr int RP = 1024 / ROWB;
-  const TileLoad<T, D, KT, LW> load_k(a.k, a.k_ld, r.t.k0, r.hk, wave * LW * RP), load_v(a.v, a.v_ld, r.t.k0, r.hk, wave * LW * RP);
-  auto issue_k = [&](int i) { load_k.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&k_lds[i & 1][0] + 1024 * LW * wave); };
-  auto issue_v = [&](int i) { load_v.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&v_lds[i & 1][0] + 1024 * LW * wave); };
+  const WholeTiles whole = r.whole(a, r.first, r.last), whole_w = r.whole(a, wfirst, wlast);
+  TileLoads<T, D, KT, LW> load_k(a.k, a.k_ld, r.t, r.hk, wave * LW * RP), load_v(a.v, a.v_ld, r.t, r.hk, wave * LW * RP);
+  auto issue_k = [&] { load_k.issue(r.keys, r.t.nk, lds_address(k_lds(load_k.next)) + 1024 * LW * wave); };
+  auto issue_v = [&] { load_v.issue(r.keys, r.t.nk, lds_address(v_lds(load_v.next)) + 1024 * LW * wave); };
 
   if (threadIdx.x == 0) dirty = 0;
-  if (n > 0) issue_k(0);
+  const T* q = reinterpret_cast<const T*>(a.q) + (size_t)(r.t.q0 + qi) * a.q_ld + (size_t)hq * D;
   Wave w;
-  w.start(a, reinterpret_cast<const T*>(a.q) + (size_t)(r.t.q0 + qi) * a.q_ld + (size_t)hq * D);
   using Scores = typename Wave::Scores;
   auto settle = [&](int i, Scores& s, float best) {
-    if (!r.whole(a, KT * i, wfirst, wlast)) best = w.mask(a, r.keys, p, KT * i, s);
+    if (!whole_w.has(i)) {
+      asm volatile("");  // (a branch, not 100 instructions of every tile)
+      best = w.mask(a, r.keys, p, KT * i, s);
+    }
     w.settle(best);
   };
-  if (n > 0) {
-    if (n > 1) issue_k(1);
-    issue_v(0);
-    asm volatile("s_barrier" ::: "memory");  // (K of tile 0 is there: each wave has waited for its loads, with those of q)
-    Scores one, two;
-    w.scores(k_lds[0], one);
-    settle(0, one, w.largest(one));
-    // (the tile behind the last one is scored too, on what its stage holds, and not used)
-    auto step = [&](int i, Scores& s, Scores& ahead) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // V of tile i and K of the next are there
-      if (i + 2 < n) issue_k(i + 2);
-      if (i + 1 < n) issue_v(i + 1);
-      if (!r.whole(a, KT * i, r.first, r.last)) {
-        if (clean_tile<T, LW>(&v_lds[i & 1][1024 * LW * wave])) dirty = 1;
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      }
-      float best;
-      w.template add<true>(v_lds[i & 1], s, k_lds[(i + 1) & 1], ahead, best);
-      if (i + 1 < n) settle(i + 1, ahead, best);
-    };
-    for (int i = 0;;) {
-      step(i, one, two);
-      if (++i >= n) break;
-      step(i, two, one);
-      if (++i >= n) break;
+  for (bool cleaning = false;; cleaning = true) {
+    int t0 = 0;
+    asm volatile("" : "+s"(t0));  // (nothing of the first tile is kept for another pass)
+    if (n > 0) {
+      load_k.start(r.keys, r.t.nk, t0);
+      load_v.start(r.keys, r.t.nk, t0);
+      issue_k();
+      issue_v();
+      if (n > 1) issue_k();
     }
+    w.start(a, q + t0);
+    if (n > 0) {
+      asm volatile("s_barrier" ::: "memory");  // (the first tiles are there: each wave has waited for its loads, with those of q)
+      Scores one, two;
+      w.scores(k_lds(0), one);
+      settle(t0, one, w.largest(one));
+      // (the tile behind the last one is scored too, on what its stage holds, and not used)
+      auto step = [&](int i, Scores& s, Scores& ahead) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // V of tile i and K of the next are there
+        if (i + 2 < n) issue_k();
+        if (i + 1 < n) issue_v();
+        if (cleaning && !whole.has(i)) {
+          if (clean_tile<T, LW>(v_lds(i) + 1024 * LW * wave)) dirty = 1;
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        float best;
+        w.template add<true>(v_lds(i), s, k_lds(i + 1), ahead, best);
+        if (i + 1 < n) settle(i + 1, ahead, best);
+      };
+      for (int i = t0;;) {
+        step(i, one, two);
+        if (++i >= n) break;
+        step(i, two, one);
+        if (++i >= n) break;
+      }
+    }
+    if (cleaning || !__builtin_expect(__syncthreads_or(w.odd()), 0)) break;
   }
-
   const float inv = p + shift < 0 ? 0.f : 1.f / w.whole_sum();
   uint32_t again = 0;  // the wave's rows that see what was zeroed
   if (n > 0 && dirty) {
     for (int i = 0; i < n; ++i)
-      if (!r.whole(a, KT * i, r.first, r.last)) again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
+      if (!whole.has(i)) again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
     again &= (uint32_t)__ballot(real);
   }
-  if (real && !(again >> m & 1)) {
-    T* orow = reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + qi) * a.Hq + hq) * D;
-#pragma unroll
-    for (int d = 0; d < Wave::DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        io<T>::store4(orow + 32 * d + 2 * e + 4 * h,
-                      make_float4(w.o[d][e] * inv, w.o[d][e + 1] * inv, w.o[d][e + 2] * inv, w.o[d][e + 3] * inv));
-  }
+  if (real && !(again >> m & 1))
+    w.store(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + qi) * a.Hq + hq) * D, inv);
   while (again != 0) {
     const int x = __builtin_ctz(again);
     again &= again - 1;
@@ -527,14 +638,16 @@ struct FewCfg {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
   constexpr int KT = FEW_KT, ROWB = D * (int)sizeof(T), LI = KT * ROWB / 1024, RING = FewCfg<T, D>::RING, PART = FewCfg<T, D>::PART;
   using Wave = RowWave<T, D, KT>;
   using R = Rows<32, KT>;
-  __shared__ __align__(1024) uint8_t ring[FEW_NW][RING][2][KT * ROWB];
+  extern __shared__ __align__(1024) uint8_t tile_lds[];  // [wave][stage][K, V][KT rows]
   __shared__ float top_of[FEW_NW][32], sum_of[FEW_NW][32];
   __shared__ uint32_t odd_of[FEW_NW];  // rows that see a value that is not finite in a tile with a mask
   const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+  auto k_lds = [&](int stage) { return tile_lds + (wave * RING + stage) * FewCfg<T, D>::TILE; };
+  auto v_lds = [&](int stage) { return k_lds(stage) + KT * ROWB; };
   const int ts = blockIdx.x / a.Hk, split = ts % a.splits;
   R r;
   if (!r.find(a, ts / a.splits, blockIdx.x % a.Hk)) return;
@@ -542,11 +655,14 @@ __global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
   const int qi = (int)(row / r.G), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
   const int p = r.past + qi - r.keys.shift;
   const int t0 = (int)((long)r.keys.n * split / a.splits), t1 = (int)((long)r.keys.n * (split + 1) / a.splits);
-  const TileLoad<T, D, KT, LI> load_k(a.k, a.k_ld, r.t.k0, r.hk, 0), load_v(a.v, a.v_ld, r.t.k0, r.hk, 0);
+  const WholeTiles whole = r.whole(a, r.first, r.last);
+  TileLoads<T, D, KT, LI> load_k(a.k, a.k_ld, r.t, r.hk, 0), load_v(a.v, a.v_ld, r.t, r.hk, 0);
   auto issue = [&](int i, int stage) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what the stage held before has been read
-    load_k.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&ring[wave][stage][0][0]);
-    load_v.issue(r.keys, r.t.nk, KT * i, (uint32_t)(uintptr_t)&ring[wave][stage][1][0]);
+    load_k.start(r.keys, r.t.nk, i);
+    load_v.start(r.keys, r.t.nk, i);
+    load_k.issue(r.keys, r.t.nk, lds_address(k_lds(stage)));
+    load_v.issue(r.keys, r.t.nk, lds_address(v_lds(stage)));
   };
   if (t0 + wave < t1) issue(t0 + wave, 0);
   Wave w;
@@ -555,16 +671,16 @@ __global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
   auto compute = [&](int i, int stage) {
     typename Wave::Scores s;
     float best;
-    w.scores(ring[wave][stage][0], s);
-    if (r.whole(a, KT * i, r.first, r.last)) {
+    w.scores(k_lds(stage), s);
+    if (whole.has(i)) {
       best = w.largest(s);
     } else {
-      if (__ballot(clean_tile<T, LI>(ring[wave][stage][1])) != 0)
+      if (__ballot(clean_tile<T, LI>(v_lds(stage))) != 0)
         again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
       best = w.mask(a, r.keys, p, KT * i, s);
     }
     w.settle(best);
-    w.template add<false>(ring[wave][stage][1], s, nullptr, s, best);
+    w.template add<false>(v_lds(stage), s, nullptr, s, best);
   };
   for (int i = t0 + wave, stage = 0; i < t1; i += FEW_NW, stage ^= RING - 1) {
     if (RING == 2 && i + FEW_NW < t1) {
@@ -579,7 +695,7 @@ __global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
 
   const float sum = w.whole_sum();
   __syncthreads();
-  float* mine = reinterpret_cast<float*>(&ring[wave][0][0][0]) + m * PART;
+  float* mine = reinterpret_cast<float*>(k_lds(0)) + m * PART;
 #pragma unroll
   for (int d = 0; d < Wave::DT; ++d)
 #pragma unroll
@@ -606,7 +722,8 @@ __global__ __launch_bounds__(64 * FEW_NW) void win_few_kernel(WinArgs a) {
 #pragma unroll
     for (int y = 0; y < FEW_NW; ++y) {
       const float f = exp2_of((top_of[y][x] - base) * a.c);
-      const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&ring[y][0][0][0]) + x * PART + d);
+      const float4 u = *reinterpret_cast<const float4*>(
+          reinterpret_cast<const float*>(tile_lds + y * RING * FewCfg<T, D>::TILE) + x * PART + d);
       v = make_float4(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w));
       all = fmaf(sum_of[y][x], f, all);
     }
@@ -708,16 +825,22 @@ size_t win_bytes(const WinPlan& p, const WinArgs& a, int D) {
 }
 
 template <typename T, int D>
-void launch_win(WinArgs a, const WinPlan& p, hipStream_t s) {
+bool launch_win(WinArgs a, const WinPlan& p, hipStream_t s) {
+  static std::atomic<signed char> ready[MAX_DEVICES];
   a.tiles = (int)p.tiles;
   a.splits = p.splits;
+  a.paired = p.rows == 128 && p.tiles * a.Hk <= 2 * device_cus();
   const unsigned n = (unsigned)(p.tiles * a.Hk);
   if (p.rows == 128) {
     hipLaunchKernelGGL((win_attn_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, a);
-    return;
+    return true;
   }
-  hipLaunchKernelGGL((win_few_kernel<T, D>), dim3(n * p.splits), dim3(64 * FEW_NW), 0, s, a);
+  constexpr int LDS = FEW_NW * FewCfg<T, D>::RING * FewCfg<T, D>::TILE;
+  const auto kernel = win_few_kernel<T, D>;
+  if (!lds_ready((const void*)kernel, LDS, ready)) return false;
+  hipLaunchKernelGGL(kernel, dim3(n * p.splits), dim3(64 * FEW_NW), LDS, s, a);
   if (p.splits > 1) hipLaunchKernelGGL((win_few_join_kernel<T, D>), dim3(4 * n), dim3(2 * D), 0, s, a);
+  return true;
 }
 
 bool win_sizes(int B, int Tq, int Tk, int Hq, int Hk, int D, int window, int sinks, int dtype) {
@@ -769,7 +892,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
   if (((uintptr_t)cu_q | (uintptr_t)cu_k) % 4) return fail(ZGDN_EINVAL, "%s: cu_q, cu_k not on 4-byte boundaries", fn);
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
-            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 1, nullptr, nullptr};
+            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 0, 1, nullptr, nullptr};
   const WinPlan p = win_plan(a);
   if (p.tiles * p.splits * Hk > (1L << 32) / 256 - 1) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
   const size_t need = win_bytes(p, a, D);
@@ -786,9 +909,8 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
     a.part_ml = a.part_o + (size_t)p.tiles * Hk * p.splits * 32 * D;
   }
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == ZGDN_F32)
-    D == 128 ? launch_win<float, 128>(a, p, s) : launch_win<float, 64>(a, p, s);
-  else
-    D == 128 ? launch_win<bf16, 128>(a, p, s) : launch_win<bf16, 64>(a, p, s);
+  const bool ok = dtype == ZGDN_F32 ? (D == 128 ? launch_win<float, 128>(a, p, s) : launch_win<float, 64>(a, p, s))
+                                    : (D == 128 ? launch_win<bf16, 128>(a, p, s) : launch_win<bf16, 64>(a, p, s));
+  if (!ok) return fail(ZGDN_EHIP, "%s: the device has too little LDS a workgroup", fn);
   return check_launch(fn);
 }

@@ -16,6 +16,7 @@
 // 32768 tokens through a window of 1024 9 us of 329.)
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "gdn_attn.h"
 #include "zonos3_attn.h"
@@ -795,8 +796,19 @@ __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
   }
 }
 
-// How a call is cut. Where 128 rows a workgroup leave CUs without any, 32 rows and a share of the keys: as many shares as
-// there are CUs for, of two tiles for each wave at least.
+// How a call is cut: 128 rows a workgroup, or 32 rows and a share of their keys, whichever is estimated to take less. What a
+// workgroup takes, in us: a start and end, then its tiles one after the other, in the first form (a tile of 64 keys for bf16, 32
+// for fp32) alone on its CU or as its part of a CU's time, in the second (tiles of 32 for each of four waves) a round at a time.
+// (Measured, first / second form, us: 1000 tokens of 8 + 2 heads 22.9 / 15.3, 1536 of 16 + 4 32 / 40, 2048 of 8 + 2 through a window
+// of 256 12.2 / 21.5; fp32: 4096 of 8 + 2 569 / 325, through a window of 256 53 / 91, 8192 of 16 + 4 2354 / 2434.)
+// Of the second form as many shares of the keys as there are CUs for, of two tiles for each wave at least.
+struct WinCost {
+  double alone, part, wave;  // a tile of the first form, alone and as a part; of the second
+};
+WinCost win_cost(int D, int dtype) {
+  if (dtype == ZGDN_F32) return D == 128 ? WinCost{4.4, 4.4, 4.6} : WinCost{2.3, 2.3, 2.5};
+  return D == 128 ? WinCost{1.05, 1.0, 1.0} : WinCost{0.85, 0.6, 0.7};
+}
 struct WinPlan {
   long tiles;  // of rows a key head
   int rows, splits;
@@ -806,19 +818,22 @@ long row_tiles(const WinArgs& a, int rows) {
   if (a.cu_q == nullptr) return a.N * ((all + rows - 1) / rows);
   return (all + rows - 1) / rows + a.N;  // (each sequence may leave a part of a tile)
 }
-WinPlan win_plan(const WinArgs& a) {
-  WinPlan p;
-  const long cus = device_cus();
-  p.rows = 128, p.splits = 1;
-  p.tiles = row_tiles(a, 128);
-  if (p.tiles * a.Hk >= cus) return p;
-  p.rows = 32;
-  p.tiles = row_tiles(a, 32);
-  long keys = a.Tk;
-  if (a.window > 0) keys = std::min(keys, (long)a.window + 32 + a.sinks);
-  const long most = std::max(1L, keys / (2 * FEW_NW * FEW_KT));
-  p.splits = (int)std::max(1L, std::min(most, cus / (p.tiles * a.Hk)));
-  return p;
+WinPlan win_plan(const WinArgs& a, int D, int dtype) {
+  constexpr double MANY = 6.0, FEW = 7.5, JOIN = 4.0;  // start and end, in us
+  const double cus = device_cus(), kt = dtype == ZGDN_F32 ? 32 : 64;
+  const WinCost cost = win_cost(D, dtype);
+  WinPlan many{row_tiles(a, 128), 128, 1}, few{row_tiles(a, 32), 32, 1};
+  // keys of the longest list and of a list in the mean (a packed batch is taken for sequences of equal length)
+  const double seqs = a.cu_q != nullptr ? a.N : 1, nk = a.Tk / seqs, nq = std::min(a.Tq / seqs, nk);
+  const double reach = a.window > 0 ? (double)a.window + a.sinks + 32 : nk;
+  const double most = std::min(nk, reach), mean = std::min(nk - nq / 2, reach);
+  const double many_us = MANY + std::max(most / kt * cost.alone, many.tiles * a.Hk / cus * mean / kt * cost.part);
+  const double slots = (D == 64 && dtype == ZGDN_BF16 ? 2 : 1) * cus, groups = (double)few.tiles * a.Hk;
+  few.splits = (int)std::max(1.0, std::min(std::floor(most / (2 * FEW_NW * FEW_KT)), std::floor(cus / groups)));
+  const double share = cost.wave / (FEW_NW * FEW_KT * few.splits);
+  const double few_us = std::max(FEW + most * share, std::ceil(groups * few.splits / slots) * (FEW + mean * share)) +
+                        (few.splits > 1 ? JOIN : 0.0);
+  return few_us < many_us ? few : many;
 }
 size_t win_bytes(const WinPlan& p, const WinArgs& a, int D) {
   return p.splits == 1 ? 0 : (size_t)p.tiles * a.Hk * p.splits * 32 * (D + 2) * sizeof(float);
@@ -860,7 +875,7 @@ extern "C" size_t zattn_window_fwd_workspace_bytes(int packed, int n_seqs, int T
   const int32_t bounds = 0;  // (told from none by its address alone)
   a.cu_q = packed ? &bounds : nullptr;
   a.N = n_seqs, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hk = Hk, a.window = window, a.sinks = sinks;
-  return win_bytes(win_plan(a), a, D);
+  return win_bytes(win_plan(a, D, dtype), a, D);
 }
 
 extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
@@ -893,7 +908,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
             fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 0, 1, nullptr, nullptr};
-  const WinPlan p = win_plan(a);
+  const WinPlan p = win_plan(a, D, dtype);
   if (p.tiles * p.splits * Hk > (1L << 32) / 256 - 1) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
   const size_t need = win_bytes(p, a, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))

@@ -11,9 +11,9 @@
 // wave see whole have no mask.
 // Scores, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
 // A masked weight is 0, but 0 times an infinity or a NaN of V is a NaN. A workgroup with an output that is not finite computes
-// its rows once more, and in tiles that a row of it does not see whole zeroes such entries in LDS ahead of the product; the
-// rows that see one of them are then computed again key by key (win_row). (Cleaned at once, with a barrier more, such tiles cost
-// 32768 tokens through a window of 1024 9 us of 329.)
+// its rows once more, and in tiles that a row of it does not see whole zeroes such entries in LDS ahead of the product; what
+// rows see of them is added in the end (patch_row). (Cleaned at once, with a barrier more, such tiles cost 32768 tokens
+// through a window of 1024 9 us of 329.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -35,7 +35,7 @@ struct WinArgs {
   int tiles;  // of rows a key head, at most
   int paired;               // two workgroups a CU hold the whole call
   int splits;               // workgroups that share a tile of 32 rows
-  float *part_o, *part_ml;  // [workgroup][32][D], [workgroup][32][2]
+  float *part_o, *part_ml;  // [workgroup][32][D], [workgroup][32][maximum, sum, whether V was zeroed, -]
 };
 
 __device__ __forceinline__ int prefix_count(int x) {  // over the lanes up to this one
@@ -103,45 +103,6 @@ __device__ __forceinline__ bool clear_odd(uint4& w) {
   return any;
 }
 
-// One row by one wave, in fp32 and from visible keys alone: q its query, k and v its key head's first rows, p its position.
-template <typename T, int D>
-__device__ __noinline__ void win_row(const T* q, const T* k, long k_ld, const T* v, long v_ld, T* o, int p, int window,
-                                     int sinks, float c) {
-  const int lane = threadIdx.x & 63;
-  const int lo = window > 0 ? max(0, p - window + 1) : 0, s = min(sinks, lo), n = s + p + 1 - lo;  // visible keys
-  float top = -INFINITY, sum = 0.f, acc[D / 64] = {};
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + lane, j = i < s ? i : lo + i - s;
-    float x = -INFINITY;
-    if (i < n) {
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot = fmaf(io<T>::load(q + d), io<T>::load(k + (size_t)j * k_ld + d), dot);
-      x = dot * c;
-    }
-    const float next = fmaxf(top, wave_max(x)), base = next == -INFINITY ? 0.f : next, keep = exp2_of(top - base);
-    top = next;
-    const float w = i < n ? exp2_of(x - base) : 0.f;
-    sum = fmaf(sum, keep, wave_sum(w));
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d) acc[d] *= keep;
-    for (int e = 0; e < min(64, n - i0); ++e) {
-      const int je = i0 + e < s ? i0 + e : lo + i0 + e - s;
-      const float we = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), e));
-#pragma unroll
-      for (int d = 0; d < D / 64; ++d) acc[d] = fmaf(we, io<T>::load(v + (size_t)je * v_ld + 64 * d + lane), acc[d]);
-    }
-  }
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) io<T>::store(o + 64 * d + lane, acc[d] / sum);
-}
-
-// The same for query qi of a workgroup's sequence, head hq.
-template <typename T, int D>
-__device__ __forceinline__ void redo_row(const WinArgs& a, const RowTile& t, const T* k, const T* v, int qi, int hq) {
-  win_row<T, D>(reinterpret_cast<const T*>(a.q) + (size_t)(t.q0 + qi) * a.q_ld + (size_t)hq * D, k, a.k_ld, v, a.v_ld,
-                reinterpret_cast<T*>(a.o) + ((size_t)(t.q0 + qi) * a.Hq + hq) * D, t.nk - t.nq + qi, a.window, a.sinks,
-                a.flip ? -a.c : a.c);
-}
 // The keys that the rows at positions first .. last see, as a list of places: the sinks ahead of the window's start, then all
 // from there on. Place u is position u, or u + shift behind the sinks.
 struct KeyList {
@@ -163,6 +124,37 @@ struct WholeTiles {
   int to, from, sunk;  // those below `to` from `from` on, or below `sunk`
   __device__ __forceinline__ bool has(int i) const { return i < to && (i >= from || i < sunk); }
 };
+
+// Adds to a row that is stored what was zeroed of the values that it sees: w v for each infinity and NaN v, w its weight, by
+// one wave. q, k, v, o: the row's and its key head's first entries; p its place, top its maximum.
+template <typename T, int D, int KT>
+__device__ __forceinline__ void patch_row(const WinArgs& a, const KeyList& keys, const WholeTiles& whole, int nk, const T* q,
+                                       const T* k, const T* v, T* o, int p, float top) {
+  const int lane = threadIdx.x & 63;
+  for (int i = 0; i < keys.n; ++i) {
+    if (whole.has(i)) continue;
+    const int u = KT * i + lane, j = keys.position(u);
+    bool odd = false;
+    if (lane < KT && u <= p && j < nk && (a.window == 0 || p - u < a.window || u < keys.sunk))
+      for (int c = 0; c < D * (int)sizeof(T) / 16; ++c) {
+        uint4 w = *reinterpret_cast<const uint4*>(v + (size_t)j * a.v_ld + c * (16 / (int)sizeof(T)));
+        odd = clear_odd<T>(w) || odd;
+      }
+    for (uint64_t left = __ballot(odd); left != 0; left &= left - 1) {
+      const size_t key = (size_t)__builtin_amdgcn_readlane(j, __builtin_ctzll(left));
+      float dot = 0.f;
+#pragma unroll
+      for (int d = lane; d < D; d += 64) dot = fmaf(io<T>::load(q + d), io<T>::load(k + key * a.k_ld + d), dot);
+      dot = wave_sum(dot);
+      const float w = exp2_of(((a.flip ? -dot : dot) - top) * a.c);
+#pragma unroll
+      for (int d = lane; d < D; d += 64) {
+        const float x = io<T>::load(v + key * a.v_ld + d);
+        if (x - x != 0.f) io<T>::store(o + d, io<T>::load(o + d) + w * x);
+      }
+    }
+  }
+}
 
 // A workgroup's rows of a sequence and key head, and their keys. Positions, from here on, are places of the list's second part
 // (p - shift): differences and bounds are the same.
@@ -194,8 +186,14 @@ struct Rows {
     w.sunk = keys.sunk / KT;
     return w;
   }
-  __device__ __forceinline__ bool sees(const WinArgs& a, int p, int u) const {
-    return u <= p && (a.window == 0 || p - u < a.window || u < keys.sunk);
+  // patch_row for query qi, head hq, whose maximum is `top`.
+  template <typename T, int D>
+  __device__ __forceinline__ void patch(const WinArgs& a, const WholeTiles& w, int qi, int hq, float top) const {
+    const size_t row = (size_t)(t.q0 + qi);
+    patch_row<T, D, KT>(a, keys, w, t.nk, reinterpret_cast<const T*>(a.q) + row * a.q_ld + (size_t)hq * D,
+                        reinterpret_cast<const T*>(a.k) + (size_t)t.k0 * a.k_ld + (size_t)hk * D,
+                        reinterpret_cast<const T*>(a.v) + (size_t)t.k0 * a.v_ld + (size_t)hk * D,
+                        reinterpret_cast<T*>(a.o) + (row * a.Hq + hq) * D, past + qi - keys.shift, top);
   }
 };
 
@@ -518,24 +516,6 @@ struct RowWave {
   }
 };
 
-// Those of the wave's 32 rows (places p, a lane each) that see a value that is not finite in the tile at place p0. (Rare: from
-// global memory, a key a lane.)
-template <typename T, int D, typename R, int KT>
-__device__ __forceinline__ uint32_t rows_that_see_odd(const WinArgs& a, const R& r, const T* v, int p, int p0) {
-  const int lane = threadIdx.x & 63, u = p0 + lane, j = r.keys.position(u);
-  bool bad = false;
-  if (lane < KT && j < r.t.nk)
-    for (int c = 0; c < D * (int)sizeof(T) / 16; ++c) {
-      uint4 w = *reinterpret_cast<const uint4*>(v + (size_t)j * a.v_ld + c * (16 / (int)sizeof(T)));
-      bad = clear_odd<T>(w) || bad;
-    }
-  uint32_t found = 0;
-  if (__ballot(bad) != 0)
-    for (int l = 0; l < 32; ++l)
-      if (__ballot(bad && r.sees(a, __builtin_amdgcn_readlane(p, l), u))) found |= 1u << l;
-  return found;
-}
-
 // Many rows: a wave for each 32 of a workgroup's, all on the same tiles. The scores of a tile are formed beside the product of
 // the one before, so that matrix and vector instructions have each other to run beside; K is loaded a tile further ahead than V.
 template <typename T, int D, int NW>
@@ -585,7 +565,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : sizeof(T) == 2 ? 2 : 1) void
     }
     w.start(a, q + t0);
     if (n > 0) {
-      asm volatile("s_barrier" ::: "memory");  // (the first tiles are there: each wave has waited for its loads, with those of q)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the first tiles are there
       Scores one, two;
       w.scores(k_lds(0), one);
       settle(t0, one, w.largest(one));
@@ -612,18 +592,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : sizeof(T) == 2 ? 2 : 1) void
     if (cleaning || !__builtin_expect(__syncthreads_or(w.odd()), 0)) break;
   }
   const float inv = p + shift < 0 ? 0.f : 1.f / w.whole_sum();
-  uint32_t again = 0;  // the wave's rows that see what was zeroed
+  if (real) w.store(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + qi) * a.Hq + hq) * D, inv);
   if (n > 0 && dirty) {
-    for (int i = 0; i < n; ++i)
-      if (!whole.has(i)) again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
-    again &= (uint32_t)__ballot(real);
-  }
-  if (real && !(again >> m & 1))
-    w.store(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + qi) * a.Hq + hq) * D, inv);
-  while (again != 0) {
-    const int x = __builtin_ctz(again);
-    again &= again - 1;
-    redo_row<T, D>(a, r.t, load_k.base, load_v.base, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x));
+    __threadfence();
+    for (uint32_t left = (uint32_t)__ballot(real); left != 0; left &= left - 1) {
+      const int x = __builtin_ctz(left);
+      r.template patch<T, D>(a, whole, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x),
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w.top), x)));
+    }
   }
 }
 
@@ -645,7 +621,7 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
   using R = Rows<32, KT>;
   extern __shared__ __align__(1024) uint8_t tile_lds[];  // [wave][stage][K, V][KT rows]
   __shared__ float top_of[FEW_NW][32], sum_of[FEW_NW][32];
-  __shared__ uint32_t odd_of[FEW_NW];  // rows that see a value that is not finite in a tile with a mask
+  __shared__ int dirty;  // something of V was zeroed
   const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
   auto k_lds = [&](int stage) { return tile_lds + (wave * RING + stage) * FewCfg<T, D>::TILE; };
   auto v_lds = [&](int stage) { return k_lds(stage) + KT * ROWB; };
@@ -666,9 +642,10 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
     load_v.issue(r.keys, r.t.nk, lds_address(v_lds(stage)));
   };
   if (t0 + wave < t1) issue(t0 + wave, 0);
+  if (threadIdx.x == 0) dirty = 0;
+  __syncthreads();
   Wave w;
   w.start(a, reinterpret_cast<const T*>(a.q) + (size_t)(r.t.q0 + qi) * a.q_ld + (size_t)hq * D);
-  uint32_t again = 0;
   auto compute = [&](int i, int stage) {
     typename Wave::Scores s;
     float best;
@@ -676,8 +653,7 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
     if (whole.has(i)) {
       best = w.largest(s);
     } else {
-      if (__ballot(clean_tile<T, LI>(v_lds(stage))) != 0)
-        again |= rows_that_see_odd<T, D, R, KT>(a, r, load_v.base, p, KT * i);
+      if (clean_tile<T, LI>(v_lds(stage))) dirty = 1;
       best = w.mask(a, r.keys, p, KT * i, s);
     }
     w.settle(best);
@@ -706,11 +682,7 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
     top_of[wave][m] = w.top;
     sum_of[wave][m] = sum;
   }
-  if ((threadIdx.x & 63) == 0) odd_of[wave] = again;
   __syncthreads();
-  uint32_t odd = 0;
-#pragma unroll
-  for (int x = 0; x < FEW_NW; ++x) odd |= odd_of[x];
   for (int i = threadIdx.x; i < 32 * D / 4; i += 64 * FEW_NW) {
     const int x = i / (D / 4), d = i % (D / 4) * 4;
     if (r.r0 + x >= r.rows) continue;
@@ -731,8 +703,8 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
     if (a.splits > 1) {
       const size_t at = (size_t)blockIdx.x * 32 + x;
       *reinterpret_cast<float4*>(a.part_o + at * D + d) = v;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(best, odd >> x & 1 ? -1.f : all);
-    } else if (!(odd >> x & 1)) {
+      if (d == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * at) = make_float4(best, all, dirty ? 1.f : 0.f, 0.f);
+    } else {
       const uint32_t rr = r.r0 + x;
       const int q = (int)(rr / r.G), hh = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
       const float inv = r.past + q < 0 ? 0.f : 1.f / all;
@@ -740,10 +712,16 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
                     make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
   }
-  if (a.splits > 1) return;
+  if (a.splits > 1 || !dirty) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int y = 0; y < FEW_NW; ++y) top = fmaxf(top, top_of[y][m]);
+  __threadfence();
+  __syncthreads();
   for (int x = wave; x < 32; x += FEW_NW)
-    if ((odd >> x & 1) && r.r0 + x < r.rows)
-      redo_row<T, D>(a, r.t, load_k.base, load_v.base, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x));
+    if (r.r0 + x < r.rows)
+      r.template patch<T, D>(a, whole, __builtin_amdgcn_readlane(qi, x), __builtin_amdgcn_readlane(hq, x),
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), x)));
 }
 
 // A workgroup joins the parts of 8 rows, D / 4 lanes each.
@@ -760,12 +738,11 @@ __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
   bool odd = false;
   constexpr int AT = 4;  // parts read at a time
   for (int i0 = 0; i0 < a.splits; i0 += AT) {
-    float2 ml[AT];
-    float4 u[AT];
+    float4 ml[AT], u[AT];
 #pragma unroll
     for (int e = 0; e < AT; ++e) {
       const size_t at = ((size_t)(tile * a.splits + min(i0 + e, a.splits - 1)) * a.Hk + r.hk) * 32 + (real ? x : 0);
-      ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+      ml[e] = *reinterpret_cast<const float4*>(a.part_ml + 4 * at);
       u[e] = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
     }
 #pragma unroll
@@ -774,7 +751,7 @@ __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
         const float next = fmaxf(top, ml[e].x), base = next == -INFINITY ? 0.f : next;
         const float keep = exp2_of((top - base) * a.c), f = exp2_of((ml[e].x - base) * a.c);
         top = next;
-        odd = odd || ml[e].y < 0.f;
+        odd = odd || ml[e].z != 0.f;
         sum = fmaf(sum, keep, ml[e].y * f);
         v = make_float4(fmaf(v.x, keep, u[e].x * f), fmaf(v.y, keep, u[e].y * f), fmaf(v.z, keep, u[e].z * f),
                         fmaf(v.w, keep, u[e].w * f));
@@ -782,17 +759,19 @@ __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
   }
   const uint32_t rr = min(r.r0 + x, r.rows - 1);
   const int q = (int)(rr / r.G), hq = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
-  odd = odd && real;
-  if (real && !odd) {
+  if (real) {
     const float inv = r.past + q < 0 ? 0.f : 1.f / sum;
     io<T>::store4(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + q) * a.Hq + hq) * D + d,
                   make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
   }
-  const T* kb = reinterpret_cast<const T*>(a.k) + (size_t)r.t.k0 * a.k_ld + (size_t)r.hk * D;
-  const T* vb = reinterpret_cast<const T*>(a.v) + (size_t)r.t.k0 * a.v_ld + (size_t)r.hk * D;
-  for (uint64_t left = __ballot(odd && d == 0); left != 0; left &= left - 1) {  // (a row's lanes are of one wave)
+  uint64_t left = __ballot(odd && real && d == 0);  // (a row's lanes are of one wave)
+  if (left == 0) return;
+  __threadfence();
+  const WholeTiles whole = r.whole(a, r.first, r.last);
+  for (; left != 0; left &= left - 1) {
     const int lane = __builtin_ctzll(left);
-    redo_row<T, D>(a, r.t, kb, vb, __builtin_amdgcn_readlane(q, lane), __builtin_amdgcn_readlane(hq, lane));
+    r.template patch<T, D>(a, whole, __builtin_amdgcn_readlane(q, lane), __builtin_amdgcn_readlane(hq, lane),
+                           __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), lane)));
   }
 }
 
@@ -836,7 +815,7 @@ WinPlan win_plan(const WinArgs& a, int D, int dtype) {
   return few_us < many_us ? few : many;
 }
 size_t win_bytes(const WinPlan& p, const WinArgs& a, int D) {
-  return p.splits == 1 ? 0 : (size_t)p.tiles * a.Hk * p.splits * 32 * (D + 2) * sizeof(float);
+  return p.splits == 1 ? 0 : (size_t)p.tiles * a.Hk * p.splits * 32 * (D + 4) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -858,6 +837,16 @@ bool launch_win(WinArgs a, const WinPlan& p, hipStream_t s) {
   return true;
 }
 
+// What a plan goes by.
+WinArgs plan_args(int packed, int n_seqs, int Tq, int Tk, int Hq, int Hk, int window, int sinks) {
+  static const int32_t bounds = 0;  // (told from none by its address alone)
+  WinArgs a{};
+  a.cu_q = packed ? &bounds : nullptr;
+  a.N = n_seqs, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hk = Hk;
+  a.window = std::min(window, 1 << 30), a.sinks = std::min(sinks, 1 << 30);
+  return a;
+}
+
 bool win_sizes(int B, int Tq, int Tk, int Hq, int Hk, int D, int window, int sinks, int dtype) {
   return B >= 1 && Tq >= 0 && Tk >= 0 && Hq >= 1 && Hk >= 1 && Hq % Hk == 0 && (D == 64 || D == 128) && window >= 0 &&
          sinks >= 0 && (dtype == ZGDN_F32 || dtype == ZGDN_BF16) && (long)B * Tq <= 1L << 30 && (long)B * Tk <= 1L << 30 &&
@@ -871,11 +860,20 @@ extern "C" size_t zattn_window_fwd_workspace_bytes(int packed, int n_seqs, int T
                                                    int sinks, int dtype) {
   using namespace zgdn;
   if (n_seqs < 1 || !win_sizes(packed ? 1 : n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, dtype) || Tq == 0) return 0;
-  WinArgs a{};
-  const int32_t bounds = 0;  // (told from none by its address alone)
-  a.cu_q = packed ? &bounds : nullptr;
-  a.N = n_seqs, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hk = Hk, a.window = window, a.sinks = sinks;
+  const WinArgs a = plan_args(packed, n_seqs, Tq, Tk, Hq, Hk, window, sinks);
   return win_bytes(win_plan(a, D, dtype), a, D);
+}
+
+// (for tests) Rows of a workgroup and workgroups that share their keys, for the same sizes.
+extern "C" int zgdn_window_fwd_form(int packed, int n_seqs, int Tq, int Tk, int Hq, int Hk, int D, int window, int sinks,
+                                    int dtype, int64_t* form) {
+  using namespace zgdn;
+  if (n_seqs < 1 || !win_sizes(packed ? 1 : n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, dtype))
+    return fail(ZGDN_EINVAL, "zgdn_window_fwd_form: bad sizes");
+  const WinPlan p = win_plan(plan_args(packed, n_seqs, Tq, Tk, Hq, Hk, window, sinks), D, dtype);
+  form[0] = p.rows;
+  form[1] = p.splits;
+  return ZGDN_OK;
 }
 
 extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,
@@ -894,6 +892,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
     return fail(ZGDN_EINVAL, "%s: packed sequences need B == 1 and n_seqs >= 1 (B=%d n_seqs=%d)", fn, B, n_seqs);
   if ((long)B * Tq > (1L << 30) || (long)B * Tk > (1L << 30) || (long)B * Tq * Hq > (1L << 31))
     return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d, Tk=%d rows", fn, B, Tq, Hq, Tk);
+  if (!std::isfinite(scale)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
   if (Tq == 0) return ZGDN_OK;
   if (!q || !o || (Tk > 0 && (!k || !v))) return fail(ZGDN_EINVAL, "%s: null tensor pointer", fn);
   const int ve = dtype == ZGDN_F32 ? 4 : 8;
@@ -906,6 +905,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
     return fail(ZGDN_EINVAL, "%s: q, k, v, o and workspace need 16-byte aligned bases", fn);
   if (((uintptr_t)cu_q | (uintptr_t)cu_k) % 4) return fail(ZGDN_EINVAL, "%s: cu_q, cu_k not on 4-byte boundaries", fn);
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
+  window = std::min(window, 1 << 30), sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
             fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 0, 1, nullptr, nullptr};
   const WinPlan p = win_plan(a, D, dtype);

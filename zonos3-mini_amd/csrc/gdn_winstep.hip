@@ -11,6 +11,7 @@
 // maximum, sum, O) are joined in LDS, those of a stream's chunks by a second kernel, in order.
 // Sums, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
 #include <algorithm>
+#include <cmath>
 
 #include "gdn_attn.h"
 #include "zonos3_attn.h"
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
       int32_t page = p < room ? a.pages[(size_t)b * a.n_pages + (p >> a.page_shift)] : -1;
       if (page < 0 || page >= a.cache_pages) {
         page = -1;
-        missing = missing || p < n;
+        missing = missing || (p < n && (p + gran > lo || p < a.sinks));
       }
       page_of[i] = page;
     }
@@ -430,7 +431,18 @@ extern "C" size_t zattn_window_step_workspace_bytes(int B, long room, int Hq, in
                                                     int dtype) {
   using namespace zgdn;
   if (!step_sizes(B, room, Hq, Hk, D, window, sinks, dtype) || B == 0) return 0;
-  return step_bytes(step_plan(B, room, Hq, Hk, window, sinks, dtype), B, Hk, D);
+  return step_bytes(step_plan(B, room, Hq, Hk, std::min(window, 1 << 30), std::min(sinks, 1 << 30), dtype), B, Hk, D);
+}
+
+// (for tests) Whether a call takes one launch of wide workgroups, and the chunks of a stream, for the same sizes.
+extern "C" int zgdn_window_step_form(int B, long room, int Hq, int Hk, int window, int sinks, int dtype, int64_t* form) {
+  using namespace zgdn;
+  if (!step_sizes(B, room, Hq, Hk, 64, window, sinks, dtype) || B == 0)
+    return fail(ZGDN_EINVAL, "zgdn_window_step_form: bad sizes");
+  const StepPlan p = step_plan(B, room, Hq, Hk, std::min(window, 1 << 30), std::min(sinks, 1 << 30), dtype);
+  form[0] = p.wide;
+  form[1] = p.splits;
+  return ZGDN_OK;
 }
 
 extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, long kc_ld, const void* v_cache, long vc_ld,
@@ -451,6 +463,8 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
                 "pages; without: one a stream)", fn, page_size, n_pages, n_rows);
   const long room = (long)page_size * n_pages;
   if (room > MOST_ROOM) return fail(ZGDN_EUNSUPPORTED, "%s: %ld positions a stream", fn, room);
+  if (!std::isfinite(scale)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
+  window = std::min(window, 1 << 30), sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   if (B == 0) return ZGDN_OK;
   if (!q || !o || !lengths || (n_rows > 0 && (!k_cache || !v_cache))) return fail(ZGDN_EINVAL, "%s: null tensor pointer", fn);
   const int ve = dtype == ZGDN_F32 ? 4 : 8;

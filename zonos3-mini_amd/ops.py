@@ -1195,8 +1195,8 @@ def _head_vectors(name: str, t, lead: tuple | None, heads: int | None, D: int | 
                            f"got {tuple(shape)}")
     if t.dtype is not dtype:
         raise RuntimeError(f"{name}: {t.dtype}, expected {dtype} as the queries")
-    if ld > 1 << 22:  # rows further apart than the kernels' 32-bit offsets reach
-        t, ld = t.contiguous(), shape[-1] * shape[-2]
+    if ld > 1 << 22 or t.data_ptr() % 16:  # rows further apart than the kernels' 32-bit offsets reach, dense ones off a boundary
+        t, ld = t.clone(memory_format=torch.contiguous_format), shape[-1] * shape[-2]
     return t, ld
 
 
@@ -1453,6 +1453,8 @@ def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=N
     elif n != B:
         raise RuntimeError(f"k_cache: {n} streams' rows for {B} streams (pages name them)")
     window, sinks = _window(window, sinks)
+    if B == 0 or page_size * n_pages == 0:
+        return q.new_zeros(q.shape)
     o = q.new_empty(q.shape)
     size = _window_step_workspace(B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
     workspace = o.new_empty(size, dtype=torch.uint8) if size else None

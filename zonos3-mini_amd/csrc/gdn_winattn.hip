@@ -7,9 +7,16 @@
 // leaves a row's scores in one lane (and its partner, lane ^ 32), so that the softmax is within a lane but for one exchange,
 // and S^T's layout is the second operand of O^T = V^T P^T as it stands: keys in the order that S^T leaves them, V read
 // transposed from LDS in the same order. One pass over the keys with a running maximum and sum.
-// Tiles of K and V are loaded straight into LDS, a tile ahead. Tiles that no row sees are left out, tiles that all rows of a
-// wave see whole have no mask.
+// Tiles of K and V are loaded straight into LDS, a tile ahead. The keys that a workgroup's rows see are one list, sinks then
+// window, so that a few sinks share a tile with the window's first keys; tiles that all rows of a wave see whole have no mask.
 // Scores, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
+// The maximum may lag by 2^8: it is taken on, and O rescaled, only where a row's rises by more.
+//
+// What bounds it: matrix products, and the card's power. 16384 tokens of 16 heads on 4, D = 128: 1010 us, 1090 TFLOP/s, 88 % of
+// the rate of a large library product; the matrix units are busy for 62 % of the cycles, at a clock that falls to 1.5-1.8 GHz
+// (1.3 times the cycles at 1.74 GHz took no longer). 32768 tokens through a window of 1024: 310 us, 47 of them what reading q
+// and writing o takes, 14.2 a tile of 64 keys. fp32: 117 TFLOP/s of 154.
+//
 // A masked weight is 0, but 0 times an infinity or a NaN of V is a NaN. A workgroup with an output that is not finite computes
 // its rows once more, and in tiles that a row of it does not see whole zeroes such entries in LDS ahead of the product; what
 // rows see of them is added in the end (patch_row). (Cleaned at once, with a barrier more, such tiles cost 32768 tokens
@@ -404,10 +411,16 @@ struct RowWave {
     const float base = top == -INFINITY ? 0.f : top * c;
     if constexpr (BF) {
       uint32_t w[2 * ST][4];
-      auto weigh = [&](int n) {  // two weights, rounded and summed (the sum of what the product takes)
+      auto weigh = [&](int n) {  // two weights, rounded, and their part of the sum
         const af32x16& x = s.t[n / 8];
-        const uint32_t y = pack_bf16x2(exp2_of(fmaf(x[2 * (n % 8)], c, -base)), exp2_of(fmaf(x[2 * (n % 8) + 1], c, -base)));
-        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(abf16x2, y), __builtin_bit_cast(abf16x2, 0x3f803f80u), sum, false);
+        const float y0 = exp2_of(fmaf(x[2 * (n % 8)], c, -base)), y1 = exp2_of(fmaf(x[2 * (n % 8) + 1], c, -base));
+        const uint32_t y = pack_bf16x2(y0, y1);
+        // one sum of two products takes about as long as three additions: at D = 64 vector instructions bind and the count of
+        // instructions tells (8192 tokens, 16 + 4 heads: 160 us, 164 with additions), at D = 128 it does not (1013, 1032 without)
+        if constexpr (D == 64)
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(abf16x2, y), __builtin_bit_cast(abf16x2, 0x3f803f80u), sum, false);
+        else
+          sum += y0, sum += y1;
         w[n / 4][n % 4] = y;
       };
       constexpr int LATE = AHEAD ? 4 : 0;  // weights of the last 8 keys of the lane's, beside the product's first steps

@@ -9,6 +9,11 @@
 // within a lane but for one exchange over the lane groups, and S^T's own layout is the second operand of
 // O^T = V^T P^T: keys in the order that S^T leaves them, V read transposed in the same order. The waves' parts (running
 // maximum, sum, O) are joined in LDS, those of a stream's chunks by a second kernel, in order.
+// What is not seen is loaded as zeros, so that nothing of it (a NaN, say) meets a weight of 0.
+// Loads bypass the caches' retention, and the key heads of one chunk stand beside one another in the grid (a cache's row is all
+// of them): 64 streams over caches of 4096 .. 8192 rows, 16 heads on 4, D = 128: 155 us, 5.4 TB/s, the rate of a copy (202 us
+// without both). One stream over 32768 rows: 20 us where its bytes take 13; two launches and the first loads' chain (length and
+// pages, rows, queries) are the rest.
 // Sums, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
 #include <algorithm>
 #include <cmath>

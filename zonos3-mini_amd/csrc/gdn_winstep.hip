@@ -327,14 +327,15 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
   }
 }
 
-// A workgroup for each stream and query head joins its chunks' parts: JG groups of D threads, every JG-th chunk each, in order,
-// with a running maximum (so that a part's statistics and values are read at one time), then the groups' sums.
-constexpr int WS_JOIN = 512;  // threads
+// A workgroup for each stream and query head joins its chunks' parts: groups of D threads, JOIN_AT parts each at a time, in
+// order, with a running maximum (so that a part's statistics and values are read at one time), then the groups' sums. The first
+// parts are read while the length is, whether there are as many or not.
+constexpr int JOIN_AT = 8, JOIN_MOST = 1024;  // parts a group at a time; threads, at most
 struct Joined {
   float top = -INFINITY, sum = 0.f, x = 0.f;
   bool any = false;
   __device__ __forceinline__ void add(float t, float l, float v) {  // (l below zero: the part saw nothing)
-    const bool saw = !(l < 0.f);
+    const bool saw = !(l < 0.f);  // (what is not there may be any bits)
     const float next = saw ? fmaxf(top, t) : top, base = next == -INFINITY ? 0.f : next, keep = exp2_of(top - base);
     const float f = exp2_of(t - base);
     top = next;
@@ -344,9 +345,9 @@ struct Joined {
   }
 };
 template <typename T, int D>
-__global__ __launch_bounds__(WS_JOIN) void win_step_join_kernel(WinStepArgs a) {
-  constexpr int JG = WS_JOIN / D;
-  __shared__ float x_of[JG][D], top_of[JG], sum_of[JG];
+__global__ __launch_bounds__(JOIN_MOST) void win_step_join_kernel(WinStepArgs a) {
+  __shared__ float x_of[JOIN_MOST / D][D], top_of[JOIN_MOST / D], sum_of[JOIN_MOST / D];
+  const int groups = blockDim.x / D;
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq, G = a.Hq / a.Hk, hk = h / G, qg = (h - hk * G) / a.gq;
   const size_t unit = ((size_t)b * a.Hk + hk) * a.q_groups + qg;
   const size_t at = unit * a.splits * a.gq + (h - hk * G - qg * a.gq);
@@ -355,19 +356,23 @@ __global__ __launch_bounds__(WS_JOIN) void win_step_join_kernel(WinStepArgs a) {
   const int used = (tiles.n + a.chunk - 1) / a.chunk;
   const int d = threadIdx.x % D, jg = threadIdx.x / D;
   Joined j;
-  constexpr int AT = 8;  // parts read at a time
-  for (int i0 = jg; i0 < used; i0 += JG * AT) {
-    float2 ml[AT];
-    float x[AT];
+  int i0 = jg;
+  do {
+    float2 ml[JOIN_AT];
+    float x[JOIN_AT];
 #pragma unroll
-    for (int e = 0; e < AT; ++e) {
-      const size_t p = at + (size_t)min(i0 + e * JG, used - 1) * a.gq;
+    for (int e = 0; e < JOIN_AT; ++e) {
+      const size_t p = at + (size_t)min(i0 + e * groups, a.splits - 1) * a.gq;
       ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
       x[e] = a.part_o[p * D + d];
     }
 #pragma unroll
-    for (int e = 0; e < AT; ++e) j.add(ml[e].x, i0 + e * JG < used ? ml[e].y : -1.f, x[e]);
-  }
+    for (int e = 0; e < JOIN_AT; ++e) {
+      const bool there = i0 + e * groups < used;
+      j.add(ml[e].x, there ? ml[e].y : -1.f, x[e]);
+    }
+    i0 += JOIN_AT * groups;
+  } while (i0 < used);
   x_of[jg][d] = j.x;
   if (d == 0) {
     top_of[jg] = j.top;
@@ -375,8 +380,7 @@ __global__ __launch_bounds__(WS_JOIN) void win_step_join_kernel(WinStepArgs a) {
   }
   __syncthreads();
   if (jg != 0) return;
-#pragma unroll
-  for (int i = 1; i < JG; ++i) j.add(top_of[i], sum_of[i], x_of[i][d]);
+  for (int i = 1; i < groups; ++i) j.add(top_of[i], sum_of[i], x_of[i][d]);
   io<T>::store(reinterpret_cast<T*>(a.o) + (size_t)blockIdx.x * D + d, j.any ? j.x / j.sum : 0.f);
 }
 
@@ -421,7 +425,9 @@ void launch_win_step(const WinStepArgs& a, bool wide, hipStream_t s) {
     return;
   }
   hipLaunchKernelGGL((win_step_kernel<T, D, WS_NW, 2>), dim3(units * a.splits), dim3(64 * WS_NW), 0, s, a);
-  if (a.splits > 1) hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(WS_JOIN), 0, s, a);
+  if (a.splits == 1) return;
+  const int groups = std::min((a.splits + JOIN_AT - 1) / JOIN_AT, JOIN_MOST / D);
+  hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(groups * D), 0, s, a);
 }
 
 bool step_sizes(int B, long room, int Hq, int Hk, int D, int window, int sinks, int dtype) {
@@ -482,7 +488,7 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
     return fail(ZGDN_EINVAL, "%s: q, caches, o and workspace need 16-byte aligned bases", fn);
   if (((uintptr_t)lengths | (uintptr_t)pages) % 4) return fail(ZGDN_EINVAL, "%s: lengths, pages not on 4-byte boundaries", fn);
   const StepPlan p = step_plan(B, room, Hq, Hk, window, sinks, dtype);
-  if ((long)B * Hk * p.q_groups * p.splits > (1L << 32) / (64 * WS_NW) - 1 || (long)B * Hq > (1L << 32) / WS_JOIN - 1)
+  if ((long)B * Hk * p.q_groups * p.splits > (1L << 32) / (64 * WS_NW) - 1 || (long)B * Hq > (1L << 32) / JOIN_MOST - 1)
     return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Hq=%d x %d chunks", fn, B, Hq, p.splits);
   const size_t need = step_bytes(p, B, Hk, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))

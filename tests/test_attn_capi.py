@@ -74,7 +74,8 @@ def test_window_fwd_refuses(native):
         (dict(q=None), "null"), (dict(v=None), "null"), (dict(o=None), "null"), (dict(q_ld=1023), "row strides"),
         (dict(k_ld=248), "row strides"), (dict(v_ld=1 << 23), "row strides"), (dict(k=ODD), "16-byte"), (dict(o=P), "overlaps"),
         (dict(o=ctypes.c_void_p(_at(2).value + 512)), "overlaps"), (dict(B=1 << 12, Tq=1 << 20), "rows"),
-        (dict(cu_q=ctypes.c_void_p(_at(4).value + 2), cu_k=_at(5), B=1, n_seqs=2), "4-byte")])
+        (dict(cu_q=ctypes.c_void_p(_at(4).value + 2), cu_k=_at(5), B=1, n_seqs=2), "4-byte"),
+        (dict(ws=ODD), "16-byte"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale")])
     assert native.lib().zattn_window_fwd(*{**args, "Tq": 0}.values()) == native.OK
 
 
@@ -95,7 +96,7 @@ def test_window_step_refuses(native):
         (dict(n_pages=1 << 25), "positions a stream"), (dict(lengths=None), "null"), (dict(vc=None), "null"), (dict(kc_ld=250), "row strides"),
         (dict(vc_ld=128), "row strides"), (dict(q_ld=1 << 23), "row strides"), (dict(kc=ODD), "16-byte"), (dict(ws=ODD), "16-byte"),
         (dict(pages=ctypes.c_void_p(_at(4).value + 2)), "4-byte"), (dict(ws=None), "workspace"), (dict(ws_bytes=need - 1), "workspace"),
-        (dict(o=P), "overlap"), (dict(ws=_at(1)), "overlap"), (dict(ws=_at(5)), "overlap")])
+        (dict(o=P), "overlap"), (dict(ws=_at(1)), "overlap"), (dict(ws=_at(5)), "overlap"), (dict(scale=float("-inf")), "scale")])
     assert native.lib().zattn_window_step(*{**args, "B": 0}.values()) == native.OK
 
 

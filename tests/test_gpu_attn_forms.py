@@ -96,6 +96,21 @@ def test_not_finite(gdn, cuda, sizes, rows, shared):
     assert torch.equal(o[0][~hit], clean[0][~hit]) and torch.equal(o[1:], clean[1:])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_windows_and_sinks_that_hold_all(gdn, cuda, dtype):
+    """A window of all keys or of more, and sinks of all, are no window: to the bit, dense, packed and for one token."""
+    announce(f"windows of all keys {dtype}")
+    q, k, v = (t.to(cuda) for t in _inputs(1, 150, 190, 4, 2, 64, dtype, 44))
+    n = torch.tensor([190], dtype=torch.int32, device=cuda)
+    for call in (lambda **kw: gdn.window_attn_fwd(q, k, v, **kw), lambda **kw: gdn.window_attn_step(q[:, -1], k, v, n, **kw),
+                 lambda **kw: gdn.window_attn_fwd(q, k, v, cu_seqlens=[0, 40, 150], cu_seqlens_k=[0, 60, 190], **kw)):
+        plain = call()
+        for kw in (dict(window=190), dict(window=191, sinks=3), dict(window=1 << 31), dict(window=1 << 40, sinks=1 << 40)):
+            assert torch.equal(call(**kw), plain), kw
+    o = gdn.window_attn_fwd(q, k, v, window=5, sinks=1 << 40)
+    _hold(o[0], q[0].cpu(), k[0].cpu(), v[0].cpu(), torch.arange(150), dtype, window=5, sinks=190)
+
+
 @pytest.mark.parametrize("sizes,rows,shared", FORMS[::2])
 def test_repeats_over_dirty_memory(gdn, cuda, sizes, rows, shared):
     """The same to the bit, whatever a call's LDS and workspace held: between them calls whose values are all NaN."""

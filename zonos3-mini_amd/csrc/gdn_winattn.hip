@@ -856,7 +856,7 @@ WinArgs plan_args(int packed, int n_seqs, int Tq, int Tk, int Hq, int Hk, int wi
   WinArgs a{};
   a.cu_q = packed ? &bounds : nullptr;
   a.N = n_seqs, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hk = Hk;
-  a.window = std::min(window, 1 << 30), a.sinks = std::min(sinks, 1 << 30);
+  a.window = window >= Tk ? 0 : window, a.sinks = std::min(sinks, 1 << 30);
   return a;
 }
 
@@ -914,11 +914,12 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
   if (bad(q_ld, wq) || bad(k_ld, wk) || bad(v_ld, wk))
     return fail(ZGDN_EINVAL, "%s: row strides q=%ld k=%ld v=%ld (multiples of %d elements, at least a row, at most 2^22)", fn,
                 q_ld, k_ld, v_ld, ve);
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 16)
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)workspace) % 16)
     return fail(ZGDN_EINVAL, "%s: q, k, v, o and workspace need 16-byte aligned bases", fn);
   if (((uintptr_t)cu_q | (uintptr_t)cu_k) % 4) return fail(ZGDN_EINVAL, "%s: cu_q, cu_k not on 4-byte boundaries", fn);
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
-  window = std::min(window, 1 << 30), sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
+  if (window >= Tk) window = 0;        // (every key up to the query)
+  sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
             fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 0, 1, nullptr, nullptr};
   const WinPlan p = win_plan(a, D, dtype);

@@ -442,7 +442,7 @@ extern "C" size_t zattn_window_step_workspace_bytes(int B, long room, int Hq, in
                                                     int dtype) {
   using namespace zgdn;
   if (!step_sizes(B, room, Hq, Hk, D, window, sinks, dtype) || B == 0) return 0;
-  return step_bytes(step_plan(B, room, Hq, Hk, std::min(window, 1 << 30), std::min(sinks, 1 << 30), dtype), B, Hk, D);
+  return step_bytes(step_plan(B, room, Hq, Hk, window >= room ? 0 : window, std::min(sinks, 1 << 30), dtype), B, Hk, D);
 }
 
 // (for tests) Whether a call takes one launch of wide workgroups, and the chunks of a stream, for the same sizes.
@@ -450,7 +450,7 @@ extern "C" int zgdn_window_step_form(int B, long room, int Hq, int Hk, int windo
   using namespace zgdn;
   if (!step_sizes(B, room, Hq, Hk, 64, window, sinks, dtype) || B == 0)
     return fail(ZGDN_EINVAL, "zgdn_window_step_form: bad sizes");
-  const StepPlan p = step_plan(B, room, Hq, Hk, std::min(window, 1 << 30), std::min(sinks, 1 << 30), dtype);
+  const StepPlan p = step_plan(B, room, Hq, Hk, window >= room ? 0 : window, std::min(sinks, 1 << 30), dtype);
   form[0] = p.wide;
   form[1] = p.splits;
   return ZGDN_OK;
@@ -475,7 +475,8 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
   const long room = (long)page_size * n_pages;
   if (room > MOST_ROOM) return fail(ZGDN_EUNSUPPORTED, "%s: %ld positions a stream", fn, room);
   if (!std::isfinite(scale)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
-  window = std::min(window, 1 << 30), sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
+  if (window >= room) window = 0;  // (every position)
+  sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   if (B == 0) return ZGDN_OK;
   if (!q || !o || !lengths || (n_rows > 0 && (!k_cache || !v_cache))) return fail(ZGDN_EINVAL, "%s: null tensor pointer", fn);
   const int ve = dtype == ZGDN_F32 ? 4 : 8;

@@ -31,6 +31,19 @@
 namespace zgdn {
 namespace {
 
+// n / d for n below 2^31, by a product: n mul / 2^(31 + shift), 2^shift >= d, with mul = 2^(31 + shift) / d rounded up by less
+// than 1, so that the result is less than n / 2^(31 + shift) <= 1 / d too large. (A division is twenty vector instructions, of
+// uniform numbers as well: 1000 tokens of 8 + 2 heads 14.6 -> 14.2 us, 64 rows behind 8192 keys 17.1 -> 16.6.)
+struct Over {
+  uint32_t mul, shift;
+  Over() = default;
+  explicit Over(uint32_t d) : shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return __umulhi(n << 1, mul) >> shift; }
+};
+
 struct WinArgs {
   const void *q, *k, *v;
   long q_ld, k_ld, v_ld;
@@ -39,7 +52,8 @@ struct WinArgs {
   int N, Tq, Tk, Hq, Hk, window, sinks;
   float c;    // |scale| log2(e)
   int flip;   // scale below zero: the queries change their signs
-  int tiles;  // of rows a key head, at most
+  int G, per;  // query heads of a key head; tiles of a sequence's rows, where all have as many
+  Over over_G, over_Hk, over_N, over_splits;
   int paired;               // two workgroups a CU hold the whole call
   int splits;               // workgroups that share a tile of 32 rows
   float *part_o, *part_ml;  // [workgroup][32][D], [workgroup][32][maximum, sum, whether V was zeroed, -]
@@ -63,29 +77,28 @@ struct RowTile {
 };
 template <int ROWS>
 __device__ __forceinline__ bool find_rows(const WinArgs& a, int i, RowTile& t) {
-  const int G = a.Hq / a.Hk;
   if (a.cu_q == nullptr) {
-    const int per = a.tiles / a.N, s = i % a.N;
-    const int j = i / a.N;
-    t = {s * a.Tq, a.Tq, s * a.Tk, a.Tk, a.paired && 2 * j >= per ? j - (per + 1) / 2 : per - 1 - j};
+    const int j = (int)a.over_N(i), s = i - j * a.N;
+    t = {s * a.Tq, a.Tq, s * a.Tk, a.Tk, a.paired && 2 * j >= a.per ? j - (a.per + 1) / 2 : a.per - 1 - j};
     return true;
   }
   const int l = threadIdx.x & 63;
   int taken = 0;
   for (int s0 = 0; s0 < a.N; s0 += 64) {
-    int b = 0, e = 0;
-    if (s0 + l < a.N) seq_bounds(a.cu_q, s0 + l, a.Tq, b, e);
-    const int mine = (int)(((long)(e - b) * G + ROWS - 1) / ROWS), upto = prefix_count(mine);
+    int b = 0, e = 0, kb = 0, ke = 0;
+    if (s0 + l < a.N) {
+      seq_bounds(a.cu_q, s0 + l, a.Tq, b, e);
+      seq_bounds(a.cu_k, s0 + l, a.Tk, kb, ke);
+    }
+    const int mine = (int)(((uint32_t)(e - b) * a.G + (ROWS - 1)) / ROWS), upto = prefix_count(mine);
     const int all = __builtin_amdgcn_readlane(upto, 63);
     if (i < taken + all) {
       const int at = __builtin_ctzll(__ballot(i - taken < upto));
-      int kb, ke;
-      seq_bounds(a.cu_k, s0 + at, a.Tk, kb, ke);
       const int n = __builtin_amdgcn_readlane(mine, at), before = __builtin_amdgcn_readlane(upto, at) - n;
       b = __builtin_amdgcn_readlane(b, at);
       e = __builtin_amdgcn_readlane(e, at);
-      kb = __builtin_amdgcn_readfirstlane(kb);
-      ke = __builtin_amdgcn_readfirstlane(ke);
+      kb = __builtin_amdgcn_readlane(kb, at);
+      ke = __builtin_amdgcn_readlane(ke, at);
       t = {b, e - b, kb, ke - kb, n - 1 - (i - taken - before)};
       return true;
     }
@@ -173,13 +186,13 @@ struct Rows {
   KeyList keys;
   __device__ __forceinline__ bool find(const WinArgs& a, int i, int key_head) {
     if (!find_rows<ROWS>(a, i, t)) return false;
-    G = a.Hq / a.Hk;
+    G = a.G;
     hk = key_head;
     rows = (uint32_t)t.nq * G;
     r0 = (uint32_t)t.tile * ROWS;
     past = t.nk - t.nq;
-    first = past + (int)(r0 / G);
-    last = past + (int)((min(rows, r0 + ROWS) - 1) / G);
+    first = past + (int)a.over_G(r0);
+    last = past + (int)a.over_G(min(rows, r0 + ROWS) - 1);
     keys = key_list<KT>(a, first, last);
     first -= keys.shift;
     last -= keys.shift;
@@ -542,13 +555,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : sizeof(T) == 2 ? 2 : 1) void
   auto v_lds = [&](int i) { return stages[2 + (i & 1)]; };
   const int wave = wave_id(), m = threadIdx.x & 31;
   R r;
-  if (!r.find(a, blockIdx.x / a.Hk, blockIdx.x % a.Hk)) return;
+  const int of_keys = (int)a.over_Hk(blockIdx.x);
+  if (!r.find(a, of_keys, blockIdx.x - of_keys * a.Hk)) return;
   const uint32_t rw = r.r0 + 32 * wave, row = min(rw + m, r.rows - 1);  // (lanes behind the last row: as that one, without stores)
   const bool real = rw + m < r.rows;
-  const int qi = (int)(row / r.G), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
+  const int qi = (int)a.over_G(row), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
   const int shift = r.keys.shift, n = r.keys.n, p = r.past + qi - shift;
-  const int wfirst = r.past + (int)(min(r.rows - 1, rw) / r.G) - shift;
-  const int wlast = r.past + (int)((min(r.rows, rw + 32) - 1) / r.G) - shift;
+  const int wfirst = r.past + (int)a.over_G(min(r.rows - 1, rw)) - shift;
+  const int wlast = r.past + (int)a.over_G(min(r.rows, rw + 32) - 1) - shift;
   constexpr int RP = 1024 / ROWB;
   const WholeTiles whole = r.whole(a, r.first, r.last), whole_w = r.whole(a, wfirst, wlast);
   TileLoads<T, D, KT, LW> load_k(a.k, a.k_ld, r.t, r.hk, wave * LW * RP), load_v(a.v, a.v_ld, r.t, r.hk, wave * LW * RP);
@@ -638,11 +652,11 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
   const int wave = wave_id(), m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
   auto k_lds = [&](int stage) { return tile_lds + (wave * RING + stage) * FewCfg<T, D>::TILE; };
   auto v_lds = [&](int stage) { return k_lds(stage) + KT * ROWB; };
-  const int ts = blockIdx.x / a.Hk, split = ts % a.splits;
+  const int ts = (int)a.over_Hk(blockIdx.x), tile = (int)a.over_splits(ts), split = ts - tile * a.splits;
   R r;
-  if (!r.find(a, ts / a.splits, blockIdx.x % a.Hk)) return;
+  if (!r.find(a, tile, blockIdx.x - ts * a.Hk)) return;
   const uint32_t row = min(r.r0 + m, r.rows - 1);
-  const int qi = (int)(row / r.G), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
+  const int qi = (int)a.over_G(row), hq = r.hk * r.G + (int)(row - (uint32_t)qi * r.G);
   const int p = r.past + qi - r.keys.shift;
   const int t0 = (int)((long)r.keys.n * split / a.splits), t1 = (int)((long)r.keys.n * (split + 1) / a.splits);
   const WholeTiles whole = r.whole(a, r.first, r.last);
@@ -719,7 +733,7 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
       if (d == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * at) = make_float4(best, all, dirty ? 1.f : 0.f, 0.f);
     } else {
       const uint32_t rr = r.r0 + x;
-      const int q = (int)(rr / r.G), hh = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
+      const int q = (int)a.over_G(rr), hh = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
       const float inv = r.past + q < 0 ? 0.f : 1.f / all;
       io<T>::store4(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + q) * a.Hq + hh) * D + d,
                     make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
@@ -741,9 +755,9 @@ __global__ __launch_bounds__(64 * FEW_NW, 2) void win_few_kernel(WinArgs a) {
 template <typename T, int D>
 __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
   using R = Rows<32, FEW_KT>;
-  const int t8 = blockIdx.x / a.Hk, tile = t8 / 4;
+  const int t8 = (int)a.over_Hk(blockIdx.x), tile = t8 / 4;
   R r;
-  if (!r.find(a, tile, blockIdx.x % a.Hk)) return;
+  if (!r.find(a, tile, blockIdx.x - t8 * a.Hk)) return;
   const int x = (t8 & 3) * 8 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   const bool real = r.r0 + x < r.rows;
   float top = -INFINITY, sum = 0.f;
@@ -771,7 +785,7 @@ __global__ __launch_bounds__(2 * D) void win_few_join_kernel(WinArgs a) {
       }
   }
   const uint32_t rr = min(r.r0 + x, r.rows - 1);
-  const int q = (int)(rr / r.G), hq = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
+  const int q = (int)a.over_G(rr), hq = r.hk * r.G + (int)(rr - (uint32_t)q * r.G);
   if (real) {
     const float inv = r.past + q < 0 ? 0.f : 1.f / sum;
     io<T>::store4(reinterpret_cast<T*>(a.o) + ((size_t)(r.t.q0 + q) * a.Hq + hq) * D + d,
@@ -834,7 +848,9 @@ size_t win_bytes(const WinPlan& p, const WinArgs& a, int D) {
 template <typename T, int D>
 bool launch_win(WinArgs a, const WinPlan& p, hipStream_t s) {
   static std::atomic<signed char> ready[MAX_DEVICES];
-  a.tiles = (int)p.tiles;
+  a.G = a.Hq / a.Hk;
+  a.per = (int)(p.tiles / a.N);
+  a.over_G = Over(a.G), a.over_Hk = Over(a.Hk), a.over_N = Over(a.N), a.over_splits = Over(p.splits);
   a.splits = p.splits;
   a.paired = p.rows == 128 && p.tiles * a.Hk <= 2 * device_cus();
   const unsigned n = (unsigned)(p.tiles * a.Hk);
@@ -921,7 +937,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
   if (window >= Tk) window = 0;        // (every key up to the query)
   sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
-            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f, 0, 0, 1, nullptr, nullptr};
+            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f};
   const WinPlan p = win_plan(a, D, dtype);
   if (p.tiles * p.splits * Hk > (1L << 32) / 256 - 1) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
   const size_t need = win_bytes(p, a, D);

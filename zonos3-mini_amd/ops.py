@@ -1239,6 +1239,17 @@ def _cache_ld(name: str, t, heads: int, D: int, dtype, index: int, dev) -> int:
     return ld
 
 
+def _norm_weight(name: str, t, D: int, index: int, dev):
+    """(dtype code, address) of a norm's weight [D]."""
+    _plain(name, t, index, dev)
+    if t.shape != (D,):
+        raise RuntimeError(f"{name}: expected [{D}], got {tuple(t.shape)}")
+    code, at = _code(t, name), t.data_ptr()
+    if at % 16:
+        raise RuntimeError(f"{name}: not on a 16-byte boundary")
+    return code, at
+
+
 def _window(window, sinks) -> tuple[int, int]:
     if window is None:
         window = 0
@@ -1283,28 +1294,28 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
     if Hq < 1 or Hk < 1:
         raise RuntimeError(f"heads: {Hq} of queries, {Hk} of keys")
     _plain("positions", positions, index, dev)
-    p32 = positions.dtype is torch.int32
-    if positions.shape != lead or not (p32 or positions.dtype is torch.int64):
+    p_type = positions.dtype
+    p32 = p_type is torch.int32
+    if positions.shape != lead or not (p32 or p_type is torch.int64):
         raise RuntimeError(f"positions: expected int64 or int32 {list(lead)}, got {positions.dtype} {tuple(positions.shape)}")
     _plain("inv_freq", inv_freq, index, dev)
-    f32 = inv_freq.dtype is torch.float32
-    if inv_freq.dim() != 1 or not (f32 or inv_freq.dtype is torch.float64):
+    f_type, turned = inv_freq.dtype, inv_freq.shape
+    f32 = f_type is torch.float32
+    if len(turned) != 1 or not (f32 or f_type is torch.float64):
         raise RuntimeError(f"inv_freq: expected float64 or float32 [R / 2], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
-    R = 2 * inv_freq.shape[0]
+    R = 2 * turned[0]
     if R % 16 or R > D:
         raise RuntimeError(f"inv_freq: turns {R} entries of a head (a multiple of 16, at most {D})")
-    w_code = F32
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _plain(name, t, index, dev)
-            if t.dim() != 1 or t.shape[0] != D:
-                raise RuntimeError(f"{name}: expected [{D}], got {tuple(t.shape)}")
-            w_code = _code(t, name)
-            if t.data_ptr() % 16:
-                raise RuntimeError(f"{name}: not on a 16-byte boundary")
-    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
-        raise RuntimeError("q_weight, k_weight: must share a dtype")
+    w_code, qw_at, kw_at = F32, None, None
+    if q_weight is not None:
+        w_code, qw_at = _norm_weight("q_weight", q_weight, D, index, dev)
+    if k_weight is not None:
+        k_code, kw_at = _norm_weight("k_weight", k_weight, D, index, dev)
+        if q_weight is not None and k_code != w_code:
+            raise RuntimeError("q_weight, k_weight: must share a dtype")
+        w_code = k_code
     v_ld = kc_ld = vc_ld = n_rows = 0
+    v_at = kc_at = vc_at = rows_at = None
     if rows is None:
         if k_cache is not None or v_cache is not None or v is not None:
             raise RuntimeError("k_cache, v and v_cache need rows")
@@ -1317,7 +1328,8 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
         if k_cache is None or (v is None) != (v_cache is None):
             raise RuntimeError("rows need k_cache, and v and v_cache go together")
         kc_ld = _cache_ld("k_cache", k_cache, Hk, D, dtype, index, dev)
-        n_rows = k_cache.shape[0] * k_cache.shape[1]
+        pages, page_size, _, _ = k_cache.shape
+        n_rows, kc_at, rows_at = pages * page_size, k_cache.data_ptr(), rows.data_ptr()
         if v is not None:
             v_ld = _heads_ld(v, dtype, index)
             if not v_ld or v.shape != k.shape:
@@ -1325,13 +1337,17 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e
             vc_ld = _cache_ld("v_cache", v_cache, Hk, D, dtype, index, dev)
             if v_cache.shape != k_cache.shape:
                 raise RuntimeError(f"v_cache: {tuple(v_cache.shape)}, expected {tuple(k_cache.shape)} as k_cache")
-    q_out = q.new_empty(shape)
-    k_out = k.new_empty(k.shape) if output_k else None
+            v_at, vc_at = v.data_ptr(), v_cache.data_ptr()
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out, k_at = None, None
+    if output_k:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_at = k_out.data_ptr()
     n = positions.numel()
     if n:
-        _launch(index, dev, "zattn_qk_norm_rope", q.data_ptr(), q_ld, k.data_ptr(), k_ld, _ptr(v), v_ld, code,
-                positions.data_ptr(), p32, inv_freq.data_ptr(), f32, _ptr(q_weight), _ptr(k_weight), w_code, eps, interleaved,
-                q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), kc_ld, _ptr(v_cache), vc_ld, _ptr(rows), n_rows, n, Hq, Hk, D, R)
+        _launch(index, dev, "zattn_qk_norm_rope", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v_at, v_ld, code,
+                positions.data_ptr(), p32, inv_freq.data_ptr(), f32, qw_at, kw_at, w_code, eps, interleaved, q_out.data_ptr(),
+                k_at, kc_at, kc_ld, vc_at, vc_ld, rows_at, n_rows, n, Hq, Hk, D, R)
     if (q.requires_grad or k.requires_grad or inv_freq.requires_grad or (q_weight is not None and q_weight.requires_grad)
             or (k_weight is not None and k_weight.requires_grad)):
         inputs = (q, k, inv_freq, q_weight, k_weight)
@@ -1387,7 +1403,7 @@ def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, 
         n_seqs = cu_seqlens.numel() - 1
         if cu_seqlens_k.numel() != n_seqs + 1:
             raise RuntimeError(f"cu_seqlens_k: {cu_seqlens_k.numel()} entries, expected {n_seqs + 1} as cu_seqlens")
-    o = q.new_empty(q.shape)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     size = _window_fwd_workspace(int(cu_seqlens is not None), n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, code)
     workspace = o.new_empty(size, dtype=torch.uint8) if size else None
     _launch(index, dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
@@ -1455,7 +1471,7 @@ def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=N
     window, sinks = _window(window, sinks)
     if B == 0 or page_size * n_pages == 0:
         return q.new_zeros(q.shape)
-    o = q.new_empty(q.shape)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     size = _window_step_workspace(B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
     workspace = o.new_empty(size, dtype=torch.uint8) if size else None
     _launch(index, dev, "zattn_window_step", q.data_ptr(), q_ld, k_cache.data_ptr(), kc_ld, v_cache.data_ptr(), vc_ld, code,

@@ -12,7 +12,7 @@
 // What is not seen is loaded as zeros, so that nothing of it (a NaN, say) meets a weight of 0.
 // Loads bypass the caches' retention, and the key heads of one chunk stand beside one another in the grid (a cache's row is all
 // of them): 64 streams over caches of 4096 .. 8192 rows, 16 heads on 4, D = 128: 155 us, 5.4 TB/s, the rate of a copy (202 us
-// without both). One stream over 32768 rows: 20 us where its bytes take 13; two launches and the first loads' chain (length and
+// without both). One stream over 32768 rows: 20.6 us where its bytes take 13; two launches and the first loads' chain (length and
 // pages, rows, queries) are the rest.
 // Sums, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
 #include <algorithm>
@@ -327,61 +327,73 @@ __global__ __launch_bounds__(64 * NW) void win_step_kernel(WinStepArgs a) {
   }
 }
 
-// A workgroup for each stream and query head joins its chunks' parts: groups of D threads, JOIN_AT parts each at a time, in
-// order, with a running maximum (so that a part's statistics and values are read at one time), then the groups' sums. The first
-// parts are read while the length is, whether there are as many or not.
-constexpr int JOIN_AT = 8, JOIN_MOST = 1024;  // parts a group at a time; threads, at most
-struct Joined {
-  float top = -INFINITY, sum = 0.f, x = 0.f;
-  bool any = false;
-  __device__ __forceinline__ void add(float t, float l, float v) {  // (l below zero: the part saw nothing)
-    const bool saw = !(l < 0.f);  // (what is not there may be any bits)
-    const float next = saw ? fmaxf(top, t) : top, base = next == -INFINITY ? 0.f : next, keep = exp2_of(top - base);
-    const float f = exp2_of(t - base);
-    top = next;
-    sum = fmaf(sum, keep, saw ? l * f : 0.f);
-    x = fmaf(x, keep, saw ? v * f : 0.f);
-    any = any || saw;
-  }
-};
+// A workgroup for each stream and query head joins its chunks' parts: groups of D / 4 lanes, JOIN_AT parts each at a time, in
+// order, with a running maximum (so that a part's statistics and values are read at one time); then its first wave the groups'
+// sums. The first parts are read while the length is, whether there are as many or not.
+constexpr int JOIN_AT = 4, JOIN_MOST = 1024;  // parts a group at a time; threads, at most
 template <typename T, int D>
 __global__ __launch_bounds__(JOIN_MOST) void win_step_join_kernel(WinStepArgs a) {
-  __shared__ float x_of[JOIN_MOST / D][D], top_of[JOIN_MOST / D], sum_of[JOIN_MOST / D];
-  const int groups = blockDim.x / D;
+  constexpr int LANES = D / 4, MOST = JOIN_MOST / LANES, EACH = D / 64;
+  __shared__ __align__(16) float x_of[MOST][D];
+  __shared__ float top_of[MOST], sum_of[MOST];
+  static_assert(MOST <= 64, "a lane for each group");
+  const int groups = blockDim.x / LANES;
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq, G = a.Hq / a.Hk, hk = h / G, qg = (h - hk * G) / a.gq;
   const size_t unit = ((size_t)b * a.Hk + hk) * a.q_groups + qg;
   const size_t at = unit * a.splits * a.gq + (h - hk * G - qg * a.gq);
   int n, lo;
   const KeyTiles tiles = stream_tiles<WsCfg<T>::TILE>(a, b, n, lo);
   const int used = (tiles.n + a.chunk - 1) / a.chunk;
-  const int d = threadIdx.x % D, jg = threadIdx.x / D;
-  Joined j;
+  const int d = 4 * (threadIdx.x % LANES), jg = threadIdx.x / LANES;
+  float top = -INFINITY, sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool any = false;
   int i0 = jg;
   do {
     float2 ml[JOIN_AT];
-    float x[JOIN_AT];
+    float4 u[JOIN_AT];
 #pragma unroll
     for (int e = 0; e < JOIN_AT; ++e) {
       const size_t p = at + (size_t)min(i0 + e * groups, a.splits - 1) * a.gq;
       ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
-      x[e] = a.part_o[p * D + d];
+      u[e] = *reinterpret_cast<const float4*>(a.part_o + p * D + d);
     }
 #pragma unroll
     for (int e = 0; e < JOIN_AT; ++e) {
-      const bool there = i0 + e * groups < used;
-      j.add(ml[e].x, there ? ml[e].y : -1.f, x[e]);
+      const bool saw = i0 + e * groups < used && !(ml[e].y < 0.f);  // (a sum below zero: the part saw nothing)
+      if (!saw) continue;                                           // (what is not there may be any bits)
+      const float next = fmaxf(top, ml[e].x), base = next == -INFINITY ? 0.f : next;
+      const float keep = exp2_of(top - base), f = exp2_of(ml[e].x - base);
+      top = next;
+      sum = fmaf(sum, keep, ml[e].y * f);
+      x = make_float4(fmaf(x.x, keep, u[e].x * f), fmaf(x.y, keep, u[e].y * f), fmaf(x.z, keep, u[e].z * f),
+                      fmaf(x.w, keep, u[e].w * f));
+      any = true;
     }
     i0 += JOIN_AT * groups;
   } while (i0 < used);
-  x_of[jg][d] = j.x;
+  *reinterpret_cast<float4*>(&x_of[jg][d]) = x;
   if (d == 0) {
-    top_of[jg] = j.top;
-    sum_of[jg] = j.any ? j.sum : -1.f;
+    top_of[jg] = top;
+    sum_of[jg] = any ? sum : -1.f;
   }
   __syncthreads();
-  if (jg != 0) return;
-  for (int i = 1; i < groups; ++i) j.add(top_of[i], sum_of[i], x_of[i][d]);
-  io<T>::store(reinterpret_cast<T*>(a.o) + (size_t)blockIdx.x * D + d, j.any ? j.x / j.sum : 0.f);
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
+  const float l = lane < groups ? sum_of[lane] : -1.f, t = lane < groups ? top_of[lane] : -INFINITY;
+  const bool saw = !(l < 0.f);
+  const float best = wave_max(t);
+  const float f = saw ? exp2_of(t - (best == -INFINITY ? 0.f : best)) : 0.f, all = wave_sum(saw ? l * f : 0.f);
+  float o[EACH] = {};
+  for (int g = 0; g < groups; ++g) {
+    const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), g));
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) o[e] = fmaf(x_of[g][64 * e + lane], w, o[e]);
+  }
+  const bool seen = __any(saw);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    io<T>::store(reinterpret_cast<T*>(a.o) + (size_t)blockIdx.x * D + 64 * e + lane, seen ? o[e] / all : 0.f);
 }
 
 // How a call is cut: chunks of at most WS_KEYS keys, of at least a tile for each wave, two workgroups for each CU where the
@@ -426,8 +438,9 @@ void launch_win_step(const WinStepArgs& a, bool wide, hipStream_t s) {
   }
   hipLaunchKernelGGL((win_step_kernel<T, D, WS_NW, 2>), dim3(units * a.splits), dim3(64 * WS_NW), 0, s, a);
   if (a.splits == 1) return;
-  const int groups = std::min((a.splits + JOIN_AT - 1) / JOIN_AT, JOIN_MOST / D);
-  hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(groups * D), 0, s, a);
+  constexpr int WAVE = 64 / (D / 4);  // groups of a wave
+  const int waves = std::min((a.splits + JOIN_AT * WAVE - 1) / (JOIN_AT * WAVE), JOIN_MOST / 64);
+  hipLaunchKernelGGL((win_step_join_kernel<T, D>), dim3((unsigned)(a.B * a.Hq)), dim3(64 * waves), 0, s, a);
 }
 
 bool step_sizes(int B, long room, int Hq, int Hk, int D, int window, int sinks, int dtype) {

@@ -32,6 +32,7 @@ extern "C" {
  *   q_weight, k_weight [D] in w_dtype, or NULL (ones). q_out [n_tokens, Hq, D] dense. k_out [n_tokens, Hk, D] dense, or NULL.
  *   k_cache, v_cache with `rows` (int64 [n_tokens]), or all NULL: token t's k (turned) and v go to rows[t] of the
  *   n_cache_rows rows, kc_ld and vc_ld elements apart; a row outside the cache is not written. k_cache alone: v is NULL.
+ *   (A cache of no rows may be NULL.)
  *   Where two tokens name one row, it holds pieces of either. Outputs overlap no other operand.
  */
 int zattn_qk_norm_rope(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, int dtype,

@@ -119,3 +119,15 @@ def test_nothing_to_do(gdn, cuda):
     q, k = gdn.qk_norm_rope(torch.empty(0, 2, 64, device=cuda), torch.empty(0, 1, 64, device=cuda),
                             torch.empty(0, dtype=torch.long, device=cuda), f)
     assert q.shape == (0, 2, 64) and k.shape == (0, 1, 64)
+
+
+def test_cache_of_no_rows(gdn, cuda):
+    """A cache without pages: no row is in it, and what comes back is what comes back without one."""
+    announce("qk_norm_rope cache of no rows")
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (A.randn(g, 5, h, 64, dtype=BF).to(cuda) for h in (4, 2, 2))
+    at, f, none = torch.arange(5, device=cuda), torch.rand(32, generator=g).to(cuda), torch.empty(0, 16, 2, 64, dtype=BF, device=cuda)
+    want = gdn.qk_norm_rope(q, k, at, f)
+    for kw in (dict(v=v, v_cache=none.clone()), dict()):
+        got = gdn.qk_norm_rope(q, k, at, f, k_cache=none, rows=at, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -251,7 +251,7 @@ extern "C" int zattn_qk_norm_rope(const void* q, long q_ld, const void* k, long 
   for (int dt : {dtype, w_dtype})
     if (dt != ZGDN_F32 && dt != ZGDN_BF16) return fail(ZGDN_EINVAL, "%s: unknown dtype code %d", fn, dt);
   if (rows == nullptr ? k_cache != nullptr || v_cache != nullptr || v != nullptr
-                      : k_cache == nullptr || (v == nullptr) != (v_cache == nullptr))
+                      : n_cache_rows > 0 && (k_cache == nullptr || (v == nullptr) != (v_cache == nullptr)))
     return fail(ZGDN_EINVAL, "%s: rows and k_cache go together, and v and v_cache with them", fn);
   if (n_tokens > 0 && (!q || !k || !positions || !q_out || (R > 0 && !inv_freq)))
     return fail(ZGDN_EINVAL, "%s: null tensor pointer", fn);

@@ -4,6 +4,7 @@ dirty memory, graphs, streams, guarded buffers, offsets past 32 bits (bounds: ``
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -326,3 +327,27 @@ def test_copies_and_empty_calls(gdn, cuda):
     assert not bool(gdn.window_attn_step(q3, c, c, n + 5, pages=torch.zeros(3, 0, dtype=torch.int32, device=cuda)).any())
     assert gdn.window_attn_step(q3[:0], c, c, n[:0], pages=torch.zeros(0, 4, dtype=torch.int32, device=cuda)).shape == (0, 4, 64)
     torch.cuda.synchronize()
+
+
+def test_threads_on_streams_of_their_own(gdn, cuda):
+    """Four threads, a stream and a window each, at one time: each its own results, of both forms and the step."""
+    announce("attention sublayer from four threads")
+    q, k, v = (t.to(cuda) for t in _inputs(1, 700, 700, 8, 2, 128, BF, 45))
+    n = torch.tensor([700], dtype=torch.int32, device=cuda)
+    calls = lambda i: (gdn.window_attn_fwd(q, k, v, window=100 + i, sinks=i),  # noqa: E731
+                       gdn.window_attn_fwd(q[:, -20:], k, v), gdn.window_attn_step(q[:, -1], k, v, n, window=300 + i))
+    want, got = [calls(i) for i in range(4)], [None] * 4
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = calls(i)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))

@@ -1404,7 +1404,8 @@ def window_attn_fwd(q, k, v, window=None, sinks=0, scale=None, cu_seqlens=None, 
         if cu_seqlens_k.numel() != n_seqs + 1:
             raise RuntimeError(f"cu_seqlens_k: {cu_seqlens_k.numel()} entries, expected {n_seqs + 1} as cu_seqlens")
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    size = _window_fwd_workspace(int(cu_seqlens is not None), n_seqs, Tq, Tk, Hq, Hk, D, window, sinks, code)
+    size = _attn_workspace(index, "zattn_window_fwd_workspace_bytes", int(cu_seqlens is not None), n_seqs, Tq, Tk, Hq, Hk, D,
+                           window, sinks, code)
     workspace = o.new_empty(size, dtype=torch.uint8) if size else None
     _launch(index, dev, "zattn_window_fwd", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, code, o.data_ptr(),
             _ptr(cu_seqlens), _ptr(cu_seqlens_k), n_seqs, B, Tq, Tk, Hq, Hk, D, window, sinks,
@@ -1425,13 +1426,10 @@ def _bounds_table(cu, total: int, dev):
 
 
 @functools.lru_cache(maxsize=1024)
-def _window_fwd_workspace(*sizes: int) -> int:
-    return int(_native.lib().zattn_window_fwd_workspace_bytes(*sizes))
-
-
-@functools.lru_cache(maxsize=1024)
-def _window_step_workspace(*sizes: int) -> int:
-    return int(_native.lib().zattn_window_step_workspace_bytes(*sizes))
+def _attn_workspace(index: int, query: str, *sizes: int) -> int:
+    """The bytes that entry point ``query`` names for a call on GPU ``index`` (how a call is cut goes by its device's CUs)."""
+    with torch.cuda.device(index):
+        return int(getattr(_native.lib(), query)(*sizes))
 
 
 def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=None, pages=None):
@@ -1472,7 +1470,7 @@ def window_attn_step(q, k_cache, v_cache, lengths, window=None, sinks=0, scale=N
     if B == 0 or page_size * n_pages == 0:
         return q.new_zeros(q.shape)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    size = _window_step_workspace(B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
+    size = _attn_workspace(index, "zattn_window_step_workspace_bytes", B, page_size * n_pages, Hq, Hk, D, window, sinks, code)
     workspace = o.new_empty(size, dtype=torch.uint8) if size else None
     _launch(index, dev, "zattn_window_step", q.data_ptr(), q_ld, k_cache.data_ptr(), kc_ld, v_cache.data_ptr(), vc_ld, code,
             lengths.data_ptr(), _ptr(pages), page_size, n_pages, n * page_size, o.data_ptr(), B, Hq, Hk, D, window, sinks,

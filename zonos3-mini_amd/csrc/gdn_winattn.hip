@@ -23,6 +23,7 @@
 // through a window of 1024 9 us of 329.)
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 
 #include "gdn_attn.h"
@@ -50,7 +51,7 @@ struct WinArgs {
   void* o;
   const int32_t *cu_q, *cu_k;
   int N, Tq, Tk, Hq, Hk, window, sinks;
-  float c;    // |scale| log2(e)
+  float c;    // |scale| log2(e), or 2^-149 (not 0: a masked score, -inf, times c stays -inf, and any other vanishes)
   int flip;   // scale below zero: the queries change their signs
   int G, per;  // query heads of a key head; tiles of a sequence's rows, where all have as many
   Over over_G, over_Hk, over_N, over_splits;
@@ -306,7 +307,7 @@ struct RowWave {
   __device__ __forceinline__ void start(const WinArgs& a, const T* q) {
     const int lane = threadIdx.x & 63;
     m = lane & 31, h = lane >> 5, l = lane & 15, l4 = (lane >> 4) & 1;
-    c = a.c, lag = 8.f / a.c, top = -INFINITY, sum = 0.f;
+    c = a.c, lag = fminf(8.f / a.c, FLT_MAX), top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int t = 0; t < QF; ++t) qf[t] = *reinterpret_cast<const uint4*>(q + (BF ? 16 * t + 8 * h : 8 * t + 4 * h));
     if (a.flip) {
@@ -936,8 +937,9 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
   const size_t es = dtype == ZGDN_F32 ? 4 : 2, nq = (size_t)B * Tq, nk = (size_t)B * Tk, cu = ((size_t)n_seqs + 1) * 4;
   if (window >= Tk) window = 0;        // (every key up to the query)
   sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
+  const float c = fabsf(scale) * LOG2E;
   WinArgs a{q, k, v, q_ld, k_ld, v_ld, o, cu_q, cu_k, cu_q != nullptr ? n_seqs : B, Tq, Tk, Hq, Hk, window, sinks,
-            fmaxf(fabsf(scale) * LOG2E, 1e-30f), scale < 0.f};
+            c > 0.f ? c : FLT_TRUE_MIN, scale < 0.f};
   const WinPlan p = win_plan(a, D, dtype);
   if (p.tiles * p.splits * Hk > (1L << 32) / 256 - 1) return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d rows", fn, B, Tq, Hq);
   const size_t need = win_bytes(p, a, D);

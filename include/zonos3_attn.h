@@ -11,7 +11,7 @@
  * Heads: query head h reads key head h / (Hq / Hk). Head sizes D: 64 or 128. A token's heads are contiguous; *_ld are the
  * elements between tokens (at least a token's, multiples of 16 bytes from 16-byte aligned bases, at most 2^22).
  * Workspaces start on 16-byte boundaries; the bytes that they need go by the CUs of the current device, so they are asked for
- * with the launch's device current. scale is finite.
+ * with the launch's device current. scale and its product with log2(e) are finite in float32.
  * A query at position p sees key j where j <= p and (p - j < window or j < sinks); window 0: no window. A row that sees
  * nothing is zeros. What a row does not see has no part in it, infinities and NaN included.
  */

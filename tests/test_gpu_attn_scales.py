@@ -1,8 +1,10 @@
-"""Attention at the ends of the scale's range: no scale, scales as small as scores are large (bounds: ``attn_testing``)."""
+"""Attention at the ends of the scale's range: no scale, scales as small as scores are large, scales that have no
+finite product with log2 e (bounds: ``attn_testing``)."""
 
 from __future__ import annotations
 
 import ctypes
+import importlib
 
 import pytest
 import torch
@@ -45,3 +47,15 @@ def test_scores_of_any_size(gdn, cuda, scale, size, T, Tq, D, window, rows, shar
     bound = A.attend_bound(want, sizes, slip + 2 * max(2.0**-24 * abs(scale), 2.0**-150) * terms, dtype, T)
     assert A.within(o[at], want, bound) <= 1
     assert A.within(x[0], want[-1], bound[-1]) <= 1
+
+
+def test_scales_without_a_product_are_refused():
+    native = importlib.import_module("zonos3-mini_amd._native")
+    at = lambda n: ctypes.c_void_p((1 << 32) + (n << 28))  # noqa: E731  (never read: calls of nothing)
+    for scale in (2.4e38, -3.4e38):
+        with pytest.raises(RuntimeError, match="scale"):
+            native.call("zattn_window_fwd", at(0), 256, at(1), 128, at(2), 128, 1, at(3), None, None, 0, 1, 0, 9, 4, 2, 64, 0, 0,
+                        scale, None, 0, None)
+        with pytest.raises(RuntimeError, match="scale"):
+            native.call("zattn_window_step", at(0), 256, at(1), 128, at(2), 128, 1, at(4), None, 9, 1, 9, at(3), 0, 4, 2, 64, 0, 0,
+                        scale, None, 0, None)

@@ -922,7 +922,7 @@ extern "C" int zattn_window_fwd(const void* q, long q_ld, const void* k, long k_
     return fail(ZGDN_EINVAL, "%s: packed sequences need B == 1 and n_seqs >= 1 (B=%d n_seqs=%d)", fn, B, n_seqs);
   if ((long)B * Tq > (1L << 30) || (long)B * Tk > (1L << 30) || (long)B * Tq * Hq > (1L << 31))
     return fail(ZGDN_EUNSUPPORTED, "%s: B=%d x Tq=%d x Hq=%d, Tk=%d rows", fn, B, Tq, Hq, Tk);
-  if (!std::isfinite(scale)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
+  if (!std::isfinite(scale * LOG2E)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
   if (Tq == 0) return ZGDN_OK;
   if (!q || !o || (Tk > 0 && (!k || !v))) return fail(ZGDN_EINVAL, "%s: null tensor pointer", fn);
   const int ve = dtype == ZGDN_F32 ? 4 : 8;

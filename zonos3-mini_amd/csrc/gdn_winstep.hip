@@ -487,7 +487,7 @@ extern "C" int zattn_window_step(const void* q, long q_ld, const void* k_cache, 
                 "pages; without: one a stream)", fn, page_size, n_pages, n_rows);
   const long room = (long)page_size * n_pages;
   if (room > MOST_ROOM) return fail(ZGDN_EUNSUPPORTED, "%s: %ld positions a stream", fn, room);
-  if (!std::isfinite(scale)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
+  if (!std::isfinite(scale * LOG2E)) return fail(ZGDN_EINVAL, "%s: scale %g", fn, scale);
   if (window >= room) window = 0;  // (every position)
   sinks = std::min(sinks, 1 << 30);  // (more than positions reach)
   if (B == 0) return ZGDN_OK;

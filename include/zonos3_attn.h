@@ -12,6 +12,8 @@
  * elements between tokens (at least a token's, multiples of 16 bytes from 16-byte aligned bases, at most 2^22).
  * Workspaces start on 16-byte boundaries; the bytes that they need go by the CUs of the current device, so they are asked for
  * with the launch's device current. scale and its product with log2(e) are finite in float32.
+ * Sums are formed in float32. A head whose squares sum to 2^128 or more comes out of its norm as zeros; values of 2^120 (for
+ * zattn_window_step 2^128) over the number of a row's keys and more may become infinities.
  * A query at position p sees key j where j <= p and (p - j < window or j < sinks); window 0: no window. A row that sees
  * nothing is zeros. What a row does not see has no part in it, infinities and NaN included.
  */

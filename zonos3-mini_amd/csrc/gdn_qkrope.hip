@@ -7,8 +7,9 @@
 // over 8 or 4 lanes. A wave takes one token: its lanes form the token's R / 2 angles once, one a lane, and hand them round
 // through LDS; then up to three groups of 64 / (D / 16) heads, all loads first. A token of more groups, or each group of
 // a few tokens, has a wave of its own.
-// Measured: 30526 rows of 16 + 2 heads, D = 128, bf16: 56 us, 5.05 TB/s, the rate of a copy; one token of 8 + 2 heads into a
-// cache 2.8 us in a graph, a launch's own time.
+// Measured: calls of 30526 rows of 16 + 2 heads, D = 128, on inputs that rotate: bf16 56 us, 5.05 TB/s, fp32 113 us, 4.96 (a copy:
+// 5.14; on the same inputs again and again the bf16 kernel takes 50, for it finds some of them in the last-level cache); one token
+// of 8 + 2 heads into a cache 2.8 us in a graph, a launch's own time.
 // The angle is reduced to a quarter turn in float64: position * inv_freq has 24 bits in float32, and at position 2^20 the
 // rest of them after the whole turns would be 7 (an error of 0.03).
 #include <type_traits>

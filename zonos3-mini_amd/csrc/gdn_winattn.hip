@@ -10,12 +10,16 @@
 // Tiles of K and V are loaded straight into LDS, a tile ahead. The keys that a workgroup's rows see are one list, sinks then
 // window, so that a few sinks share a tile with the window's first keys; tiles that all rows of a wave see whole have no mask.
 // Scores, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
+// What a row is divided by is the sum of its weights as they are at D = 128 and as they are rounded at D = 64, whichever costs
+// fewer cycles there (RowWave::add): a weight's rounding is then the output's alone, or the sum's with it.
 // The maximum may lag by 2^8: it is taken on, and O rescaled, only where a row's rises by more.
 //
-// What bounds it: matrix products, and the card's power. 16384 tokens of 16 heads on 4, D = 128: 1010 us, 1090 TFLOP/s, 88 % of
-// the rate of a large library product; the matrix units are busy for 62 % of the cycles, at a clock that falls to 1.5-1.8 GHz
-// (1.3 times the cycles at 1.74 GHz took no longer). 32768 tokens through a window of 1024: 310 us, 47 of them what reading q
-// and writing o takes, 14.2 a tile of 64 keys. fp32: 117 TFLOP/s of 154.
+// What bounds it: matrix products, and the card's power. 16384 tokens of 16 heads on 4, D = 128: 977 .. 1094 us by card and by
+// how long it has been busy, 1005 .. 1125 TFLOP/s, 81 .. 90 % of the rate of a large library product; the matrix units are busy
+// for 62 % of the cycles, at a clock that falls to 1.5-1.8 GHz (1.3 times the cycles at 1.74 GHz took no longer). 32768 tokens
+// through a window of 1024: 316 .. 335 us, eight rounds of two workgroups a CU of which 17 tiles of 64 keys take 33 us and start
+// and end 6 each. fp32, 16 heads on 4: 8192 tokens 2355 us at D = 128 and 1140 at D = 64, 117 and 121 TFLOP/s of 154; 4096 tokens
+// 765 and 311, 90 and 111.
 //
 // A masked weight is 0, but 0 times an infinity or a NaN of V is a NaN. A workgroup with an output that is not finite computes
 // its rows once more, and in tiles that a row of it does not see whole zeroes such entries in LDS ahead of the product; what
@@ -545,6 +549,8 @@ struct RowWave {
 
 // Many rows: a wave for each 32 of a workgroup's, all on the same tiles. The scores of a tile are formed beside the product of
 // the one before, so that matrix and vector instructions have each other to run beside; K is loaded a tile further ahead than V.
+// (Three workgroups a CU at D = 64. For fp32 there 10 of a wave's registers are then spilled; two a CU, which would need none to
+// be, have not been measured.)
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : sizeof(T) == 2 ? 2 : 1) void win_attn_kernel(WinArgs a) {
   constexpr int KT = sizeof(T) == 2 ? 64 : 32, ROWB = D * (int)sizeof(T), LW = KT * ROWB / 1024 / NW, ROWS = 32 * NW;
@@ -830,7 +836,9 @@ WinPlan win_plan(const WinArgs& a, int D, int dtype) {
   const double cus = device_cus(), kt = dtype == ZGDN_F32 ? 32 : 64;
   const WinCost cost = win_cost(D, dtype);
   WinPlan many{row_tiles(a, 128), 128, 1}, few{row_tiles(a, 32), 32, 1};
-  // keys of the longest list and of a list in the mean (a packed batch is taken for sequences of equal length)
+  // Keys of the longest list and of a list in the mean. The lengths of a packed batch are on the device: it is taken for
+  // sequences of equal length, so that `most` is no bound there. One of 30008 keys among 63 of 108, 8 queries each: 496 us, its list
+  // walked by one workgroup a key head, where it alone is shared out and takes 26.
   const double seqs = a.cu_q != nullptr ? a.N : 1, nk = a.Tk / seqs, nq = std::min(a.Tq / seqs, nk);
   const double reach = a.window > 0 ? (double)a.window + a.sinks + 32 : nk;
   const double most = std::min(nk, reach), mean = std::min(nk - nq / 2, reach);

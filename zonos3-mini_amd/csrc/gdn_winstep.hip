@@ -11,9 +11,10 @@
 // maximum, sum, O) are joined in LDS, those of a stream's chunks by a second kernel, in order.
 // What is not seen is loaded as zeros, so that nothing of it (a NaN, say) meets a weight of 0.
 // Loads bypass the caches' retention, and the key heads of one chunk stand beside one another in the grid (a cache's row is all
-// of them): 64 streams over caches of 4096 .. 8192 rows, 16 heads on 4, D = 128: 155 us, 5.4 TB/s, the rate of a copy (202 us
-// without both). One stream over 32768 rows: 20.6 us where its bytes take 13; two launches and the first loads' chain (length and
-// pages, rows, queries) are the rest.
+// of them): a call of 64 streams over caches of 4096 .. 8192 rows, 16 heads on 4, D = 128: 150 us, 5.5 TB/s (202 us without
+// both), of 256 streams over 3.2 GB 580 us, 5.6 TB/s, so that it is memory and not a cache that gives them: reads alone, a tenth
+// faster than a copy (5.14). One stream over 32768 rows: 20.2 us where its bytes take 13; two launches and the first loads' chain
+// (length and pages, rows, queries) are the rest.
 // Sums, statistics and O are fp32; P is rounded to bf16 for the product where V is bf16 (at most 2^-8 of each weight, as V's own).
 #include <algorithm>
 #include <cmath>

@@ -60,3 +60,24 @@ def test_workspaces_go_by_the_tensors_device(gdn, launches, order):
         gdn.window_attn_fwd(q, k, k, window=9, sinks=1)
         gdn.window_attn_step(q[0, :2], c, c, z(2, dtype=torch.int32), window=9)
     assert launches == [(i, n, 64 * CUS[i] + s) for i in order for n, s in (("zattn_window_fwd", 10), ("zattn_window_step", 8))]
+
+
+@pytest.mark.gpu
+def test_sizes_first_met_in_a_capture(gdn, cuda):
+    """A workspace's size is asked for, and its device made current, while a graph is captured: sizes that no call had before."""
+    importlib.import_module("zonos3-mini_amd.ops")._attn_workspace.cache_clear()
+    g = torch.Generator().manual_seed(91)
+    r = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(cuda)  # noqa: E731
+    q, k, v, n = r(1, 11, 8, 128), r(1, 2900, 2, 128), r(1, 2900, 2, 128), torch.tensor([2801], dtype=torch.int32, device=cuda)
+    calls = lambda: (gdn.window_attn_fwd(q, k, v), gdn.window_attn_step(q[:, -1], k, v, n))  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    want = calls()
+    for _ in range(3):
+        for o in out:
+            o.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        want = calls()
